@@ -328,6 +328,37 @@ B2Q_API int b2q_moe_gemm_fp8(const void* x, int act_dtype, int64_t ldx,
                      int64_t rows, int64_t N, int64_t K, int act,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- 8-bit integer operators -------------------------------------------------
+ * Weights int8 [N, K] with one scale per output channel, activations int8 with one scale per token ("W8A8 int8").  The reference
+ * has no such format; everything here is an addition.
+ *
+ * Rows to codes:  a = max(max_k |x[m, k]|, 1e-12);  scale[m] = a / 127;  q[m, k] = rint(127 x[m, k] / a), halves to even, decided
+ * exactly.  A row that holds an infinity or a NaN gets the scale NaN and zero codes.  Serves tokens and, at load time, the rows of a
+ * weight.  x bf16, fp16 or fp32 [M, K] with row pitch ldx (elements), any K >= 1, any alignment of the elements' own size; q is
+ * contiguous [M, K].  Rows of 16-byte aligned 16-bit values with K % 8 == 0 are read once, others twice and more slowly.   */
+B2Q_API int b2q_quantize_int8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* scale, int64_t M, int64_t K, void* stream);
+/* The same of silu(x[:, :K]) * x[:, K:2K] in fp32, never rounded to 16 bits in between; ldx >= 2K, 16-bit types.        */
+B2Q_API int b2q_silu_mul_quantize_int8(const void* gate_up, int act_dtype, int64_t ldx, int8_t* q, float* scale, int64_t M, int64_t K,
+                               void* stream);
+/* The same of RMSNorm(v) * norm_weight with v = hidden + residual in fp32; residual_out <- v in act_dtype, and may be residual
+ * itself.  All tensors contiguous [M, K].                                                                               */
+B2Q_API int b2q_resadd_rmsnorm_quantize_int8(const void* hidden, const void* residual, const void* norm_weight, void* residual_out,
+                                     int act_dtype, float eps, int8_t* q, float* scale, int64_t M, int64_t K, void* stream);
+
+/* out[m, n] = scale[m] * wscale[n] * sum_k q[m, k] w[n, k] (+ bias[n]): the sum exact in 32-bit integers, the rest in fp32, one
+ * rounding to out_dtype (bf16 / fp16, also bias's type).  q [M, K] with row pitch ldq (bytes), w contiguous [N, K], wscale [N] in
+ * any of the three types.  Any M, N; K % 16 == 0, K < 131072 (no sum can overflow); q, w and ldq 16-byte aligned, out only to its
+ * elements.  No scratch.  Results do not depend on how the work is divided: integer sums are exact in any order.        */
+B2Q_API int b2q_linear_int8(const int8_t* q, int64_t ldq, const float* scale, const int8_t* w, const void* wscale, int wscale_dtype,
+                    const void* bias, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, void* stream);
+/* b2q_quantize_int8 and b2q_linear_int8 as one call on 16-bit rows, with the same codes and results; out and bias in act_dtype.  A
+ * few tokens take one launch and no scratch; b2q_linear_int8_dynamic_workspace_bytes says what is needed.  Scratch is the
+ * call's own until its last kernel has completed.                                                                        */
+B2Q_API size_t b2q_linear_int8_dynamic_workspace_bytes(int64_t M, int64_t N, int64_t K);
+B2Q_API int b2q_linear_int8_dynamic(const void* x, int act_dtype, int64_t ldx, const int8_t* w, const void* wscale, int wscale_dtype,
+                            const void* bias, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* ---- sum of row-parallel partial results over the GPUs of one box ----------------------------
  * The exchange step behind a row-parallel linear (o_proj, down) of a tensor-parallel decoder layer; the
  * reference calls the serving framework's all-reduce there (vllm/patches/vllm_for_multi_arc.patch:10185,

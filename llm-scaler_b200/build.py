@@ -18,6 +18,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 OUT = os.path.join(HERE, "custom_esimd_kernels_vllm", "libb2q.so")
 OUT_TORCH = os.path.join(HERE, "custom_esimd_kernels_vllm", "libb2q_torch.so")
+OUT_INT8 = os.path.join(HERE, "custom_esimd_kernels_vllm", "libb2q_int8.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC_FLAGS = [
@@ -72,33 +73,35 @@ def build(force=False, verbose=False):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
-    build_torch_ops(force or bool(jobs))
+    with cf.ThreadPoolExecutor() as ex:
+        list(ex.map(lambda a: build_torch_ops(force or bool(jobs), *a), ((OUT_TORCH, "torch_ops.cpp"), (OUT_INT8, "torch_int8.cpp"))))
     return OUT
 
 
-def build_torch_ops(force=False):
-    """libb2q_torch.so: the C++ torch-op registration of the dense linears (csrc/torch_ops.cpp) over libb2q.so.
+def build_torch_ops(force=False, out=OUT_TORCH, source="torch_ops.cpp"):
+    """libb2q_torch.so: the C++ torch-op registration of the dense linears (csrc/torch_ops.cpp) over libb2q.so; libb2q_int8.so: that of
+    the 8-bit integer operators (csrc/torch_int8.cpp).
     Host code only: compiled with g++ against the installed torch's headers and linked with its libraries."""
-    src = os.path.join(CSRC, "torch_ops.cpp")
+    src = os.path.join(CSRC, source)
     hdr = os.path.join(INCLUDE, "b2q.h")
-    if not force and os.path.exists(OUT_TORCH) and os.path.getmtime(OUT_TORCH) >= max(os.path.getmtime(src), os.path.getmtime(hdr), os.path.getmtime(OUT)):
-        return OUT_TORCH
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(hdr), os.path.getmtime(OUT)):
+        return out
     import torch
     tdir = os.path.dirname(torch.__file__)
     cuda_home = os.environ.get("CUDA_HOME") or os.path.dirname(os.path.dirname(_nvcc()))
     gxx = os.environ.get("CXX") or shutil.which("g++")
     if not gxx:
-        raise RuntimeError("g++ not found; libb2q_torch.so cannot be built")
+        raise RuntimeError("g++ not found; %s cannot be built" % os.path.basename(out))
     cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
            "-I", INCLUDE, "-I", os.path.join(tdir, "include"), "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
-           "-I", os.path.join(cuda_home, "include"), src, "-o", OUT_TORCH,
+           "-I", os.path.join(cuda_home, "include"), src, "-o", out,
            "-L", os.path.dirname(OUT), "-l:libb2q.so", "-L", os.path.join(tdir, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
            "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("g++ failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
-    return OUT_TORCH
+    return out
 
 
 if __name__ == "__main__":

@@ -1,0 +1,313 @@
+// Rows to int8 codes and one scale per row: a = max(max |x|, 1e-12), scale = a / 127, code = rint(127 x / a) with halves to even, decided
+// exactly (i8.cuh).  A row that holds an infinity or a NaN gets the scale NaN and zero codes, so that everything made from it is NaN.
+//
+// Three forms of x: a row of 16-bit (or fp32) values; silu(gate) * up; and the RMSNorm of hidden + residual, whose codes need no
+// 1 / rms: it cancels out of v w / max |v w|, so that one reduction gives both the sum of squares and the maximum.
+//
+// Memory-bound: a row is read once and stays in registers between the maximum and the codes.  Rows of up to 1024 values take a warp
+// each, longer ones a CTA with one barrier; what is not 16-byte aligned, or longer than 1024 threads hold, is read twice.
+#include "i8.cuh"
+
+namespace b2q {
+
+namespace i8q {
+enum { PLAIN, SILU, NORM };
+
+struct Params {
+  const void* x; int64_t ldx;                              // elements
+  const void* residual; const void* nw; void* residual_out; float eps;
+  const int32_t* idx; int div; const int32_t* n_valid;
+  int8_t* q; float* s; int64_t M; int K;
+};
+
+__device__ __forceinline__ void enter() {                  // as in moe_aux.cu: a grid that fills the GPU lets the next one begin later
+  const bool few = gridDim.x <= 148;
+  if (few) grid_dep_release();
+  grid_dep_wait();
+  if (!few) grid_dep_release();
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }      // orders as |v|, NaN above all
+
+// Scale of a row whose largest |value| has these bits; a and r for the codes.  False where the row is not finite.
+__device__ __forceinline__ bool row_scale(uint32_t bits, float& a, float& r, float& scale) {
+  a = fmaxf(__uint_as_float(bits), I8_MIN_AMAX);
+  scale = a / 127.f;
+  r = 127.f / a;
+  if (bits < 0x7F800000u) return true;
+  scale = __uint_as_float(0x7FC00000u);
+  return false;
+}
+
+template <bool BF16> __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  unpack2<BF16>(v.x, f[0], f[1]); unpack2<BF16>(v.y, f[2], f[3]); unpack2<BF16>(v.z, f[4], f[5]); unpack2<BF16>(v.w, f[6], f[7]);
+}
+
+// Eight values of a row as they are to be quantised.  PLAIN keeps the raw words, the other forms the eight floats.
+template <int MODE, bool BF16> struct Piece {
+  float f[8];
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = f[i];
+  }
+};
+template <bool BF16> struct Piece<PLAIN, BF16> {
+  uint4 v;
+  __device__ __forceinline__ void get(float (&o)[8]) const { unpack8<BF16>(v, o); }
+};
+
+// WARP: a row per warp, V pieces per lane.  Otherwise a row per CTA, V pieces per thread.
+template <int MODE, bool BF16, int V, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Params p) {
+  __shared__ uint32_t red_max[32];
+  __shared__ float red_sum[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int step = WARP ? 32 : blockDim.x, first = WARP ? lane : threadIdx.x;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
+  enter();
+  if (row >= p.M) return;                                  // whole warps, or the whole CTA
+  int64_t src = row;
+  if constexpr (MODE == PLAIN) {
+    if (p.idx) {
+      if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
+      src = *reinterpret_cast<const volatile int32_t*>(p.idx + row) / p.div;
+    }
+  }
+  const int n8 = p.K >> 3;
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + src * p.ldx;
+  Piece<MODE, BF16> pc[V];
+  uint32_t mx = 0;
+  float sum = 0.f;
+  if constexpr (MODE == PLAIN) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = first + i * step;
+      pc[i].v = c < n8 ? ld_vec(x + 8 * c) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float f[8];
+      pc[i].get(f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx = max(mx, abs_bits(f[j]));
+    }
+  } else if constexpr (MODE == SILU) {
+    uint4 g[V], u[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = first + i * step;
+      const bool in = c < n8;
+      g[i] = in ? ld_vec(x + 8 * c) : make_uint4(0, 0, 0, 0);
+      u[i] = in ? ld_vec(x + p.K + 8 * c) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float a[8], b[8];
+      unpack8<BF16>(g[i], a);
+      unpack8<BF16>(u[i], b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        pc[i].f[j] = silu_mul_f(a[j], b[j]);
+        mx = max(mx, abs_bits(pc[i].f[j]));
+      }
+    }
+  } else {
+    const uint16_t* rs = reinterpret_cast<const uint16_t*>(p.residual) + row * p.K;
+    uint16_t* ro = reinterpret_cast<uint16_t*>(p.residual_out) + row * p.K;
+    uint4 h[V], r[V], w[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = first + i * step;
+      const bool in = c < n8;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      h[i] = in ? ld_vec(x + 8 * c) : zero;
+      r[i] = in ? ld_vec(rs + 8 * c) : zero;
+      w[i] = in ? ld_vec(reinterpret_cast<const uint16_t*>(p.nw) + 8 * c) : zero;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = first + i * step;
+      float a[8], b[8];
+      unpack8<BF16>(h[i], a);
+      unpack8<BF16>(r[i], b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { a[j] += b[j]; sum = fmaf(a[j], a[j], sum); }
+      if (c < n8)
+        *reinterpret_cast<uint4*>(ro + 8 * c) =
+            make_uint4(pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3]), pack2<BF16>(a[4], a[5]), pack2<BF16>(a[6], a[7]));
+      unpack8<BF16>(w[i], b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        pc[i].f[j] = a[j] * b[j];
+        mx = max(mx, abs_bits(pc[i].f[j]));
+      }
+    }
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if constexpr (MODE == NORM) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  if constexpr (!WARP) {                                   // every warp finishes the reduction itself: one barrier
+    if (lane == 0) { red_max[warp] = mx; if constexpr (MODE == NORM) red_sum[warp] = sum; }
+    __syncthreads();
+    const bool in = lane < (int)(blockDim.x >> 5);
+    mx = __reduce_max_sync(0xffffffffu, in ? red_max[lane] : 0u);
+    if constexpr (MODE == NORM) {
+      sum = in ? red_sum[lane] : 0.f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+  }
+  float a, r, scale;
+  bool finite;
+  if constexpr (MODE == NORM) {
+    const float rstd = rsqrtf(sum / (float)p.K + p.eps), an = __uint_as_float(mx) * rstd;
+    finite = row_scale(abs_bits(an), a, r, scale) && mx < 0x7F800000u && abs_bits(sum) <= 0x7F800000u;
+    if (!finite) scale = __uint_as_float(0x7FC00000u);
+    // codes of v w, whose maximum stands for the normed row's; of a row that is nearly nothing, of v w rstd against the floor
+    a = fmaxf(__uint_as_float(mx), I8_MIN_AMAX / rstd);
+    r = 127.f / a;
+  } else {
+    finite = row_scale(mx, a, r, scale);
+  }
+  if (first == 0) p.s[row] = scale;
+  uint8_t* q = reinterpret_cast<uint8_t*>(p.q) + row * p.K;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = first + i * step;
+    if (c < n8) {
+      float f[8];
+      pc[i].get(f);
+      const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+      uint2 o = make_uint2(0, 0);
+      if (finite) o = make_uint2(i8_codes4(lo, a, r), i8_codes4(hi, a, r));
+      *reinterpret_cast<uint2*>(q + 8 * c) = o;
+    }
+  }
+}
+
+// Any K, any alignment: element by element, the row read twice.
+template <int MODE, int DT>
+__global__ void __launch_bounds__(512) quantize_i8_any_kernel(const Params p) {
+  __shared__ uint32_t red_max[16];
+  __shared__ float red_sum[16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
+  enter();
+  int64_t src = row;
+  if constexpr (MODE == PLAIN) {
+    if (p.idx) {
+      if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
+      src = *reinterpret_cast<const volatile int32_t*>(p.idx + row) / p.div;
+    }
+  }
+  auto at = [&](const void* b, int64_t i) -> float {
+    if constexpr (DT == B2Q_F32) return reinterpret_cast<const volatile float*>(b)[i];
+    else return scalar_from_raw(reinterpret_cast<const volatile unsigned short*>(b)[i], DT);
+  };
+  uint32_t mx = 0;
+  float sum = 0.f;
+  for (int c = threadIdx.x; c < p.K; c += 512) {
+    float v = at(p.x, src * p.ldx + c);
+    if constexpr (MODE == SILU) v = silu_mul_f(v, at(p.x, src * p.ldx + p.K + c));
+    if constexpr (MODE == NORM) {
+      v += at(p.residual, row * p.K + c);
+      sum = fmaf(v, v, sum);
+      v *= at(p.nw, c);
+    }
+    mx = max(mx, abs_bits(v));
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) { red_max[warp] = mx; red_sum[warp] = sum; }
+  __syncthreads();
+  mx = __reduce_max_sync(0xffffffffu, lane < 16 ? red_max[lane] : 0u);
+  sum = lane < 16 ? red_sum[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  float a, r, scale;
+  bool finite;
+  if constexpr (MODE == NORM) {
+    const float rstd = rsqrtf(sum / (float)p.K + p.eps), an = __uint_as_float(mx) * rstd;
+    finite = row_scale(abs_bits(an), a, r, scale) && mx < 0x7F800000u && abs_bits(sum) <= 0x7F800000u;
+    if (!finite) scale = __uint_as_float(0x7FC00000u);
+    a = fmaxf(__uint_as_float(mx), I8_MIN_AMAX / rstd);
+    r = 127.f / a;
+  } else {
+    finite = row_scale(mx, a, r, scale);
+  }
+  if (threadIdx.x == 0) p.s[row] = scale;
+  for (int c = threadIdx.x; c < p.K; c += 512) {
+    float v = at(p.x, src * p.ldx + c);
+    if constexpr (MODE == SILU) v = silu_mul_f(v, at(p.x, src * p.ldx + p.K + c));
+    if constexpr (MODE == NORM) {
+      v += at(p.residual, row * p.K + c);
+      store_scalar(p.residual_out, row * p.K + c, DT, v);
+      v *= at(p.nw, c);
+    }
+    p.q[row * p.K + c] = finite ? (int8_t)i8_code_exact(v, a, r) : (int8_t)0;
+  }
+}
+
+template <typename... KArgs, typename... Args>
+static int launch(void (*kern)(KArgs...), int64_t grid, int block, cudaStream_t st, Args&&... args) {
+  if (grid > INT32_MAX) return B2Q_ERR_LIMIT;
+  launch_overlapped(kern, dim3((unsigned)grid), dim3(block), 0, st, tls().overlap_mode > 0, args...);
+  note_launch("quantize_i8");
+  return launch_status();
+}
+
+template <int MODE, bool BF16> static int run_vec(const Params& p, cudaStream_t st) {
+  const int n8 = p.K / 8;
+  // short rows, and enough of them to fill the SMs: a warp each
+  if (n8 <= 128 && p.M >= 148) {
+    const int64_t grid = (p.M + 7) / 8;
+    if (n8 <= 32) return launch(quantize_i8_kernel<MODE, BF16, 1, true>, grid, 256, st, p);
+    if (n8 <= 64) return launch(quantize_i8_kernel<MODE, BF16, 2, true>, grid, 256, st, p);
+    return launch(quantize_i8_kernel<MODE, BF16, 4, true>, grid, 256, st, p);
+  }
+  auto block = [&](int v) { return (n8 + 32 * v - 1) / (32 * v) * 32; };
+  const bool few = p.M <= 148;                             // one CTA per SM at most: as many threads as a row gives work to
+  if (few ? n8 <= 1024 : n8 <= 256) return launch(quantize_i8_kernel<MODE, BF16, 1, false>, p.M, block(1), st, p);
+  if (few ? n8 <= 2048 : n8 <= 1024) return launch(quantize_i8_kernel<MODE, BF16, 2, false>, p.M, block(2), st, p);
+  return launch(quantize_i8_kernel<MODE, BF16, 4, false>, p.M, block(4), st, p);
+}
+
+template <int MODE> static int run(const Params& p, int dt, bool vec, cudaStream_t st) {
+  if (p.M == 0) return B2Q_OK;
+  if (vec && p.K % 8 == 0 && p.K <= 32768 && dt != B2Q_F32) return dt == B2Q_BF16 ? run_vec<MODE, true>(p, st) : run_vec<MODE, false>(p, st);
+  if (dt == B2Q_BF16) return launch(quantize_i8_any_kernel<MODE, B2Q_BF16>, p.M, 512, st, p);
+  if (dt == B2Q_F16) return launch(quantize_i8_any_kernel<MODE, B2Q_F16>, p.M, 512, st, p);
+  if constexpr (MODE == PLAIN) return launch(quantize_i8_any_kernel<MODE, B2Q_F32>, p.M, 512, st, p);
+  return B2Q_ERR_DTYPE;
+}
+static bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+}  // namespace i8q
+
+int quantize_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
+  i8q::Params p{};
+  p.x = x; p.ldx = ldx; p.q = q; p.s = s; p.M = M; p.K = K;
+  return i8q::run<i8q::PLAIN>(p, x_dtype, aligned16(x) && i8q::aligned8(q) && ldx % 8 == 0, st);
+}
+int quantize_i8_gather(const void* x, bool bf16, int64_t ldx, const int32_t* idx, int div, const int32_t* n_valid, int8_t* q, float* s, int64_t rows, int K,
+                       cudaStream_t st) {
+  i8q::Params p{};
+  p.x = x; p.ldx = ldx; p.idx = idx; p.div = div; p.n_valid = n_valid; p.q = q; p.s = s; p.M = rows; p.K = K;
+  return i8q::run<i8q::PLAIN>(p, bf16 ? B2Q_BF16 : B2Q_F16, aligned16(x) && i8q::aligned8(q) && ldx % 8 == 0, st);
+}
+int silu_mul_quantize_i8(const void* gate_up, bool bf16, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
+  i8q::Params p{};
+  p.x = gate_up; p.ldx = ldx; p.q = q; p.s = s; p.M = M; p.K = K;
+  return i8q::run<i8q::SILU>(p, bf16 ? B2Q_BF16 : B2Q_F16, aligned16(gate_up) && i8q::aligned8(q) && ldx % 8 == 0, st);
+}
+int resadd_rmsnorm_quantize_i8(const void* hidden, const void* residual, const void* w, void* residual_out, bool bf16, float eps, int8_t* q, float* s,
+                               int64_t M, int K, cudaStream_t st) {
+  i8q::Params p{};
+  p.x = hidden; p.ldx = K; p.residual = residual; p.nw = w; p.residual_out = residual_out; p.eps = eps; p.q = q; p.s = s; p.M = M; p.K = K;
+  return i8q::run<i8q::NORM>(p, bf16 ? B2Q_BF16 : B2Q_F16,
+                             aligned16(hidden) && aligned16(residual) && aligned16(w) && aligned16(residual_out) && i8q::aligned8(q), st);
+}
+
+}  // namespace b2q

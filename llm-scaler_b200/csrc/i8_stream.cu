@@ -1,0 +1,224 @@
+// Int8 linear of up to sixteen tokens: out[m, n] = scale[m] wscale[n] sum_k codes[m, k] w[n, k] (+ bias[n]).
+//
+// HBM-bound: the weights are read once and nothing else is large.  They go from global memory straight into the registers that
+// mma.sync m16n8k32 takes them from: with the k of a 64-byte piece permuted the same way on both sides, a lane's sixteen bytes of a weight
+// row are the B operands of two MMAs (rows as the MMA's columns, tokens as its rows), so there is nothing to stage, convert or wait for
+// but the loads themselves.
+//
+// Every CTA has rows of its own, dealt out evenly over two CTAs per SM.  Its eight warps share the work in units of eight 16-byte
+// loads per lane (32 rows x 128 k, 16 x 256 or 8 x 512), an equal run of units each; the next unit's loads are on their way while a unit is
+// multiplied.  Integer sums are exact in any order, so warps that share rows add into shared memory by atomics and every result is
+// bit-identical whatever the division.
+//
+// The 16-bit form quantises the tokens by itself: each CTA makes all codes in its shared memory while its first weights arrive.
+#include "i8.cuh"
+
+namespace b2q {
+
+namespace i8s {
+constexpr int WARPS = 8, THREADS = 32 * WARPS, LOADS = 8;
+constexpr int CODES_MAX = 96 * 1024;                       // bytes of shared memory for the codes of the 16-bit form
+
+struct Params {
+  const int8_t* xq; int64_t ldx; const float* xs;
+  const uint16_t* x16; int64_t ldx16;
+  const int8_t* w; const void* ws; int ws_dtype; const void* bias;
+  void* out; int64_t ldo;
+  int M, N, K;
+  int row_cap, code_pitch;                                 // rows of sums per token; bytes between two tokens' codes
+  int early;                                               // weights may be read before the kernels in front are done
+};
+
+__device__ __forceinline__ void add_shared(int* p, int v) {
+  asm volatile("red.shared.add.s32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(p)), "r"(v) : "memory");
+}
+
+// R: eights of rows in a unit
+template <int R, bool FROM16, bool BF16>
+__global__ void __launch_bounds__(THREADS, 2) i8_stream_kernel(const Params p) {
+  constexpr int S = LOADS / R, ROWS = 8 * R, KU = 64 * S;
+  extern __shared__ __align__(16) uint8_t smem[];
+  int* sums = reinterpret_cast<int*>(smem);                // [M][row_cap]
+  uint8_t* codes = smem + (size_t)p.M * p.row_cap * 4;     // [M][code_pitch]
+  __shared__ float token_scale[I8_STREAM_MAX_TOK];
+  __shared__ uint32_t token_max[I8_STREAM_MAX_TOK];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int r0 = (int)((int64_t)blockIdx.x * p.N / gridDim.x), rows = (int)((int64_t)(blockIdx.x + 1) * p.N / gridDim.x) - r0;
+  const int nck = (p.K + KU - 1) / KU, units = (rows + ROWS - 1) / ROWS * nck;
+  const int u0 = (int)((int64_t)warp * units / WARPS), u1 = (int)((int64_t)(warp + 1) * units / WARPS);
+
+  grid_dep_release();
+  uint4 cur[LOADS], nxt[LOADS];
+  auto load = [&](int u, uint4 (&v)[LOADS]) {
+    const int group = u / nck, k0 = (u - group * nck) * KU + 16 * t;
+    const int8_t* base = p.w + (int64_t)(r0 + group * ROWS + g) * p.K + k0;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        const bool in = group * ROWS + 8 * i + g < rows && k0 + 64 * j < p.K;
+        v[i * S + j] = in ? ld_weight(base + (int64_t)(8 * i) * p.K + 64 * j) : make_uint4(0, 0, 0, 0);
+      }
+  };
+  if (!p.early) grid_dep_wait();
+  if (u0 < u1) load(u0, cur);
+  for (int i = threadIdx.x; i < p.M * p.row_cap; i += THREADS) sums[i] = 0;
+  if (FROM16 && threadIdx.x < I8_STREAM_MAX_TOK) token_max[threadIdx.x] = 0;
+  if (p.early) grid_dep_wait();
+  __syncthreads();
+
+  if constexpr (FROM16) {
+    const int n8 = p.K >> 3, total = p.M * n8;
+    for (int i = threadIdx.x; i < (total + 31) / 32 * 32; i += THREADS) {      // whole warps; a warp may straddle two tokens
+      const int m = min(i / n8, p.M - 1);
+      uint32_t mx = 0;
+      if (i < total) {
+        const uint4 v = ld_vec(p.x16 + m * p.ldx16 + 8 * (i - m * n8));
+        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float a, b;
+          unpack2<BF16>(e[j], a, b);
+          mx = max(mx, max(__float_as_uint(a) & 0x7FFFFFFFu, __float_as_uint(b) & 0x7FFFFFFFu));
+        }
+      }
+      if (__match_any_sync(0xffffffffu, m) == 0xffffffffu) {
+        mx = __reduce_max_sync(0xffffffffu, mx);
+        if (lane == 0) atomicMax(&token_max[m], mx);
+      } else {
+        atomicMax(&token_max[m], mx);
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < total; i += THREADS) {
+      const int m = i / n8, c = i - m * n8;
+      const uint4 v = ld_vec(p.x16 + m * p.ldx16 + 8 * c);
+      const uint32_t bits = token_max[m];
+      const float a = fmaxf(__uint_as_float(bits), I8_MIN_AMAX), r = 127.f / a;
+      const bool finite = bits < 0x7F800000u;
+      float lo[4], hi[4];
+      unpack2<BF16>(v.x, lo[0], lo[1]); unpack2<BF16>(v.y, lo[2], lo[3]); unpack2<BF16>(v.z, hi[0], hi[1]); unpack2<BF16>(v.w, hi[2], hi[3]);
+      uint2 o = make_uint2(0, 0);
+      if (finite) o = make_uint2(i8_codes4(lo, a, r), i8_codes4(hi, a, r));
+      *reinterpret_cast<uint2*>(codes + m * p.code_pitch + 8 * c) = o;
+      if (c == 0) token_scale[m] = finite ? a / 127.f : __uint_as_float(0x7FC00000u);
+    }
+    __syncthreads();
+  }
+
+  int acc[R][4];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[i][c] = 0;
+  auto multiply = [&](int u, const uint4 (&v)[LOADS]) {
+    const int group = u / nck, k0 = (u - group * nck) * KU + 16 * t;
+    uint4 xa[S], xb[S];
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      const int k = k0 + 64 * j;
+      xa[j] = xb[j] = make_uint4(0, 0, 0, 0);
+      if constexpr (FROM16) {
+        if (g < p.M && k < p.K) xa[j] = *reinterpret_cast<const uint4*>(codes + g * p.code_pitch + k);
+        if (g + 8 < p.M && k < p.K) xb[j] = *reinterpret_cast<const uint4*>(codes + (g + 8) * p.code_pitch + k);
+      } else {
+        if (g < p.M && k < p.K) xa[j] = ld_vec(p.xq + g * p.ldx + k);
+        if (g + 8 < p.M && k < p.K) xb[j] = ld_vec(p.xq + (g + 8) * p.ldx + k);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        const uint4 w = v[i * S + j];
+        mma_s8(acc[i], xa[j].x, xb[j].x, xa[j].y, xb[j].y, w.x, w.y);
+        mma_s8(acc[i], xa[j].z, xb[j].z, xa[j].w, xb[j].w, w.z, w.w);
+      }
+  };
+  auto flush = [&](int group) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int m = g + (c & 2) * 4, r = group * ROWS + 8 * i + 2 * t + (c & 1);
+        if (m < p.M && r < rows) add_shared(sums + m * p.row_cap + r, acc[i][c]);
+        acc[i][c] = 0;
+      }
+    }
+  };
+  for (int u = u0; u < u1; ++u) {
+    if (u + 1 < u1) load(u + 1, nxt);
+    multiply(u, cur);
+    const int group = u / nck;
+    if (u + 1 == u1 || (u + 1) / nck != group) flush(group);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) cur[i] = nxt[i];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.M * rows; i += THREADS) {
+    const int m = i / rows, r = i - m * rows, n = r0 + r;
+    const float s = FROM16 ? token_scale[m] : ld_f32(p.xs + m);
+    const float v = i8_output(sums[m * p.row_cap + r], s, load_scalar(p.ws, n, p.ws_dtype), p.bias ? load_scalar(p.bias, n, BF16 ? B2Q_BF16 : B2Q_F16) : 0.f);
+    reinterpret_cast<uint16_t*>(p.out)[m * p.ldo + n] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+  }
+}
+
+static int sm_count() {
+  static thread_local int sms[16] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 16) return 148;
+  if (!sms[dev]) {
+    cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    if (sms[dev] <= 0) sms[dev] = 148;
+  }
+  return sms[dev];
+}
+
+// codes of neighbouring tokens 64 bytes apart in the banks: a quarter warp reads two tokens' 64 bytes without a conflict
+static int code_pitch(int K) { return (K + 127) / 128 * 128 + 64; }
+
+template <int R, bool FROM16, bool BF16> static int launch(Params& p, int grid, cudaStream_t st) {
+  p.row_cap = (p.N + grid - 1) / grid;
+  p.row_cap = (p.row_cap + 3) / 4 * 4;                     // the codes behind the sums stay 16-byte aligned
+  p.code_pitch = code_pitch(p.K);
+  const int smem = p.M * p.row_cap * 4 + (FROM16 ? p.M * p.code_pitch : 0);
+  auto kern = i8_stream_kernel<R, FROM16, BF16>;
+  static thread_local int configured[16] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (smem > 47 * 1024 && (dev >= 16 || configured[dev] < smem)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return B2Q_ERR_CUDA;
+    if (dev < 16) configured[dev] = smem;
+  }
+  launch_overlapped(kern, dim3(grid), dim3(THREADS), smem, st, tls().overlap_mode > 0, p);
+  note_launch("i8_stream");
+  return launch_status();
+}
+
+template <bool FROM16, bool BF16> static int pick(Params& p, cudaStream_t st) {
+  // two CTAs per SM; more where the sums of that many rows would not fit beside the codes
+  int grid = 2 * sm_count();
+  while ((int64_t)p.M * ((p.N + grid - 1) / grid) * 4 > 64 * 1024) grid *= 2;
+  if (grid > p.N) grid = p.N;
+  const int rows = (p.N + grid - 1) / grid;
+  if (rows <= 8) return launch<1, FROM16, BF16>(p, grid, st);
+  if (rows <= 16) return launch<2, FROM16, BF16>(p, grid, st);
+  return launch<4, FROM16, BF16>(p, grid, st);
+}
+}  // namespace i8s
+
+bool i8_stream_supported(const I8LinearArgs& a) {
+  return a.M <= I8_STREAM_MAX_TOK && (!a.x16 || (a.M * i8s::code_pitch(a.K) <= i8s::CODES_MAX && aligned16(a.x16) && a.ldx16 % 8 == 0));
+}
+
+int i8_stream_linear(const I8LinearArgs& a, cudaStream_t st) {
+  i8s::Params p{};
+  p.xq = a.xq; p.ldx = a.ldx; p.xs = a.xs; p.x16 = reinterpret_cast<const uint16_t*>(a.x16); p.ldx16 = a.ldx16;
+  p.w = a.w; p.ws = a.ws; p.ws_dtype = a.ws_dtype; p.bias = a.bias; p.out = a.out; p.ldo = a.ldo; p.M = a.M; p.N = a.N; p.K = a.K;
+  p.early = tls().overlap_mode == 2;
+  if (a.x16) return a.out_bf16 ? i8s::pick<true, true>(p, st) : i8s::pick<true, false>(p, st);
+  return a.out_bf16 ? i8s::pick<false, true>(p, st) : i8s::pick<false, false>(p, st);
+}
+
+}  // namespace b2q

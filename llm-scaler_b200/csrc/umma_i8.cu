@@ -1,0 +1,474 @@
+// Int8 GEMM on tcgen05: out[m, n] = scale[m] wscale[n] sum_k codes[m, k] w[n, k] (+ bias[n]), dense from seventeen tokens on, and grouped by
+// expert for any number.
+//
+// Both operands go from TMA (128-byte-swizzled boxes of 128 k) straight into tcgen05.mma kind::i8; sums are exact 32-bit integers in
+// tensor memory, and scales, bias and rounding happen once per output.  The 128 tokens of a tile are the MMA's rows, up to 256 weight rows
+// its columns: a thread of the epilogue then has consecutive outputs of one token.  With the weights as columns a tile can have any
+// multiple of sixteen of them, so that the weight rows of a layer are dealt out evenly to the SMs, whatever their number.
+//
+// Three forms of one kernel, persistent but for the second:
+//  * one CTA per tile; two accumulators, so that a tile is drained and stored while the next one is multiplied;
+//  * SPLIT: a cluster of up to eight CTAs per tile, each with a share of k.  The partial sums meet in distributed shared memory; being
+//    integers, they add up to the same whatever the division.  For layers of few rows, whose tiles would leave SMs idle;
+//  * PAIR: two CTAs share a tile of 256 x 256 (cta_group::2), each loading 128 tokens and 128 weight rows.  A CTA then pulls 64 bytes
+//    per cycle of MMA through L2 where a tile of its own would take 96.
+// GATED (grouped, expert up projection): half of a tile's columns are gate rows, half the up rows of the same outputs, and the epilogue
+// stores silu(gate) * up.
+//
+// No multicast load; every mbarrier wait is bounded, as in the other tcgen05 kernels.
+#include "umma_gemm.cuh"
+#include "sm100.cuh"
+#include "i8.cuh"
+
+namespace b2q {
+
+using namespace sm100;
+
+namespace ui8 {
+enum { ST_EMPTY = 801, ST_FULL = 802, ST_ACCEMPTY = 803, ST_ACCFULL = 804 };
+constexpr int EPI = 8, THREADS = 64 + 32 * EPI;
+constexpr int MAX_STAGES = 16, TABLE = 256;
+constexpr int STG_BYTES = EPI * 2048;                      // 32 rows x 64 bytes for every epilogue warp
+constexpr int TAIL = STG_BYTES + 2 * 2 * TABLE * 4 + 512;  // staging, scale and bias tables of two tiles, barriers
+constexpr int SMEM_MAX = 232448;
+constexpr int OVERREAD = 16384;                            // an MMA reads 128 token rows, however few are loaded
+
+struct Params {
+  const float* xs; const void* ws; int ws_dtype; const void* bias;
+  uint16_t* out; int64_t ldo; int out_bf16, vec_out;
+  int M, N, nkb;
+  int h;                                                   // weight rows (MMA columns) per tile
+  int n_strips, m_tiles, m_group, total;                   // total: tiles of a dense launch
+  int tok_rows, tok_box;                                   // tokens per tile; rows of the token box
+  int stages, a_bytes, stage_bytes, split;
+  const int32_t* tiles; const int32_t* offsets;            // grouped
+  int early;
+  int* status;
+};
+
+struct Tile { int tok0, rows, n0, cols, w0, w1, e; };      // cols: valid outputs; w0: first weight row in memory, w1: of the up half
+
+template <bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(const Params& p, int id) {
+  Tile t;
+  if constexpr (GROUPED) {
+    const int ti = id / p.n_strips, st = id - ti * p.n_strips;
+    const int e = p.tiles[4 + 2 * ti], r0 = p.tiles[4 + 2 * ti + 1];
+    const int width = GATED ? p.h / 2 : p.h;
+    t.e = e;
+    t.tok0 = p.offsets[e] + r0;
+    t.rows = min(p.tok_rows, p.offsets[e + 1] - t.tok0);
+    t.n0 = st * width;
+    t.cols = min(width, p.N - t.n0);
+    t.w0 = (GATED ? 2 : 1) * e * p.N + t.n0;
+    t.w1 = t.w0 + p.N;
+  } else {
+    // m_group token tiles against all strips before the next group: what runs at one time shares both operands in L2
+    const int per = p.m_group * p.n_strips, gi = id / per, left = id - gi * per, m0 = gi * p.m_group;
+    const int gm = min(p.m_group, p.m_tiles - m0), st = left / gm, mt = m0 + left - st * gm;
+    t.e = 0;
+    t.tok0 = mt * p.tok_rows;
+    t.rows = min(p.tok_rows, p.M - t.tok0);
+    t.n0 = st * p.h;
+    t.cols = min(p.h, p.N - t.n0);
+    t.w0 = t.n0;
+    t.w1 = 0;
+  }
+  return t;
+}
+
+__device__ __forceinline__ uint4 ld_cluster(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 lds128v(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t pack_out(float a, float b, int bf16) { return bf16 ? pack2<true>(a, b) : pack2<false>(a, b); }
+}  // namespace ui8
+
+template <bool PAIR, bool SPLIT, bool GROUPED, bool GATED>
+__global__ void __launch_bounds__(ui8::THREADS, 1)
+umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const ui8::Params p) {
+  using namespace ui8;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  // [stages of (token box, weight box)] [room for the MMA's reads beyond a low token box] [staging] [tables] [barriers]
+  const uint32_t stg_off = p.stages * p.stage_bytes + (p.tok_box < 128 ? OVERREAD : 0);
+  const uint32_t tab_off = stg_off + STG_BYTES, bar = base + tab_off + 4 * TABLE * 4;
+  float* tab = reinterpret_cast<float*>(gen + tab_off);    // [2 tiles][scales, biases][TABLE]
+  const uint32_t full = bar, empty = bar + 8 * MAX_STAGES, acc_full = bar + 16 * MAX_STAGES, acc_empty = acc_full + 16;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + (acc_empty + 16 - base));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + (acc_empty + 24 - base));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR || SPLIT ? cluster_ctarank() : 0;
+  const int group = PAIR ? 2 : (SPLIT ? p.split : 1);      // CTAs that work on one tile
+  const int first = (int)blockIdx.x / group, step = (int)gridDim.x / group;
+  const int kb0 = SPLIT ? (int)rank * p.nkb / p.split : 0, kb1 = SPLIT ? ((int)rank + 1) * p.nkb / p.split : p.nkb;
+
+  grid_dep_release();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, PAIR ? 2 * EPI : EPI); }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) { tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512); tmem_relinquish_pair(); }
+    else { tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512); tmem_relinquish(); }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();                  // both CTAs' barriers exist before anything is signalled across
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // the tile list comes from the kernels in front; a dense launch knows its tiles
+  if constexpr (GROUPED) grid_dep_wait();
+  const int total = GROUPED ? p.tiles[0] * p.n_strips : p.total;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&tm_x);
+      tma_prefetch_desc(&tm_w);
+      const int wbox = PAIR ? 128 : (GATED ? p.h / 2 : p.h);
+      const uint32_t bytes = (uint32_t)p.stage_bytes * (PAIR ? 2u : 1u);
+      int s = 0, issued = 0;
+      uint32_t par = 1u;
+      bool ok = true;
+      auto put_w = [&](int st, int kb, const Tile& t) {
+        const uint32_t dst = base + st * p.stage_bytes + p.a_bytes;
+        if constexpr (PAIR) {
+          tma_load_2d_pair(dst, &tm_w, kb * 128, t.w0 + (int)rank * 128, map_to_cta(full + 8 * st, 0));
+        } else {
+          tma_load_2d(dst, &tm_w, kb * 128, t.w0, full + 8 * st);
+          if constexpr (GATED) tma_load_2d(dst + wbox * 128, &tm_w, kb * 128, t.w1, full + 8 * st);
+        }
+      };
+      auto put_x = [&](int st, int kb, const Tile& t) {
+        const uint32_t dst = base + st * p.stage_bytes;
+        if constexpr (PAIR) tma_load_2d_pair(dst, &tm_x, kb * 128, t.tok0 + (int)rank * 128, map_to_cta(full + 8 * st, 0));
+        else tma_load_2d(dst, &tm_x, kb * 128, t.tok0, full + 8 * st);
+      };
+      // Weights do not depend on the kernels in front: the first stages' are on their way before the wait for the tokens.
+      int ahead = 0;
+      if constexpr (!GROUPED) {
+        if (p.early && first < total) {
+          const Tile t = tile_at<GROUPED, GATED>(p, first);
+          ahead = min(p.stages, kb1 - kb0);
+          for (int i = 0; i < ahead; ++i) {
+            if (rank == 0 || !PAIR) mbar_expect_tx(full + 8 * i, bytes);
+            put_w(i, kb0 + i, t);
+          }
+        }
+        grid_dep_wait();
+      }
+      for (int id = first; ok && id < total; id += step) {
+        const Tile t = tile_at<GROUPED, GATED>(p, id);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_EMPTY);
+          if (!ok) break;
+          if (issued >= ahead) {
+            if (rank == 0 || !PAIR) mbar_expect_tx(full + 8 * s, bytes);
+            put_w(s, kb, t);
+          }
+          put_x(s, kb, t);
+          ++issued;
+          if (++s == p.stages) { s = 0; par ^= 1u; }
+        }
+      }
+      // gave up: the copies issued land before the CTA leaves (a pair's are counted on the leader's barriers, and the peer stays with it)
+      if (!ok && (rank == 0 || !PAIR)) drain_issued(full, p.stages, issued);
+    }
+  } else if (warp == 1) {
+    if ((!PAIR || rank == 0) && elect_one()) {
+      const uint32_t idesc = instr_desc_i8(1u, 1u, PAIR ? 256u : 128u, (uint32_t)p.h);
+      int s = 0, it = 0;
+      uint32_t par = 0u;
+      bool ok = true;
+      for (int id = first; ok && id < total; id += step, ++it) {
+        const int b = it & 1;
+        if (it >= 2) ok = mbar_wait(acc_empty + 8 * b, ((it >> 1) - 1) & 1, abort_flag, p.status, ST_ACCEMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + b * 256;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = mbar_wait(full + 8 * s, par, abort_flag, p.status, ST_FULL);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t da = smem_desc_sw128(base + s * p.stage_bytes);
+          const uint64_t db = smem_desc_sw128(base + s * p.stage_bytes + p.a_bytes);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (PAIR) mma_i8_pair(d, da + 2 * i, db + 2 * i, idesc, kb > kb0 || i > 0);
+            else mma_i8(d, da + 2 * i, db + 2 * i, idesc, kb > kb0 || i > 0);
+          }
+          if constexpr (PAIR) tc_commit_pair(empty + 8 * s, 3); else tc_commit(empty + 8 * s);
+          if (++s == p.stages) { s = 0; par ^= 1u; }
+        }
+        if (!ok) break;
+        if constexpr (PAIR) tc_commit_pair(acc_full + 8 * b, 3); else tc_commit(acc_full + 8 * b);
+      }
+    }
+  } else {
+    // ---- epilogue: lane quadrant = warp & 3 (tokens), column chunks of 32 shared by the two warps of a quadrant ----
+    const int quad = warp & 3, half = (warp - 2) >> 2, etid = threadIdx.x - 64;
+    const uint32_t stg = base + stg_off + (warp - 2) * 2048;
+    if constexpr (!GROUPED) grid_dep_wait();
+    int it = 0;
+    for (int id = first; id < total; id += step, ++it) {
+      const Tile t = tile_at<GROUPED, GATED>(p, id);
+      const int b = it & 1;
+      float* sc = tab + b * 2 * TABLE;
+      float* bi = sc + TABLE;
+      {
+        // scales of the tile's columns: thread i has column i (gated: gate columns, then up columns)
+        const int width = GATED ? p.h / 2 : p.h, col = GATED && etid >= width ? etid - width : etid;
+        float v = 0.f, w = 0.f;
+        if (etid < p.h && col < t.cols) {
+          const int64_t at = GATED ? (int64_t)(etid >= width ? t.w1 : t.w0) + col : (int64_t)t.w0 + col;
+          v = load_scalar(p.ws, at, p.ws_dtype);
+          if (p.bias) w = load_scalar(p.bias, t.n0 + col, p.out_bf16 ? B2Q_BF16 : B2Q_F16);
+        }
+        sc[etid] = v;
+        bi[etid] = w;
+      }
+      const int trow = (PAIR ? (int)rank * 128 : 0) + quad * 32 + lane;      // this lane's token within the tile
+      const float xs = trow < t.rows ? ld_f32(p.xs + t.tok0 + trow) : 0.f;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI) : "memory");
+      if (!mbar_wait_warp(acc_full + 8 * b, (it >> 1) & 1, abort_flag, p.status, ST_ACCFULL)) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + b * 256;
+      const int row0 = (PAIR ? (int)rank * 128 : 0) + quad * 32;
+      if constexpr (SPLIT) {
+        // partial sums into this CTA's shared memory, whose stages nobody uses any more
+        const int pitch = p.h + 4;
+        for (int c = half * 32; row0 < t.rows && c < t.cols; c += 64) {
+          uint32_t r[32];
+          tmem_ld32(acc + c, r);
+          tmem_ld_wait();
+          const uint32_t at = base + (uint32_t)((quad * 32 + lane) * pitch + c) * 4;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            if (c + i < p.h) sts128(at + i * 4, r[i], r[i + 1], r[i + 2], r[i + 3]);
+        }
+      } else {
+        uint16_t* out = p.out + (int64_t)(t.tok0 + row0) * p.ldo + t.n0;
+        for (int c = half * 32; row0 < t.rows && c < t.cols; c += 64) {
+          uint32_t r[32], o[16];
+          tmem_ld32(acc + c, r);
+          if constexpr (GATED) {
+            uint32_t u[32];
+            tmem_ld32(acc + p.h / 2 + c, u);
+            tmem_ld_wait();
+            const float* us = sc + p.h / 2 + c;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float g0 = i8_scaled((int)r[2 * i], xs, sc[c + 2 * i]), g1 = i8_scaled((int)r[2 * i + 1], xs, sc[c + 2 * i + 1]);
+              const float u0 = i8_scaled((int)u[2 * i], xs, us[2 * i]), u1 = i8_scaled((int)u[2 * i + 1], xs, us[2 * i + 1]);
+              o[i] = pack_out(silu_mul_f(g0, u0), silu_mul_f(g1, u1), p.out_bf16);
+            }
+          } else {
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float v0 = i8_output((int)r[2 * i], xs, sc[c + 2 * i], bi[c + 2 * i]);
+              const float v1 = i8_output((int)r[2 * i + 1], xs, sc[c + 2 * i + 1], bi[c + 2 * i + 1]);
+              o[i] = pack_out(v0, v1, p.out_bf16);
+            }
+          }
+          // through shared memory, so that four lanes store 64 bytes of a token; 16-byte pieces are permuted against bank conflicts
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) sts128(stg + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          __syncwarp();
+          if (p.vec_out && c + 32 <= t.cols) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int rr = i * 8 + (lane >> 2), q = lane & 3;
+              const uint4 v = lds128v(stg + rr * 64 + ((q ^ ((rr >> 1) & 3)) << 4));
+              if (row0 + rr < t.rows) *reinterpret_cast<uint4*>(out + rr * p.ldo + c + q * 8) = v;
+            }
+          } else {
+            for (int rr = 0; rr < 32 && row0 + rr < t.rows; ++rr) {
+              const int q = lane >> 3;
+              uint16_t v;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(stg + rr * 64 + ((q ^ ((rr >> 1) & 3)) << 4) + (lane & 7) * 2) : "memory");
+              if (c + lane < t.cols) out[rr * p.ldo + c + lane] = v;
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(acc_empty + 8 * b, 0));
+          else mbar_arrive(acc_empty + 8 * b);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (SPLIT) {
+    cluster_sync_all();                                    // every CTA's partial sums are there
+    if (first < total && !*abort_flag) {
+      const Tile t = tile_at<GROUPED, GATED>(p, first);
+      const int pitch = p.h + 4, eights = (t.cols + 7) / 8, items = t.rows * eights;
+      for (int i = (int)rank * THREADS + threadIdx.x; i < items; i += p.split * THREADS) {
+        const int row = i / eights, c = (i - row * eights) * 8;
+        int sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const uint32_t at = base + (uint32_t)(row * pitch + c) * 4;
+        for (int j = 0; j < p.split; ++j) {
+          const uint32_t from = map_to_cta(at, j);
+          const uint4 a = ld_cluster(from), d = ld_cluster(from + 16);
+          sum[0] += (int)a.x; sum[1] += (int)a.y; sum[2] += (int)a.z; sum[3] += (int)a.w;
+          sum[4] += (int)d.x; sum[5] += (int)d.y; sum[6] += (int)d.z; sum[7] += (int)d.w;
+        }
+        const float xs = ld_f32(p.xs + t.tok0 + row);
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = i8_output(sum[k], xs, tab[c + k], tab[TABLE + c + k]);
+        uint16_t* out = p.out + (int64_t)(t.tok0 + row) * p.ldo + t.n0 + c;
+        const uint4 o = make_uint4(pack_out(v[0], v[1], p.out_bf16), pack_out(v[2], v[3], p.out_bf16), pack_out(v[4], v[5], p.out_bf16),
+                                   pack_out(v[6], v[7], p.out_bf16));
+        if (p.vec_out && c + 8 <= t.cols) {
+          *reinterpret_cast<uint4*>(out) = o;
+        } else {
+          const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (c + k < t.cols) out[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+        }
+      }
+    }
+    cluster_sync_all();                                    // nobody leaves while its sums may be read
+  }
+  if constexpr (PAIR) cluster_sync_all();                  // nor while the partner may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, 512); else tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+namespace ui8 {
+static int sm_count() {
+  static thread_local int sms[16] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 16) return 148;
+  if (!sms[dev]) {
+    cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    if (sms[dev] <= 0) sms[dev] = 148;
+  }
+  return sms[dev];
+}
+static int round_up(int v, int a) { return (v + a - 1) / a * a; }
+
+template <bool PAIR, bool SPLIT, bool GROUPED, bool GATED>
+static int launch(const CUtensorMap& tx, const CUtensorMap& tw, Params& p, int grid, cudaStream_t st) {
+  p.stage_bytes = p.a_bytes + (PAIR ? 128 : p.h) * 128;
+  const int over = p.tok_box < 128 ? OVERREAD : 0, room = SMEM_MAX - 1024 - TAIL - over;
+  p.stages = room / p.stage_bytes;
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  int bytes = p.stages * p.stage_bytes;
+  if (SPLIT && bytes < p.tok_box * (p.h + 4) * 4) return B2Q_ERR_LIMIT;      // partial sums use the stages' room
+  const int smem = 1024 + bytes + over + TAIL;
+  auto kern = umma_i8_kernel<PAIR, SPLIT, GROUPED, GATED>;
+  static thread_local bool configured[16] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 16 || !configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX) != cudaSuccess) return B2Q_ERR_CUDA;
+    if (dev < 16) configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (PAIR || SPLIT) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = PAIR ? 2 : p.split; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (tls().overlap_mode > 0) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at; cfg.numAttrs = n;
+  if (cudaLaunchKernelEx(&cfg, kern, tx, tw, p) != cudaSuccess) return B2Q_ERR_CUDA;
+  note_launch(PAIR ? "umma_i8_pair" : (SPLIT ? "umma_i8_split" : "umma_i8"));
+  return launch_status();
+}
+
+// How a dense launch is divided: weight rows per tile and CTAs per tile, by what a tile's stages cost in cycles of an SM.
+struct Plan { int h, split; };
+static Plan plan(int M, int N, int nkb, int tok_box) {
+  const int sms = sm_count(), m_tiles = (M + 127) / 128;
+  Plan best{256, 1};
+  double best_cost = 1e30;
+  for (int split = 1; split <= 8 && split <= nkb; ++split) {
+    const int slots = sms / split;
+    for (int waves = 1; waves <= 4; ++waves) {
+      const int strips_max = slots * waves / m_tiles;
+      if (strips_max == 0) continue;
+      int h = round_up((N + strips_max - 1) / strips_max, 16);
+      if (h > 256) continue;
+      if (split > 1 && waves > 1) continue;
+      const int strips = (N + h - 1) / h, rounds = (strips * m_tiles + slots - 1) / slots;
+      const double stage = 60 + fmax(2.0 * h, fmax(h * 128 / 30.0, (h + tok_box) * 128 / 55.0));
+      const double cost = rounds * ((nkb + split - 1) / split * stage + 1500) + (split > 1 ? 2500 : 0);
+      if (cost < best_cost) { best_cost = cost; best = Plan{h, split}; }
+    }
+  }
+  return best;
+}
+}  // namespace ui8
+
+int umma_i8_linear(const I8LinearArgs& a, cudaStream_t st) {
+  using namespace ui8;
+  if (!tensor_map_encoder()) return B2Q_ERR_CUDA;
+  Params p{};
+  p.xs = a.xs; p.ws = a.ws; p.ws_dtype = a.ws_dtype; p.bias = a.bias;
+  p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.ldo; p.out_bf16 = a.out_bf16; p.vec_out = aligned16(a.out) && a.ldo % 8 == 0;
+  p.M = a.M; p.N = a.N; p.nkb = (a.K + 127) / 128;
+  p.early = tls().overlap_mode == 2;
+  p.status = umma_status_ptr();
+  if (!p.status) return B2Q_ERR_CUDA;
+  const int sms = sm_count();
+  const int pair_tiles = (a.M + 255) / 256 * ((a.N + 255) / 256);
+  const bool pair = a.M > 256 && pair_tiles >= sms / 4;
+  CUtensorMap tx, tw;
+  if (pair) {
+    p.h = 256; p.tok_rows = 256; p.tok_box = 128; p.split = 1;
+  } else {
+    p.tok_box = a.M <= 32 ? 32 : (a.M <= 64 ? 64 : 128);
+    p.tok_rows = 128;
+    const Plan pl = plan(a.M, a.N, p.nkb, p.tok_box);
+    p.h = pl.h; p.split = pl.split;
+  }
+  p.a_bytes = p.tok_box * 128;
+  p.n_strips = (a.N + p.h - 1) / p.h;
+  p.m_tiles = (a.M + p.tok_rows - 1) / p.tok_rows;
+  p.m_group = p.m_tiles < 16 ? p.m_tiles : 16;
+  if ((int64_t)p.n_strips * p.m_tiles > INT32_MAX / 8) return B2Q_ERR_LIMIT;
+  p.total = p.n_strips * p.m_tiles;
+  int rc = make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.xq, a.M, a.K, (uint64_t)a.ldx, p.tok_box, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.N, a.K, (uint64_t)a.K, pair ? 128 : p.h, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  if (pair) return launch<true, false, false, false>(tx, tw, p, 2 * (p.total < sms / 2 ? p.total : sms / 2), st);
+  if (p.split > 1) return launch<false, true, false, false>(tx, tw, p, p.total * p.split, st);
+  return launch<false, false, false, false>(tx, tw, p, p.total < sms ? p.total : sms, st);
+}
+
+}  // namespace b2q

@@ -21,6 +21,9 @@ from .ops import (  # noqa: F401
     moe_router_forward_int4, moe_router_topk_int4, moe_forward_full_int4, moe_shared_expert_forward_int4_nmajor,
     moe_forward_cutlass_nmajor_int4_full, esimd_scaled_resadd_norm_gemv_fp8_pert, esimd_norm_gemv_norm_fp16,
 )
+from .int8 import (  # noqa: F401
+    quantize_int8, silu_mul_quantize_int8, resadd_rmsnorm_quantize_int8, linear_int8, linear_int8_dynamic,
+)
 
 launch_count = _lib.launch_count
 last_kernel = _lib.last_kernel

@@ -75,6 +75,12 @@ _SIGS = {
     "b2q_moe_forward_workspace_bytes": (sz, [i64, i32, i32, i64, i64, i64]),
     "b2q_moe_forward_int4": (i32, [C.POINTER(MoeInt4), vp, sz, vp]),
     "b2q_moe_forward_fp8": (i32, [C.POINTER(MoeFp8), vp, sz, vp]),
+    "b2q_quantize_int8": (i32, [vp, i32, i64, vp, vp, i64, i64, vp]),
+    "b2q_silu_mul_quantize_int8": (i32, [vp, i32, i64, vp, vp, i64, i64, vp]),
+    "b2q_resadd_rmsnorm_quantize_int8": (i32, [vp, vp, vp, vp, i32, C.c_float, vp, vp, i64, i64, vp]),
+    "b2q_linear_int8": (i32, [vp, i64, vp, vp, vp, i32, vp, vp, i32, i64, i64, i64, i64, vp]),
+    "b2q_linear_int8_dynamic_workspace_bytes": (sz, [i64, i64, i64]),
+    "b2q_linear_int8_dynamic": (i32, [vp, i32, i64, vp, vp, i32, vp, vp, i64, i64, i64, i64, vp, sz, vp]),
     "b2q_comm_create": (i32, [i32, i32, i64, i64, vp, vp]),
     "b2q_comm_create_mode": (i32, [i32, i32, i64, i64, i32, vp, vp]),
     "b2q_comm_connect": (i32, [vp, vp]),

@@ -1,0 +1,60 @@
+"""8-bit integer operators: int8 weights with one scale per output channel, activations quantised to int8 with one scale per token.
+
+The reference has no such format, so these have names of their own and the torch namespace `b2q_int8` (csrc/torch_int8.cpp ->
+libb2q_int8.so, over the C ABI of include/b2q.h).  All of them run on torch's current stream and may be captured in a CUDA graph.
+"""
+import os
+
+import torch
+
+from . import _lib as L
+
+_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libb2q_int8.so")
+if not os.path.exists(_PATH):
+    raise ImportError("b2q: %s is missing; build it with `python llm-scaler_b200/build.py`" % _PATH)
+torch.ops.load_library(_PATH)
+_ops = torch.ops.b2q_int8
+
+if os.environ.get("B2Q_CHECK_STATUS") == "1":
+    # debugging, as for the other ops: every call synchronises and raises if a bounded device-side wait has expired
+    class _Checked:
+        def __getattr__(self, name):
+            op = getattr(torch.ops.b2q_int8, name)
+
+            def run(*args):
+                out = op(*args)
+                code = L.device_status()
+                if code:
+                    raise RuntimeError("b2q: b2q_int8::%s: a bounded device-side wait expired (code %d); results are not valid" % (name, code))
+                return out
+            return run
+
+    _ops = _Checked()
+
+
+def quantize_int8(x):
+    """Rows of x (bf16, fp16 or fp32 [M, K], rows contiguous) -> codes int8 [M, K], scale fp32 [M].
+
+    scale = max(amax, 1e-12) / 127, codes = rint(127 x / amax), halves to even, decided exactly.  A row with an infinity or a NaN gets
+    the scale NaN and zero codes.  Tokens, or at load time the rows of a weight."""
+    return _ops.quantize(x)
+
+
+def silu_mul_quantize_int8(gate_up):
+    """quantize_int8 of silu(gate) * up, gate_up bf16 / fp16 [M, 2K]; the product is not rounded to 16 bits in between."""
+    return _ops.silu_mul_quantize(gate_up)
+
+
+def resadd_rmsnorm_quantize_int8(hidden, residual, norm_weight, eps, residual_out=None):
+    """v = hidden + residual; residual_out (residual itself by default) <- v; returns quantize_int8 of rmsnorm(v) * norm_weight."""
+    return _ops.resadd_rmsnorm_quantize(hidden, residual, norm_weight, eps, residual_out)
+
+
+def linear_int8(codes, scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
+    """out[m, n] = scale[m] * weight_scale[n] * (codes[m] . weight[n]) (+ bias[n]); codes int8 [M, K], weight int8 [N, K], K % 16 == 0."""
+    return _ops.linear(codes, scale, weight, weight_scale, bias, out_dtype)
+
+
+def linear_int8_dynamic(x, weight, weight_scale, bias=None):
+    """linear_int8(*quantize_int8(x), ...) in x's type; for a few tokens one launch."""
+    return _ops.linear_dynamic(x, weight, weight_scale, bias)
