@@ -359,6 +359,26 @@ B2Q_API int b2q_linear_int8_dynamic(const void* x, int act_dtype, int64_t ldx, c
                             const void* bias, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/* A whole expert layer, from router logits to the weighted sum, on int8 experts:
+ *   ids, w = the top_k largest logits of a token, the lowest index first among equals; w their softmax over all E, divided by its sum
+ *   over the chosen if renormalize;  (q, s) = codes of x[t];  g, u = s s13[e, j] q.w13[e, j] and the same of row I + j;  h = silu(g) u;
+ *   (d, r) = codes of h;  out[t] = sum over the chosen of w r s2[e, n] d.w2[e, n], in fp32, one rounding.
+ * A token whose logits hold a NaN, or none that is finite at the top, goes to no expert: its row of out is zero.
+ * x [T, H], logits [T, E], out [T, H]; w13 int8 [E, 2I, H] (gate rows, then up), s13 [E, 2I], w2 int8 [E, H, I], s2 [E, H], all contiguous.
+ * H % 16 == 0, I % 16 == 0, E <= 1024, top_k <= 32.  h stays fp32 until its codes are made.  Up to sixteen tokens (while their codes
+ * fit shared memory) take two kernels; more are sorted by expert and go through grouped GEMMs, and each expert's output is rounded to
+ * act_dtype before the weighted sum.  workspace: 256-byte aligned, b2q_moe_forward_int8_workspace_bytes() bytes, the call's own until its last kernel has
+ * completed; what it holds before does not matter.                                                                       */
+typedef struct b2q_moe_int8 {
+  const void *x, *logits;
+  const int8_t* w13; const void* s13; const int8_t* w2; const void* s2;
+  void* out;
+  int64_t T, E, top_k, H, I;
+  int act_dtype, logits_dtype, s13_dtype, s2_dtype, renormalize;
+} b2q_moe_int8;
+B2Q_API size_t b2q_moe_forward_int8_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I);
+B2Q_API int b2q_moe_forward_int8(const b2q_moe_int8* args, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- sum of row-parallel partial results over the GPUs of one box ----------------------------
  * The exchange step behind a row-parallel linear (o_proj, down) of a tensor-parallel decoder layer; the
  * reference calls the serving framework's all-reduce there (vllm/patches/vllm_for_multi_arc.patch:10185,

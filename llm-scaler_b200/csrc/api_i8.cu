@@ -1,6 +1,17 @@
 // C ABI of the 8-bit integer operators: argument validation and kernel selection, as in api.cu.
 #include "i8.cuh"
 
+namespace b2q {
+// implemented in moe_aux.cu
+int moe_topk(const void*, int, int64_t, int, int, int, void*, int, int32_t*, cudaStream_t);
+size_t moe_route_workspace_bytes(int64_t, int);
+int moe_route(const int32_t*, int64_t, int, int32_t*, int32_t*, int32_t*, int32_t*, void*, cudaStream_t);
+int moe_build_tiles(const int32_t*, int, int, int32_t*, cudaStream_t);
+bool moe_route_fused_fits(int64_t, int, int);
+int moe_route_fused(const void*, int, int64_t, int, int, void*, int, int32_t*, int32_t*, int32_t*, int, int32_t*, int, cudaStream_t);
+int moe_combine(const void*, const void*, int, const int32_t*, void*, int, int64_t, int, int64_t, int, cudaStream_t);
+}  // namespace b2q
+
 using namespace b2q;
 
 namespace {
@@ -17,6 +28,8 @@ int linear_check(const I8LinearArgs& a, int64_t M, int64_t N, int64_t K) {
   if (!aligned16(a.w) || !aligned_to(a.out, 2) || !aligned_to(a.bias, 2) || !aligned_to(a.ws, dtype_bytes(a.ws_dtype))) return B2Q_ERR_ALIGN;
   return B2Q_OK;
 }
+// set_force_kernel(2): tcgen05 for any number of tokens
+bool use_stream(const I8LinearArgs& a) { return a.M <= I8_STREAM_MAX_TOK && tls().force_kernel != 2; }
 }  // namespace
 
 extern "C" {
@@ -63,7 +76,7 @@ int b2q_linear_int8(const int8_t* q, int64_t ldq, const float* scale, const int8
   if (ldq < K) return B2Q_ERR_SHAPE;
   if (!aligned16(q) || ldq % 16 != 0 || !aligned_to(scale, 4)) return B2Q_ERR_ALIGN;
   if (M == 0 || N == 0) return B2Q_OK;
-  return M <= I8_STREAM_MAX_TOK ? i8_stream_linear(a, (cudaStream_t)stream) : umma_i8_linear(a, (cudaStream_t)stream);
+  return use_stream(a) ? i8_stream_linear(a, (cudaStream_t)stream) : umma_i8_linear(a, (cudaStream_t)stream);
 }
 
 size_t b2q_linear_int8_dynamic_workspace_bytes(int64_t M, int64_t N, int64_t K) {
@@ -93,7 +106,92 @@ int b2q_linear_int8_dynamic(const void* x, int act_dtype, int64_t ldx, const int
   rc = quantize_i8(x, act_dtype, ldx, q, s, M, (int)K, (cudaStream_t)stream);
   if (rc) return rc;
   a.x16 = nullptr; a.xq = q; a.ldx = K; a.xs = s;
-  return M <= I8_STREAM_MAX_TOK ? i8_stream_linear(a, (cudaStream_t)stream) : umma_i8_linear(a, (cudaStream_t)stream);
+  return use_stream(a) ? i8_stream_linear(a, (cudaStream_t)stream) : umma_i8_linear(a, (cudaStream_t)stream);
+}
+
+}  // extern "C"
+
+namespace {
+// Workspace of an expert layer in its grouped form, part by part.
+struct MoeParts {
+  uint8_t *weights, *ids, *offsets, *tokens, *perm, *route, *tiles, *xq, *xs, *h, *hq, *hs, *y;
+  size_t total;
+};
+MoeParts moe_parts(void* ws, int64_t T, int E, int k, int64_t H, int64_t I) {
+  MoeParts p{};
+  uint8_t* base = reinterpret_cast<uint8_t*>(ws);
+  size_t at = 0;
+  auto take = [&](size_t bytes) { uint8_t* q = base + at; at += align_up(bytes, 256); return q; };
+  const size_t rows = (size_t)T * k;
+  p.weights = take(rows * 4); p.ids = take(rows * 4); p.offsets = take((size_t)(E + 2) * 4); p.tokens = take(rows * 4); p.perm = take(rows * 4);
+  p.route = take(moe_route_workspace_bytes((int64_t)rows, E));
+  p.tiles = take(16 + 8 * (rows / 32 + 1 + E));
+  p.xq = take(rows * H); p.xs = take(rows * 4); p.h = take(rows * I * 4); p.hq = take(rows * I); p.hs = take(rows * 4); p.y = take(rows * H * 2);
+  p.total = at;
+  return p;
+}
+}  // namespace
+
+extern "C" {
+
+size_t b2q_moe_forward_int8_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I) {
+  if (T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || top_k > 32 || H <= 0 || I <= 0 || T > INT32_MAX / 32) return 0;
+  if (moe_i8_few_supported(T, E, top_k, H, I)) return moe_i8_few_bytes(T, top_k, I);
+  return moe_parts(nullptr, T, (int)E, (int)top_k, H, I).total;
+}
+
+int b2q_moe_forward_int8(const b2q_moe_int8* m, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!m) return B2Q_ERR_NULL;
+  const b2q_moe_int8& a = *m;
+  if (!a.x || !a.logits || !a.w13 || !a.s13 || !a.w2 || !a.s2 || !a.out) return B2Q_ERR_NULL;
+  if (!is16(a.act_dtype) || !known(a.logits_dtype) || !known(a.s13_dtype) || !known(a.s2_dtype)) return B2Q_ERR_DTYPE;
+  if (a.T < 0 || a.E <= 0 || a.top_k <= 0 || a.top_k > a.E || a.H <= 0 || a.I <= 0 || a.H % 16 != 0 || a.I % 16 != 0) return B2Q_ERR_SHAPE;
+  if (a.E > 1024 || a.top_k > 32 || a.H > MAX_K || a.I > MAX_K || a.T > INT32_MAX / 32 || 2 * a.E * a.I > INT32_MAX || a.E * a.H > INT32_MAX) return B2Q_ERR_LIMIT;
+  if (!aligned16(a.x) || !aligned16(a.w13) || !aligned16(a.w2) || !aligned16(a.out) || !aligned_to(a.logits, dtype_bytes(a.logits_dtype)) ||
+      !aligned_to(a.s13, dtype_bytes(a.s13_dtype)) || !aligned_to(a.s2, dtype_bytes(a.s2_dtype)))
+    return B2Q_ERR_ALIGN;
+  if (a.T == 0) return B2Q_OK;
+  if (!workspace) return B2Q_ERR_NULL;
+  if (!aligned_to(workspace, 256)) return B2Q_ERR_ALIGN;
+  if (workspace_bytes < b2q_moe_forward_int8_workspace_bytes(a.T, a.E, a.top_k, a.H, a.I)) return B2Q_ERR_WORKSPACE;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool bf16 = a.act_dtype == B2Q_BF16;
+  const int E = (int)a.E, k = (int)a.top_k, H = (int)a.H, I = (int)a.I;
+  if (moe_i8_few_supported(a.T, E, k, H, I)) {
+    I8FewArgs f{};
+    f.x = a.x; f.bf16 = bf16; f.logits = a.logits; f.logits_dtype = a.logits_dtype;
+    f.w13 = a.w13; f.s13 = a.s13; f.s13_dtype = a.s13_dtype; f.w2 = a.w2; f.s2 = a.s2; f.s2_dtype = a.s2_dtype;
+    f.out = a.out; f.T = (int)a.T; f.E = E; f.k = k; f.H = H; f.I = I; f.renorm = a.renormalize != 0; f.scratch = workspace;
+    return moe_i8_few(f, st);
+  }
+  const MoeParts p = moe_parts(workspace, a.T, E, k, H, I);
+  const int64_t rows = a.T * k;
+  int32_t *off = reinterpret_cast<int32_t*>(p.offsets), *tok = reinterpret_cast<int32_t*>(p.tokens), *perm = reinterpret_cast<int32_t*>(p.perm);
+  int32_t* tiles = reinterpret_cast<int32_t*>(p.tiles);
+  const int tile = i8_grouped_tile(rows, E);
+  int rc;
+  if (a.renormalize && moe_route_fused_fits(a.T, E, k)) {
+    rc = moe_route_fused(a.logits, a.logits_dtype, a.T, E, k, p.weights, B2Q_F32, off, tok, perm, tile, tiles, 0, st);
+  } else {
+    int32_t* ids = reinterpret_cast<int32_t*>(p.ids);
+    rc = moe_topk(a.logits, a.logits_dtype, a.T, E, k, a.renormalize != 0, p.weights, B2Q_F32, ids, st);
+    if (!rc) rc = moe_route(ids, rows, E, off, tok, perm, nullptr, p.route, st);
+    if (!rc) rc = moe_build_tiles(off, E, tile, tiles, st);
+  }
+  if (rc) return rc;
+  I8GroupedArgs g{};
+  g.xq = reinterpret_cast<int8_t*>(p.xq); g.xs = reinterpret_cast<float*>(p.xs); g.w = a.w13; g.ws = a.s13; g.ws_dtype = a.s13_dtype;
+  g.offsets = off; g.tiles = tiles; g.tile = tile; g.tile_cap = (int)((rows + tile - 1) / tile + E); g.E = E;
+  g.out = p.h; g.out_bf16 = bf16; g.rows = (int)rows; g.N = I; g.K = H; g.gated = true;
+  I8GroupedArgs d = g;
+  d.xq = reinterpret_cast<int8_t*>(p.hq); d.xs = reinterpret_cast<float*>(p.hs); d.w = a.w2; d.ws = a.s2; d.ws_dtype = a.s2_dtype;
+  d.out = p.y; d.N = H; d.K = I; d.gated = false;
+  rc = quantize_i8_gather(a.x, a.act_dtype, H, tok, k, off + E, reinterpret_cast<int8_t*>(p.xq), reinterpret_cast<float*>(p.xs), rows, H, st);
+  if (!rc) rc = umma_i8_grouped(g, st);
+  if (!rc) rc = quantize_i8_gather(p.h, B2Q_F32, I, nullptr, 1, off + E, reinterpret_cast<int8_t*>(p.hq), reinterpret_cast<float*>(p.hs), rows, I, st);
+  if (!rc) rc = umma_i8_grouped(d, st);
+  if (!rc) rc = moe_combine(p.y, p.weights, B2Q_F32, perm, a.out, a.act_dtype, a.T, k, H, 0, st);
+  return rc;
 }
 
 }  // extern "C"

@@ -23,34 +23,46 @@ int i8_stream_linear(const I8LinearArgs& a, cudaStream_t st);
 int umma_i8_linear(const I8LinearArgs& a, cudaStream_t st);
 
 // Grouped form: rows [offsets[e], offsets[e + 1]) of xq meet expert e's [N, K] of w.  gated: N is I and w holds 2 I rows per expert, gate then
-// up; the output is silu(gate) * up in fp32.  Otherwise y in fp32.
+// up; the output is silu(gate) * up.
 struct I8GroupedArgs {
   const int8_t* xq; const float* xs; const int8_t* w; const void* ws; int ws_dtype;
-  const int32_t* offsets; const int32_t* tiles; int tile_cap; int E;
-  float* out; int rows, N, K; bool gated;
+  const int32_t* offsets; const int32_t* tiles; int tile, tile_cap, E;      // tile list of this height (i8_grouped_tile)
+  void* out; bool out_bf16; int rows, N, K; bool gated;    // gated: out is fp32
 };
-constexpr int I8_GROUPED_TILE = 128;
+int i8_grouped_tile(int64_t rows, int E);
 int umma_i8_grouped(const I8GroupedArgs& a, cudaStream_t st);
+
+// A whole expert layer of up to sixteen tokens in two kernels (moe_i8.cu).
+struct I8FewArgs {
+  const void* x; bool bf16; const void* logits; int logits_dtype;
+  const int8_t* w13; const void* s13; int s13_dtype; const int8_t* w2; const void* s2; int s2_dtype;
+  void* out; int T, E, k, H, I; bool renorm;
+  void* scratch;                                           // moe_i8_few_bytes(), 256-byte aligned
+};
+bool moe_i8_few_supported(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I);
+size_t moe_i8_few_bytes(int64_t T, int64_t k, int64_t I);
+int moe_i8_few(const I8FewArgs& a, cudaStream_t st);
 
 // q [M, K] codes, s [M] scales of rows of x; x_dtype B2Q_BF16 / F16 / F32.
 int quantize_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
-// row r of the output belongs to row idx[r] / div of x (16 bit); rows from *n_valid on are left alone
-int quantize_i8_gather(const void* x, bool bf16, int64_t ldx, const int32_t* idx, int div, const int32_t* n_valid, int8_t* q, float* s, int64_t rows, int K,
+// row r of the output belongs to row idx[r] / div of x, or to row r without idx; rows from *n_valid on are left alone
+int quantize_i8_gather(const void* x, int x_dtype, int64_t ldx, const int32_t* idx, int div, const int32_t* n_valid, int8_t* q, float* s, int64_t rows, int K,
                        cudaStream_t st);
 int silu_mul_quantize_i8(const void* gate_up, bool bf16, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
 int resadd_rmsnorm_quantize_i8(const void* hidden, const void* residual, const void* w, void* residual_out, bool bf16, float eps, int8_t* q, float* s,
                                int64_t M, int K, cudaStream_t st);
 
 #ifdef __CUDACC__
-// Ordinary loads, never by the read-only path: these kernels begin while the kernel that writes their inputs is still running.
+// Ordinary loads, never by the read-only path: these kernels begin while the kernel that writes their inputs is still running.  Volatile
+// keeps them behind the wait for it; without a memory clobber several are on their way at a time.
 __device__ __forceinline__ uint4 ld_vec(const void* p) {
   uint4 v;
-  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 __device__ __forceinline__ float ld_f32(const float* p) {
   float v;
-  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
   return v;
 }
 // Sixteen bytes of a weight: read once per call by one thread, so not worth a line of L1.
@@ -68,41 +80,135 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b)
   else { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 }
 
-// rint(127 x / a), half to even, decided exactly.  r = 127 / a rounded; x * r is then off by 2e-5 at most, and only within that of a half
-// can the two round differently (a bf16 row holds exact halves often: every value that is half its row's largest).
-__device__ __forceinline__ int i8_code_exact(float x, float a, float r) {
-  const float t = fabsf(x) * r;
-  float k = floorf(t);
-  if (fabsf(t - k - 0.5f) < 1e-4f) {
-    const double d = 254.0 * (double)fabsf(x), h = (2.0 * (double)k + 1.0) * (double)a;      // both exact
-    if (d > h || (d == h && ((int)k & 1))) k += 1.f;
-  } else {
-    k = rintf(t);
-  }
-  return x < 0.f ? -(int)k : (int)k;
+// What the codes of a row need of its largest value: rint(127 x / a), halves to even, decided exactly.  The quotient of y = 127 x by a is
+// corrected once by its remainder, which is exact in fp32; a quotient that is a half then comes out as one, and of 16-bit values no other
+// quotient is nearer to a half than 2^-13.  (A bf16 row has exact halves by the dozen: every value that is half its row's largest.  Deciding
+// the near ones in a branch of their own cost more than this: three of ten warps went there.)  Rows of huge values are taken 2^-40 of.
+struct I8Row {
+  float c, a, ra;                                          // 127, a, 1 / a, or the first two 2^-40 times that
+};
+__device__ __forceinline__ I8Row i8_row(float a) {
+  const float f = a > 1e30f ? 9.094947e-13f : 1.f;
+  return I8Row{127.f * f, a * f, 1.f / (a * f)};
 }
-// Four codes, lowest byte first.  Adding 1.5 * 2^23 leaves the rounded product in the low byte; what the product is off from it says
-// whether one of the four is near a half.
-__device__ __forceinline__ uint32_t i8_codes4(const float (&x)[4], float a, float r) {
-  constexpr float MAGIC = 12582912.f;
-  uint32_t b[4];
-  float off = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float m = fmaf(x[i], r, MAGIC);
-    off = fmaxf(off, fabsf(fmaf(x[i], r, -(m - MAGIC))));
-    b[i] = __float_as_uint(m);
+constexpr float I8_ROUND = 12582912.f;                     // 1.5 * 2^23: added, it leaves a small value's nearest integer in the low byte
+__device__ __forceinline__ uint32_t i8_pack4(const float (&m)[4]) {      // values plus I8_ROUND -> four codes, lowest byte first
+  return __byte_perm(__byte_perm(__float_as_uint(m[0]), __float_as_uint(m[1]), 0x0040), __byte_perm(__float_as_uint(m[2]), __float_as_uint(m[3]), 0x0040), 0x5410);
+}
+// WIDE: x has more than eleven significant bits, so that 127 x needs a second word.
+template <bool WIDE> __device__ __forceinline__ float i8_place(float x, const I8Row& r) {
+  const float y = __fmul_rn(x, r.c), t = __fmul_rn(y, r.ra);
+  float rem = __fmaf_rn(-t, r.a, y);
+  if constexpr (WIDE) {
+    const float low = __fmaf_rn(x, r.c, -y), q = __fmaf_rn(__fadd_rn(rem, low), r.ra, t);
+    // the quotient may be rounded to a half without being one: its own remainder tells
+    rem = __fadd_rn(__fmaf_rn(-q, r.a, y), low);
+    return fabsf(q - rintf(q)) == 0.5f && rem != 0.f ? q + copysignf(0.0009765625f, rem) : q;
+  } else {
+    return __fmaf_rn(rem, r.ra, t);
   }
-  if (off > 0.4999f) {
+}
+template <bool WIDE> __device__ __forceinline__ uint32_t i8_codes4(const float (&x)[4], const I8Row& r) {
+  float m[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = (uint32_t)i8_code_exact(x[i], a, r);
-  }
-  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  for (int i = 0; i < 4; ++i) m[i] = __fadd_rn(i8_place<WIDE>(x[i], r), I8_ROUND);
+  return i8_pack4(m);
+}
+// Of values that are rounded themselves, where the last bit of the quotient means nothing: r = 127 / a.
+__device__ __forceinline__ uint32_t i8_codes4_computed(const float (&x)[4], float r) {
+  float m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = __fmaf_rn(x[i], r, I8_ROUND);
+  return i8_pack4(m);
 }
 // Never contracted, so that every kernel gives the same bits.
 __device__ __forceinline__ float i8_scaled(int sum, float scale, float wscale) { return __fmul_rn(__fmul_rn((float)sum, scale), wscale); }
 __device__ __forceinline__ float i8_output(int sum, float scale, float wscale, float bias) { return __fadd_rn(i8_scaled(sum, scale, wscale), bias); }
-__device__ __forceinline__ float silu_mul_f(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// To within a few units in the last place: codes are made from it, and each that lands on the other side of a half is a step off (with the
+// fast exponential an fp16 layer of 14336 wide experts was off by 4.3e-4 of its norm instead of 2.1e-4).
+__device__ __forceinline__ float silu_mul_f(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
+
+// Bytes between two tokens' codes in shared memory: 64 apart in the banks, so that a quarter warp reads two tokens' 64 bytes without a conflict.
+__host__ __device__ constexpr int i8_code_pitch(int K) { return (K + 127) / 128 * 128 + 64; }
+
+// All codes of M rows x [M, ldx] into shared memory, by the first THREADS threads of a CTA, which meet() in between; tok.max is zero before,
+// K % 8 == 0.  A thread's pieces of eight stay in registers between the maximum and the codes, sixteen of them; more are read twice.
+struct I8Tokens {
+  uint32_t max[I8_STREAM_MAX_TOK];
+  float scale[I8_STREAM_MAX_TOK];
+  I8Row row[I8_STREAM_MAX_TOK];
+};
+template <bool BF16, int THREADS, class Meet>
+__device__ __forceinline__ void i8_quantize_tokens(const uint16_t* x, int64_t ldx, int M, int K, uint8_t* codes, int pitch, I8Tokens& tok, Meet meet) {
+  constexpr int V = 16;
+  const int n8 = K >> 3, total = M * n8, lane = threadIdx.x & 31;
+  const uint32_t inv = 0xFFFFFFFFu / (uint32_t)n8 + 1;     // i / n8 = i * inv >> 32 for the sizes that fit shared memory (i < 2^17, n8 < 2^14)
+  auto token = [&](int i) { return n8 == 1 ? i : (int)__umulhi((uint32_t)i, inv); };
+  const bool once = total <= V * THREADS;
+  uint4 v[V];
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i = base + j * THREADS + threadIdx.x, m = token(i);
+      v[j] = i < total ? ld_vec(x + m * ldx + 8 * (i - m * n8)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  for (int base = 0; base < total; base += V * THREADS) {
+    fetch(base);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i0 = base + j * THREADS + (int)(threadIdx.x & ~31u);
+      if (i0 >= total) break;                              // whole warps
+      const uint32_t e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+      uint32_t mx = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float a, b;
+        unpack2<BF16>(e[c], a, b);
+        mx = max(mx, max(__float_as_uint(a) & 0x7FFFFFFFu, __float_as_uint(b) & 0x7FFFFFFFu));
+      }
+      const int m = token(i0);
+      if (token(i0 + 31) == m) {
+        mx = __reduce_max_sync(0xffffffffu, mx);
+        if (lane == 0) atomicMax(&tok.max[m], mx);
+      } else if (i0 + lane < total) {                      // a warp that straddles tokens
+        atomicMax(&tok.max[token(i0 + lane)], mx);
+      }
+      __syncwarp();
+    }
+  }
+  meet();
+  if (threadIdx.x < M) {
+    const uint32_t bits = tok.max[threadIdx.x];
+    const float a = fmaxf(__uint_as_float(bits), I8_MIN_AMAX);
+    I8Row r = i8_row(a);
+    if (bits >= 0x7F800000u) r = I8Row{0.f, 0.f, 0.f};     // not finite
+    tok.row[threadIdx.x] = r;
+    tok.scale[threadIdx.x] = bits < 0x7F800000u ? a / 127.f : __uint_as_float(0x7FC00000u);
+  }
+  __syncwarp();
+  meet();
+  for (int base = 0; base < total; base += V * THREADS) {
+    if (!once) fetch(base);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i = base + j * THREADS + threadIdx.x;
+      if (i >= total) break;
+      const int m = token(i);
+      const I8Row r = tok.row[m];
+      float lo[4], hi[4];
+      unpack2<BF16>(v[j].x, lo[0], lo[1]); unpack2<BF16>(v[j].y, lo[2], lo[3]); unpack2<BF16>(v[j].z, hi[0], hi[1]); unpack2<BF16>(v[j].w, hi[2], hi[3]);
+      uint2 o = make_uint2(0, 0);
+      if (r.c != 0.f) o = make_uint2(i8_codes4<false>(lo, r), i8_codes4<false>(hi, r));
+      *reinterpret_cast<uint2*>(codes + m * pitch + 8 * (i - m * n8)) = o;
+    }
+  }
+  __syncwarp();
+  meet();
+}
+__device__ __forceinline__ void add_shared(int* p, int v) {
+  asm volatile("red.shared.add.s32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(p)), "r"(v) : "memory");
+}
 
 // D += A * B, 16 x 8 x 32, signed bytes: A rows are tokens, B columns weight rows
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

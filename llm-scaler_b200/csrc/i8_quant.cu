@@ -29,35 +29,52 @@ __device__ __forceinline__ void enter() {                  // as in moe_aux.cu: 
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }      // orders as |v|, NaN above all
 
-// Scale of a row whose largest |value| has these bits; a and r for the codes.  False where the row is not finite.
-__device__ __forceinline__ bool row_scale(uint32_t bits, float& a, float& r, float& scale) {
-  a = fmaxf(__uint_as_float(bits), I8_MIN_AMAX);
-  scale = a / 127.f;
-  r = 127.f / a;
-  if (bits < 0x7F800000u) return true;
-  scale = __uint_as_float(0x7FC00000u);
-  return false;
+// What a row's codes are made with: a stored row's exactly (row), a computed one's by r = 127 / a.
+struct Scale {
+  I8Row row;
+  float r, scale;
+  bool finite;
+};
+template <int MODE> __device__ __forceinline__ Scale row_scale(uint32_t mx, float sum, int K, float eps) {
+  Scale s;
+  if constexpr (MODE == NORM) {
+    // codes of v w, whose maximum stands for the normed row's; of a row that is nearly nothing, of v w against the floor over 1 / rms
+    const float rstd = rsqrtf(sum / (float)K + eps), an = __uint_as_float(mx) * rstd;
+    s.finite = abs_bits(an) < 0x7F800000u && mx < 0x7F800000u && abs_bits(sum) <= 0x7F800000u;
+    s.scale = fmaxf(an, I8_MIN_AMAX) / 127.f;
+    s.r = 127.f / fmaxf(__uint_as_float(mx), I8_MIN_AMAX / rstd);
+  } else {
+    const float a = fmaxf(__uint_as_float(mx), I8_MIN_AMAX);
+    s.finite = mx < 0x7F800000u;
+    s.scale = a / 127.f;
+    if constexpr (MODE == PLAIN) s.row = i8_row(a); else s.r = 127.f / a;
+  }
+  if (!s.finite) s.scale = __uint_as_float(0x7FC00000u);
+  return s;
 }
 
-template <bool BF16> __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+template <int DT> __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  constexpr bool BF16 = DT == B2Q_BF16;
   unpack2<BF16>(v.x, f[0], f[1]); unpack2<BF16>(v.y, f[2], f[3]); unpack2<BF16>(v.z, f[4], f[5]); unpack2<BF16>(v.w, f[6], f[7]);
 }
 
-// Eight values of a row as they are to be quantised.  PLAIN keeps the raw words, the other forms the eight floats.
-template <int MODE, bool BF16> struct Piece {
+// Eight values of a row as they are to be quantised.  16-bit PLAIN keeps the raw words, the other forms the eight floats.
+template <int MODE, int DT> struct Piece {
   float f[8];
   __device__ __forceinline__ void get(float (&o)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = f[i];
   }
 };
-template <bool BF16> struct Piece<PLAIN, BF16> {
+template <int DT> struct RawPiece {
   uint4 v;
-  __device__ __forceinline__ void get(float (&o)[8]) const { unpack8<BF16>(v, o); }
+  __device__ __forceinline__ void get(float (&o)[8]) const { unpack8<DT>(v, o); }
 };
+template <> struct Piece<PLAIN, B2Q_BF16> : RawPiece<B2Q_BF16> {};
+template <> struct Piece<PLAIN, B2Q_F16> : RawPiece<B2Q_F16> {};
 
 // WARP: a row per warp, V pieces per lane.  Otherwise a row per CTA, V pieces per thread.
-template <int MODE, bool BF16, int V, bool WARP>
+template <int MODE, int DT, int V, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Params p) {
   __shared__ uint32_t red_max[32];
   __shared__ float red_sum[32];
@@ -68,21 +85,27 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Pa
   if (row >= p.M) return;                                  // whole warps, or the whole CTA
   int64_t src = row;
   if constexpr (MODE == PLAIN) {
-    if (p.idx) {
-      if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
-      src = *reinterpret_cast<const volatile int32_t*>(p.idx + row) / p.div;
-    }
+    if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
+    if (p.idx) src = *reinterpret_cast<const volatile int32_t*>(p.idx + row) / p.div;
   }
   const int n8 = p.K >> 3;
-  const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + src * p.ldx;
-  Piece<MODE, BF16> pc[V];
+  constexpr bool BF16 = DT == B2Q_BF16;
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + src * p.ldx * (DT == B2Q_F32 ? 2 : 1);
+  Piece<MODE, DT> pc[V];
   uint32_t mx = 0;
   float sum = 0.f;
   if constexpr (MODE == PLAIN) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = first + i * step;
-      pc[i].v = c < n8 ? ld_vec(x + 8 * c) : make_uint4(0, 0, 0, 0);
+      if constexpr (DT == B2Q_F32) {
+        const uint4 a = c < n8 ? ld_vec(x + 16 * c) : make_uint4(0, 0, 0, 0), b = c < n8 ? ld_vec(x + 16 * c + 8) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pc[i].f[j] = __uint_as_float(w[j]);
+      } else {
+        pc[i].v = c < n8 ? ld_vec(x + 8 * c) : make_uint4(0, 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -103,8 +126,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Pa
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float a[8], b[8];
-      unpack8<BF16>(g[i], a);
-      unpack8<BF16>(u[i], b);
+      unpack8<DT>(g[i], a);
+      unpack8<DT>(u[i], b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         pc[i].f[j] = silu_mul_f(a[j], b[j]);
@@ -128,14 +151,14 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Pa
     for (int i = 0; i < V; ++i) {
       const int c = first + i * step;
       float a[8], b[8];
-      unpack8<BF16>(h[i], a);
-      unpack8<BF16>(r[i], b);
+      unpack8<DT>(h[i], a);
+      unpack8<DT>(r[i], b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) { a[j] += b[j]; sum = fmaf(a[j], a[j], sum); }
       if (c < n8)
         *reinterpret_cast<uint4*>(ro + 8 * c) =
             make_uint4(pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3]), pack2<BF16>(a[4], a[5]), pack2<BF16>(a[6], a[7]));
-      unpack8<BF16>(w[i], b);
+      unpack8<DT>(w[i], b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         pc[i].f[j] = a[j] * b[j];
@@ -159,19 +182,8 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Pa
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
   }
-  float a, r, scale;
-  bool finite;
-  if constexpr (MODE == NORM) {
-    const float rstd = rsqrtf(sum / (float)p.K + p.eps), an = __uint_as_float(mx) * rstd;
-    finite = row_scale(abs_bits(an), a, r, scale) && mx < 0x7F800000u && abs_bits(sum) <= 0x7F800000u;
-    if (!finite) scale = __uint_as_float(0x7FC00000u);
-    // codes of v w, whose maximum stands for the normed row's; of a row that is nearly nothing, of v w rstd against the floor
-    a = fmaxf(__uint_as_float(mx), I8_MIN_AMAX / rstd);
-    r = 127.f / a;
-  } else {
-    finite = row_scale(mx, a, r, scale);
-  }
-  if (first == 0) p.s[row] = scale;
+  const Scale sc = row_scale<MODE>(mx, sum, p.K, p.eps);
+  if (first == 0) p.s[row] = sc.scale;
   uint8_t* q = reinterpret_cast<uint8_t*>(p.q) + row * p.K;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -181,7 +193,10 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Pa
       pc[i].get(f);
       const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
       uint2 o = make_uint2(0, 0);
-      if (finite) o = make_uint2(i8_codes4(lo, a, r), i8_codes4(hi, a, r));
+      if (sc.finite) {
+        if constexpr (MODE == PLAIN) o = make_uint2(i8_codes4<DT == B2Q_F32>(lo, sc.row), i8_codes4<DT == B2Q_F32>(hi, sc.row));
+        else o = make_uint2(i8_codes4_computed(lo, sc.r), i8_codes4_computed(hi, sc.r));
+      }
       *reinterpret_cast<uint2*>(q + 8 * c) = o;
     }
   }
@@ -197,10 +212,8 @@ __global__ void __launch_bounds__(512) quantize_i8_any_kernel(const Params p) {
   enter();
   int64_t src = row;
   if constexpr (MODE == PLAIN) {
-    if (p.idx) {
-      if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
-      src = *reinterpret_cast<const volatile int32_t*>(p.idx + row) / p.div;
-    }
+    if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
+    if (p.idx) src = *reinterpret_cast<const volatile int32_t*>(p.idx + row) / p.div;
   }
   auto at = [&](const void* b, int64_t i) -> float {
     if constexpr (DT == B2Q_F32) return reinterpret_cast<const volatile float*>(b)[i];
@@ -227,18 +240,8 @@ __global__ void __launch_bounds__(512) quantize_i8_any_kernel(const Params p) {
   sum = lane < 16 ? red_sum[lane] : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  float a, r, scale;
-  bool finite;
-  if constexpr (MODE == NORM) {
-    const float rstd = rsqrtf(sum / (float)p.K + p.eps), an = __uint_as_float(mx) * rstd;
-    finite = row_scale(abs_bits(an), a, r, scale) && mx < 0x7F800000u && abs_bits(sum) <= 0x7F800000u;
-    if (!finite) scale = __uint_as_float(0x7FC00000u);
-    a = fmaxf(__uint_as_float(mx), I8_MIN_AMAX / rstd);
-    r = 127.f / a;
-  } else {
-    finite = row_scale(mx, a, r, scale);
-  }
-  if (threadIdx.x == 0) p.s[row] = scale;
+  const Scale sc = row_scale<MODE>(mx, sum, p.K, p.eps);
+  if (threadIdx.x == 0) p.s[row] = sc.scale;
   for (int c = threadIdx.x; c < p.K; c += 512) {
     float v = at(p.x, src * p.ldx + c);
     if constexpr (MODE == SILU) v = silu_mul_f(v, at(p.x, src * p.ldx + p.K + c));
@@ -247,7 +250,10 @@ __global__ void __launch_bounds__(512) quantize_i8_any_kernel(const Params p) {
       store_scalar(p.residual_out, row * p.K + c, DT, v);
       v *= at(p.nw, c);
     }
-    p.q[row * p.K + c] = finite ? (int8_t)i8_code_exact(v, a, r) : (int8_t)0;
+    float m;
+    if constexpr (MODE == PLAIN) m = __fadd_rn(i8_place<DT == B2Q_F32>(v, sc.row), I8_ROUND);
+    else m = __fmaf_rn(v, sc.r, I8_ROUND);
+    p.q[row * p.K + c] = sc.finite ? (int8_t)(__float_as_uint(m) & 255u) : (int8_t)0;
   }
 }
 
@@ -259,25 +265,29 @@ static int launch(void (*kern)(KArgs...), int64_t grid, int block, cudaStream_t 
   return launch_status();
 }
 
-template <int MODE, bool BF16> static int run_vec(const Params& p, cudaStream_t st) {
+template <int MODE, int DT> static int run_vec(const Params& p, cudaStream_t st) {
   const int n8 = p.K / 8;
   // short rows, and enough of them to fill the SMs: a warp each
   if (n8 <= 128 && p.M >= 148) {
     const int64_t grid = (p.M + 7) / 8;
-    if (n8 <= 32) return launch(quantize_i8_kernel<MODE, BF16, 1, true>, grid, 256, st, p);
-    if (n8 <= 64) return launch(quantize_i8_kernel<MODE, BF16, 2, true>, grid, 256, st, p);
-    return launch(quantize_i8_kernel<MODE, BF16, 4, true>, grid, 256, st, p);
+    if (n8 <= 32) return launch(quantize_i8_kernel<MODE, DT, 1, true>, grid, 256, st, p);
+    if (n8 <= 64) return launch(quantize_i8_kernel<MODE, DT, 2, true>, grid, 256, st, p);
+    return launch(quantize_i8_kernel<MODE, DT, 4, true>, grid, 256, st, p);
   }
   auto block = [&](int v) { return (n8 + 32 * v - 1) / (32 * v) * 32; };
   const bool few = p.M <= 148;                             // one CTA per SM at most: as many threads as a row gives work to
-  if (few ? n8 <= 1024 : n8 <= 256) return launch(quantize_i8_kernel<MODE, BF16, 1, false>, p.M, block(1), st, p);
-  if (few ? n8 <= 2048 : n8 <= 1024) return launch(quantize_i8_kernel<MODE, BF16, 2, false>, p.M, block(2), st, p);
-  return launch(quantize_i8_kernel<MODE, BF16, 4, false>, p.M, block(4), st, p);
+  if (few ? n8 <= 1024 : n8 <= 256) return launch(quantize_i8_kernel<MODE, DT, 1, false>, p.M, block(1), st, p);
+  if (few ? n8 <= 2048 : n8 <= 1024) return launch(quantize_i8_kernel<MODE, DT, 2, false>, p.M, block(2), st, p);
+  return launch(quantize_i8_kernel<MODE, DT, 4, false>, p.M, block(4), st, p);
 }
 
 template <int MODE> static int run(const Params& p, int dt, bool vec, cudaStream_t st) {
   if (p.M == 0) return B2Q_OK;
-  if (vec && p.K % 8 == 0 && p.K <= 32768 && dt != B2Q_F32) return dt == B2Q_BF16 ? run_vec<MODE, true>(p, st) : run_vec<MODE, false>(p, st);
+  if (vec && p.K % 8 == 0 && p.K <= 32768) {
+    if (dt == B2Q_BF16) return run_vec<MODE, B2Q_BF16>(p, st);
+    if (dt == B2Q_F16) return run_vec<MODE, B2Q_F16>(p, st);
+    if constexpr (MODE == PLAIN) return run_vec<MODE, B2Q_F32>(p, st);
+  }
   if (dt == B2Q_BF16) return launch(quantize_i8_any_kernel<MODE, B2Q_BF16>, p.M, 512, st, p);
   if (dt == B2Q_F16) return launch(quantize_i8_any_kernel<MODE, B2Q_F16>, p.M, 512, st, p);
   if constexpr (MODE == PLAIN) return launch(quantize_i8_any_kernel<MODE, B2Q_F32>, p.M, 512, st, p);
@@ -291,11 +301,11 @@ int quantize_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* s, in
   p.x = x; p.ldx = ldx; p.q = q; p.s = s; p.M = M; p.K = K;
   return i8q::run<i8q::PLAIN>(p, x_dtype, aligned16(x) && i8q::aligned8(q) && ldx % 8 == 0, st);
 }
-int quantize_i8_gather(const void* x, bool bf16, int64_t ldx, const int32_t* idx, int div, const int32_t* n_valid, int8_t* q, float* s, int64_t rows, int K,
+int quantize_i8_gather(const void* x, int x_dtype, int64_t ldx, const int32_t* idx, int div, const int32_t* n_valid, int8_t* q, float* s, int64_t rows, int K,
                        cudaStream_t st) {
   i8q::Params p{};
   p.x = x; p.ldx = ldx; p.idx = idx; p.div = div; p.n_valid = n_valid; p.q = q; p.s = s; p.M = rows; p.K = K;
-  return i8q::run<i8q::PLAIN>(p, bf16 ? B2Q_BF16 : B2Q_F16, aligned16(x) && i8q::aligned8(q) && ldx % 8 == 0, st);
+  return i8q::run<i8q::PLAIN>(p, x_dtype, aligned16(x) && i8q::aligned8(q) && ldx % 8 == 0, st);
 }
 int silu_mul_quantize_i8(const void* gate_up, bool bf16, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
   i8q::Params p{};

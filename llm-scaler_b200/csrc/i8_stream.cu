@@ -29,10 +29,6 @@ struct Params {
   int early;                                               // weights may be read before the kernels in front are done
 };
 
-__device__ __forceinline__ void add_shared(int* p, int v) {
-  asm volatile("red.shared.add.s32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(p)), "r"(v) : "memory");
-}
-
 // R: eights of rows in a unit
 template <int R, bool FROM16, bool BF16>
 __global__ void __launch_bounds__(THREADS, 2) i8_stream_kernel(const Params p) {
@@ -40,8 +36,7 @@ __global__ void __launch_bounds__(THREADS, 2) i8_stream_kernel(const Params p) {
   extern __shared__ __align__(16) uint8_t smem[];
   int* sums = reinterpret_cast<int*>(smem);                // [M][row_cap]
   uint8_t* codes = smem + (size_t)p.M * p.row_cap * 4;     // [M][code_pitch]
-  __shared__ float token_scale[I8_STREAM_MAX_TOK];
-  __shared__ uint32_t token_max[I8_STREAM_MAX_TOK];
+  __shared__ I8Tokens tok;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int r0 = (int)((int64_t)blockIdx.x * p.N / gridDim.x), rows = (int)((int64_t)(blockIdx.x + 1) * p.N / gridDim.x) - r0;
   const int nck = (p.K + KU - 1) / KU, units = (rows + ROWS - 1) / ROWS * nck;
@@ -63,48 +58,11 @@ __global__ void __launch_bounds__(THREADS, 2) i8_stream_kernel(const Params p) {
   if (!p.early) grid_dep_wait();
   if (u0 < u1) load(u0, cur);
   for (int i = threadIdx.x; i < p.M * p.row_cap; i += THREADS) sums[i] = 0;
-  if (FROM16 && threadIdx.x < I8_STREAM_MAX_TOK) token_max[threadIdx.x] = 0;
+  if (FROM16 && threadIdx.x < I8_STREAM_MAX_TOK) tok.max[threadIdx.x] = 0;
   if (p.early) grid_dep_wait();
   __syncthreads();
 
-  if constexpr (FROM16) {
-    const int n8 = p.K >> 3, total = p.M * n8;
-    for (int i = threadIdx.x; i < (total + 31) / 32 * 32; i += THREADS) {      // whole warps; a warp may straddle two tokens
-      const int m = min(i / n8, p.M - 1);
-      uint32_t mx = 0;
-      if (i < total) {
-        const uint4 v = ld_vec(p.x16 + m * p.ldx16 + 8 * (i - m * n8));
-        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float a, b;
-          unpack2<BF16>(e[j], a, b);
-          mx = max(mx, max(__float_as_uint(a) & 0x7FFFFFFFu, __float_as_uint(b) & 0x7FFFFFFFu));
-        }
-      }
-      if (__match_any_sync(0xffffffffu, m) == 0xffffffffu) {
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        if (lane == 0) atomicMax(&token_max[m], mx);
-      } else {
-        atomicMax(&token_max[m], mx);
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < total; i += THREADS) {
-      const int m = i / n8, c = i - m * n8;
-      const uint4 v = ld_vec(p.x16 + m * p.ldx16 + 8 * c);
-      const uint32_t bits = token_max[m];
-      const float a = fmaxf(__uint_as_float(bits), I8_MIN_AMAX), r = 127.f / a;
-      const bool finite = bits < 0x7F800000u;
-      float lo[4], hi[4];
-      unpack2<BF16>(v.x, lo[0], lo[1]); unpack2<BF16>(v.y, lo[2], lo[3]); unpack2<BF16>(v.z, hi[0], hi[1]); unpack2<BF16>(v.w, hi[2], hi[3]);
-      uint2 o = make_uint2(0, 0);
-      if (finite) o = make_uint2(i8_codes4(lo, a, r), i8_codes4(hi, a, r));
-      *reinterpret_cast<uint2*>(codes + m * p.code_pitch + 8 * c) = o;
-      if (c == 0) token_scale[m] = finite ? a / 127.f : __uint_as_float(0x7FC00000u);
-    }
-    __syncthreads();
-  }
+  if constexpr (FROM16) i8_quantize_tokens<BF16, THREADS>(p.x16, p.ldx16, p.M, p.K, codes, p.code_pitch, tok, [] { __syncthreads(); });
 
   int acc[R][4];
 #pragma unroll
@@ -157,7 +115,7 @@ __global__ void __launch_bounds__(THREADS, 2) i8_stream_kernel(const Params p) {
   __syncthreads();
   for (int i = threadIdx.x; i < p.M * rows; i += THREADS) {
     const int m = i / rows, r = i - m * rows, n = r0 + r;
-    const float s = FROM16 ? token_scale[m] : ld_f32(p.xs + m);
+    const float s = FROM16 ? tok.scale[m] : ld_f32(p.xs + m);
     const float v = i8_output(sums[m * p.row_cap + r], s, load_scalar(p.ws, n, p.ws_dtype), p.bias ? load_scalar(p.bias, n, BF16 ? B2Q_BF16 : B2Q_F16) : 0.f);
     reinterpret_cast<uint16_t*>(p.out)[m * p.ldo + n] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
   }
@@ -175,13 +133,10 @@ static int sm_count() {
   return sms[dev];
 }
 
-// codes of neighbouring tokens 64 bytes apart in the banks: a quarter warp reads two tokens' 64 bytes without a conflict
-static int code_pitch(int K) { return (K + 127) / 128 * 128 + 64; }
-
 template <int R, bool FROM16, bool BF16> static int launch(Params& p, int grid, cudaStream_t st) {
   p.row_cap = (p.N + grid - 1) / grid;
   p.row_cap = (p.row_cap + 3) / 4 * 4;                     // the codes behind the sums stay 16-byte aligned
-  p.code_pitch = code_pitch(p.K);
+  p.code_pitch = i8_code_pitch(p.K);
   const int smem = p.M * p.row_cap * 4 + (FROM16 ? p.M * p.code_pitch : 0);
   auto kern = i8_stream_kernel<R, FROM16, BF16>;
   static thread_local int configured[16] = {0};
@@ -209,7 +164,7 @@ template <bool FROM16, bool BF16> static int pick(Params& p, cudaStream_t st) {
 }  // namespace i8s
 
 bool i8_stream_supported(const I8LinearArgs& a) {
-  return a.M <= I8_STREAM_MAX_TOK && (!a.x16 || (a.M * i8s::code_pitch(a.K) <= i8s::CODES_MAX && aligned16(a.x16) && a.ldx16 % 8 == 0));
+  return a.M <= I8_STREAM_MAX_TOK && (!a.x16 || (a.M * i8_code_pitch(a.K) <= i8s::CODES_MAX && aligned16(a.x16) && a.ldx16 % 8 == 0));
 }
 
 int i8_stream_linear(const I8LinearArgs& a, cudaStream_t st) {

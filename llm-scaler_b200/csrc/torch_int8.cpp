@@ -137,6 +137,34 @@ Tensor linear_dynamic(const Tensor& x, const Tensor& weight, const Tensor& weigh
   return out;
 }
 
+Tensor moe_forward(const Tensor& x, const Tensor& logits, const Tensor& w13, const Tensor& s13, const Tensor& w2, const Tensor& s2, int64_t top_k,
+                   bool renormalize) {
+  same_device({&x, &logits, &w13, &s13, &w2, &s2});
+  TORCH_CHECK(x.dim() == 2 && is16(x.scalar_type()) && x.is_contiguous(), "x must be a contiguous bf16 / fp16 [T, H] tensor");
+  TORCH_CHECK(logits.dim() == 2 && logits.size(0) == x.size(0) && logits.is_contiguous(), "router_logits must be a contiguous [T, E] tensor");
+  const int64_t T = x.size(0), H = x.size(1), E = logits.size(1);
+  TORCH_CHECK(w13.dim() == 3 && w13.scalar_type() == at::kChar && w13.is_contiguous() && w13.size(0) == E && w13.size(2) == H && w13.size(1) % 2 == 0,
+              "gate_up_weight must be a contiguous int8 [E, 2I, H] tensor");
+  const int64_t I = w13.size(1) / 2;
+  TORCH_CHECK(w2.dim() == 3 && w2.scalar_type() == at::kChar && w2.is_contiguous() && w2.size(0) == E && w2.size(1) == H && w2.size(2) == I,
+              "down_weight must be a contiguous int8 [E, H, I] tensor");
+  TORCH_CHECK(s13.numel() == E * 2 * I && s13.is_contiguous(), "gate_up_scale must have E * 2I contiguous elements");
+  TORCH_CHECK(s2.numel() == E * H && s2.is_contiguous(), "down_scale must have E * H contiguous elements");
+  TORCH_CHECK(top_k > 0 && top_k <= E, "top_k must be between 1 and the number of experts");
+  TORCH_CHECK(H > 0 && I > 0 && H % 16 == 0 && I % 16 == 0, "H and I must be multiples of 16");
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor out = at::empty({T, H}, x.options());
+  if (T == 0) return out;
+  b2q_moe_int8 a{};
+  a.x = x.data_ptr(); a.logits = logits.data_ptr(); a.w13 = w13.data_ptr<int8_t>(); a.s13 = s13.data_ptr(); a.w2 = w2.data_ptr<int8_t>(); a.s2 = s2.data_ptr();
+  a.out = out.data_ptr(); a.T = T; a.E = E; a.top_k = top_k; a.H = H; a.I = I;
+  a.act_dtype = dtype_of(x); a.logits_dtype = dtype_of(logits); a.s13_dtype = dtype_of(s13); a.s2_dtype = dtype_of(s2); a.renormalize = renormalize;
+  const size_t wsb = b2q_moe_forward_int8_workspace_bytes(T, E, top_k, H, I);
+  const Tensor ws = at::empty({(int64_t)wsb}, x.options().dtype(at::kByte));
+  check(b2q_moe_forward_int8(&a, ws.data_ptr(), wsb, stream_of(x)));
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(b2q_int8, m) {
@@ -145,6 +173,8 @@ TORCH_LIBRARY(b2q_int8, m) {
   m.def("resadd_rmsnorm_quantize(Tensor hidden, Tensor(a!) residual, Tensor norm_weight, float eps, Tensor(b!)? residual_out) -> (Tensor, Tensor)");
   m.def("linear(Tensor codes, Tensor scale, Tensor weight, Tensor weight_scale, Tensor? bias, ScalarType out_dtype) -> Tensor");
   m.def("linear_dynamic(Tensor x, Tensor weight, Tensor weight_scale, Tensor? bias) -> Tensor");
+  m.def("moe_forward(Tensor x, Tensor router_logits, Tensor gate_up_weight, Tensor gate_up_scale, Tensor down_weight, Tensor down_scale, "
+        "int top_k, bool renormalize) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(b2q_int8, CUDA, m) {
@@ -153,4 +183,5 @@ TORCH_LIBRARY_IMPL(b2q_int8, CUDA, m) {
   m.impl("resadd_rmsnorm_quantize", &resadd_rmsnorm_quantize);
   m.impl("linear", &linear);
   m.impl("linear_dynamic", &linear_dynamic);
+  m.impl("moe_forward", &moe_forward);
 }

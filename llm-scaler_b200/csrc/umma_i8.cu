@@ -25,8 +25,8 @@ namespace b2q {
 using namespace sm100;
 
 namespace ui8 {
-enum { ST_EMPTY = 801, ST_FULL = 802, ST_ACCEMPTY = 803, ST_ACCFULL = 804 };
-constexpr int EPI = 8, THREADS = 64 + 32 * EPI;
+enum { ST_EMPTY = 801, ST_FULL = 802, ST_ACCEMPTY = 803, ST_ACCFULL = 804, ST_XEMPTY = 805 };
+constexpr int EPI = 8, FIRST_EPI = 4, THREADS = 32 * (FIRST_EPI + EPI);      // warps: weights, MMA, tokens, (none), epilogue
 constexpr int MAX_STAGES = 16, TABLE = 256;
 constexpr int STG_BYTES = EPI * 2048;                      // 32 rows x 64 bytes for every epilogue warp
 constexpr int TAIL = STG_BYTES + 2 * 2 * TABLE * 4 + 512;  // staging, scale and bias tables of two tiles, barriers
@@ -36,7 +36,8 @@ constexpr int OVERREAD = 16384;                            // an MMA reads 128 t
 struct Params {
   const float* xs; const void* ws; int ws_dtype; const void* bias;
   uint16_t* out; int64_t ldo; int out_bf16, vec_out;
-  int M, N, nkb;
+  int M, N;
+  int nks;                                                 // stages that K takes
   int h;                                                   // weight rows (MMA columns) per tile
   int n_strips, m_tiles, m_group, total;                   // total: tiles of a dense launch
   int tok_rows, tok_box;                                   // tokens per tile; rows of the token box
@@ -90,9 +91,25 @@ __device__ __forceinline__ uint4 lds128v(uint32_t at) {
   return v;
 }
 __device__ __forceinline__ uint32_t pack_out(float a, float b, int bf16) { return bf16 ? pack2<true>(a, b) : pack2<false>(a, b); }
+// A warp's 32 rows of 64 bytes through shared memory, so that four lanes store a row's 64 bytes together; 16-byte pieces are permuted
+// against bank conflicts.
+__device__ __forceinline__ void stage_rows(uint32_t stg, int lane, const uint32_t (&o)[16]) {
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) sts128(stg + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+  __syncwarp();
+}
+__device__ __forceinline__ void store_rows(uint32_t stg, int lane, int rows, uint8_t* out, int64_t pitch) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rr = i * 8 + (lane >> 2), q = lane & 3;
+    const uint4 v = lds128v(stg + rr * 64 + ((q ^ ((rr >> 1) & 3)) << 4));
+    if (rr < rows) *reinterpret_cast<uint4*>(out + rr * pitch + q * 16) = v;
+  }
+}
 }  // namespace ui8
 
-template <bool PAIR, bool SPLIT, bool GROUPED, bool GATED>
+template <int KPS, bool PAIR, bool SPLIT, bool GROUPED, bool GATED>      // KPS: 128-k boxes of each operand in a stage
 __global__ void __launch_bounds__(ui8::THREADS, 1)
 umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const ui8::Params p) {
   using namespace ui8;
@@ -111,11 +128,11 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
   const uint32_t rank = PAIR || SPLIT ? cluster_ctarank() : 0;
   const int group = PAIR ? 2 : (SPLIT ? p.split : 1);      // CTAs that work on one tile
   const int first = (int)blockIdx.x / group, step = (int)gridDim.x / group;
-  const int kb0 = SPLIT ? (int)rank * p.nkb / p.split : 0, kb1 = SPLIT ? ((int)rank + 1) * p.nkb / p.split : p.nkb;
+  const int ks0 = SPLIT ? (int)rank * p.nks / p.split : 0, ks1 = SPLIT ? ((int)rank + 1) * p.nks / p.split : p.nks;
 
   grid_dep_release();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
+    for (int i = 0; i < p.stages; ++i) { mbar_init(full + 8 * i, 2); mbar_init(empty + 8 * i, 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, PAIR ? 2 * EPI : EPI); }
     *abort_flag = 0;
     fence_barrier_init();
@@ -134,51 +151,33 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
   const int total = GROUPED ? p.tiles[0] * p.n_strips : p.total;
 
   if (warp == 0) {
+    // ---- weights; boxes that begin beyond K read as zero ----
     if (elect_one()) {
-      tma_prefetch_desc(&tm_x);
       tma_prefetch_desc(&tm_w);
-      const int wbox = PAIR ? 128 : (GATED ? p.h / 2 : p.h);
-      const uint32_t bytes = (uint32_t)p.stage_bytes * (PAIR ? 2u : 1u);
+      const int box = PAIR ? 128 : (GATED ? p.h / 2 : p.h);
+      const uint32_t bytes = (uint32_t)(p.stage_bytes - p.a_bytes) * (PAIR ? 2u : 1u);
       int s = 0, issued = 0;
       uint32_t par = 1u;
       bool ok = true;
-      auto put_w = [&](int st, int kb, const Tile& t) {
-        const uint32_t dst = base + st * p.stage_bytes + p.a_bytes;
-        if constexpr (PAIR) {
-          tma_load_2d_pair(dst, &tm_w, kb * 128, t.w0 + (int)rank * 128, map_to_cta(full + 8 * st, 0));
-        } else {
-          tma_load_2d(dst, &tm_w, kb * 128, t.w0, full + 8 * st);
-          if constexpr (GATED) tma_load_2d(dst + wbox * 128, &tm_w, kb * 128, t.w1, full + 8 * st);
-        }
-      };
-      auto put_x = [&](int st, int kb, const Tile& t) {
-        const uint32_t dst = base + st * p.stage_bytes;
-        if constexpr (PAIR) tma_load_2d_pair(dst, &tm_x, kb * 128, t.tok0 + (int)rank * 128, map_to_cta(full + 8 * st, 0));
-        else tma_load_2d(dst, &tm_x, kb * 128, t.tok0, full + 8 * st);
-      };
-      // Weights do not depend on the kernels in front: the first stages' are on their way before the wait for the tokens.
-      int ahead = 0;
-      if constexpr (!GROUPED) {
-        if (p.early && first < total) {
-          const Tile t = tile_at<GROUPED, GATED>(p, first);
-          ahead = min(p.stages, kb1 - kb0);
-          for (int i = 0; i < ahead; ++i) {
-            if (rank == 0 || !PAIR) mbar_expect_tx(full + 8 * i, bytes);
-            put_w(i, kb0 + i, t);
-          }
-        }
-        grid_dep_wait();
-      }
+      // a dense launch's weights do not depend on the kernels in front
+      if (!GROUPED && !p.early) grid_dep_wait();
       for (int id = first; ok && id < total; id += step) {
         const Tile t = tile_at<GROUPED, GATED>(p, id);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int ks = ks0; ks < ks1; ++ks) {
           ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_EMPTY);
           if (!ok) break;
-          if (issued >= ahead) {
-            if (rank == 0 || !PAIR) mbar_expect_tx(full + 8 * s, bytes);
-            put_w(s, kb, t);
+          const uint32_t dst = base + s * p.stage_bytes + p.a_bytes;
+          if (rank == 0 || !PAIR) mbar_expect_tx(full + 8 * s, bytes);
+#pragma unroll
+          for (int i = 0; i < KPS; ++i) {
+            const int k = (ks * KPS + i) * 128;
+            if constexpr (PAIR) {
+              tma_load_2d_pair(dst + i * 16384, &tm_w, k, t.w0 + (int)rank * 128, map_to_cta(full + 8 * s, 0));
+            } else {
+              tma_load_2d(dst + i * p.h * 128, &tm_w, k, t.w0, full + 8 * s);
+              if constexpr (GATED) tma_load_2d(dst + i * p.h * 128 + box * 128, &tm_w, k, t.w1, full + 8 * s);
+            }
           }
-          put_x(s, kb, t);
           ++issued;
           if (++s == p.stages) { s = 0; par ^= 1u; }
         }
@@ -186,9 +185,38 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       // gave up: the copies issued land before the CTA leaves (a pair's are counted on the leader's barriers, and the peer stays with it)
       if (!ok && (rank == 0 || !PAIR)) drain_issued(full, p.stages, issued);
     }
+  } else if (warp == 2) {
+    // ---- tokens ----
+    if (elect_one()) {
+      tma_prefetch_desc(&tm_x);
+      const uint32_t bytes = (uint32_t)p.a_bytes * (PAIR ? 2u : 1u);
+      int s = 0, issued = 0;
+      uint32_t par = 1u;
+      bool ok = true;
+      if constexpr (!GROUPED) grid_dep_wait();
+      for (int id = first; ok && id < total; id += step) {
+        const Tile t = tile_at<GROUPED, GATED>(p, id);
+        for (int ks = ks0; ks < ks1; ++ks) {
+          ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_XEMPTY);
+          if (!ok) break;
+          const uint32_t dst = base + s * p.stage_bytes;
+          if (rank == 0 || !PAIR) mbar_expect_tx(full + 8 * s, bytes);
+#pragma unroll
+          for (int i = 0; i < KPS; ++i) {
+            const int k = (ks * KPS + i) * 128;
+            if constexpr (PAIR) tma_load_2d_pair(dst + i * 16384, &tm_x, k, t.tok0 + (int)rank * 128, map_to_cta(full + 8 * s, 0));
+            else tma_load_2d(dst + i * p.tok_box * 128, &tm_x, k, t.tok0, full + 8 * s);
+          }
+          ++issued;
+          if (++s == p.stages) { s = 0; par ^= 1u; }
+        }
+      }
+      if (!ok && (rank == 0 || !PAIR)) drain_issued(full, p.stages, issued);
+    }
   } else if (warp == 1) {
     if ((!PAIR || rank == 0) && elect_one()) {
       const uint32_t idesc = instr_desc_i8(1u, 1u, PAIR ? 256u : 128u, (uint32_t)p.h);
+      const uint64_t x_step = (uint64_t)(PAIR ? 128 : p.tok_box) * 8, w_step = (uint64_t)(PAIR ? 128 : p.h) * 8;      // from box to box, in 16 bytes
       int s = 0, it = 0;
       uint32_t par = 0u;
       bool ok = true;
@@ -198,16 +226,19 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + b * 256;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int ks = ks0; ks < ks1; ++ks) {
           ok = mbar_wait(full + 8 * s, par, abort_flag, p.status, ST_FULL);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t da = smem_desc_sw128(base + s * p.stage_bytes);
-          const uint64_t db = smem_desc_sw128(base + s * p.stage_bytes + p.a_bytes);
+          uint64_t da = smem_desc_sw128(base + s * p.stage_bytes);
+          uint64_t db = smem_desc_sw128(base + s * p.stage_bytes + p.a_bytes);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (PAIR) mma_i8_pair(d, da + 2 * i, db + 2 * i, idesc, kb > kb0 || i > 0);
-            else mma_i8(d, da + 2 * i, db + 2 * i, idesc, kb > kb0 || i > 0);
+          for (int j = 0; j < KPS; ++j, da += x_step, db += w_step) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (PAIR) mma_i8_pair(d, da + 2 * i, db + 2 * i, idesc, ks > ks0 || j > 0 || i > 0);
+              else mma_i8(d, da + 2 * i, db + 2 * i, idesc, ks > ks0 || j > 0 || i > 0);
+            }
           }
           if constexpr (PAIR) tc_commit_pair(empty + 8 * s, 3); else tc_commit(empty + 8 * s);
           if (++s == p.stages) { s = 0; par ^= 1u; }
@@ -216,10 +247,10 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         if constexpr (PAIR) tc_commit_pair(acc_full + 8 * b, 3); else tc_commit(acc_full + 8 * b);
       }
     }
-  } else {
+  } else if (warp >= FIRST_EPI) {
     // ---- epilogue: lane quadrant = warp & 3 (tokens), column chunks of 32 shared by the two warps of a quadrant ----
-    const int quad = warp & 3, half = (warp - 2) >> 2, etid = threadIdx.x - 64;
-    const uint32_t stg = base + stg_off + (warp - 2) * 2048;
+    const int quad = warp & 3, half = (warp - FIRST_EPI) >> 2, etid = threadIdx.x - 32 * FIRST_EPI;
+    const uint32_t stg = base + stg_off + (warp - FIRST_EPI) * 2048;
     if constexpr (!GROUPED) grid_dep_wait();
     int it = 0;
     for (int id = first; id < total; id += step, ++it) {
@@ -259,22 +290,35 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
             if (c + i < p.h) sts128(at + i * 4, r[i], r[i + 1], r[i + 2], r[i + 3]);
         }
       } else {
-        uint16_t* out = p.out + (int64_t)(t.tok0 + row0) * p.ldo + t.n0;
-        for (int c = half * 32; row0 < t.rows && c < t.cols; c += 64) {
-          uint32_t r[32], o[16];
-          tmem_ld32(acc + c, r);
-          if constexpr (GATED) {
-            uint32_t u[32];
-            tmem_ld32(acc + p.h / 2 + c, u);
+        if constexpr (GATED) {
+          // sixteen outputs in fp32 at a time
+          float* out = reinterpret_cast<float*>(p.out) + (int64_t)(t.tok0 + row0) * p.ldo + t.n0;
+          const float* us = sc + p.h / 2;
+          for (int c = half * 16; row0 < t.rows && c < t.cols; c += 32) {
+            uint32_t r[16], u[16];
+            tmem_ld16(acc + c, r);
+            tmem_ld16(acc + p.h / 2 + c, u);
             tmem_ld_wait();
-            const float* us = sc + p.h / 2 + c;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float g0 = i8_scaled((int)r[2 * i], xs, sc[c + 2 * i]), g1 = i8_scaled((int)r[2 * i + 1], xs, sc[c + 2 * i + 1]);
-              const float u0 = i8_scaled((int)u[2 * i], xs, us[2 * i]), u1 = i8_scaled((int)u[2 * i + 1], xs, us[2 * i + 1]);
-              o[i] = pack_out(silu_mul_f(g0, u0), silu_mul_f(g1, u1), p.out_bf16);
+            for (int i = 0; i < 16; ++i)
+              r[i] = __float_as_uint(silu_mul_f(i8_scaled((int)r[i], xs, sc[c + i]), i8_scaled((int)u[i], xs, us[c + i])));
+            stage_rows(stg, lane, r);
+            if (c + 16 <= t.cols) {
+              store_rows(stg, lane, t.rows - row0, reinterpret_cast<uint8_t*>(out + c), p.ldo * 4);
+            } else {
+              for (int rr = 0; rr < 32 && row0 + rr < t.rows; ++rr) {
+                const int i = lane & 15;
+                uint32_t v;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(stg + rr * 64 + (((i >> 2) ^ ((rr >> 1) & 3)) << 4) + (i & 3) * 4) : "memory");
+                if (lane < 16 && c + i < t.cols) out[rr * p.ldo + c + i] = __uint_as_float(v);
+              }
             }
-          } else {
+          }
+        } else {
+          uint16_t* out = p.out + (int64_t)(t.tok0 + row0) * p.ldo + t.n0;
+          for (int c = half * 32; row0 < t.rows && c < t.cols; c += 64) {
+            uint32_t r[32], o[16];
+            tmem_ld32(acc + c, r);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -282,25 +326,16 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
               const float v1 = i8_output((int)r[2 * i + 1], xs, sc[c + 2 * i + 1], bi[c + 2 * i + 1]);
               o[i] = pack_out(v0, v1, p.out_bf16);
             }
-          }
-          // through shared memory, so that four lanes store 64 bytes of a token; 16-byte pieces are permuted against bank conflicts
-          __syncwarp();
-#pragma unroll
-          for (int q = 0; q < 4; ++q) sts128(stg + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-          __syncwarp();
-          if (p.vec_out && c + 32 <= t.cols) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int rr = i * 8 + (lane >> 2), q = lane & 3;
-              const uint4 v = lds128v(stg + rr * 64 + ((q ^ ((rr >> 1) & 3)) << 4));
-              if (row0 + rr < t.rows) *reinterpret_cast<uint4*>(out + rr * p.ldo + c + q * 8) = v;
-            }
-          } else {
-            for (int rr = 0; rr < 32 && row0 + rr < t.rows; ++rr) {
-              const int q = lane >> 3;
-              uint16_t v;
-              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(stg + rr * 64 + ((q ^ ((rr >> 1) & 3)) << 4) + (lane & 7) * 2) : "memory");
-              if (c + lane < t.cols) out[rr * p.ldo + c + lane] = v;
+            stage_rows(stg, lane, o);
+            if (p.vec_out && c + 32 <= t.cols) {
+              store_rows(stg, lane, t.rows - row0, reinterpret_cast<uint8_t*>(out + c), p.ldo * 2);
+            } else {
+              for (int rr = 0; rr < 32 && row0 + rr < t.rows; ++rr) {
+                const int q = lane >> 3;
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(stg + rr * 64 + ((q ^ ((rr >> 1) & 3)) << 4) + (lane & 7) * 2) : "memory");
+                if (c + lane < t.cols) out[rr * p.ldo + c + lane] = v;
+              }
             }
           }
         }
@@ -374,16 +409,17 @@ static int sm_count() {
 }
 static int round_up(int v, int a) { return (v + a - 1) / a * a; }
 
-template <bool PAIR, bool SPLIT, bool GROUPED, bool GATED>
-static int launch(const CUtensorMap& tx, const CUtensorMap& tw, Params& p, int grid, cudaStream_t st) {
-  p.stage_bytes = p.a_bytes + (PAIR ? 128 : p.h) * 128;
+template <int KPS, bool PAIR, bool SPLIT, bool GROUPED, bool GATED>
+static int launch_form(const CUtensorMap& tx, const CUtensorMap& tw, Params& p, int grid, cudaStream_t st) {
+  p.a_bytes = KPS * p.tok_box * 128;
+  p.stage_bytes = p.a_bytes + KPS * (PAIR ? 128 : p.h) * 128;
   const int over = p.tok_box < 128 ? OVERREAD : 0, room = SMEM_MAX - 1024 - TAIL - over;
   p.stages = room / p.stage_bytes;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   int bytes = p.stages * p.stage_bytes;
-  if (SPLIT && bytes < p.tok_box * (p.h + 4) * 4) return B2Q_ERR_LIMIT;      // partial sums use the stages' room
+  if (SPLIT && bytes < (p.tok_box < 32 ? 32 : p.tok_box) * (p.h + 4) * 4) return B2Q_ERR_LIMIT;      // partial sums use the stages' room
   const int smem = 1024 + bytes + over + TAIL;
-  auto kern = umma_i8_kernel<PAIR, SPLIT, GROUPED, GATED>;
+  auto kern = umma_i8_kernel<KPS, PAIR, SPLIT, GROUPED, GATED>;
   static thread_local bool configured[16] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -411,25 +447,40 @@ static int launch(const CUtensorMap& tx, const CUtensorMap& tw, Params& p, int g
   return launch_status();
 }
 
-// How a dense launch is divided: weight rows per tile and CTAs per tile, by what a tile's stages cost in cycles of an SM.
-struct Plan { int h, split; };
+template <bool SPLIT, bool GROUPED, bool GATED>
+static int launch(int kps, const CUtensorMap& tx, const CUtensorMap& tw, Params& p, int grid, cudaStream_t st) {
+  return kps == 1 ? launch_form<1, false, SPLIT, GROUPED, GATED>(tx, tw, p, grid, st) : launch_form<2, false, SPLIT, GROUPED, GATED>(tx, tw, p, grid, st);
+}
+
+// A stage costs its producers and the MMA's issuer some 150 ns whatever is in it, so low weight boxes come in twos (one / two / four per
+// stage: 8 x 5120 x 5120, 48 rows, 9.1 / 8.0 / 8.0 us; 64 x 4096 x 4096, 32 rows, 7.8 / 6.9 / 7.3; 8 x 17408 x 5120, 128 rows, 16.0 / 16.5).
+static int boxes_per_stage(int h) { return h <= 64 ? 2 : 1; }
+
+// How a dense launch is divided: weight rows per tile, CTAs per tile, or pairs of CTAs with tiles of 256 x 256, by estimated nanoseconds.
+// A tile's 128 k cost what its boxes take out of L2 (160 bytes per ns and SM) or 90 ns, the whole launch at least what the weights take
+// out of DRAM; a split tile 2 us more, for the meeting of its partial sums (128 x 4096 x 14336: 32 rows 17.8 us, 64 rows on two CTAs
+// 16.9; 64 x 4096 x 4096: 6.9 and 8.3).  Clusters of four and eight do not fit on all SMs: 37 of four took two rounds, 32 one.
+struct Plan { int h, split; bool pair; };
 static Plan plan(int M, int N, int nkb, int tok_box) {
   const int sms = sm_count(), m_tiles = (M + 127) / 128;
-  Plan best{256, 1};
-  double best_cost = 1e30;
-  for (int split = 1; split <= 8 && split <= nkb; ++split) {
-    const int slots = sms / split;
-    for (int waves = 1; waves <= 4; ++waves) {
-      const int strips_max = slots * waves / m_tiles;
-      if (strips_max == 0) continue;
-      int h = round_up((N + strips_max - 1) / strips_max, 16);
+  Plan best{256, 1, false};
+  double least = 1e30;
+  const double dram = (double)N * nkb * 128 / 6300;
+  for (int split = 1; split <= 8 && 2 * split <= nkb; split *= 2) {
+    const int slots = split <= 2 ? sms / split : (split == 4 ? sms * 7 / 32 : sms / 9);
+    for (int rounds = 1; rounds <= (split > 1 ? 1 : 8); ++rounds) {
+      const int strips = slots * rounds / m_tiles;
+      if (strips == 0) continue;
+      int h = round_up((N + strips - 1) / strips, 16);
       if (h > 256) continue;
-      if (split > 1 && waves > 1) continue;
-      const int strips = (N + h - 1) / h, rounds = (strips * m_tiles + slots - 1) / slots;
-      const double stage = 60 + fmax(2.0 * h, fmax(h * 128 / 30.0, (h + tok_box) * 128 / 55.0));
-      const double cost = rounds * ((nkb + split - 1) / split * stage + 1500) + (split > 1 ? 2500 : 0);
-      if (cost < best_cost) { best_cost = cost; best = Plan{h, split}; }
+      const double ns = fmax(dram, rounds * ((nkb + split - 1) / split) * fmax(90.0, (h + tok_box) * 128 / 160.0)) + rounds * 700 + (split > 1 ? 2000 : 0);
+      if (ns < least) { least = ns; best = Plan{h, split, false}; }
     }
+  }
+  if (M > 128) {
+    const int rounds = ((M + 255) / 256 * ((N + 255) / 256) + sms / 2 - 1) / (sms / 2);
+    const double ns = fmax(dram, rounds * nkb * 330.0) + rounds * 300 + 1000;
+    if (ns < least) best = Plan{256, 1, true};
   }
   return best;
 }
@@ -441,23 +492,20 @@ int umma_i8_linear(const I8LinearArgs& a, cudaStream_t st) {
   Params p{};
   p.xs = a.xs; p.ws = a.ws; p.ws_dtype = a.ws_dtype; p.bias = a.bias;
   p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.ldo; p.out_bf16 = a.out_bf16; p.vec_out = aligned16(a.out) && a.ldo % 8 == 0;
-  p.M = a.M; p.N = a.N; p.nkb = (a.K + 127) / 128;
+  p.M = a.M; p.N = a.N;
+  const int nkb = (a.K + 127) / 128;
   p.early = tls().overlap_mode == 2;
   p.status = umma_status_ptr();
   if (!p.status) return B2Q_ERR_CUDA;
   const int sms = sm_count();
-  const int pair_tiles = (a.M + 255) / 256 * ((a.N + 255) / 256);
-  const bool pair = a.M > 256 && pair_tiles >= sms / 4;
+  p.tok_box = a.M <= 16 ? 16 : (a.M <= 32 ? 32 : (a.M <= 64 ? 64 : 128));
+  const Plan pl = plan(a.M, a.N, nkb, p.tok_box);
+  const bool pair = pl.pair;
   CUtensorMap tx, tw;
-  if (pair) {
-    p.h = 256; p.tok_rows = 256; p.tok_box = 128; p.split = 1;
-  } else {
-    p.tok_box = a.M <= 32 ? 32 : (a.M <= 64 ? 64 : 128);
-    p.tok_rows = 128;
-    const Plan pl = plan(a.M, a.N, p.nkb, p.tok_box);
-    p.h = pl.h; p.split = pl.split;
-  }
-  p.a_bytes = p.tok_box * 128;
+  p.h = pl.h; p.split = pl.split; p.tok_rows = pair ? 256 : 128;
+  const int kps = pair ? 1 : boxes_per_stage(p.h);
+  p.nks = (nkb + kps - 1) / kps;
+  if (p.split > p.nks) p.split = p.nks;
   p.n_strips = (a.N + p.h - 1) / p.h;
   p.m_tiles = (a.M + p.tok_rows - 1) / p.tok_rows;
   p.m_group = p.m_tiles < 16 ? p.m_tiles : 16;
@@ -466,9 +514,42 @@ int umma_i8_linear(const I8LinearArgs& a, cudaStream_t st) {
   int rc = make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.xq, a.M, a.K, (uint64_t)a.ldx, p.tok_box, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (!rc) rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.N, a.K, (uint64_t)a.K, pair ? 128 : p.h, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  if (pair) return launch<true, false, false, false>(tx, tw, p, 2 * (p.total < sms / 2 ? p.total : sms / 2), st);
-  if (p.split > 1) return launch<false, true, false, false>(tx, tw, p, p.total * p.split, st);
-  return launch<false, false, false, false>(tx, tw, p, p.total < sms ? p.total : sms, st);
+  if (pair) return launch_form<1, true, false, false, false>(tx, tw, p, 2 * (p.total < sms / 2 ? p.total : sms / 2), st);
+  if (p.split > 1) return launch<true, false, false>(kps, tx, tw, p, p.total * p.split, st);
+  return launch<false, false, false>(kps, tx, tw, p, p.total < sms ? p.total : sms, st);
+}
+
+// Token height of the tiles: an MMA has 128 token rows however few are loaded, so this is about bytes of tokens per tile only.
+int i8_grouped_tile(int64_t rows, int E) {
+  const int64_t avg = (rows + E - 1) / E;
+  return avg <= 24 ? 32 : (avg <= 48 ? 64 : 128);
+}
+
+int umma_i8_grouped(const I8GroupedArgs& a, cudaStream_t st) {
+  using namespace ui8;
+  if (!tensor_map_encoder()) return B2Q_ERR_CUDA;
+  Params p{};
+  p.xs = a.xs; p.ws = a.ws; p.ws_dtype = a.ws_dtype;
+  p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.N; p.out_bf16 = a.out_bf16; p.vec_out = aligned16(a.out) && a.N % 8 == 0;
+  p.M = a.rows; p.N = a.N;
+  p.tiles = a.tiles; p.offsets = a.offsets; p.split = 1;
+  p.status = umma_status_ptr();
+  if (!p.status) return B2Q_ERR_CUDA;
+  const int most = a.gated ? 128 : 256;                    // outputs of a tile
+  p.n_strips = (a.N + most - 1) / most;
+  const int width = round_up((a.N + p.n_strips - 1) / p.n_strips, 16);
+  p.h = a.gated ? 2 * width : width;
+  p.tok_rows = p.tok_box = a.tile;
+  const int kps = boxes_per_stage(p.h);
+  p.nks = ((a.K + 127) / 128 + kps - 1) / kps;
+  const int64_t w_rows = (int64_t)a.E * a.N * (a.gated ? 2 : 1);
+  if (w_rows > INT32_MAX || (int64_t)a.tile_cap * p.n_strips > INT32_MAX / 2) return B2Q_ERR_LIMIT;
+  CUtensorMap tx, tw;
+  int rc = make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.xq, a.rows, a.K, (uint64_t)a.K, a.tile, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, w_rows, a.K, (uint64_t)a.K, width, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  const int most_tiles = a.tile_cap * p.n_strips, grid = most_tiles < sm_count() ? most_tiles : sm_count();
+  return a.gated ? launch<false, true, true>(kps, tx, tw, p, grid, st) : launch<false, true, false>(kps, tx, tw, p, grid, st);
 }
 
 }  // namespace b2q

@@ -23,6 +23,7 @@ from .ops import (  # noqa: F401
 )
 from .int8 import (  # noqa: F401
     quantize_int8, silu_mul_quantize_int8, resadd_rmsnorm_quantize_int8, linear_int8, linear_int8_dynamic,
+    moe_forward_int8,
 )
 
 launch_count = _lib.launch_count

@@ -36,6 +36,12 @@ class MoeFp8(C.Structure):
         + [(n, i64) for n in ("T", "E", "top_k", "H", "I")] + [(n, i32) for n in ("act_dtype", "logits_dtype", "fp8_format")]
 
 
+class MoeInt8(C.Structure):
+    """struct b2q_moe_int8"""
+    _fields_ = [(n, vp) for n in ("x", "logits", "w13", "s13", "w2", "s2", "out")] + [(n, i64) for n in ("T", "E", "top_k", "H", "I")] \
+        + [(n, i32) for n in ("act_dtype", "logits_dtype", "s13_dtype", "s2_dtype", "renormalize")]
+
+
 _SIGS = {
     "b2q_strerror": (C.c_char_p, [i32]),
     "b2q_version": (i32, []),
@@ -81,6 +87,8 @@ _SIGS = {
     "b2q_linear_int8": (i32, [vp, i64, vp, vp, vp, i32, vp, vp, i32, i64, i64, i64, i64, vp]),
     "b2q_linear_int8_dynamic_workspace_bytes": (sz, [i64, i64, i64]),
     "b2q_linear_int8_dynamic": (i32, [vp, i32, i64, vp, vp, i32, vp, vp, i64, i64, i64, i64, vp, sz, vp]),
+    "b2q_moe_forward_int8_workspace_bytes": (sz, [i64, i64, i64, i64, i64]),
+    "b2q_moe_forward_int8": (i32, [C.POINTER(MoeInt8), vp, sz, vp]),
     "b2q_comm_create": (i32, [i32, i32, i64, i64, vp, vp]),
     "b2q_comm_create_mode": (i32, [i32, i32, i64, i64, i32, vp, vp]),
     "b2q_comm_connect": (i32, [vp, vp]),

@@ -58,3 +58,12 @@ def linear_int8(codes, scale, weight, weight_scale, bias=None, out_dtype=torch.b
 def linear_int8_dynamic(x, weight, weight_scale, bias=None):
     """linear_int8(*quantize_int8(x), ...) in x's type; for a few tokens one launch."""
     return _ops.linear_dynamic(x, weight, weight_scale, bias)
+
+
+def moe_forward_int8(x, router_logits, gate_up_weight, gate_up_scale, down_weight, down_scale, top_k, renormalize=True):
+    """A whole expert layer: top_k of router_logits [T, E], silu(x W_gate) * (x W_up), down projection, weighted sum -> [T, H] in x's type.
+
+    gate_up_weight int8 [E, 2I, H] (gate rows, then up), gate_up_scale [E, 2I], down_weight int8 [E, H, I], down_scale [E, H]; x and the
+    intermediate rows are quantised to int8 per row.  Weights of the chosen experts are their softmax, renormalised over the chosen or
+    not.  Up to sixteen tokens take two kernels."""
+    return _ops.moe_forward(x, router_logits, gate_up_weight, gate_up_scale, down_weight, down_scale, top_k, renormalize)
