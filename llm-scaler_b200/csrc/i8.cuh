@@ -32,7 +32,7 @@ struct I8GroupedArgs {
 int i8_grouped_tile(int64_t rows, int E);
 int umma_i8_grouped(const I8GroupedArgs& a, cudaStream_t st);
 
-// A whole expert layer of up to sixteen tokens in two kernels (moe_i8.cu).
+// A whole expert layer of up to sixteen tokens in one kernel (moe_i8.cu).
 struct I8FewArgs {
   const void* x; bool bf16; const void* logits; int logits_dtype;
   const int8_t* w13; const void* s13; int s13_dtype; const int8_t* w2; const void* s2; int s2_dtype;
@@ -131,81 +131,87 @@ __device__ __forceinline__ float silu_mul_f(float g, float u) { return __fdivide
 // Bytes between two tokens' codes in shared memory: 64 apart in the banks, so that a quarter warp reads two tokens' 64 bytes without a conflict.
 __host__ __device__ constexpr int i8_code_pitch(int K) { return (K + 127) / 128 * 128 + 64; }
 
-// All codes of M rows x [M, ldx] into shared memory, by the first THREADS threads of a CTA, which meet() in between; tok.max is zero before,
-// K % 8 == 0.  A thread's pieces of eight stay in registers between the maximum and the codes, sixteen of them; more are read twice.
+// All codes of M rows x [M, ldx] into shared memory, by the first THREADS threads of a CTA, in three steps with a barrier of theirs between two:
+// maximum, rows, codes.  tok.max is zero before, K % 8 == 0.  A thread's pieces of eight stay in registers from the first step to the
+// last, V of them; more are read twice.
 struct I8Tokens {
   uint32_t max[I8_STREAM_MAX_TOK];
   float scale[I8_STREAM_MAX_TOK];
   I8Row row[I8_STREAM_MAX_TOK];
 };
-template <bool BF16, int THREADS, class Meet>
-__device__ __forceinline__ void i8_quantize_tokens(const uint16_t* x, int64_t ldx, int M, int K, uint8_t* codes, int pitch, I8Tokens& tok, Meet meet) {
-  constexpr int V = 16;
-  const int n8 = K >> 3, total = M * n8, lane = threadIdx.x & 31;
-  const uint32_t inv = 0xFFFFFFFFu / (uint32_t)n8 + 1;     // i / n8 = i * inv >> 32 for the sizes that fit shared memory (i < 2^17, n8 < 2^14)
-  auto token = [&](int i) { return n8 == 1 ? i : (int)__umulhi((uint32_t)i, inv); };
-  const bool once = total <= V * THREADS;
+template <bool BF16, int THREADS, int V> struct I8TokenCodes {
+  const uint16_t* x; int64_t ldx;
+  int M, n8, total;
+  uint32_t inv;                                            // i / n8 = i * inv >> 32 for the sizes that fit shared memory (i < 2^17, n8 < 2^14)
   uint4 v[V];
-  auto fetch = [&](int base) {
+  __device__ __forceinline__ I8TokenCodes(const uint16_t* x_, int64_t ldx_, int M_, int K) : x(x_), ldx(ldx_), M(M_), n8(K >> 3), total(M_ * (K >> 3)) {
+    inv = 0xFFFFFFFFu / (uint32_t)n8 + 1;
+  }
+  __device__ __forceinline__ int token(int i) const { return n8 == 1 ? i : (int)__umulhi((uint32_t)i, inv); }
+  __device__ __forceinline__ void fetch(int base = 0) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int i = base + j * THREADS + threadIdx.x, m = token(i);
       v[j] = i < total ? ld_vec(x + m * ldx + 8 * (i - m * n8)) : make_uint4(0, 0, 0, 0);
     }
-  };
-  for (int base = 0; base < total; base += V * THREADS) {
-    fetch(base);
+  }
+  __device__ __forceinline__ void maximum(I8Tokens& tok) { // behind fetch()
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base < total; base += V * THREADS) {
+      if (base) fetch(base);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int i0 = base + j * THREADS + (int)(threadIdx.x & ~31u);
-      if (i0 >= total) break;                              // whole warps
-      const uint32_t e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-      uint32_t mx = 0;
+      for (int j = 0; j < V; ++j) {
+        const int i0 = base + j * THREADS + (int)(threadIdx.x & ~31u);
+        if (i0 >= total) break;                            // whole warps
+        const uint32_t e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+        uint32_t mx = 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float a, b;
-        unpack2<BF16>(e[c], a, b);
-        mx = max(mx, max(__float_as_uint(a) & 0x7FFFFFFFu, __float_as_uint(b) & 0x7FFFFFFFu));
+        for (int c = 0; c < 4; ++c) {
+          float a, b;
+          unpack2<BF16>(e[c], a, b);
+          mx = max(mx, max(__float_as_uint(a) & 0x7FFFFFFFu, __float_as_uint(b) & 0x7FFFFFFFu));
+        }
+        const int m = token(i0);
+        if (token(i0 + 31) == m) {
+          mx = __reduce_max_sync(0xffffffffu, mx);
+          if (lane == 0) atomicMax(&tok.max[m], mx);
+        } else if (i0 + lane < total) {                    // a warp that straddles tokens
+          atomicMax(&tok.max[token(i0 + lane)], mx);
+        }
+        __syncwarp();
       }
-      const int m = token(i0);
-      if (token(i0 + 31) == m) {
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        if (lane == 0) atomicMax(&tok.max[m], mx);
-      } else if (i0 + lane < total) {                      // a warp that straddles tokens
-        atomicMax(&tok.max[token(i0 + lane)], mx);
-      }
-      __syncwarp();
     }
   }
-  meet();
-  if (threadIdx.x < M) {
-    const uint32_t bits = tok.max[threadIdx.x];
-    const float a = fmaxf(__uint_as_float(bits), I8_MIN_AMAX);
-    I8Row r = i8_row(a);
-    if (bits >= 0x7F800000u) r = I8Row{0.f, 0.f, 0.f};     // not finite
-    tok.row[threadIdx.x] = r;
-    tok.scale[threadIdx.x] = bits < 0x7F800000u ? a / 127.f : __uint_as_float(0x7FC00000u);
-  }
-  __syncwarp();
-  meet();
-  for (int base = 0; base < total; base += V * THREADS) {
-    if (!once) fetch(base);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int i = base + j * THREADS + threadIdx.x;
-      if (i >= total) break;
-      const int m = token(i);
-      const I8Row r = tok.row[m];
-      float lo[4], hi[4];
-      unpack2<BF16>(v[j].x, lo[0], lo[1]); unpack2<BF16>(v[j].y, lo[2], lo[3]); unpack2<BF16>(v[j].z, hi[0], hi[1]); unpack2<BF16>(v[j].w, hi[2], hi[3]);
-      uint2 o = make_uint2(0, 0);
-      if (r.c != 0.f) o = make_uint2(i8_codes4<false>(lo, r), i8_codes4<false>(hi, r));
-      *reinterpret_cast<uint2*>(codes + m * pitch + 8 * (i - m * n8)) = o;
+  __device__ __forceinline__ void rows(I8Tokens& tok) const {
+    if (threadIdx.x < M) {
+      const uint32_t bits = tok.max[threadIdx.x];
+      const float a = fmaxf(__uint_as_float(bits), I8_MIN_AMAX);
+      I8Row r = i8_row(a);
+      if (bits >= 0x7F800000u) r = I8Row{0.f, 0.f, 0.f};   // not finite
+      tok.row[threadIdx.x] = r;
+      tok.scale[threadIdx.x] = bits < 0x7F800000u ? a / 127.f : __uint_as_float(0x7FC00000u);
     }
+    __syncwarp();
   }
-  __syncwarp();
-  meet();
-}
+  __device__ __forceinline__ void codes(const I8Tokens& tok, uint8_t* to, int pitch) {
+    for (int base = 0; base < total; base += V * THREADS) {
+      if (total > V * THREADS) fetch(base);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int i = base + j * THREADS + threadIdx.x;
+        if (i >= total) break;
+        const int m = token(i);
+        const I8Row r = tok.row[m];
+        float lo[4], hi[4];
+        unpack2<BF16>(v[j].x, lo[0], lo[1]); unpack2<BF16>(v[j].y, lo[2], lo[3]); unpack2<BF16>(v[j].z, hi[0], hi[1]); unpack2<BF16>(v[j].w, hi[2], hi[3]);
+        uint2 o = make_uint2(0, 0);
+        if (r.c != 0.f) o = make_uint2(i8_codes4<false>(lo, r), i8_codes4<false>(hi, r));
+        *reinterpret_cast<uint2*>(to + m * pitch + 8 * (i - m * n8)) = o;
+      }
+    }
+    __syncwarp();
+  }
+};
 __device__ __forceinline__ void add_shared(int* p, int v) {
   asm volatile("red.shared.add.s32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(p)), "r"(v) : "memory");
 }

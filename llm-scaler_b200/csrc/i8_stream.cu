@@ -62,7 +62,16 @@ __global__ void __launch_bounds__(THREADS, 2) i8_stream_kernel(const Params p) {
   if (p.early) grid_dep_wait();
   __syncthreads();
 
-  if constexpr (FROM16) i8_quantize_tokens<BF16, THREADS>(p.x16, p.ldx16, p.M, p.K, codes, p.code_pitch, tok, [] { __syncthreads(); });
+  if constexpr (FROM16) {
+    I8TokenCodes<BF16, THREADS, 4> tc(p.x16, p.ldx16, p.M, p.K);
+    tc.fetch();
+    tc.maximum(tok);
+    __syncthreads();
+    tc.rows(tok);
+    __syncthreads();
+    tc.codes(tok, codes, p.code_pitch);
+    __syncthreads();
+  }
 
   int acc[R][4];
 #pragma unroll

@@ -1,22 +1,26 @@
-// A whole int8 expert layer of up to sixteen tokens in two kernels:
+// A whole int8 expert layer of up to sixteen tokens in one kernel:
 //   ids, w = top-k of the logits;  h = silu(x W_gate) * (x W_up) per (token, expert) pair;  out = sum of w * (h W_down),
 // where x and h meet the int8 weights as int8 codes with one scale per row.
 //
-// HBM-bound: the chosen experts' matrices, once.  One thread fetches them, eight or sixteen rows at a time, into a ring that fills the SM's
-// shared memory: rows that are taken whole are one contiguous run and one untiled bulk copy of exactly the rows that are wanted; pieces of
-// longer rows are TMA boxes.  Eight warps feed them to mma.sync m16n8k32 (the up to sixteen pairs of an expert are the MMA's rows, with k permuted
-// alike on both sides so that a lane reads sixteen bytes of a row at a time).  A stage is one warp's, whose sums are added up in shared
-// memory, in integers, so that no division of the work changes a bit.
+// HBM-bound: the chosen experts' matrices, once.  One CTA per SM; one thread fetches weights, eight or up to sixteen rows at a time, into a
+// ring that fills the SM's shared memory, first of the up and gate matrices, then, without a pause, of the down matrices: rows that are
+// taken whole are one contiguous run and one untiled bulk copy of exactly the rows that are wanted; pieces of longer rows are TMA boxes.
+// Eight warps feed them to mma.sync m16n8k32 (the up to sixteen pairs of an expert are the MMA's rows, with k permuted alike on both sides so
+// that a lane reads sixteen bytes of a row at a time).  A stage is one warp's, whose sums are added up in shared memory, in integers, so
+// that no division of the work changes a bit.
 //
-// Up kernel.  Every CTA routes all tokens and makes all their codes by itself, which costs less than a launch.  The columns j of all chosen
-// experts, one expert behind the other, are dealt out evenly to the column; eight columns are eight gate rows and eight up rows.  h is
-// written in fp32.  An expert's rows of h become codes as soon as its last CTA has delivered (arrivals.cuh): that one CTA does it.
-// Down kernel.  A CTA owns output columns and runs through all chosen experts, so no sum crosses CTAs: the pairs' products add up in the
-// order of the slots.  It routes the tokens again rather than wait for the up kernel to tell, and has its first weights on their way
-// before that has finished; nothing it reads there is written by a kernel that may still run (the up kernel lets it start only
-// behind its own wait).
+// Up.  Every CTA routes all tokens and makes all their codes by itself, which costs less than a launch.  The columns j of all chosen experts,
+// one expert behind the other, are dealt out evenly to the column; eight columns are eight gate rows and eight up rows.  h is written in
+// fp32.  An expert's rows of h become codes as soon as its last CTA has delivered (arrivals.cuh): that one CTA makes them and
+// raises the expert's flag.
+// Down.  A CTA owns output columns and runs through all chosen experts, so no sum crosses CTAs: the pairs' products add up in the order of
+// the slots.  The codes of h that go with a stage of weights are fetched by the warp that owns the stage, as soon as it has done with it,
+// behind the expert's flag (one thread for all stages took 580 ns per stage, 48 us with sixteen tokens).
 //
-// Every mbarrier wait is bounded; a warp that gives up still goes to the barriers where the others expect it.
+// CTAs wait for one another's flags, so the launch is cooperative.  128 experts of 2048 x 768, top-8, one / sixteen tokens: as two kernels, each
+// with its own routing and an empty ring to begin with, 23.4 / 98 us.
+//
+// Every wait is bounded; a warp that gives up still goes to the barriers where the others expect it.
 #include "arrivals.cuh"
 #include "i8.cuh"
 #include "sm100.cuh"
@@ -27,15 +31,17 @@ namespace b2q {
 using namespace sm100;
 
 namespace mi8 {
-enum { ST_UP_EMPTY = 901, ST_UP_FULL = 902, ST_DOWN_EMPTY = 903, ST_DOWN_FULL = 904, ST_DOWN_XEMPTY = 905 };
+enum { ST_EMPTY = 901, ST_UP_FULL = 902, ST_DOWN_FULL = 903, ST_FLAG = 904 };
 constexpr int WARPS = 8, WORKERS = 32 * WARPS;              // the warps that multiply
-constexpr int UP_THREADS = WORKERS + 32, DOWN_THREADS = WORKERS + 64;      // and those that fetch: weights; codes
+constexpr int THREADS = 512, W_WARP = 15;                  // and the one that fetches weights; all sixteen route
+constexpr int HELPERS = 32 * W_WARP;                       // threads that make the tokens' codes, fill tables and store
 constexpr int MAX_TOK = I8_STREAM_MAX_TOK, MAX_K = 32, MAX_PAIRS = MAX_TOK * MAX_K, MAX_E = 1024;
-constexpr int CODES_MAX = 68 * 1024;                       // bytes of the tokens' codes in the up kernel's shared memory
+constexpr int CODES_MAX = 68 * 1024;                       // bytes of the tokens' codes in shared memory
 constexpr int PASS = 16;                                   // groups of eight columns whose sums are held at a time
-constexpr int TABLE_MAX = 24 * 1024;                       // bytes of sums in the down kernel's, and of scales
+constexpr int TABLE_MAX = 24 * 1024;                       // bytes of the down part's sums, and of its scales
+constexpr int XR = 4;                                      // pairs of a down stage; an expert with more fetches its rows again, from L2
 constexpr int PIECE = 2048;                                // longest k of a stage: 256 elements of eight bytes in a TMA box
-constexpr int MAX_STAGES = 4 * WARPS, BAR_BYTES = 16 * MAX_STAGES + 16;
+constexpr int MAX_STAGES = 32, BAR_BYTES = 16 * MAX_STAGES + 16;
 constexpr int SMEM_MAX = 232448 - 1024;                    // of a CTA, static part included
 
 struct Params {
@@ -44,12 +50,14 @@ struct Params {
   const int8_t* w2; const void* s2; int s2_dt;
   uint16_t* out;
   int T, E, k, H, I, renorm;
-  float* h; int8_t* hq; float* hs;                         // [pairs, I], [pairs, I], [pairs]
-  Arrivals* counts; Arrivals tag; const Arrivals* epoch;
-  int pitch, row_cap;
-  // the ring: k and weight rows of a stage; a multiple of WARPS of them, so that a stage always comes back to the same warp (a parity wait
-  // cannot tell the phase it waits for from the one two before)
-  int piece, stage_rows, stages, stage_bytes;
+  float* h; int8_t* hq;                                    // [pairs, I]; [pairs, I + 16]: codes, then their scale
+  Arrivals *counts, *flags, *left;                         // of slots; of slots; CTAs that have seen all flags
+  Arrivals tag; const Arrivals* epoch;
+  int pitch, row_cap, front;                               // front: bytes of the codes, or of the tables that take their place
+  // The ring.  Stage s is always warp s % WARPS's (a parity wait cannot tell the phase it waits for from the one two before, so nobody may
+  // come to a stage that another has not finished).
+  int stages, stage_bytes;
+  int up_piece, down_piece, down_rows;                     // k of a stage; weight rows of a down stage
   int* status;
 };
 
@@ -63,7 +71,9 @@ struct Route {
   int16_t slot_expert[MAX_PAIRS];
   int16_t slot_first[MAX_PAIRS + 1];                       // into list
   int16_t list[MAX_PAIRS];                                 // pairs by slot
-  int slots;
+  int16_t chunk_slot[MAX_PAIRS], chunk_first[MAX_PAIRS];   // up to XR pairs of a slot each; where in list
+  int slots, chunks;
+  __device__ __forceinline__ int chunk_pairs(int c) const { return min(XR, slot_first[chunk_slot[c] + 1] - chunk_first[c]); }
 };
 
 // Larger logits have larger keys, equal ones equal keys, none has key 0.
@@ -72,13 +82,11 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// One warp: the k largest of E logits, the lowest index first among equals; softmax over all or over the chosen.  A token whose logits
+// One warp: a token's logits, and the k largest of them, the lowest index first among equals; softmax over all or over the chosen.  A token whose logits
 // hold a NaN, or have no finite maximum, goes to no expert.
-template <int PER> __device__ __forceinline__ void route_token(const Params& p, int tok, Route& r) {
+template <int PER> __device__ __forceinline__ void load_logits(const Params& p, int tok, float (&v)[PER]) {
   const int lane = threadIdx.x & 31;
   const int64_t at = (int64_t)tok * p.E;
-  float v[PER];
-  uint32_t key[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int e = lane + 32 * j;
@@ -87,6 +95,10 @@ template <int PER> __device__ __forceinline__ void route_token(const Params& p, 
       v[j] = p.ldt == B2Q_F32 ? __ldcg(reinterpret_cast<const float*>(p.logits) + at + e)
                               : scalar_from_raw(__ldcg(reinterpret_cast<const unsigned short*>(p.logits) + at + e), p.ldt);
   }
+}
+template <int PER> __device__ __forceinline__ void route_token(const Params& p, int tok, const float (&v)[PER], Route& r) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[PER];
   float mx = -INFINITY;
   bool nan = false;
 #pragma unroll
@@ -135,12 +147,13 @@ template <int PER> __device__ __forceinline__ void route_token(const Params& p, 
   }
 }
 
-// The whole CTA; barriers inside.  Which place a pair gets among its expert's is a matter of chance and changes no result.
-template <int PER> __device__ __forceinline__ void route(const Params& p, Route& r) {
+// The whole CTA.  Which place a pair gets among its expert's is a matter of chance and changes no result.  between(0) runs behind the barrier
+// that has all tokens' choices, in every warp but the first, which finds the slots; between(1) behind the one that has the slots.
+// r.first is p.T * p.k and r.count zero before, for everybody.
+template <int PER, class Between> __device__ __forceinline__ void route(const Params& p, Route& r, const float (&logits)[PER], Between between) {
+  static_assert(THREADS / 32 >= MAX_TOK, "a warp per token");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pairs = p.T * p.k;
-  for (int i = threadIdx.x; i < p.E; i += blockDim.x) { r.first[i] = pairs; r.count[i] = 0; }
-  __syncthreads();
-  for (int t = warp; t < p.T; t += blockDim.x / 32) route_token<PER>(p, t, r);
+  if (warp < p.T) route_token<PER>(p, warp, logits, r);
   __syncthreads();
   if (warp == 0) {
     int slots = 0, before = 0;
@@ -148,28 +161,33 @@ template <int PER> __device__ __forceinline__ void route(const Params& p, Route&
       const int e = b + lane < pairs ? r.expert[b + lane] : -1;
       const bool names = e >= 0 && r.first[e] == b + lane;
       const unsigned some = __ballot_sync(0xffffffffu, names);
-      const int c = names ? r.count[e] : 0;
-      int upto = c;
+      const int c = names ? r.count[e] : 0, n = (c + XR - 1) / XR;
+      int upto = c | n << 16;                              // pairs and chunks up to here
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
       }
       if (names) {
-        const int s = slots + __popc(some & ((1u << lane) - 1u));
+        const int s = slots + __popc(some & ((1u << lane) - 1u)), first = (before + upto & 0xFFFF) - c;
+        int chunk = (before + upto >> 16) - n;
         r.slot_expert[s] = (int16_t)e;
-        r.slot_first[s] = (int16_t)(before + upto - c);
+        r.slot_first[s] = (int16_t)first;
+        for (int i = 0; i < c; i += XR, ++chunk) { r.chunk_slot[chunk] = (int16_t)s; r.chunk_first[chunk] = (int16_t)(first + i); }
         r.first[e] = s;                                    // a slot is no larger than the pair that named it: nobody looks at it as one again
       }
       slots += __popc(some);
       before += __shfl_sync(0xffffffffu, upto, 31);
       __syncwarp();
     }
-    if (lane == 0) { r.slots = slots; r.slot_first[slots] = (int16_t)before; }
+    if (lane == 0) { r.slots = slots; r.slot_first[slots] = (int16_t)(before & 0xFFFF); r.chunks = before >> 16; }
+    __syncwarp();
   }
+  between(0);
   __syncthreads();
-  for (int i = threadIdx.x; i < pairs; i += blockDim.x)
+  for (int i = threadIdx.x; i < pairs; i += THREADS)
     if (r.expert[i] >= 0) r.list[r.slot_first[r.first[r.expert[i]]] + r.place[i]] = (int16_t)i;
+  between(1);
   __syncthreads();
 }
 
@@ -183,49 +201,39 @@ __device__ __forceinline__ int owner(int64_t c, int64_t n, int64_t G) {
 
 __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }      // the eight warps
 
-// Codes of an expert's rows of h, by the eight warps.  Rows of up to 8192 stay in registers between the maximum and the codes.
-__device__ __forceinline__ void quantize_rows(const Params& p, const Route& r, int slot, uint32_t* red) {
+// Codes of one row of h, by one warp.  Up to 1024 values stay in registers between the maximum and the codes.
+__device__ __forceinline__ void quantize_row(const Params& p, int pair) {
   constexpr int V = 8;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n4 = p.I >> 2;
-  const bool once = n4 <= V * WORKERS;
-  for (int i = r.slot_first[slot]; i < r.slot_first[slot + 1]; ++i) {
-    const int pair = r.list[i];
-    const float4* h = reinterpret_cast<const float4*>(p.h + (int64_t)pair * p.I);
-    float4 v[V];
-    auto fetch = [&](int base) {
+  const int lane = threadIdx.x & 31, n4 = p.I >> 2;
+  const float4* h = reinterpret_cast<const float4*>(p.h + (int64_t)pair * p.I);
+  float4 v[V];
+  auto fetch = [&](int base) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int c = base + j * WORKERS + threadIdx.x;
-        v[j] = c < n4 ? __ldcg(h + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-    };
-    uint32_t mx = 0;
-    for (int base = 0; base < n4; base += V * WORKERS) {
-      fetch(base);
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        mx = max(max(mx, __float_as_uint(v[j].x) & 0x7FFFFFFFu), max(__float_as_uint(v[j].y) & 0x7FFFFFFFu, max(__float_as_uint(v[j].z) & 0x7FFFFFFFu, __float_as_uint(v[j].w) & 0x7FFFFFFFu)));
+    for (int j = 0; j < V; ++j) {
+      const int c = base + j * 32 + lane;
+      v[j] = c < n4 ? __ldcg(h + c) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    mx = __reduce_max_sync(0xffffffffu, mx);
-    if (lane == 0) red[warp] = mx;
-    __syncwarp();
-    meet();
-    mx = __reduce_max_sync(0xffffffffu, red[lane & (WARPS - 1)]);
-    const bool finite = mx < 0x7F800000u;
-    const float a = fmaxf(__uint_as_float(mx), I8_MIN_AMAX), s = 127.f / a;
-    if (threadIdx.x == 0) p.hs[pair] = finite ? a / 127.f : __uint_as_float(0x7FC00000u);
-    uint32_t* q = reinterpret_cast<uint32_t*>(p.hq + (int64_t)pair * p.I);
-    for (int base = 0; base < n4; base += V * WORKERS) {
-      if (!once) fetch(base);
+  };
+  uint32_t mx = 0;
+  for (int base = 0; base < n4; base += V * 32) {
+    fetch(base);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int c = base + j * WORKERS + threadIdx.x;
-        const float f[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-        if (c < n4) q[c] = finite ? i8_codes4_computed(f, s) : 0u;
-      }
+    for (int j = 0; j < V; ++j)
+      mx = max(max(mx, __float_as_uint(v[j].x) & 0x7FFFFFFFu), max(__float_as_uint(v[j].y) & 0x7FFFFFFFu, max(__float_as_uint(v[j].z) & 0x7FFFFFFFu, __float_as_uint(v[j].w) & 0x7FFFFFFFu)));
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  const bool finite = mx < 0x7F800000u;
+  const float a = fmaxf(__uint_as_float(mx), I8_MIN_AMAX), s = 127.f / a;
+  uint32_t* q = reinterpret_cast<uint32_t*>(p.hq + (int64_t)pair * (p.I + 16));
+  if (lane == 0) q[n4] = __float_as_uint(finite ? a / 127.f : __uint_as_float(0x7FC00000u));
+  for (int base = 0; base < n4; base += V * 32) {
+    if (n4 > V * 32) fetch(base);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = base + j * 32 + lane;
+      const float f[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+      if (c < n4) q[c] = finite ? i8_codes4_computed(f, s) : 0u;
     }
-    __syncwarp();
-    meet();                                                // red is used again
   }
 }
 
@@ -255,42 +263,97 @@ __device__ __forceinline__ void multiply(int (&acc)[4], uint32_t w, uint32_t xa,
   for (int c = 0; c < 4; ++c) acc[c] += more[c];
 }
 
+// Sixteen weight rows, at u and v, against up to eight rows of codes at x.
+__device__ __forceinline__ void multiply16(int (&acc)[2][4], uint32_t u, uint32_t v, uint32_t x, bool has, int len) {
+  const int t16 = 16 * (threadIdx.x & 3);
+  int more[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  auto step = [&](int k, bool in) {
+    uint4 a = make_uint4(0, 0, 0, 0), b = a, c = a;
+    if (in) { b = lds(u + k); c = lds(v + k); }
+    if (in && has) a = lds(x + k);
+    mma_s8(acc[0], a.x, 0u, a.y, 0u, b.x, b.y);
+    mma_s8(acc[1], a.x, 0u, a.y, 0u, c.x, c.y);
+    mma_s8(more[0], a.z, 0u, a.w, 0u, b.z, b.w);
+    mma_s8(more[1], a.z, 0u, a.w, 0u, c.z, c.w);
+  };
+  const int whole = len & ~63;
+#pragma unroll 4
+  for (int k = 0; k < whole; k += 64) step(k, true);
+  if (whole < len) step(whole, whole + t16 < len);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) { acc[0][c] += more[0][c]; acc[1][c] += more[1][c]; }
+}
+
+// The whole warp: how many of the slots from `from` on, up to 32, have their flags raised without a gap.  At least one, or 0 after two seconds.
+__device__ __forceinline__ int wait_flags(const Arrivals* flags, int from, int slots, Arrivals mark, volatile int* abort_flag, int* status) {
+  const int slot = from + (threadIdx.x & 31);
+  const long long t0 = clock64();
+  for (;;) {
+    Arrivals v = 0;
+    if (slot < slots) asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(flags + slot) : "memory");
+    const unsigned down = ~__ballot_sync(0xffffffffu, slot < slots && v == mark);
+    if (!(down & 1u)) {
+      asm volatile("fence.proxy.async;" ::: "memory");     // what the flags stand for was written by ordinary stores and is read by bulk copies
+      return down ? __ffs(down) - 1 : 32;
+    }
+    if (__any_sync(0xffffffffu, *abort_flag || clock64() - t0 > WAIT_LIMIT_TICKS)) break;
+  }
+  if ((threadIdx.x & 31) == 0 && !*abort_flag) {
+    *abort_flag = 1;
+    atomicCAS(status, 0, (int)ST_FLAG);
+  }
+  __syncwarp();
+  return 0;
+}
+
 template <bool BF16, int PER>
-__global__ void __launch_bounds__(UP_THREADS, 1) moe_i8_up_kernel(const __grid_constant__ CUtensorMap tm_w, const Params p) {
+__global__ void __launch_bounds__(THREADS, 1) moe_i8_kernel(const __grid_constant__ CUtensorMap tm_up, const __grid_constant__ CUtensorMap tm_down, const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Route rt;
   __shared__ I8Tokens tok;
-  __shared__ uint32_t red[WARPS];
-  __shared__ int last;
-  // [ring: eight gate or up rows x piece] [codes: T x pitch] [sums of two passes: 2 x PASS x T x 16] [barriers]
+  __shared__ int done[WORKERS];                            // slots of this CTA that it is the last to deliver
+  __shared__ float code_scale[MAX_PAIRS];
+  // [ring] [codes: T x pitch; later sums: pairs x row_cap, scales: the same] [sums of two passes: 2 x PASS x T x 16] [barriers]
+  const int pairs = p.T * p.k;
   const uint32_t ring = smem_u32(smem);
   uint8_t* codes = smem + p.stages * p.stage_bytes;
-  int* sums = reinterpret_cast<int*>(codes + p.T * p.pitch);
+  int* down_sums = reinterpret_cast<int*>(codes);
+  float* down_scales = reinterpret_cast<float*>(down_sums + pairs * p.row_cap);
+  int* sums = reinterpret_cast<int*>(codes + p.front);
   const uint32_t full = smem_u32(sums + 2 * PASS * p.T * 16), empty = full + 8 * MAX_STAGES;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(sums + 2 * PASS * p.T * 16) + 16 * MAX_STAGES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
+    // full: the weights and, of a down stage, the codes
+    for (int i = 0; i < p.stages; ++i) { mbar_init(full + 8 * i, 2); mbar_init(empty + 8 * i, 1); }
     *abort_flag = 0;
     fence_barrier_init();
   }
   if (threadIdx.x < MAX_TOK) tok.max[threadIdx.x] = 0;
-  for (int i = threadIdx.x; i < 2 * PASS * p.T * 16; i += UP_THREADS) sums[i] = 0;
-  grid_dep_wait();
-  grid_dep_release();                                      // not before the wait: see the down kernel
-  route<PER>(p, rt);
-  const int64_t n = (int64_t)rt.slots * p.I;               // columns of all slots
-  const int64_t G = min((int64_t)gridDim.x, n);            // no CTA without a column
-  if (blockIdx.x >= G) return;                             // the whole CTA
-  const int64_t c0 = blockIdx.x * n / G, c1 = (blockIdx.x + 1) * n / G;
-  const int slot0 = (int)(c0 / p.I), slot1 = (int)((c1 - 1) / p.I);
+  for (int i = threadIdx.x; i < 2 * PASS * p.T * 16; i += THREADS) sums[i] = 0;
+  for (int i = threadIdx.x; i < p.E; i += THREADS) { rt.first[i] = pairs; rt.count[i] = 0; }
+  float logits[PER];
+  if (warp < p.T) load_logits<PER>(p, warp, logits);
+  I8TokenCodes<BF16, HELPERS, 10> tc(p.x, p.H, p.T, p.H);
+  if (warp < W_WARP) tc.fetch();
+  __syncthreads();
+  route<PER>(p, rt, logits, [&](int step) {
+    if (warp < W_WARP) { if (step == 0) tc.maximum(tok); else tc.rows(tok); }
+  });
+  grid_dep_release();
 
-  // groups of eight columns: those of the first slot's part, then of whole slots; the last slot's part may end early
+  // ---- this CTA's share of the up part: columns [c0, c1) of all slots' columns, as groups of eight: those of the first slot's part, then of
+  // whole slots; the last slot's part may end early ----
+  const int64_t n = (int64_t)rt.slots * p.I;
+  const int64_t G = min((int64_t)gridDim.x, n);            // CTAs that have a column
+  const bool any = blockIdx.x < G;
+  const int64_t c0 = any ? blockIdx.x * n / G : 0, c1 = any ? (blockIdx.x + 1) * n / G : 0;
+  const int slot0 = (int)(c0 / p.I), slot1 = any ? (int)((c1 - 1) / p.I) : -1;
   const int j0 = (int)(c0 - (int64_t)slot0 * p.I), per_slot = (p.I + 7) / 8;
   const int len0 = (int)min((int64_t)p.I - j0, c1 - c0), groups0 = (len0 + 7) / 8;
   const int end1 = (int)(c1 - (int64_t)slot1 * p.I);       // columns of the last slot end here
-  const int groups = slot0 == slot1 ? groups0 : groups0 + (slot1 - slot0 - 1) * per_slot + (end1 + 7) / 8;
+  const int groups = !any ? 0 : (slot0 == slot1 ? groups0 : groups0 + (slot1 - slot0 - 1) * per_slot + (end1 + 7) / 8);
   struct Group { int slot, j, n; };                        // n: valid columns
   auto group_at = [&](int i) {
     Group q;
@@ -303,34 +366,57 @@ __global__ void __launch_bounds__(UP_THREADS, 1) moe_i8_up_kernel(const __grid_c
     }
     return q;
   };
-  const int pieces = (p.H + p.piece - 1) / p.piece, per_group = 2 * pieces;      // stages of a group: its gate rows' pieces, its up rows'
+  const int up_pieces = (p.H + p.up_piece - 1) / p.up_piece, per_group = 2 * up_pieces;      // stages of a group: its gate rows' pieces, its up rows'
+  const int up_items = groups * per_group;
+  // ---- and of the down part: rows [r0, r0 + rows) of every slot's matrix ----
+  const int r0 = (int)((int64_t)blockIdx.x * p.H / gridDim.x), rows = (int)((int64_t)(blockIdx.x + 1) * p.H / gridDim.x) - r0;
+  const int sr = p.down_rows, nrg = (rows + sr - 1) / sr, down_pieces = (p.I + p.down_piece - 1) / p.down_piece;
+  const int per_chunk = nrg * down_pieces, items = up_items + rt.chunks * per_chunk;
+  const Arrivals mark = p.tag ^ *reinterpret_cast<const volatile Arrivals*>(p.epoch) << ARRIVALS_BITS;
 
-  if (warp == WARPS) {
+  if (warp == W_WARP) {
+    // ---------------- weights ----------------
     if (elect_one()) {
       int s = 0, issued = 0;
       uint32_t par = 1u;
       bool ok = true;
+      // n rows of K bytes, len of them from k on: whole rows follow one another; eight pieces are a box, zeros beyond K
+      auto put = [&](const int8_t* base, const CUtensorMap* map, int64_t row, int n, int K, int k, int piece, int pieces) {
+        const int len = min(piece, K - k);
+        const uint32_t dst = ring + s * p.stage_bytes, bar = full + 8 * s;
+        const int8_t* src = base + row * K + k;
+        if (pieces == 1) {
+          mbar_expect_tx(bar, n * len);
+          bulk_load(dst, src, n * len, bar);
+        } else if (n == 8) {
+          mbar_expect_tx(bar, 8 * piece);
+          tma_load_2d(dst, map, k / 8, (int)row, bar);
+        } else {
+          mbar_expect_tx(bar, n * len);
+          for (int r = 0; r < n; ++r) bulk_load(dst + r * piece, src + (int64_t)r * K, len, bar);
+        }
+        ++issued;
+      };
       for (int i = 0; ok && i < groups; ++i) {
         const Group q = group_at(i);
         for (int h = 0; ok && h < 2; ++h) {
           const int64_t row = (int64_t)(2 * rt.slot_expert[q.slot] + h) * p.I + q.j;
-          for (int k = 0; k < p.H; k += p.piece) {
-            ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_UP_EMPTY);
+          for (int k = 0; k < p.H; k += p.up_piece) {
+            ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_EMPTY);
             if (!ok) break;
-            const int len = min(p.piece, p.H - k);
-            const uint32_t dst = ring + s * p.stage_bytes, bar = full + 8 * s;
-            const int8_t* src = p.w13 + row * p.H + k;
-            if (pieces == 1) {                             // whole rows: they follow one another
-              mbar_expect_tx(bar, q.n * len);
-              bulk_load(dst, src, q.n * len, bar);
-            } else if (q.n == 8) {                         // a box, zeros beyond H
-              mbar_expect_tx(bar, 8 * p.piece);
-              tma_load_2d(dst, &tm_w, k / 8, (int)row, bar);
-            } else {
-              mbar_expect_tx(bar, q.n * len);
-              for (int r = 0; r < q.n; ++r) bulk_load(dst + r * p.piece, src + (int64_t)r * p.H, len, bar);
-            }
-            ++issued;
+            put(p.w13, &tm_up, row, q.n, p.H, k, p.up_piece, up_pieces);
+            mbar_arrive(full + 8 * s);                     // no codes come with it
+            if (++s == p.stages) { s = 0; par ^= 1u; }
+          }
+        }
+      }
+      for (int c = 0; ok && c < rt.chunks; ++c) {
+        const int64_t row = (int64_t)rt.slot_expert[rt.chunk_slot[c]] * p.H + r0;
+        for (int rg = 0; ok && rg < nrg; ++rg) {
+          for (int k = 0; k < p.I; k += p.down_piece) {
+            ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_EMPTY);
+            if (!ok) break;
+            put(p.w2, &tm_down, row + sr * rg, min(sr, rows - sr * rg), p.I, k, p.down_piece, down_pieces);
             if (++s == p.stages) { s = 0; par ^= 1u; }
           }
         }
@@ -339,199 +425,170 @@ __global__ void __launch_bounds__(UP_THREADS, 1) moe_i8_up_kernel(const __grid_c
     }
     return;
   }
+  tc.codes(tok, codes, p.pitch);
+  __syncwarp();
+  asm volatile("bar.sync 2, %0;" ::"n"(HELPERS) : "memory");
 
-  for (int s = slot0 + threadIdx.x; s <= slot1; s += WORKERS) arrivals_open(p.counts + s, p.tag, p.epoch);
-  i8_quantize_tokens<BF16, WORKERS>(p.x, p.H, p.T, p.H, codes, p.pitch, tok, meet);
-  const uint32_t codes_at = smem_u32(codes) + 16 * t;
-  int item = warp;                                         // stages are dealt out to the warps in turn
+  // ---------------- up: eight warps ----------------
+  // a warp's items are those of its stages: stage, then the round of the ring
+  int stage = warp, item = warp;
+  uint32_t par = 0u;
   bool ok = true;
-  for (int pass = 0, b = 0; pass < groups; pass += PASS, b ^= 1) {
-    const int here = min(PASS, groups - pass);
-    int* mine = sums + b * PASS * p.T * 16;
-    // the scales of the columns that this warp will finish, fetched under the stream: groups warp and warp + 8 of the pass
-    float sg[PASS / WARPS], su[PASS / WARPS];
+  if (warp >= p.stages || warp >= WARPS) item = items;     // none
+  auto next = [&] {
+    stage += WARPS; item += WARPS;
+    if (stage >= p.stages) { item += p.stages - stage + warp; stage = warp; par ^= 1u; }
+  };
+  if (warp < WARPS) {
+    if (threadIdx.x == 0) arrivals_open(p.left, p.tag, p.epoch);
+    for (int s = slot0 + threadIdx.x; s <= slot1; s += WORKERS) arrivals_open(p.counts + s, p.tag, p.epoch);
+    const uint32_t codes_at = smem_u32(codes) + 16 * t;
+    for (int pass = 0, b = 0; pass < groups; pass += PASS, b ^= 1) {
+      const int here = min(PASS, groups - pass);
+      int* mine = sums + b * PASS * p.T * 16;
+      // the scales of the columns that this warp will finish, fetched under the stream: groups warp and warp + 8 of the pass
+      float sg[PASS / WARPS], su[PASS / WARPS];
 #pragma unroll
-    for (int i = 0; i < PASS / WARPS; ++i) {
-      sg[i] = su[i] = 0.f;
-      if (warp + i * WARPS < here) {
+      for (int i = 0; i < PASS / WARPS; ++i) {
+        sg[i] = su[i] = 0.f;
+        if (warp + i * WARPS < here) {
+          const Group q = group_at(pass + warp + i * WARPS);
+          const int64_t at = (int64_t)rt.slot_expert[q.slot] * 2 * p.I + q.j + (lane & 7);
+          if ((lane & 7) < q.n) { sg[i] = load_scalar(p.s13, at, p.s13_dt); su[i] = load_scalar(p.s13, at + p.I, p.s13_dt); }
+        }
+      }
+      for (; item < (pass + here) * per_group; next()) {
+        const int gi = item / per_group, sub = item - gi * per_group, h = sub >= up_pieces, k0 = (sub - h * up_pieces) * p.up_piece;
+        const int slot = group_at(gi).slot, first = rt.slot_first[slot], nrows = rt.slot_first[slot + 1] - first;
+        const uint32_t xa = codes_at + (g < nrows ? rt.list[first + g] / p.k : 0) * p.pitch + k0;
+        const uint32_t xb = codes_at + (g + 8 < nrows ? rt.list[first + g + 8] / p.k : 0) * p.pitch + k0;
+        ok = ok && mbar_wait_warp(full + 8 * stage, par, abort_flag, p.status, ST_UP_FULL);
+        if (!ok) continue;
+        int acc[4] = {0, 0, 0, 0};
+        multiply(acc, ring + stage * p.stage_bytes + g * p.up_piece + 16 * t, xa, xb, g < nrows, g + 8 < nrows, min(p.up_piece, p.H - k0));
+        mbar_arrive_read(empty + 8 * stage);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int row = g + (c & 2) * 4;
+          if (row < nrows) add_shared(mine + ((gi - pass) * p.T + row) * 16 + 8 * h + 2 * t + (c & 1), acc[c]);
+        }
+      }
+      __syncwarp();
+      meet();                                              // the pass's sums are complete, and those before it have been read
+#pragma unroll
+      for (int i = 0; i < PASS / WARPS; ++i) {
+        if (warp + i * WARPS >= here) break;
         const Group q = group_at(pass + warp + i * WARPS);
-        const int64_t at = (int64_t)rt.slot_expert[q.slot] * 2 * p.I + q.j + (lane & 7);
-        if ((lane & 7) < q.n) { sg[i] = load_scalar(p.s13, at, p.s13_dt); su[i] = load_scalar(p.s13, at + p.I, p.s13_dt); }
+        const int first = rt.slot_first[q.slot], nrows = rt.slot_first[q.slot + 1] - first, col = lane & 7;
+        for (int row = lane >> 3; row < nrows; row += 4) {
+          const int pair = rt.list[first + row];
+          int* v = mine + ((warp + i * WARPS) * p.T + row) * 16 + col;
+          const float xs = tok.scale[pair / p.k];
+          if (col < q.n) p.h[(int64_t)pair * p.I + q.j + col] = silu_mul_f(i8_scaled(v[0], xs, sg[i]), i8_scaled(v[8], xs, su[i]));
+          v[0] = v[8] = 0;
+        }
       }
     }
-    for (; item < (pass + here) * per_group; item += WARPS) {
-      const int gi = item / per_group, sub = item - gi * per_group, h = sub >= pieces, k0 = (sub - h * pieces) * p.piece;
-      const int slot = group_at(gi).slot, first = rt.slot_first[slot], rows = rt.slot_first[slot + 1] - first;
-      const uint32_t xa = codes_at + (g < rows ? rt.list[first + g] / p.k : 0) * p.pitch + k0;
-      const uint32_t xb = codes_at + (g + 8 < rows ? rt.list[first + g + 8] / p.k : 0) * p.pitch + k0;
-      const int s = item % p.stages;
-      ok = ok && mbar_wait_warp(full + 8 * s, (item / p.stages) & 1, abort_flag, p.status, ST_UP_FULL);
-      if (!ok) continue;
-      int acc[4] = {0, 0, 0, 0};
-      multiply(acc, ring + s * p.stage_bytes + g * p.piece + 16 * t, xa, xb, g < rows, g + 8 < rows, min(p.piece, p.H - k0));
-      mbar_arrive_read(empty + 8 * s);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int row = g + (c & 2) * 4;
-        if (row < rows) add_shared(mine + ((gi - pass) * p.T + row) * 16 + 8 * h + 2 * t + (c & 1), acc[c]);
-      }
-    }
+    // deliver: whoever is the last of a slot makes its rows' codes, a warp each, and raises its flag
+    __threadfence();
     __syncwarp();
-    meet();                                                // the pass's sums are complete, and those before it have been read
-#pragma unroll
-    for (int i = 0; i < PASS / WARPS; ++i) {
-      if (warp + i * WARPS >= here) break;
-      const Group q = group_at(pass + warp + i * WARPS);
-      const int first = rt.slot_first[q.slot], rows = rt.slot_first[q.slot + 1] - first, col = lane & 7;
-      for (int row = lane >> 3; row < rows; row += 4) {
-        const int pair = rt.list[first + row];
-        int* v = mine + ((warp + i * WARPS) * p.T + row) * 16 + col;
-        const float xs = tok.scale[pair / p.k];
-        if (col < q.n) p.h[(int64_t)pair * p.I + q.j + col] = silu_mul_f(i8_scaled(v[0], xs, sg[i]), i8_scaled(v[8], xs, su[i]));
-        v[0] = v[8] = 0;
+    meet();
+    for (int base = slot0; base <= slot1; base += WORKERS) {
+      const int slot = base + threadIdx.x;
+      int last = 0;
+      if (slot <= slot1) {
+        last = arrivals_last(p.counts + slot, owner((int64_t)(slot + 1) * p.I - 1, n, G) - owner((int64_t)slot * p.I, n, G));
+        __threadfence();
       }
-    }
-  }
-  // deliver: whoever is the last of a slot makes its rows' codes
-  __threadfence();
-  __syncwarp();
-  meet();
-  for (int i = slot0; i <= slot1; ++i) {
-    if (threadIdx.x == 0) {
-      const int others = owner((int64_t)(i + 1) * p.I - 1, n, G) - owner((int64_t)i * p.I, n, G);
-      last = arrivals_last(p.counts + i, others);
+      done[threadIdx.x] = last;
+      __syncwarp();
+      meet();
+      int at = 0;
+      for (int i = base; i <= min(slot1, base + WORKERS - 1); ++i) {
+        if (!done[i - base]) continue;
+        for (int r = rt.slot_first[i]; r < rt.slot_first[i + 1]; ++r, ++at)
+          if ((at & (WARPS - 1)) == warp) quantize_row(p, rt.list[r]);
+      }
       __threadfence();
+      __syncwarp();
+      meet();
+      if (last && ok) asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(p.flags + slot), "l"(mark) : "memory");
+      __syncwarp();
+    }
+  }
+  __syncwarp();
+  asm volatile("bar.sync 2, %0;" ::"n"(HELPERS) : "memory");      // the tokens' codes are done with: the tables take their place
+
+  // ---------------- down ----------------
+  for (int i = threadIdx.x; i < pairs * p.row_cap; i += HELPERS) {
+    const int pair = i / p.row_cap, r = i - pair * p.row_cap, e = rt.expert[pair];
+    down_sums[i] = 0;
+    down_scales[i] = e >= 0 && r < rows ? load_scalar(p.s2, (int64_t)e * p.H + r0 + r, p.s2_dt) : 0.f;
+  }
+  __syncwarp();
+  asm volatile("bar.sync 2, %0;" ::"n"(HELPERS) : "memory");
+  int raised = 0;                                          // slots whose flags this warp has seen
+  // the codes of an item of this warp's, to the stage that it goes through
+  auto fetch = [&](int it, int at) {
+    const int chunk = (it - up_items) / per_chunk, k0 = (it - up_items - chunk * per_chunk) % down_pieces * p.down_piece;
+    while (ok && rt.chunk_slot[chunk] >= raised) {
+      const int more = wait_flags(p.flags, raised, rt.slots, mark, abort_flag, p.status);
+      ok = more > 0;
+      raised += more;
+    }
+    if (!ok) return;
+    const int first = rt.chunk_first[chunk], nx = rt.chunk_pairs(chunk);
+    const int len = min(p.down_piece, p.I - k0) + (k0 + p.down_piece >= p.I ? 16 : 0);      // the scale comes with the last piece
+    const uint32_t dst = ring + at * p.stage_bytes + sr * p.down_piece, bar = full + 8 * at;
+    if (elect_one()) {
+      mbar_expect_tx(bar, nx * len);
+      for (int r = 0; r < nx; ++r) bulk_load(dst + r * (p.down_piece + 16), p.hq + (int64_t)rt.list[first + r] * (p.I + 16) + k0, len, bar);
     }
     __syncwarp();
-    meet();
-    const bool mine = last != 0;
-    meet();
-    if (mine) quantize_rows(p, rt, i, red);
+  };
+  // the first down items of this warp's stages; later ones when the stage comes free
+  for (int s = warp; warp < WARPS && s < p.stages; s += WARPS) {
+    const int it = up_items + (s - up_items % p.stages + p.stages) % p.stages;
+    if (it < items) fetch(it, s);
   }
-}
-
-template <bool BF16, int PER>
-__global__ void __launch_bounds__(DOWN_THREADS, 1) moe_i8_down_kernel(const __grid_constant__ CUtensorMap tm_w, const Params p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ Route rt;
-  __shared__ float code_scale[MAX_PAIRS];
-  // [ring: weight rows and T rows of codes x piece] [sums: pairs x row_cap] [scales: the same] [barriers]
-  const int pairs = p.T * p.k;
-  const uint32_t ring = smem_u32(smem);
-  int* sums = reinterpret_cast<int*>(smem + p.stages * p.stage_bytes);
-  float* scales = reinterpret_cast<float*>(sums + pairs * p.row_cap);
-  const uint32_t full = smem_u32(scales + pairs * p.row_cap), empty = full + 8 * MAX_STAGES;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(scales + pairs * p.row_cap) + 16 * MAX_STAGES);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int r0 = (int)((int64_t)blockIdx.x * p.H / gridDim.x), rows = (int)((int64_t)(blockIdx.x + 1) * p.H / gridDim.x) - r0;
-
-  grid_dep_release();
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) { mbar_init(full + 8 * i, 2); mbar_init(empty + 8 * i, 1); }
-    *abort_flag = 0;
-    fence_barrier_init();
-  }
-  for (int i = threadIdx.x; i < pairs * p.row_cap; i += DOWN_THREADS) sums[i] = 0;
-  route<PER>(p, rt);
-  const int sr = p.stage_rows, nrg = (rows + sr - 1) / sr, pieces = (p.I + p.piece - 1) / p.piece;
-
-  if (warp == WARPS) {
-    // ---- weights: before the up kernel has finished ----
-    if (elect_one()) {
-      int s = 0, issued = 0;
-      uint32_t par = 1u;
-      bool ok = true;
-      for (int slot = 0; ok && slot < rt.slots; ++slot) {
-        const int64_t row0 = (int64_t)rt.slot_expert[slot] * p.H + r0;
-        for (int rg = 0; ok && rg < nrg; ++rg) {
-          const int nr = min(sr, rows - sr * rg);
-          const int8_t* src = p.w2 + (row0 + sr * rg) * p.I;
-          for (int k = 0; k < p.I; k += p.piece) {
-            ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_DOWN_EMPTY);
-            if (!ok) break;
-            const int len = min(p.piece, p.I - k);
-            const uint32_t dst = ring + s * p.stage_bytes, bar = full + 8 * s;
-            if (pieces == 1) {
-              mbar_expect_tx(bar, nr * len);
-              bulk_load(dst, src, nr * len, bar);
-            } else if (nr == 8) {
-              mbar_expect_tx(bar, 8 * p.piece);
-              tma_load_2d(dst, &tm_w, k / 8, (int)row0 + sr * rg, bar);
-            } else {
-              mbar_expect_tx(bar, nr * len);
-              for (int r = 0; r < nr; ++r) bulk_load(dst + r * p.piece, src + (int64_t)r * p.I + k, len, bar);
-            }
-            ++issued;
-            if (++s == p.stages) { s = 0; par ^= 1u; }
-          }
-        }
-      }
-      if (!ok) drain_issued(full, p.stages, issued);
-    }
-    return;
-  }
-  if (warp == WARPS + 1) {
-    // ---- the pairs' codes of the same k, which the up kernel makes ----
-    if (elect_one()) {
-      grid_dep_wait();
-      int s = 0, issued = 0;
-      uint32_t par = 1u;
-      bool ok = true;
-      for (int slot = 0; ok && slot < rt.slots; ++slot) {
-        const int first = rt.slot_first[slot], nx = rt.slot_first[slot + 1] - first;
-        for (int rg = 0; ok && rg < nrg; ++rg) {
-          for (int k = 0; k < p.I; k += p.piece) {
-            ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_DOWN_XEMPTY);
-            if (!ok) break;
-            const int len = min(p.piece, p.I - k);
-            const uint32_t dst = ring + s * p.stage_bytes + sr * p.piece, bar = full + 8 * s;
-            mbar_expect_tx(bar, nx * len);
-            for (int r = 0; r < nx; ++r) bulk_load(dst + r * p.piece, p.hq + (int64_t)rt.list[first + r] * p.I + k, len, bar);
-            ++issued;
-            if (++s == p.stages) { s = 0; par ^= 1u; }
-          }
-        }
-      }
-      if (!ok) drain_issued(full, p.stages, issued);
-    }
-    return;
-  }
-
-  for (int i = threadIdx.x; i < pairs * rows; i += WORKERS) {
-    const int pair = i / rows, r = i - pair * rows, e = rt.expert[pair];
-    scales[pair * p.row_cap + r] = e >= 0 ? load_scalar(p.s2, (int64_t)e * p.H + r0 + r, p.s2_dt) : 0.f;
-  }
-  bool ok = true;
-  const int per_slot = nrg * pieces, items = rt.slots * per_slot;
-  for (int item = warp; ok && item < items; item += WARPS) {
-    const int slot = item / per_slot, sub = item - slot * per_slot, rg = sub / pieces, k0 = (sub - rg * pieces) * p.piece;
-    const int first = rt.slot_first[slot], nx = rt.slot_first[slot + 1] - first, s = item % p.stages;
-    ok = mbar_wait_warp(full + 8 * s, (item / p.stages) & 1, abort_flag, p.status, ST_DOWN_FULL);
+  for (; ok && item < items; next()) {
+    const int chunk = (item - up_items) / per_chunk, sub = item - up_items - chunk * per_chunk, rg = sub / down_pieces, k0 = (sub - rg * down_pieces) * p.down_piece;
+    const int first = rt.chunk_first[chunk], nx = rt.chunk_pairs(chunk);
+    ok = mbar_wait_warp(full + 8 * stage, par, abort_flag, p.status, ST_DOWN_FULL);
     if (!ok) break;
-    const uint32_t w = ring + s * p.stage_bytes + g * p.piece + 16 * t, x = w + sr * p.piece;
-    const int len = min(p.piece, p.I - k0), left = rows - sr * rg;
+    const uint32_t w = ring + stage * p.stage_bytes + g * p.down_piece + 16 * t, x = ring + stage * p.stage_bytes + sr * p.down_piece + g * (p.down_piece + 16) + 16 * t;
+    const int len = min(p.down_piece, p.I - k0), left = rows - sr * rg;
     int acc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    multiply(acc[0], w, x, x + 8 * p.piece, g < nx, g + 8 < nx, len);
-    if (sr > 8 && left > 8) multiply(acc[1], w + 8 * p.piece, x, x + 8 * p.piece, g < nx, g + 8 < nx, len);
-    mbar_arrive_read(empty + 8 * s);
+    if (sr > 8 && left > 8) multiply16(acc, w, w + 8 * p.down_piece, x, g < nx, len);
+    else multiply(acc[0], w, x, 0, g < nx, false, len);
+    if (k0 + len == p.I && rg == 0 && t == 0 && g < nx) {
+      uint32_t v;
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(x + len) : "memory");
+      code_scale[rt.list[first + g]] = __uint_as_float(v);
+    }
+    mbar_arrive_read(empty + 8 * stage);
+    if (item + p.stages < items) fetch(item + p.stages, stage);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const int row = g + (c & 2) * 4, r = sr * rg + (c & 4) * 2 + 2 * t + (c & 1);
-      if (row < nx && (c & 4) * 2 + 2 * t + (c & 1) < sr && r < rows) add_shared(sums + rt.list[first + row] * p.row_cap + r, acc[c >> 2][c & 3]);
+    for (int c = 0; c < 4; ++c) {
+      const int r = 8 * (c >> 1) + 2 * t + (c & 1);
+      if (g < nx && r < sr && sr * rg + r < rows) add_shared(down_sums + rt.list[first + g] * p.row_cap + sr * rg + r, acc[c >> 1][c & 1]);
     }
   }
-  grid_dep_wait();                                         // over by now; the scales of the codes are the up kernel's
-  for (int i = threadIdx.x; i < pairs; i += WORKERS) code_scale[i] = rt.expert[i] >= 0 ? ld_f32(p.hs + i) : 0.f;
+  if (!ok && lane == 0) drain_issued(full, p.stages, item);      // copies of this warp's may be on their way
   __syncwarp();
-  meet();
-  for (int i = threadIdx.x; i < p.T * rows; i += WORKERS) {
-    const int tok = i / rows, r = i - tok * rows;
+  asm volatile("bar.sync 2, %0;" ::"n"(HELPERS) : "memory");
+  // The last CTA that has seen all flags lowers them: a graph's replays have the same mark.  (What a CTA that gave up leaves raised, the
+  // reset of the status words makes another launch's.)
+  if (threadIdx.x == 32 * WARPS && !*abort_flag && arrivals_last(p.left, gridDim.x - 1))
+    for (int i = 0; i < rt.slots; ++i) p.flags[i] = 0;
+  for (int i = threadIdx.x; i < p.T * rows; i += HELPERS) {
+    const int token = i / rows, r = i - token * rows;
     float v = 0.f;
     for (int q = 0; q < p.k; ++q) {
-      const int pair = tok * p.k + q;
-      if (rt.expert[pair] >= 0) v = fmaf(rt.weight[pair], i8_scaled(sums[pair * p.row_cap + r], code_scale[pair], scales[pair * p.row_cap + r]), v);
+      const int pair = token * p.k + q;
+      if (rt.expert[pair] >= 0) v = fmaf(rt.weight[pair], i8_scaled(down_sums[pair * p.row_cap + r], code_scale[pair], down_scales[pair * p.row_cap + r]), v);
     }
-    p.out[(int64_t)tok * p.H + r0 + r] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+    p.out[(int64_t)token * p.H + r0 + r] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
   }
 }
 
@@ -550,71 +607,72 @@ static int sm_count() {
   return sms[dev];
 }
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
-static int down_grid(int64_t H) { return (int)(sm_count() < H ? sm_count() : H); }
-static int up_fixed(int T, int pitch) { return T * pitch + 2 * PASS * T * 16 * 4 + BAR_BYTES; }
-static int down_fixed(int pairs, int cap) { return 2 * pairs * cap * 4 + BAR_BYTES; }
+static int grid_of(int64_t H) { return (int)(sm_count() < H ? sm_count() : H); }
+static int room(int fixed) { return SMEM_MAX - (int)sizeof(Route) - (int)sizeof(I8Tokens) - 4 * (WORKERS + MAX_PAIRS) - 256 - fixed; }
 
-static int room(int fixed) { return SMEM_MAX - (int)sizeof(Route) - 4 * MAX_PAIRS - 512 - fixed; }
-
-static int launch(void (*kern)(const CUtensorMap, const Params), const char* name, int grid, int threads, int fixed, const int8_t* w, int64_t rows, int K, Params& p,
-                  int* configured, cudaStream_t st) {
-  p.stages = room(fixed) / p.stage_bytes / WARPS * WARPS;
-  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-  const int smem = p.stages * p.stage_bytes + fixed;
-  CUtensorMap tm{};
-  if (p.piece < K) {
-    const int rc = make_tmap_2d(&tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 8, w, rows, K / 8, (uint64_t)K, 8, p.piece / 8, CU_TENSOR_MAP_SWIZZLE_NONE);
-    if (rc) return rc;
-  }
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 16 || configured[dev] < smem) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return B2Q_ERR_CUDA;
-    if (dev < 16) configured[dev] = smem;
-  }
-  launch_overlapped(kern, dim3(grid), dim3(threads), smem, st, tls().overlap_mode > 0, tm, p);
-  note_launch(name);
-  return launch_status();
-}
-
-// k of a stage: the whole row where a stage of that for every warp fits, else what fits (a TMA box has 2048 bytes of a row at most)
-static int piece_of(int K, int bytes_per_k, int fixed) {
-  const int fits = room(fixed) / WARPS / bytes_per_k;
+// k of a stage: the whole row where six stages of that fit, else what fits (a TMA box has 2048 bytes of a row at most)
+static int piece_of(int K, int rows, int more, int fixed) {
+  const int fits = (room(fixed) / 6 - more) / rows;
   if (K <= fits && K <= PIECE) return K;
   const int v = fits < PIECE ? fits : PIECE;
   return v / 64 * 64;
 }
 
 template <bool BF16, int PER> static int run(Params& p, cudaStream_t st) {
-  static thread_local int configured[2][16] = {{0}};
+  const int grid = grid_of(p.H), pairs = p.T * p.k, xr = p.T < XR ? p.T : XR;
   p.pitch = i8_code_pitch(p.H);
-  int fixed = up_fixed(p.T, p.pitch);
-  p.stage_rows = 8;
-  p.piece = piece_of(p.H, 8, fixed);
-  p.stage_bytes = 8 * p.piece;
-  int rc = launch(moe_i8_up_kernel<BF16, PER>, "moe_i8_up", sm_count(), UP_THREADS, fixed, p.w13, (int64_t)p.E * 2 * p.I, p.H, p, configured[0], st);
-  if (rc) return rc;
-  const int grid = down_grid(p.H);
   p.row_cap = (p.H + grid - 1) / grid;
-  fixed = down_fixed(p.T * p.k, p.row_cap);
-  // sixteen rows that are one run of memory, if there are that many and they fit; else eight
-  p.stage_rows = p.row_cap > 8 && piece_of(p.I, 16 + p.T, fixed) == p.I ? 16 : 8;
-  p.piece = piece_of(p.I, p.stage_rows + p.T, fixed);
-  p.stage_bytes = (p.stage_rows + p.T) * p.piece;
-  return launch(moe_i8_down_kernel<BF16, PER>, "moe_i8_down", grid, DOWN_THREADS, fixed, p.w2, (int64_t)p.E * p.H, p.I, p, configured[1], st);
+  const int tables = 2 * pairs * p.row_cap * 4;
+  p.front = (int)align256(p.T * p.pitch > tables ? p.T * p.pitch : tables);
+  const int fixed = p.front + 2 * PASS * p.T * 16 * 4 + BAR_BYTES;
+  p.up_piece = piece_of(p.H, 8, 0, fixed);
+  // up to sixteen rows that are one run of memory, if there are more than eight and they fit; else eight
+  const int most = p.row_cap < 16 ? p.row_cap : 16;
+  p.down_rows = p.row_cap > 8 && piece_of(p.I, most + xr, 16 * xr, fixed) == p.I ? most : 8;
+  p.down_piece = piece_of(p.I, p.down_rows + xr, 16 * xr, fixed);
+  const int up = 8 * p.up_piece, down = p.down_rows * p.down_piece + xr * (p.down_piece + 16);
+  p.stage_bytes = ((up > down ? up : down) + 127) / 128 * 128;
+  p.stages = room(fixed) / p.stage_bytes;
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  const int smem = p.stages * p.stage_bytes + fixed;
+  CUtensorMap tu{}, td{};
+  int rc = B2Q_OK;
+  if (p.up_piece < p.H)
+    rc = make_tmap_2d(&tu, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 8, p.w13, (uint64_t)p.E * 2 * p.I, p.H / 8, p.H, 8, p.up_piece / 8, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (!rc && p.down_piece < p.I)
+    rc = make_tmap_2d(&td, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 8, p.w2, (uint64_t)p.E * p.H, p.I / 8, p.I, 8, p.down_piece / 8, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (rc) return rc;
+  auto kern = moe_i8_kernel<BF16, PER>;
+  static thread_local int configured[16] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 16 || configured[dev] < smem) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return B2Q_ERR_CUDA;
+    if (dev < 16) configured[dev] = smem;
+  }
+  // No early start: CTAs that wait for one another are launched together or not at all.
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeCooperative;
+  at[0].val.cooperative = 1;
+  cfg.attrs = at; cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, tu, td, p) != cudaSuccess) return B2Q_ERR_CUDA;
+  note_launch("moe_i8");
+  return launch_status();
 }
 }  // namespace mi8
 
 bool moe_i8_few_supported(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
   using namespace mi8;
   if (T > MAX_TOK || E > MAX_E || k > MAX_K || H > INT32_MAX / 64 || I > INT32_MAX / 64) return false;
-  const int64_t cap = (H + down_grid(H) - 1) / down_grid(H);
+  const int64_t cap = (H + grid_of(H) - 1) / grid_of(H);
   return T * i8_code_pitch((int)H) <= CODES_MAX && T * k * cap * 4 <= TABLE_MAX;
 }
 
 size_t moe_i8_few_bytes(int64_t T, int64_t k, int64_t I) {
   const size_t pairs = (size_t)T * k;
-  return mi8::align256(pairs * I * 4) + mi8::align256(pairs * I) + mi8::align256(pairs * 4) + mi8::align256(pairs * 8);
+  return mi8::align256(pairs * I * 4) + mi8::align256(pairs * (I + 16)) + 2 * mi8::align256(pairs * 8) + 256;
 }
 
 int moe_i8_few(const I8FewArgs& a, cudaStream_t st) {
@@ -627,9 +685,10 @@ int moe_i8_few(const I8FewArgs& a, cudaStream_t st) {
   const size_t pairs = (size_t)a.T * a.k;
   uint8_t* at = reinterpret_cast<uint8_t*>(a.scratch);
   p.h = reinterpret_cast<float*>(at); at += align256(pairs * a.I * 4);
-  p.hq = reinterpret_cast<int8_t*>(at); at += align256(pairs * a.I);
-  p.hs = reinterpret_cast<float*>(at); at += align256(pairs * 4);
-  p.counts = reinterpret_cast<Arrivals*>(at);
+  p.hq = reinterpret_cast<int8_t*>(at); at += align256(pairs * (a.I + 16));
+  p.counts = reinterpret_cast<Arrivals*>(at); at += align256(pairs * 8);
+  p.flags = reinterpret_cast<Arrivals*>(at); at += align256(pairs * 8);
+  p.left = reinterpret_cast<Arrivals*>(at);
   p.tag = arrivals_tag();
   p.epoch = arrivals_epoch();
   p.status = umma_status_ptr();

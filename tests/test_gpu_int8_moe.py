@@ -39,8 +39,8 @@ def on_gpu(a):
     return [t.to(DEV) for t in a]
 
 
-def two_kernels(T, H):
-    """Whether the tokens' codes fit the shared memory of the two-kernel form."""
+def one_kernel(T, H):
+    """Whether the tokens' codes fit the shared memory of the one-kernel form."""
     return T <= 16 and T * ((H + 127) // 128 * 128 + 64) <= 68 * 1024
 
 
@@ -60,7 +60,7 @@ def experts_interval(h, w2, s2, dt, few):
 
 def check(out, a, k, renorm=True):
     x, logits, w13, s13, w2, s2 = a
-    few, dt = two_kernels(*x.shape), x.dtype
+    few, dt = one_kernel(*x.shape), x.dtype
     ids, w = int8.route(logits, k, renorm)
     codes, _, scale = int8.quantize_rows(x)
     lo, hi = torch.zeros(2, *out.shape, dtype=torch.float64)
@@ -90,7 +90,7 @@ def test_expert_layer(ops, T, E, k, H, I, dt):
     a = make(T, E, H, I, dt, T * E + k, sdt)
     out = ops.moe_forward_int8(*on_gpu(a), k)
     assert out.shape == (T, H) and out.dtype == dt
-    assert (ops.last_kernel() == "moe_i8_down") == two_kernels(T, H)
+    assert (ops.last_kernel() == "moe_i8") == one_kernel(T, H)
     check(out, a, k)
 
 
@@ -143,11 +143,11 @@ def test_a_layer_is_repeatable_and_a_token_does_not_see_the_others(ops):
         assert torch.equal(ops.moe_forward_int8(a[0][:n].contiguous(), a[1][:n].contiguous(), *a[2:], 6), out[:n])
 
 
-def test_few_tokens_take_two_kernels(ops):
+def test_few_tokens_take_one_kernel(ops):
     a = on_gpu(make(16, 128, 256, 128, torch.bfloat16, 1))
     before = ops.launch_count()
     ops.moe_forward_int8(*a, 8)
-    assert ops.launch_count() - before == 2 and ops.last_kernel() == "moe_i8_down"
+    assert ops.launch_count() - before == 1 and ops.last_kernel() == "moe_i8"
 
 
 @pytest.mark.parametrize("mode", [0, 1, 2])
