@@ -146,7 +146,7 @@ int b2q_moe_forward_int8(const b2q_moe_int8* m, void* workspace, size_t workspac
   if (!a.x || !a.logits || !a.w13 || !a.s13 || !a.w2 || !a.s2 || !a.out) return B2Q_ERR_NULL;
   if (!is16(a.act_dtype) || !known(a.logits_dtype) || !known(a.s13_dtype) || !known(a.s2_dtype)) return B2Q_ERR_DTYPE;
   if (a.T < 0 || a.E <= 0 || a.top_k <= 0 || a.top_k > a.E || a.H <= 0 || a.I <= 0 || a.H % 16 != 0 || a.I % 16 != 0) return B2Q_ERR_SHAPE;
-  if (a.E > 1024 || a.top_k > 32 || a.H > MAX_K || a.I > MAX_K || a.T > INT32_MAX / 32 || 2 * a.E * a.I > INT32_MAX || a.E * a.H > INT32_MAX) return B2Q_ERR_LIMIT;
+  if (a.E > 1024 || a.top_k > 32 || a.H > 32768 || a.I > MAX_K || a.T > INT32_MAX / 32 || 2 * a.E * a.I > INT32_MAX || a.E * a.H > INT32_MAX) return B2Q_ERR_LIMIT;
   if (!aligned16(a.x) || !aligned16(a.w13) || !aligned16(a.w2) || !aligned16(a.out) || !aligned_to(a.logits, dtype_bytes(a.logits_dtype)) ||
       !aligned_to(a.s13, dtype_bytes(a.s13_dtype)) || !aligned_to(a.s2, dtype_bytes(a.s2_dtype)))
     return B2Q_ERR_ALIGN;
@@ -186,9 +186,9 @@ int b2q_moe_forward_int8(const b2q_moe_int8* m, void* workspace, size_t workspac
   I8GroupedArgs d = g;
   d.xq = reinterpret_cast<int8_t*>(p.hq); d.xs = reinterpret_cast<float*>(p.hs); d.w = a.w2; d.ws = a.s2; d.ws_dtype = a.s2_dtype;
   d.out = p.y; d.N = H; d.K = I; d.gated = false;
-  rc = quantize_i8_gather(a.x, a.act_dtype, H, tok, k, off + E, reinterpret_cast<int8_t*>(p.xq), reinterpret_cast<float*>(p.xs), rows, H, st);
+  rc = quantize_i8_copies(a.x, bf16, perm, k, reinterpret_cast<int8_t*>(p.xq), reinterpret_cast<float*>(p.xs), a.T, H, st);
   if (!rc) rc = umma_i8_grouped(g, st);
-  if (!rc) rc = quantize_i8_gather(p.h, B2Q_F32, I, nullptr, 1, off + E, reinterpret_cast<int8_t*>(p.hq), reinterpret_cast<float*>(p.hs), rows, I, st);
+  if (!rc) rc = quantize_i8_some(p.h, B2Q_F32, I, off + E, reinterpret_cast<int8_t*>(p.hq), reinterpret_cast<float*>(p.hs), rows, I, st);
   if (!rc) rc = umma_i8_grouped(d, st);
   if (!rc) rc = moe_combine(p.y, p.weights, B2Q_F32, perm, a.out, a.act_dtype, a.T, k, H, 0, st);
   return rc;

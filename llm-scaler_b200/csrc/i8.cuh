@@ -45,9 +45,10 @@ int moe_i8_few(const I8FewArgs& a, cudaStream_t st);
 
 // q [M, K] codes, s [M] scales of rows of x; x_dtype B2Q_BF16 / F16 / F32.
 int quantize_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
-// row r of the output belongs to row idx[r] / div of x, or to row r without idx; rows from *n_valid on are left alone
-int quantize_i8_gather(const void* x, int x_dtype, int64_t ldx, const int32_t* idx, int div, const int32_t* n_valid, int8_t* q, float* s, int64_t rows, int K,
-                       cudaStream_t st);
+// the same for the first *n_valid of M rows, a number that only the device knows
+int quantize_i8_some(const void* x, int x_dtype, int64_t ldx, const int32_t* n_valid, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
+// the same with k copies of row r, at rows to[r * k] ... of q and s (none where that is negative); x contiguous, 16 bit, K % 16 == 0
+int quantize_i8_copies(const void* x, bool bf16, const int32_t* to, int k, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
 int silu_mul_quantize_i8(const void* gate_up, bool bf16, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
 int resadd_rmsnorm_quantize_i8(const void* hidden, const void* residual, const void* w, void* residual_out, bool bf16, float eps, int8_t* q, float* s,
                                int64_t M, int K, cudaStream_t st);

@@ -11,12 +11,13 @@
 namespace b2q {
 
 namespace i8q {
-enum { PLAIN, SILU, NORM };
+enum { PLAIN, SILU, NORM, COPIES };
 
 struct Params {
   const void* x; int64_t ldx;                              // elements
   const void* residual; const void* nw; void* residual_out; float eps;
-  const int32_t* idx; int div; const int32_t* n_valid;
+  const int32_t* n_valid;
+  const int32_t* to; int copies;                           // COPIES: where the copies of a row go
   int8_t* q; float* s; int64_t M; int K;
 };
 
@@ -47,7 +48,7 @@ template <int MODE> __device__ __forceinline__ Scale row_scale(uint32_t mx, floa
     const float a = fmaxf(__uint_as_float(mx), I8_MIN_AMAX);
     s.finite = mx < 0x7F800000u;
     s.scale = a / 127.f;
-    if constexpr (MODE == PLAIN) s.row = i8_row(a); else s.r = 127.f / a;
+    if constexpr (MODE == PLAIN || MODE == COPIES) s.row = i8_row(a); else s.r = 127.f / a;
   }
   if (!s.finite) s.scale = __uint_as_float(0x7FC00000u);
   return s;
@@ -72,6 +73,8 @@ template <int DT> struct RawPiece {
 };
 template <> struct Piece<PLAIN, B2Q_BF16> : RawPiece<B2Q_BF16> {};
 template <> struct Piece<PLAIN, B2Q_F16> : RawPiece<B2Q_F16> {};
+template <> struct Piece<COPIES, B2Q_BF16> : RawPiece<B2Q_BF16> {};
+template <> struct Piece<COPIES, B2Q_F16> : RawPiece<B2Q_F16> {};
 
 // WARP: a row per warp, V pieces per lane.  Otherwise a row per CTA, V pieces per thread.
 template <int MODE, int DT, int V, bool WARP>
@@ -83,18 +86,16 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Pa
   const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
   enter();
   if (row >= p.M) return;                                  // whole warps, or the whole CTA
-  int64_t src = row;
   if constexpr (MODE == PLAIN) {
     if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
-    if (p.idx) src = *reinterpret_cast<const volatile int32_t*>(p.idx + row) / p.div;
   }
   const int n8 = p.K >> 3;
   constexpr bool BF16 = DT == B2Q_BF16;
-  const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + src * p.ldx * (DT == B2Q_F32 ? 2 : 1);
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + row * p.ldx * (DT == B2Q_F32 ? 2 : 1);
   Piece<MODE, DT> pc[V];
   uint32_t mx = 0;
   float sum = 0.f;
-  if constexpr (MODE == PLAIN) {
+  if constexpr (MODE == PLAIN || MODE == COPIES) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = first + i * step;
@@ -183,8 +184,15 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Pa
     }
   }
   const Scale sc = row_scale<MODE>(mx, sum, p.K, p.eps);
-  if (first == 0) p.s[row] = sc.scale;
-  uint8_t* q = reinterpret_cast<uint8_t*>(p.q) + row * p.K;
+  if constexpr (MODE == COPIES) {
+    if (first < p.copies) {
+      const int32_t r = *reinterpret_cast<const volatile int32_t*>(p.to + row * p.copies + first);
+      if (r >= 0) p.s[r] = sc.scale;
+    }
+  } else {
+    if (first == 0) p.s[row] = sc.scale;
+  }
+  uint8_t* q = reinterpret_cast<uint8_t*>(p.q) + (MODE == COPIES ? 0 : row * p.K);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = first + i * step;
@@ -194,10 +202,17 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Pa
       const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
       uint2 o = make_uint2(0, 0);
       if (sc.finite) {
-        if constexpr (MODE == PLAIN) o = make_uint2(i8_codes4<DT == B2Q_F32>(lo, sc.row), i8_codes4<DT == B2Q_F32>(hi, sc.row));
+        if constexpr (MODE == PLAIN || MODE == COPIES) o = make_uint2(i8_codes4<DT == B2Q_F32>(lo, sc.row), i8_codes4<DT == B2Q_F32>(hi, sc.row));
         else o = make_uint2(i8_codes4_computed(lo, sc.r), i8_codes4_computed(hi, sc.r));
       }
-      *reinterpret_cast<uint2*>(q + 8 * c) = o;
+      if constexpr (MODE == COPIES) {
+        for (int n = 0; n < p.copies; ++n) {
+          const int32_t r = __ldcg(p.to + row * p.copies + n);
+          if (r >= 0) *reinterpret_cast<uint2*>(q + (int64_t)r * p.K + 8 * c) = o;
+        }
+      } else {
+        *reinterpret_cast<uint2*>(q + 8 * c) = o;
+      }
     }
   }
 }
@@ -210,10 +225,8 @@ __global__ void __launch_bounds__(512) quantize_i8_any_kernel(const Params p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x;
   enter();
-  int64_t src = row;
   if constexpr (MODE == PLAIN) {
     if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
-    if (p.idx) src = *reinterpret_cast<const volatile int32_t*>(p.idx + row) / p.div;
   }
   auto at = [&](const void* b, int64_t i) -> float {
     if constexpr (DT == B2Q_F32) return reinterpret_cast<const volatile float*>(b)[i];
@@ -222,8 +235,8 @@ __global__ void __launch_bounds__(512) quantize_i8_any_kernel(const Params p) {
   uint32_t mx = 0;
   float sum = 0.f;
   for (int c = threadIdx.x; c < p.K; c += 512) {
-    float v = at(p.x, src * p.ldx + c);
-    if constexpr (MODE == SILU) v = silu_mul_f(v, at(p.x, src * p.ldx + p.K + c));
+    float v = at(p.x, row * p.ldx + c);
+    if constexpr (MODE == SILU) v = silu_mul_f(v, at(p.x, row * p.ldx + p.K + c));
     if constexpr (MODE == NORM) {
       v += at(p.residual, row * p.K + c);
       sum = fmaf(v, v, sum);
@@ -243,8 +256,8 @@ __global__ void __launch_bounds__(512) quantize_i8_any_kernel(const Params p) {
   const Scale sc = row_scale<MODE>(mx, sum, p.K, p.eps);
   if (threadIdx.x == 0) p.s[row] = sc.scale;
   for (int c = threadIdx.x; c < p.K; c += 512) {
-    float v = at(p.x, src * p.ldx + c);
-    if constexpr (MODE == SILU) v = silu_mul_f(v, at(p.x, src * p.ldx + p.K + c));
+    float v = at(p.x, row * p.ldx + c);
+    if constexpr (MODE == SILU) v = silu_mul_f(v, at(p.x, row * p.ldx + p.K + c));
     if constexpr (MODE == NORM) {
       v += at(p.residual, row * p.K + c);
       store_scalar(p.residual_out, row * p.K + c, DT, v);
@@ -296,16 +309,20 @@ template <int MODE> static int run(const Params& p, int dt, bool vec, cudaStream
 static bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 }  // namespace i8q
 
-int quantize_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
+int quantize_i8_some(const void* x, int x_dtype, int64_t ldx, const int32_t* n_valid, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
   i8q::Params p{};
-  p.x = x; p.ldx = ldx; p.q = q; p.s = s; p.M = M; p.K = K;
+  p.x = x; p.ldx = ldx; p.n_valid = n_valid; p.q = q; p.s = s; p.M = M; p.K = K;
   return i8q::run<i8q::PLAIN>(p, x_dtype, aligned16(x) && i8q::aligned8(q) && ldx % 8 == 0, st);
 }
-int quantize_i8_gather(const void* x, int x_dtype, int64_t ldx, const int32_t* idx, int div, const int32_t* n_valid, int8_t* q, float* s, int64_t rows, int K,
-                       cudaStream_t st) {
-  i8q::Params p{};
-  p.x = x; p.ldx = ldx; p.idx = idx; p.div = div; p.n_valid = n_valid; p.q = q; p.s = s; p.M = rows; p.K = K;
-  return i8q::run<i8q::PLAIN>(p, x_dtype, aligned16(x) && i8q::aligned8(q) && ldx % 8 == 0, st);
+int quantize_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
+  return quantize_i8_some(x, x_dtype, ldx, nullptr, q, s, M, K, st);
+}
+int quantize_i8_copies(const void* x, bool bf16, const int32_t* to, int k, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
+  using namespace i8q;
+  if (K > 32768) return B2Q_ERR_LIMIT;
+  Params p{};
+  p.x = x; p.ldx = K; p.to = to; p.copies = k; p.q = q; p.s = s; p.M = M; p.K = K;
+  return bf16 ? run_vec<COPIES, B2Q_BF16>(p, st) : run_vec<COPIES, B2Q_F16>(p, st);
 }
 int silu_mul_quantize_i8(const void* gate_up, bool bf16, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
   i8q::Params p{};
