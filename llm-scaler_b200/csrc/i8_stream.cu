@@ -17,7 +17,9 @@ namespace b2q {
 
 namespace i8s {
 constexpr int WARPS = 8, THREADS = 32 * WARPS, LOADS = 8;
-constexpr int CODES_MAX = 96 * 1024;                       // bytes of shared memory for the codes of the 16-bit form
+// Values that the 16-bit form quantises in every CTA; beyond, a launch of its own costs less (2048 x 2048, 1 / 2 / 4 / 8 tokens 3.6 / 3.9 / 4.6 / 6.7 us
+// in one launch, where codes given beforehand take 3.1 / 3.1 / 3.1 / 3.2 and a quantiser in front 1.2 more).
+constexpr int FROM16_MAX = 8192;
 
 struct Params {
   const int8_t* xq; int64_t ldx; const float* xs;
@@ -148,22 +150,15 @@ template <int R, bool FROM16, bool BF16> static int launch(Params& p, int grid, 
   p.code_pitch = i8_code_pitch(p.K);
   const int smem = p.M * p.row_cap * 4 + (FROM16 ? p.M * p.code_pitch : 0);
   auto kern = i8_stream_kernel<R, FROM16, BF16>;
-  static thread_local int configured[16] = {0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (smem > 47 * 1024 && (dev >= 16 || configured[dev] < smem)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return B2Q_ERR_CUDA;
-    if (dev < 16) configured[dev] = smem;
-  }
   launch_overlapped(kern, dim3(grid), dim3(THREADS), smem, st, tls().overlap_mode > 0, p);
   note_launch("i8_stream");
   return launch_status();
 }
 
 template <bool FROM16, bool BF16> static int pick(Params& p, cudaStream_t st) {
-  // two CTAs per SM; more where the sums of that many rows would not fit beside the codes
+  // two CTAs per SM; more where the sums of that many rows would not fit the default shared memory beside the codes
   int grid = 2 * sm_count();
-  while ((int64_t)p.M * ((p.N + grid - 1) / grid) * 4 > 64 * 1024) grid *= 2;
+  while ((int64_t)p.M * ((p.N + grid - 1) / grid + 4) * 4 > 24 * 1024) grid *= 2;
   if (grid > p.N) grid = p.N;
   const int rows = (p.N + grid - 1) / grid;
   if (rows <= 8) return launch<1, FROM16, BF16>(p, grid, st);
@@ -173,7 +168,7 @@ template <bool FROM16, bool BF16> static int pick(Params& p, cudaStream_t st) {
 }  // namespace i8s
 
 bool i8_stream_supported(const I8LinearArgs& a) {
-  return a.M <= I8_STREAM_MAX_TOK && (!a.x16 || (a.M * i8_code_pitch(a.K) <= i8s::CODES_MAX && aligned16(a.x16) && a.ldx16 % 8 == 0));
+  return a.M <= I8_STREAM_MAX_TOK && (!a.x16 || ((int64_t)a.M * a.K <= i8s::FROM16_MAX && aligned16(a.x16) && a.ldx16 % 8 == 0));
 }
 
 int i8_stream_linear(const I8LinearArgs& a, cudaStream_t st) {

@@ -8,7 +8,7 @@
 //
 // Three forms of one kernel, persistent but for the second:
 //  * one CTA per tile; two accumulators, so that a tile is drained and stored while the next one is multiplied;
-//  * SPLIT: a cluster of up to eight CTAs per tile, each with a share of k.  The partial sums meet in distributed shared memory; being
+//  * SPLIT: a cluster of two or four CTAs per tile, each with a share of k.  The partial sums meet in distributed shared memory; being
 //    integers, they add up to the same whatever the division.  For layers of few rows, whose tiles would leave SMs idle;
 //  * PAIR: two CTAs share a tile of 256 x 256 (cta_group::2), each loading 128 tokens and 128 weight rows.  A CTA then pulls 64 bytes
 //    per cycle of MMA through L2 where a tile of its own would take 96.
@@ -99,12 +99,12 @@ __device__ __forceinline__ void stage_rows(uint32_t stg, int lane, const uint32_
   for (int q = 0; q < 4; ++q) sts128(stg + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
   __syncwarp();
 }
-__device__ __forceinline__ void store_rows(uint32_t stg, int lane, int rows, uint8_t* out, int64_t pitch) {
+__device__ __forceinline__ void store_rows(uint32_t stg, int lane, int rows, int bytes, uint8_t* out, int64_t pitch) {      // bytes: of a row, of 64
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int rr = i * 8 + (lane >> 2), q = lane & 3;
     const uint4 v = lds128v(stg + rr * 64 + ((q ^ ((rr >> 1) & 3)) << 4));
-    if (rr < rows) *reinterpret_cast<uint4*>(out + rr * pitch + q * 16) = v;
+    if (rr < rows && 16 * q < bytes) *reinterpret_cast<uint4*>(out + rr * pitch + q * 16) = v;
   }
 }
 }  // namespace ui8
@@ -303,8 +303,8 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
             for (int i = 0; i < 16; ++i)
               r[i] = __float_as_uint(silu_mul_f(i8_scaled((int)r[i], xs, sc[c + i]), i8_scaled((int)u[i], xs, us[c + i])));
             stage_rows(stg, lane, r);
-            if (c + 16 <= t.cols) {
-              store_rows(stg, lane, t.rows - row0, reinterpret_cast<uint8_t*>(out + c), p.ldo * 4);
+            if (p.vec_out && (t.cols - c) % 4 == 0) {
+              store_rows(stg, lane, t.rows - row0, (t.cols - c) * 4, reinterpret_cast<uint8_t*>(out + c), p.ldo * 4);
             } else {
               for (int rr = 0; rr < 32 && row0 + rr < t.rows; ++rr) {
                 const int i = lane & 15;
@@ -327,8 +327,8 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
               o[i] = pack_out(v0, v1, p.out_bf16);
             }
             stage_rows(stg, lane, o);
-            if (p.vec_out && c + 32 <= t.cols) {
-              store_rows(stg, lane, t.rows - row0, reinterpret_cast<uint8_t*>(out + c), p.ldo * 2);
+            if (p.vec_out && (t.cols - c) % 8 == 0) {
+              store_rows(stg, lane, t.rows - row0, (t.cols - c) * 2, reinterpret_cast<uint8_t*>(out + c), p.ldo * 2);
             } else {
               for (int rr = 0; rr < 32 && row0 + rr < t.rows; ++rr) {
                 const int q = lane >> 3;
@@ -456,32 +456,38 @@ static int launch(int kps, const CUtensorMap& tx, const CUtensorMap& tw, Params&
 // stage: 8 x 5120 x 5120, 48 rows, 9.1 / 8.0 / 8.0 us; 64 x 4096 x 4096, 32 rows, 7.8 / 6.9 / 7.3; 8 x 17408 x 5120, 128 rows, 16.0 / 16.5).
 static int boxes_per_stage(int h) { return h <= 64 ? 2 : 1; }
 
-// How a dense launch is divided: weight rows per tile, CTAs per tile, or pairs of CTAs with tiles of 256 x 256, by estimated nanoseconds.
-// A tile's 128 k cost what its boxes take out of L2 (160 bytes per ns and SM) or 90 ns, the whole launch at least what the weights take
-// out of DRAM; a split tile 2 us more, for the meeting of its partial sums (128 x 4096 x 14336: 32 rows 17.8 us, 64 rows on two CTAs
-// 16.9; 64 x 4096 x 4096: 6.9 and 8.3).  Clusters of four and eight do not fit on all SMs: 37 of four took two rounds, 32 one.
+// How a dense launch is divided: weight rows per tile, CTAs per tile, or pairs of CTAs with tiles of 256 x 256, by a fitted time in ns.
+// A tile's 128 k cost 0.45 ns per token row of its box and 1.55 per weight row, 90 at least (a pair's 365), and 1.2 and 0.3 more where K is no
+// multiple of 128, so that a row of a box lies in two lines; its outputs 0.1 each, behind the next tile's k but for the last; a launch
+// 3500, another round 500; the meeting of a split tile's sums 1800 and 0.22 per output; and all of it at least what the bytes take out of
+// DRAM.  Over 70 shapes of 17 to 4096 tokens the choice took 1.02 times as long as the best division tried (16 x 1024 x 8192: one / two / four CTAs per
+// tile 9.6 / 8.0 / 6.8 us, 256 x 4096 x 4096: 8.5 / 11.2 / 16.3, 1024 x 4096 x 14336: 49.0 alone, 42.1 in pairs).  Eight CTAs per tile lost everywhere;
+// of clusters of four 32 fit the SMs at a time, not 37.
 struct Plan { int h, split; bool pair; };
-static Plan plan(int M, int N, int nkb, int tok_box) {
-  const int sms = sm_count(), m_tiles = (M + 127) / 128;
+static Plan plan(int M, int N, int K, int tok_box) {
+  const int sms = sm_count(), nkb = (K + 127) / 128, m_tiles = (M + 127) / 128, rows = M < 128 ? M : 128;
   Plan best{256, 1, false};
   double least = 1e30;
-  const double dram = (double)N * nkb * 128 / 6300;
-  for (int split = 1; split <= 8 && 2 * split <= nkb; split *= 2) {
-    const int slots = split <= 2 ? sms / split : (split == 4 ? sms * 7 / 32 : sms / 9);
+  const double dram = ((double)N * nkb * 128 + (double)M * nkb * 128 + 2.0 * M * N) / 6300;
+  for (int split = 1; split <= 4 && 2 * split <= nkb; split *= 2) {
+    const int slots = split == 4 ? sms * 7 / 32 : sms / split;
     for (int rounds = 1; rounds <= (split > 1 ? 1 : 8); ++rounds) {
       const int strips = slots * rounds / m_tiles;
       if (strips == 0) continue;
-      int h = round_up((N + strips - 1) / strips, 16);
+      const int h = round_up((N + strips - 1) / strips, 16);
       if (h > 256) continue;
-      const double ns = fmax(dram, rounds * ((nkb + split - 1) / split) * fmax(90.0, (h + tok_box) * 128 / 160.0)) + rounds * 700 + (split > 1 ? 2000 : 0);
+      const double k128 = fmax(90, 0.45 * tok_box + 1.55 * h) + (K % 128 ? 1.2 * tok_box + 0.3 * h : 0), drain = 0.1 * rows * h;
+      double ns = fmax(dram, rounds * fmax(drain, (nkb + split - 1) / split * k128)) + 500.0 * (rounds - 1) + drain;
+      if (split > 1) ns += 1800 + 0.22 * rows * h;
       if (ns < least) { least = ns; best = Plan{h, split, false}; }
     }
   }
   if (M > 128) {
     const int rounds = ((M + 255) / 256 * ((N + 255) / 256) + sms / 2 - 1) / (sms / 2);
-    const double ns = fmax(dram, rounds * nkb * 330.0) + rounds * 300 + 1000;
-    if (ns < least) best = Plan{256, 1, true};
+    const double ns = fmax(dram, rounds * fmax(3300, nkb * 365.0)) + 500.0 * (rounds - 1) + 3300;
+    if (ns < least) { least = ns; best = Plan{256, 1, true}; }
   }
+  if (least >= 1e30) best.pair = M > 128;                  // more tiles than eight rounds hold
   return best;
 }
 }  // namespace ui8
@@ -499,7 +505,7 @@ int umma_i8_linear(const I8LinearArgs& a, cudaStream_t st) {
   if (!p.status) return B2Q_ERR_CUDA;
   const int sms = sm_count();
   p.tok_box = a.M <= 16 ? 16 : (a.M <= 32 ? 32 : (a.M <= 64 ? 64 : 128));
-  const Plan pl = plan(a.M, a.N, nkb, p.tok_box);
+  const Plan pl = plan(a.M, a.N, a.K, p.tok_box);
   const bool pair = pl.pair;
   CUtensorMap tx, tw;
   p.h = pl.h; p.split = pl.split; p.tok_rows = pair ? 256 : 128;
