@@ -78,7 +78,7 @@ template <> struct Piece<COPIES, B2Q_F16> : RawPiece<B2Q_F16> {};
 
 // WARP: a row per warp, V pieces per lane.  Otherwise a row per CTA, V pieces per thread.
 template <int MODE, int DT, int V, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) quantize_i8_kernel(const Params p) {
+__global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i8_kernel(const Params p) {
   __shared__ uint32_t red_max[32];
   __shared__ float red_sum[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -288,9 +288,19 @@ template <int MODE, int DT> static int run_vec(const Params& p, cudaStream_t st)
     return launch(quantize_i8_kernel<MODE, DT, 4, true>, grid, 256, st, p);
   }
   auto block = [&](int v) { return (n8 + 32 * v - 1) / (32 * v) * 32; };
-  const bool few = p.M <= 148;                             // one CTA per SM at most: as many threads as a row gives work to
-  if (few ? n8 <= 1024 : n8 <= 256) return launch(quantize_i8_kernel<MODE, DT, 1, false>, p.M, block(1), st, p);
-  if (few ? n8 <= 2048 : n8 <= 1024) return launch(quantize_i8_kernel<MODE, DT, 2, false>, p.M, block(2), st, p);
+  // one CTA per SM at most: as many threads as a row gives work to
+  if (p.M <= 148) {
+    if (n8 <= 1024) return launch(quantize_i8_kernel<MODE, DT, 1, false>, p.M, block(1), st, p);
+    if (n8 <= 2048) return launch(quantize_i8_kernel<MODE, DT, 2, false>, p.M, block(2), st, p);
+    return launch(quantize_i8_kernel<MODE, DT, 4, false>, p.M, block(4), st, p);
+  }
+  // Many rows: smaller CTAs with more in flight each.  Stored rows of 2047 x 8192 with two / four / eight pieces a thread 11.8 / 12.0 / 10.4 us (4.8
+  // TB/s), 2048 x 28672 with four / eight 52.5 / 33.4 (5.3 TB/s), 4096 x 2048 with one / two / eight 7.2 / 6.4 / 6.8; the other forms hold floats, and
+  // eight pieces of those do not fit the registers: norm 2047 x 8192 with two / four 21.5 / 19.7, 4096 x 5120 23.6 / 24.4, SiLU 20.1 / 18.8 and 22.7 / 22.4.
+  if constexpr (MODE == PLAIN || MODE == COPIES) {
+    if (n8 > 256) return launch(quantize_i8_kernel<MODE, DT, 8, false>, p.M, block(8), st, p);
+  }
+  if (n8 <= 768) return launch(quantize_i8_kernel<MODE, DT, 2, false>, p.M, block(2), st, p);
   return launch(quantize_i8_kernel<MODE, DT, 4, false>, p.M, block(4), st, p);
 }
 
