@@ -28,10 +28,9 @@ int linear_check(const I8LinearArgs& a, int64_t M, int64_t N, int64_t K) {
   if (!aligned16(a.w) || !aligned_to(a.out, 2) || !aligned_to(a.bias, 2) || !aligned_to(a.ws, dtype_bytes(a.ws_dtype))) return B2Q_ERR_ALIGN;
   return B2Q_OK;
 }
-// Up to sixteen tokens and 20 Mi weights: straight from global memory (1 / 16 tokens, 2048 x 2048 3.1 / 3.5 us against 4.3 / 4.8 on tcgen05, 4096 x
-// 4096 5.2 / 5.8 against 6.7 / 6.6, 2048 x 8192 6.4 / 8.2 against 7.8 / 8.2); more weights want the deeper ring (5120 x 5120 9.0 / 9.7 and
-// 7.9 / 8.4, 17408 x 5120 19.4 / 22.4 and 15.6 / 16.0).  set_force_kernel(2): tcgen05 for everything.
-bool use_stream(const I8LinearArgs& a) { return a.M <= I8_STREAM_MAX_TOK && (int64_t)a.N * a.K <= (int64_t)20 << 20 && tls().force_kernel != 2; }
+// set_force_kernel(2): tcgen05 for everything
+bool use_stream(const I8LinearArgs& a) { return tls().force_kernel != 2 && i8_stream_preferred(a.M, a.N, a.K); }
+bool use_from16(int64_t M, int64_t N, int64_t K) { return tls().force_kernel != 2 && i8_stream_from16(M, N, K); }
 }  // namespace
 
 extern "C" {
@@ -83,7 +82,7 @@ int b2q_linear_int8(const int8_t* q, int64_t ldq, const float* scale, const int8
 
 size_t b2q_linear_int8_dynamic_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  // also where one launch does without: rows that are not 16-byte aligned go through the quantiser whatever their number
+  if (use_from16(M, N, K)) return 0;
   return align_up((size_t)M * (size_t)K, 256) + align_up((size_t)M * 4, 256);
 }
 
@@ -99,7 +98,7 @@ int b2q_linear_int8_dynamic(const void* x, int act_dtype, int64_t ldx, const int
   if (ldx < K) return B2Q_ERR_SHAPE;
   if (!aligned_to(x, 2)) return B2Q_ERR_ALIGN;
   if (M == 0 || N == 0) return B2Q_OK;
-  if (use_stream(a) && i8_stream_supported(a)) return i8_stream_linear(a, (cudaStream_t)stream);
+  if (use_from16(M, N, K)) return i8_stream_linear(a, (cudaStream_t)stream);
   if (!workspace) return B2Q_ERR_NULL;
   if (!aligned16(workspace)) return B2Q_ERR_ALIGN;
   if (workspace_bytes < b2q_linear_int8_dynamic_workspace_bytes(M, N, K)) return B2Q_ERR_WORKSPACE;

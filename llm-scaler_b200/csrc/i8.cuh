@@ -18,7 +18,8 @@ struct I8LinearArgs {
   void* out; int64_t ldo; bool out_bf16;
   int M, N, K;
 };
-bool i8_stream_supported(const I8LinearArgs& a);           // of the 16-bit form: whether its codes fit the CTA's shared memory
+bool i8_stream_from16(int64_t M, int64_t N, int64_t K);    // whether the 16-bit form is worth its quantising in every CTA
+bool i8_stream_preferred(int64_t M, int64_t N, int64_t K);
 int i8_stream_linear(const I8LinearArgs& a, cudaStream_t st);
 int umma_i8_linear(const I8LinearArgs& a, cudaStream_t st);
 
@@ -59,6 +60,11 @@ int resadd_rmsnorm_quantize_i8(const void* hidden, const void* residual, const v
 __device__ __forceinline__ uint4 ld_vec(const void* p) {
   uint4 v;
   asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_u16(const uint16_t* p) {
+  unsigned short v;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
   return v;
 }
 __device__ __forceinline__ float ld_f32(const float* p) {
@@ -142,10 +148,12 @@ struct I8Tokens {
 };
 template <bool BF16, int THREADS, int V> struct I8TokenCodes {
   const uint16_t* x; int64_t ldx;
+  bool vec;                                                // rows are 16-byte aligned
   int M, n8, total;
   uint32_t inv;                                            // i / n8 = i * inv >> 32 for the sizes that fit shared memory (i < 2^17, n8 < 2^14)
   uint4 v[V];
   __device__ __forceinline__ I8TokenCodes(const uint16_t* x_, int64_t ldx_, int M_, int K) : x(x_), ldx(ldx_), M(M_), n8(K >> 3), total(M_ * (K >> 3)) {
+    vec = ((reinterpret_cast<uintptr_t>(x_) | (uintptr_t)(2 * ldx_)) & 15u) == 0;
     inv = 0xFFFFFFFFu / (uint32_t)n8 + 1;
   }
   __device__ __forceinline__ int token(int i) const { return n8 == 1 ? i : (int)__umulhi((uint32_t)i, inv); }
@@ -153,7 +161,12 @@ template <bool BF16, int THREADS, int V> struct I8TokenCodes {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int i = base + j * THREADS + threadIdx.x, m = token(i);
-      v[j] = i < total ? ld_vec(x + m * ldx + 8 * (i - m * n8)) : make_uint4(0, 0, 0, 0);
+      const uint16_t* at = x + m * ldx + 8 * (i - m * n8);
+      v[j] = make_uint4(0, 0, 0, 0);
+      if (i < total) {
+        if (vec) v[j] = ld_vec(at);
+        else v[j] = make_uint4(ld_u16(at) | ld_u16(at + 1) << 16, ld_u16(at + 2) | ld_u16(at + 3) << 16, ld_u16(at + 4) | ld_u16(at + 5) << 16, ld_u16(at + 6) | ld_u16(at + 7) << 16);
+      }
     }
   }
   __device__ __forceinline__ void maximum(I8Tokens& tok) { // behind fetch()

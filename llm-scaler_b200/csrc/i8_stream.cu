@@ -167,9 +167,11 @@ template <bool FROM16, bool BF16> static int pick(Params& p, cudaStream_t st) {
 }
 }  // namespace i8s
 
-bool i8_stream_supported(const I8LinearArgs& a) {
-  return a.M <= I8_STREAM_MAX_TOK && (!a.x16 || ((int64_t)a.M * a.K <= i8s::FROM16_MAX && aligned16(a.x16) && a.ldx16 % 8 == 0));
-}
+// Up to sixteen tokens and 20 Mi weights: straight from global memory (1 / 16 tokens, 2048 x 2048 3.1 / 3.5 us against 4.3 / 4.8 on tcgen05, 4096 x
+// 4096 5.2 / 5.8 against 6.7 / 6.6, 2048 x 8192 6.4 / 8.2 against 7.8 / 8.2); more weights want the deeper ring (5120 x 5120 9.0 / 9.7 and
+// 7.9 / 8.4, 17408 x 5120 19.4 / 22.4 and 15.6 / 16.0).
+bool i8_stream_preferred(int64_t M, int64_t N, int64_t K) { return M <= I8_STREAM_MAX_TOK && N * K <= (int64_t)20 << 20; }
+bool i8_stream_from16(int64_t M, int64_t N, int64_t K) { return i8_stream_preferred(M, N, K) && M * K <= i8s::FROM16_MAX; }
 
 int i8_stream_linear(const I8LinearArgs& a, cudaStream_t st) {
   i8s::Params p{};

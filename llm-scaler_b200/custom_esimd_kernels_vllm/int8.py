@@ -13,7 +13,17 @@ _PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libb2q_int8.so
 if not os.path.exists(_PATH):
     raise ImportError("b2q: %s is missing; build it with `python llm-scaler_b200/build.py`" % _PATH)
 torch.ops.load_library(_PATH)
-_ops = torch.ops.b2q_int8
+
+
+class _Ops:
+    """The ops' only overloads, looked up once: a call is worth a few microseconds."""
+
+    def __init__(self):
+        for name in ("quantize", "silu_mul_quantize", "resadd_rmsnorm_quantize", "linear", "linear_dynamic", "moe_forward"):
+            setattr(self, name, getattr(torch.ops.b2q_int8, name).default)
+
+
+_ops = _Ops()
 
 if os.environ.get("B2Q_CHECK_STATUS") == "1":
     # debugging, as for the other ops: every call synchronises and raises if a bounded device-side wait has expired
