@@ -10,7 +10,7 @@
 //  * one CTA per tile; two accumulators, so that a tile is drained and stored while the next one is multiplied;
 //  * SPLIT: a cluster of two or four CTAs per tile, each with a share of k.  The partial sums meet in distributed shared memory; being
 //    integers, they add up to the same whatever the division.  For layers of few rows, whose tiles would leave SMs idle;
-//  * PAIR: two CTAs share a tile of 256 x 256 (cta_group::2), each loading 128 tokens and 128 weight rows.  A CTA then pulls 64 bytes
+//  * PAIR: two CTAs share a tile of 256 tokens and up to 256 weight rows (cta_group::2), each loading half of either.  A CTA then pulls 64 bytes
 //    per cycle of MMA through L2 where a tile of its own would take 96.
 // GATED (grouped, expert up projection): half of a tile's columns are gate rows, half the up rows of the same outputs, and the epilogue
 // stores silu(gate) * up.
@@ -154,7 +154,7 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
     // ---- weights; boxes that begin beyond K read as zero ----
     if (elect_one()) {
       tma_prefetch_desc(&tm_w);
-      const int box = PAIR ? 128 : (GATED ? p.h / 2 : p.h);
+      const int box = PAIR || GATED ? p.h / 2 : p.h;
       const uint32_t bytes = (uint32_t)(p.stage_bytes - p.a_bytes) * (PAIR ? 2u : 1u);
       int s = 0, issued = 0;
       uint32_t par = 1u;
@@ -172,7 +172,7 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
           for (int i = 0; i < KPS; ++i) {
             const int k = (ks * KPS + i) * 128;
             if constexpr (PAIR) {
-              tma_load_2d_pair(dst + i * 16384, &tm_w, k, t.w0 + (int)rank * 128, map_to_cta(full + 8 * s, 0));
+              tma_load_2d_pair(dst + i * box * 128, &tm_w, k, t.w0 + (int)rank * box, map_to_cta(full + 8 * s, 0));
             } else {
               tma_load_2d(dst + i * p.h * 128, &tm_w, k, t.w0, full + 8 * s);
               if constexpr (GATED) tma_load_2d(dst + i * p.h * 128 + box * 128, &tm_w, k, t.w1, full + 8 * s);
@@ -216,7 +216,7 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
   } else if (warp == 1) {
     if ((!PAIR || rank == 0) && elect_one()) {
       const uint32_t idesc = instr_desc_i8(1u, 1u, PAIR ? 256u : 128u, (uint32_t)p.h);
-      const uint64_t x_step = (uint64_t)(PAIR ? 128 : p.tok_box) * 8, w_step = (uint64_t)(PAIR ? 128 : p.h) * 8;      // from box to box, in 16 bytes
+      const uint64_t x_step = (uint64_t)(PAIR ? 128 : p.tok_box) * 8, w_step = (uint64_t)(PAIR ? p.h / 2 : p.h) * 8;      // from box to box, in 16 bytes
       int s = 0, it = 0;
       uint32_t par = 0u;
       bool ok = true;
@@ -294,38 +294,54 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
           // sixteen outputs in fp32 at a time
           float* out = reinterpret_cast<float*>(p.out) + (int64_t)(t.tok0 + row0) * p.ldo + t.n0;
           const float* us = sc + p.h / 2;
-          for (int c = half * 16; row0 < t.rows && c < t.cols; c += 32) {
-            uint32_t r[16], u[16];
+          const int end = row0 < t.rows ? t.cols : 0;
+          uint32_t r[16], u[16], v[16];
+          auto fetch = [&](int c) {
             tmem_ld16(acc + c, r);
             tmem_ld16(acc + p.h / 2 + c, u);
+          };
+          if (half * 16 < end) fetch(half * 16);
+          for (int c = half * 16; c < end; c += 32) {
             tmem_ld_wait();
+            const float4* g4 = reinterpret_cast<const float4*>(sc + c);
+            const float4* u4 = reinterpret_cast<const float4*>(us + c);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              r[i] = __float_as_uint(silu_mul_f(i8_scaled((int)r[i], xs, sc[c + i]), i8_scaled((int)u[i], xs, us[c + i])));
-            stage_rows(stg, lane, r);
+            for (int i = 0; i < 4; ++i) {
+              const float4 gs = g4[i], uv = u4[i];
+              const float gv[4] = {gs.x, gs.y, gs.z, gs.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                v[4 * i + j] = __float_as_uint(silu_mul_f(i8_scaled((int)r[4 * i + j], xs, gv[j]), i8_scaled((int)u[4 * i + j], xs, uw[j])));
+            }
+            if (c + 32 < end) fetch(c + 32);               // on its way while these are stored
+            stage_rows(stg, lane, v);
             if (p.vec_out && (t.cols - c) % 4 == 0) {
               store_rows(stg, lane, t.rows - row0, (t.cols - c) * 4, reinterpret_cast<uint8_t*>(out + c), p.ldo * 4);
             } else {
               for (int rr = 0; rr < 32 && row0 + rr < t.rows; ++rr) {
                 const int i = lane & 15;
-                uint32_t v;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(stg + rr * 64 + (((i >> 2) ^ ((rr >> 1) & 3)) << 4) + (i & 3) * 4) : "memory");
-                if (lane < 16 && c + i < t.cols) out[rr * p.ldo + c + i] = __uint_as_float(v);
+                uint32_t w;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(stg + rr * 64 + (((i >> 2) ^ ((rr >> 1) & 3)) << 4) + (i & 3) * 4) : "memory");
+                if (lane < 16 && c + i < t.cols) out[rr * p.ldo + c + i] = __uint_as_float(w);
               }
             }
           }
         } else {
           uint16_t* out = p.out + (int64_t)(t.tok0 + row0) * p.ldo + t.n0;
-          for (int c = half * 32; row0 < t.rows && c < t.cols; c += 64) {
-            uint32_t r[32], o[16];
-            tmem_ld32(acc + c, r);
+          const int end = row0 < t.rows ? t.cols : 0;
+          uint32_t r[32], o[16];
+          if (half * 32 < end) tmem_ld32(acc + half * 32, r);
+          for (int c = half * 32; c < end; c += 64) {
             tmem_ld_wait();
+            const float4* s4 = reinterpret_cast<const float4*>(sc + c);
+            const float4* b4 = reinterpret_cast<const float4*>(bi + c);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float v0 = i8_output((int)r[2 * i], xs, sc[c + 2 * i], bi[c + 2 * i]);
-              const float v1 = i8_output((int)r[2 * i + 1], xs, sc[c + 2 * i + 1], bi[c + 2 * i + 1]);
-              o[i] = pack_out(v0, v1, p.out_bf16);
+            for (int i = 0; i < 8; ++i) {
+              const float4 sv = s4[i], bv = p.bias ? b4[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+              o[2 * i] = pack_out(i8_output((int)r[4 * i], xs, sv.x, bv.x), i8_output((int)r[4 * i + 1], xs, sv.y, bv.y), p.out_bf16);
+              o[2 * i + 1] = pack_out(i8_output((int)r[4 * i + 2], xs, sv.z, bv.z), i8_output((int)r[4 * i + 3], xs, sv.w, bv.w), p.out_bf16);
             }
+            if (c + 64 < end) tmem_ld32(acc + c + 64, r);  // on its way while this chunk is stored
             stage_rows(stg, lane, o);
             if (p.vec_out && (t.cols - c) % 8 == 0) {
               store_rows(stg, lane, t.rows - row0, (t.cols - c) * 2, reinterpret_cast<uint8_t*>(out + c), p.ldo * 2);
@@ -412,7 +428,7 @@ static int round_up(int v, int a) { return (v + a - 1) / a * a; }
 template <int KPS, bool PAIR, bool SPLIT, bool GROUPED, bool GATED>
 static int launch_form(const CUtensorMap& tx, const CUtensorMap& tw, Params& p, int grid, cudaStream_t st) {
   p.a_bytes = KPS * p.tok_box * 128;
-  p.stage_bytes = p.a_bytes + KPS * (PAIR ? 128 : p.h) * 128;
+  p.stage_bytes = p.a_bytes + KPS * (PAIR ? p.h / 2 : p.h) * 128;
   const int over = p.tok_box < 128 ? OVERREAD : 0, room = SMEM_MAX - 1024 - TAIL - over;
   p.stages = room / p.stage_bytes;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
@@ -456,12 +472,12 @@ static int launch(int kps, const CUtensorMap& tx, const CUtensorMap& tw, Params&
 // stage: 8 x 5120 x 5120, 48 rows, 9.1 / 8.0 / 8.0 us; 64 x 4096 x 4096, 32 rows, 7.8 / 6.9 / 7.3; 8 x 17408 x 5120, 128 rows, 16.0 / 16.5).
 static int boxes_per_stage(int h) { return h <= 64 ? 2 : 1; }
 
-// How a dense launch is divided: weight rows per tile, CTAs per tile, or pairs of CTAs with tiles of 256 x 256, by a fitted time in ns.
-// A tile's 128 k cost 0.45 ns per token row of its box and 1.55 per weight row, 90 at least (a pair's 365), and 1.2 and 0.3 more where K is no
+// How a dense launch is divided: weight rows per tile, CTAs per tile, or pairs of CTAs with tiles of 256 tokens, by a fitted time in ns.
+// A tile's 128 k cost 0.45 ns per token row of its box and 1.55 per weight row, 90 at least (a pair's 45 and 1.25 per weight row), and 1.2 and 0.3 more where K is no
 // multiple of 128, so that a row of a box lies in two lines; its outputs 0.1 each, behind the next tile's k but for the last; a launch
 // 3500, another round 500; the meeting of a split tile's sums 1800 and 0.22 per output; and all of it at least what the bytes take out of
-// DRAM.  Over 70 shapes of 17 to 4096 tokens the choice took 1.02 times as long as the best division tried (16 x 1024 x 8192: one / two / four CTAs per
-// tile 9.6 / 8.0 / 6.8 us, 256 x 4096 x 4096: 8.5 / 11.2 / 16.3, 1024 x 4096 x 14336: 49.0 alone, 42.1 in pairs).  Eight CTAs per tile lost everywhere;
+// DRAM.  Over 46 shapes of 17 to 4096 tokens the choice took 1.02 times as long as the best division tried (16 x 1024 x 8192: one / two / four CTAs per
+// tile 9.6 / 8.0 / 6.8 us, 256 x 4096 x 4096: 8.5 / 11.2 / 16.3, 1024 x 8192 x 8192: 53.0 alone, 47.3 in pairs of 256 rows, 45.8 of 224).  Eight CTAs per tile lost everywhere;
 // of clusters of four 32 fit the SMs at a time, not 37.
 struct Plan { int h, split; bool pair; };
 static Plan plan(int M, int N, int K, int tok_box) {
@@ -482,10 +498,10 @@ static Plan plan(int M, int N, int K, int tok_box) {
       if (ns < least) { least = ns; best = Plan{h, split, false}; }
     }
   }
-  if (M > 128) {
-    const int rounds = ((M + 255) / 256 * ((N + 255) / 256) + sms / 2 - 1) / (sms / 2);
-    const double ns = fmax(dram, rounds * fmax(3300, nkb * 365.0)) + 500.0 * (rounds - 1) + 3300;
-    if (ns < least) { least = ns; best = Plan{256, 1, true}; }
+  for (int h = 256; M > 128 && h >= 128; h -= 32) {        // a pair's columns come in 32s
+    const int rounds = ((M + 255) / 256 * ((N + h - 1) / h) + sms / 2 - 1) / (sms / 2);
+    const double ns = fmax(dram, rounds * fmax(13.0 * h, nkb * (45 + 1.25 * h))) + 500.0 * (rounds - 1) + 13.0 * h;
+    if (ns < least) { least = ns; best = Plan{h, 1, true}; }
   }
   if (least >= 1e30) best.pair = M > 128;                  // more tiles than eight rounds hold
   return best;
@@ -518,7 +534,7 @@ int umma_i8_linear(const I8LinearArgs& a, cudaStream_t st) {
   if ((int64_t)p.n_strips * p.m_tiles > INT32_MAX / 8) return B2Q_ERR_LIMIT;
   p.total = p.n_strips * p.m_tiles;
   int rc = make_tmap_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.xq, a.M, a.K, (uint64_t)a.ldx, p.tok_box, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (!rc) rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.N, a.K, (uint64_t)a.K, pair ? 128 : p.h, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.N, a.K, (uint64_t)a.K, pair ? p.h / 2 : p.h, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   if (pair) return launch_form<1, true, false, false, false>(tx, tw, p, 2 * (p.total < sms / 2 ? p.total : sms / 2), st);
   if (p.split > 1) return launch<true, false, false>(kps, tx, tw, p, p.total * p.split, st);
