@@ -145,13 +145,22 @@ struct I8Tokens {
   uint32_t max[I8_STREAM_MAX_TOK];
   float scale[I8_STREAM_MAX_TOK];
   I8Row row[I8_STREAM_MAX_TOK];
+  int16_t list[I8_STREAM_MAX_TOK];                         // of the tokens that are wanted, where that is not all of them
+  int count;
 };
 template <bool BF16, int THREADS, int V> struct I8TokenCodes {
   const uint16_t* x; int64_t ldx;
   bool vec;                                                // rows are 16-byte aligned
   int M, n8, total;
   uint32_t inv;                                            // i / n8 = i * inv >> 32 for the sizes that fit shared memory (i < 2^17, n8 < 2^14)
+  const int16_t* list = nullptr;
   uint4 v[V];
+  __device__ __forceinline__ void only(const I8Tokens& tok) {      // those of tok.list
+    list = tok.list;
+    M = tok.count;
+    total = M * n8;
+  }
+  __device__ __forceinline__ int actual(int m) const { return list ? list[min(m, M - 1)] : m; }
   __device__ __forceinline__ I8TokenCodes(const uint16_t* x_, int64_t ldx_, int M_, int K) : x(x_), ldx(ldx_), M(M_), n8(K >> 3), total(M_ * (K >> 3)) {
     vec = ((reinterpret_cast<uintptr_t>(x_) | (uintptr_t)(2 * ldx_)) & 15u) == 0;
     inv = 0xFFFFFFFFu / (uint32_t)n8 + 1;
@@ -161,9 +170,9 @@ template <bool BF16, int THREADS, int V> struct I8TokenCodes {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int i = base + j * THREADS + threadIdx.x, m = token(i);
-      const uint16_t* at = x + m * ldx + 8 * (i - m * n8);
       v[j] = make_uint4(0, 0, 0, 0);
       if (i < total) {
+        const uint16_t* at = x + actual(m) * ldx + 8 * (i - m * n8);
         if (vec) v[j] = ld_vec(at);
         else v[j] = make_uint4(ld_u16(at) | ld_u16(at + 1) << 16, ld_u16(at + 2) | ld_u16(at + 3) << 16, ld_u16(at + 4) | ld_u16(at + 5) << 16, ld_u16(at + 6) | ld_u16(at + 7) << 16);
       }
@@ -188,9 +197,9 @@ template <bool BF16, int THREADS, int V> struct I8TokenCodes {
         const int m = token(i0);
         if (token(i0 + 31) == m) {
           mx = __reduce_max_sync(0xffffffffu, mx);
-          if (lane == 0) atomicMax(&tok.max[m], mx);
+          if (lane == 0) atomicMax(&tok.max[actual(m)], mx);
         } else if (i0 + lane < total) {                    // a warp that straddles tokens
-          atomicMax(&tok.max[token(i0 + lane)], mx);
+          atomicMax(&tok.max[actual(token(i0 + lane))], mx);
         }
         __syncwarp();
       }
@@ -198,12 +207,13 @@ template <bool BF16, int THREADS, int V> struct I8TokenCodes {
   }
   __device__ __forceinline__ void rows(I8Tokens& tok) const {
     if (threadIdx.x < M) {
-      const uint32_t bits = tok.max[threadIdx.x];
+      const int m = actual(threadIdx.x);
+      const uint32_t bits = tok.max[m];
       const float a = fmaxf(__uint_as_float(bits), I8_MIN_AMAX);
       I8Row r = i8_row(a);
       if (bits >= 0x7F800000u) r = I8Row{0.f, 0.f, 0.f};   // not finite
-      tok.row[threadIdx.x] = r;
-      tok.scale[threadIdx.x] = bits < 0x7F800000u ? a / 127.f : __uint_as_float(0x7FC00000u);
+      tok.row[m] = r;
+      tok.scale[m] = bits < 0x7F800000u ? a / 127.f : __uint_as_float(0x7FC00000u);
     }
     __syncwarp();
   }
@@ -214,13 +224,13 @@ template <bool BF16, int THREADS, int V> struct I8TokenCodes {
       for (int j = 0; j < V; ++j) {
         const int i = base + j * THREADS + threadIdx.x;
         if (i >= total) break;
-        const int m = token(i);
+        const int n = token(i), m = actual(n);
         const I8Row r = tok.row[m];
         float lo[4], hi[4];
         unpack2<BF16>(v[j].x, lo[0], lo[1]); unpack2<BF16>(v[j].y, lo[2], lo[3]); unpack2<BF16>(v[j].z, hi[0], hi[1]); unpack2<BF16>(v[j].w, hi[2], hi[3]);
         uint2 o = make_uint2(0, 0);
         if (r.c != 0.f) o = make_uint2(i8_codes4<false>(lo, r), i8_codes4<false>(hi, r));
-        *reinterpret_cast<uint2*>(to + m * pitch + 8 * (i - m * n8)) = o;
+        *reinterpret_cast<uint2*>(to + m * pitch + 8 * (i - n * n8)) = o;
       }
     }
     __syncwarp();

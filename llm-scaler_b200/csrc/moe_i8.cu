@@ -191,13 +191,16 @@ template <int PER, class Between> __device__ __forceinline__ void route(const Pa
   __syncthreads();
 }
 
-// The CTA that has column c when n columns are dealt out to G CTAs, [b n / G, (b + 1) n / G) to CTA b.
-__device__ __forceinline__ int owner(int64_t c, int64_t n, int64_t G) {
-  int64_t b = c * G / n;
-  while ((b + 1) * n / G <= c) ++b;
-  while (b * n / G > c) --b;
-  return (int)b;
-}
+// n things dealt out to G CTAs in turn: the first n % G have one more.
+struct Share {
+  int each, more;
+  __device__ __forceinline__ Share(int n, int G) : each(n / G), more(n - n / G * G) {}
+  __device__ __forceinline__ int begin(int b) const { return b * each + min(b, more); }
+  __device__ __forceinline__ int owner(int c) const {      // each > 0
+    const int big = more * (each + 1);
+    return c < big ? c / (each + 1) : more + (c - big) / each;
+  }
+};
 
 __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(WORKERS) : "memory"); }      // the eight warps
 
@@ -335,24 +338,27 @@ __global__ void __launch_bounds__(THREADS, 1) moe_i8_kernel(const __grid_constan
   for (int i = threadIdx.x; i < p.E; i += THREADS) { rt.first[i] = pairs; rt.count[i] = 0; }
   float logits[PER];
   if (warp < p.T) load_logits<PER>(p, warp, logits);
-  I8TokenCodes<BF16, HELPERS, 10> tc(p.x, p.H, p.T, p.H);
-  if (warp < W_WARP) tc.fetch();
+  // One or two tokens' codes are made alongside the routing; of more, only those that this CTA's columns need, behind it.
+  const bool soon = p.T <= 2;
+  I8TokenCodes<BF16, HELPERS, 6> tc(p.x, p.H, p.T, p.H);
+  if (soon && warp < W_WARP) tc.fetch();
   __syncthreads();
   route<PER>(p, rt, logits, [&](int step) {
-    if (warp < W_WARP) { if (step == 0) tc.maximum(tok); else tc.rows(tok); }
+    if (soon && warp < W_WARP) { if (step == 0) tc.maximum(tok); else tc.rows(tok); }
   });
   grid_dep_release();
 
   // ---- this CTA's share of the up part: columns [c0, c1) of all slots' columns, as groups of eight: those of the first slot's part, then of
   // whole slots; the last slot's part may end early ----
-  const int64_t n = (int64_t)rt.slots * p.I;
-  const int64_t G = min((int64_t)gridDim.x, n);            // CTAs that have a column
-  const bool any = blockIdx.x < G;
-  const int64_t c0 = any ? blockIdx.x * n / G : 0, c1 = any ? (blockIdx.x + 1) * n / G : 0;
-  const int slot0 = (int)(c0 / p.I), slot1 = any ? (int)((c1 - 1) / p.I) : -1;
-  const int j0 = (int)(c0 - (int64_t)slot0 * p.I), per_slot = (p.I + 7) / 8;
-  const int len0 = (int)min((int64_t)p.I - j0, c1 - c0), groups0 = (len0 + 7) / 8;
-  const int end1 = (int)(c1 - (int64_t)slot1 * p.I);       // columns of the last slot end here
+  const int n = rt.slots * p.I;                            // at most 512 * 131071
+  const int G = min((int)gridDim.x, n);                    // CTAs that have a column
+  const bool any = (int)blockIdx.x < G;
+  const Share share(n, max(G, 1));
+  const int c0 = any ? share.begin(blockIdx.x) : 0, c1 = any ? share.begin(blockIdx.x + 1) : 0;
+  const int slot0 = c0 / p.I, slot1 = any ? (c1 - 1) / p.I : -1;
+  const int j0 = c0 - slot0 * p.I, per_slot = (p.I + 7) / 8;
+  const int len0 = min(p.I - j0, c1 - c0), groups0 = (len0 + 7) / 8;
+  const int end1 = c1 - slot1 * p.I;                       // columns of the last slot end here
   const int groups = !any ? 0 : (slot0 == slot1 ? groups0 : groups0 + (slot1 - slot0 - 1) * per_slot + (end1 + 7) / 8);
   struct Group { int slot, j, n; };                        // n: valid columns
   auto group_at = [&](int i) {
@@ -369,7 +375,8 @@ __global__ void __launch_bounds__(THREADS, 1) moe_i8_kernel(const __grid_constan
   const int up_pieces = (p.H + p.up_piece - 1) / p.up_piece, per_group = 2 * up_pieces;      // stages of a group: its gate rows' pieces, its up rows'
   const int up_items = groups * per_group;
   // ---- and of the down part: rows [r0, r0 + rows) of every slot's matrix ----
-  const int r0 = (int)((int64_t)blockIdx.x * p.H / gridDim.x), rows = (int)((int64_t)(blockIdx.x + 1) * p.H / gridDim.x) - r0;
+  const Share row_share(p.H, gridDim.x);
+  const int r0 = row_share.begin(blockIdx.x), rows = row_share.begin(blockIdx.x + 1) - r0;
   const int sr = p.down_rows, nrg = (rows + sr - 1) / sr, down_pieces = (p.I + p.down_piece - 1) / p.down_piece;
   const int per_chunk = nrg * down_pieces, items = up_items + rt.chunks * per_chunk;
   const Arrivals mark = p.tag ^ *reinterpret_cast<const volatile Arrivals*>(p.epoch) << ARRIVALS_BITS;
@@ -424,6 +431,24 @@ __global__ void __launch_bounds__(THREADS, 1) moe_i8_kernel(const __grid_constan
       if (!ok) drain_issued(full, p.stages, issued);
     }
     return;
+  }
+  if (!soon) {
+    if (warp == 0) {
+      uint32_t mask = 0;
+      if (any)
+        for (int i = rt.slot_first[slot0] + lane; i < rt.slot_first[slot1 + 1]; i += 32) mask |= 1u << (rt.list[i] / p.k);
+      mask = __reduce_or_sync(0xffffffffu, mask);
+      if (lane == 0) tok.count = __popc(mask);
+      if (mask >> lane & 1) tok.list[__popc(mask & ((1u << lane) - 1u))] = (int16_t)lane;
+      __syncwarp();
+    }
+    asm volatile("bar.sync 2, %0;" ::"n"(HELPERS) : "memory");
+    tc.only(tok);
+    tc.fetch();
+    tc.maximum(tok);
+    asm volatile("bar.sync 2, %0;" ::"n"(HELPERS) : "memory");
+    tc.rows(tok);
+    asm volatile("bar.sync 2, %0;" ::"n"(HELPERS) : "memory");
   }
   tc.codes(tok, codes, p.pitch);
   __syncwarp();
@@ -497,7 +522,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_i8_kernel(const __grid_constan
       const int slot = base + threadIdx.x;
       int last = 0;
       if (slot <= slot1) {
-        last = arrivals_last(p.counts + slot, owner((int64_t)(slot + 1) * p.I - 1, n, G) - owner((int64_t)slot * p.I, n, G));
+        last = arrivals_last(p.counts + slot, share.owner((slot + 1) * p.I - 1) - share.owner(slot * p.I));
         __threadfence();
       }
       done[threadIdx.x] = last;
