@@ -1,17 +1,6 @@
 // C ABI of the 8-bit integer operators: argument validation and kernel selection, as in api.cu.
 #include "i8.cuh"
 
-namespace b2q {
-// implemented in moe_aux.cu
-int moe_topk(const void*, int, int64_t, int, int, int, void*, int, int32_t*, cudaStream_t);
-size_t moe_route_workspace_bytes(int64_t, int);
-int moe_route(const int32_t*, int64_t, int, int32_t*, int32_t*, int32_t*, int32_t*, void*, cudaStream_t);
-int moe_build_tiles(const int32_t*, int, int, int32_t*, cudaStream_t);
-bool moe_route_fused_fits(int64_t, int, int);
-int moe_route_fused(const void*, int, int64_t, int, int, void*, int, int32_t*, int32_t*, int32_t*, int, int32_t*, int, cudaStream_t);
-int moe_combine(const void*, const void*, int, const int32_t*, void*, int, int64_t, int, int64_t, int, cudaStream_t);
-}  // namespace b2q
-
 using namespace b2q;
 
 namespace {
@@ -115,7 +104,7 @@ int b2q_linear_int8_dynamic(const void* x, int act_dtype, int64_t ldx, const int
 namespace {
 // Workspace of an expert layer in its grouped form, part by part.
 struct MoeParts {
-  uint8_t *weights, *ids, *offsets, *tokens, *perm, *route, *tiles, *xq, *xs, *h, *hq, *hs, *y;
+  uint8_t *weights, *ids, *place, *rows, *base, *offsets, *count, *tiles, *xq, *xs, *h, *hq, *hs, *y;
   size_t total;
 };
 MoeParts moe_parts(void* ws, int64_t T, int E, int k, int64_t H, int64_t I) {
@@ -124,8 +113,8 @@ MoeParts moe_parts(void* ws, int64_t T, int E, int k, int64_t H, int64_t I) {
   size_t at = 0;
   auto take = [&](size_t bytes) { uint8_t* q = base + at; at += align_up(bytes, 256); return q; };
   const size_t rows = (size_t)T * k;
-  p.weights = take(rows * 4); p.ids = take(rows * 4); p.offsets = take((size_t)(E + 2) * 4); p.tokens = take(rows * 4); p.perm = take(rows * 4);
-  p.route = take(moe_route_workspace_bytes((int64_t)rows, E));
+  p.weights = take(rows * 4); p.ids = take(rows * 4); p.place = take(rows * 4); p.rows = take(rows * 4);
+  p.base = take((size_t)moe_i8_route_ctas(T) * E * 4); p.offsets = take((size_t)(E + 1) * 4); p.count = take(8);
   p.tiles = take(16 + 8 * (rows / 32 + 1 + E));
   p.xq = take(rows * H); p.xs = take(rows * 4); p.h = take(rows * I * 4); p.hq = take(rows * I); p.hs = take(rows * 4); p.y = take(rows * H * 2);
   p.total = at;
@@ -167,18 +156,13 @@ int b2q_moe_forward_int8(const b2q_moe_int8* m, void* workspace, size_t workspac
   }
   const MoeParts p = moe_parts(workspace, a.T, E, k, H, I);
   const int64_t rows = a.T * k;
-  int32_t *off = reinterpret_cast<int32_t*>(p.offsets), *tok = reinterpret_cast<int32_t*>(p.tokens), *perm = reinterpret_cast<int32_t*>(p.perm);
-  int32_t* tiles = reinterpret_cast<int32_t*>(p.tiles);
-  const int tile = i8_grouped_tile(rows, E);
-  int rc;
-  if (a.renormalize && moe_route_fused_fits(a.T, E, k)) {
-    rc = moe_route_fused(a.logits, a.logits_dtype, a.T, E, k, p.weights, B2Q_F32, off, tok, perm, tile, tiles, 0, st);
-  } else {
-    int32_t* ids = reinterpret_cast<int32_t*>(p.ids);
-    rc = moe_topk(a.logits, a.logits_dtype, a.T, E, k, a.renormalize != 0, p.weights, B2Q_F32, ids, st);
-    if (!rc) rc = moe_route(ids, rows, E, off, tok, perm, nullptr, p.route, st);
-    if (!rc) rc = moe_build_tiles(off, E, tile, tiles, st);
-  }
+  int32_t *off = reinterpret_cast<int32_t*>(p.offsets), *tiles = reinterpret_cast<int32_t*>(p.tiles), *out_rows = reinterpret_cast<int32_t*>(p.rows);
+  const int tile = i8_grouped_tile(rows, E), ctas = moe_i8_route_ctas(a.T);
+  I8Copies to{};
+  to.ids = reinterpret_cast<int32_t*>(p.ids); to.place = reinterpret_cast<int32_t*>(p.place); to.base = reinterpret_cast<int32_t*>(p.base);
+  to.rows = out_rows; to.k = k; to.E = E; to.run = (int)((a.T + ctas - 1) / ctas);
+  int rc = moe_i8_route(a.logits, a.logits_dtype, a.T, E, k, a.renormalize != 0, tile, reinterpret_cast<float*>(p.weights), reinterpret_cast<int32_t*>(p.ids),
+                        reinterpret_cast<int32_t*>(p.place), reinterpret_cast<int32_t*>(p.base), off, tiles, p.count, st);
   if (rc) return rc;
   I8GroupedArgs g{};
   g.xq = reinterpret_cast<int8_t*>(p.xq); g.xs = reinterpret_cast<float*>(p.xs); g.w = a.w13; g.ws = a.s13; g.ws_dtype = a.s13_dtype;
@@ -187,11 +171,11 @@ int b2q_moe_forward_int8(const b2q_moe_int8* m, void* workspace, size_t workspac
   I8GroupedArgs d = g;
   d.xq = reinterpret_cast<int8_t*>(p.hq); d.xs = reinterpret_cast<float*>(p.hs); d.w = a.w2; d.ws = a.s2; d.ws_dtype = a.s2_dtype;
   d.out = p.y; d.N = H; d.K = I; d.gated = false;
-  rc = quantize_i8_copies(a.x, bf16, perm, k, reinterpret_cast<int8_t*>(p.xq), reinterpret_cast<float*>(p.xs), a.T, H, st);
+  rc = quantize_i8_copies(a.x, bf16, to, reinterpret_cast<int8_t*>(p.xq), reinterpret_cast<float*>(p.xs), a.T, H, st);
   if (!rc) rc = umma_i8_grouped(g, st);
-  if (!rc) rc = quantize_i8_some(p.h, B2Q_F32, I, off + E, reinterpret_cast<int8_t*>(p.hq), reinterpret_cast<float*>(p.hs), rows, I, st);
+  if (!rc) rc = quantize_i8_computed(reinterpret_cast<float*>(p.h), off + E, reinterpret_cast<int8_t*>(p.hq), reinterpret_cast<float*>(p.hs), rows, I, st);
   if (!rc) rc = umma_i8_grouped(d, st);
-  if (!rc) rc = moe_combine(p.y, p.weights, B2Q_F32, perm, a.out, a.act_dtype, a.T, k, H, 0, st);
+  if (!rc) rc = moe_i8_sum(p.y, reinterpret_cast<float*>(p.weights), out_rows, a.out, bf16, a.T, k, H, st);
   return rc;
 }
 

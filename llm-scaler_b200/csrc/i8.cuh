@@ -46,13 +46,26 @@ int moe_i8_few(const I8FewArgs& a, cudaStream_t st);
 
 // q [M, K] codes, s [M] scales of rows of x; x_dtype B2Q_BF16 / F16 / F32.
 int quantize_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
-// the same for the first *n_valid of M rows, a number that only the device knows
-int quantize_i8_some(const void* x, int x_dtype, int64_t ldx, const int32_t* n_valid, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
-// the same with k copies of row r, at rows to[r * k] ... of q and s (none where that is negative); x contiguous, 16 bit, K % 16 == 0
-int quantize_i8_copies(const void* x, bool bf16, const int32_t* to, int k, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
+// codes of the first *n_valid of M fp32 rows, a number that only the device knows; the rows are results themselves, so that halves are not decided
+// to the last bit.  x 16-byte aligned, K % 8 == 0
+int quantize_i8_computed(const float* x, const int32_t* n_valid, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
+// the same with a copy of row r for each of its k pairs, at rows[pair] = base[r / run, ids[pair]] + place[pair] (moe_i8_route), which it also writes;
+// -1, and no copy, where the pair has no expert.  x contiguous, 16 bit, K % 8 == 0
+struct I8Copies {
+  const int32_t *ids, *place, *base;
+  int32_t* rows;
+  int k, E, run;
+};
+int quantize_i8_copies(const void* x, bool bf16, const I8Copies& to, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
 int silu_mul_quantize_i8(const void* gate_up, bool bf16, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st);
 int resadd_rmsnorm_quantize_i8(const void* hidden, const void* residual, const void* w, void* residual_out, bool bf16, float eps, int8_t* q, float* s,
                                int64_t M, int K, cudaStream_t st);
+
+// The expert layer of many tokens (moe_i8_many.cu): routing, with base for moe_i8_route_ctas(T) runs of ceil(T / that) tokens; weighted sum.
+int moe_i8_route_ctas(int64_t T);
+int moe_i8_route(const void* logits, int dt, int64_t T, int E, int k, bool renorm, int tile, float* weights, int32_t* ids, int32_t* place, int32_t* base,
+                 int32_t* offsets, int32_t* tiles, void* count, cudaStream_t st);
+int moe_i8_sum(const void* y, const float* weights, const int32_t* rows, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st);
 
 #ifdef __CUDACC__
 // Ordinary loads, never by the read-only path: these kernels begin while the kernel that writes their inputs is still running.  Volatile

@@ -11,13 +11,13 @@
 namespace b2q {
 
 namespace i8q {
-enum { PLAIN, SILU, NORM, COPIES };
+enum { PLAIN, SILU, NORM, COPIES, COMPUTED };              // COMPUTED: fp32 rows that are results themselves
 
 struct Params {
   const void* x; int64_t ldx;                              // elements
   const void* residual; const void* nw; void* residual_out; float eps;
   const int32_t* n_valid;
-  const int32_t* to; int copies;                           // COPIES: where the copies of a row go
+  I8Copies to;                                             // COPIES
   int8_t* q; float* s; int64_t M; int K;
 };
 
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
   const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
   enter();
   if (row >= p.M) return;                                  // whole warps, or the whole CTA
-  if constexpr (MODE == PLAIN) {
+  if constexpr (MODE == PLAIN || MODE == COMPUTED) {
     if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
   }
   const int n8 = p.K >> 3;
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
   Piece<MODE, DT> pc[V];
   uint32_t mx = 0;
   float sum = 0.f;
-  if constexpr (MODE == PLAIN || MODE == COPIES) {
+  if constexpr (MODE == PLAIN || MODE == COPIES || MODE == COMPUTED) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = first + i * step;
@@ -184,11 +184,18 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
     }
   }
   const Scale sc = row_scale<MODE>(mx, sum, p.K, p.eps);
+  int32_t copy = -1;                                       // lane n: the row of the n-th copy
   if constexpr (MODE == COPIES) {
-    if (first < p.copies) {
-      const int32_t r = *reinterpret_cast<const volatile int32_t*>(p.to + row * p.copies + first);
-      if (r >= 0) p.s[r] = sc.scale;
+    if (lane < p.to.k) {
+      const int64_t pair = row * p.to.k + lane;
+      const int32_t e = __ldcg(p.to.ids + pair);
+      if (e >= 0) copy = __ldcg(p.to.base + row / p.to.run * p.to.E + e) + __ldcg(p.to.place + pair);
+      if (WARP || warp == 0) {
+        p.to.rows[pair] = copy;
+        if (copy >= 0) p.s[copy] = sc.scale;
+      }
     }
+    __syncwarp();
   } else {
     if (first == 0) p.s[row] = sc.scale;
   }
@@ -196,23 +203,21 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = first + i * step;
-    if (c < n8) {
-      float f[8];
-      pc[i].get(f);
-      const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
-      uint2 o = make_uint2(0, 0);
-      if (sc.finite) {
-        if constexpr (MODE == PLAIN || MODE == COPIES) o = make_uint2(i8_codes4<DT == B2Q_F32>(lo, sc.row), i8_codes4<DT == B2Q_F32>(hi, sc.row));
-        else o = make_uint2(i8_codes4_computed(lo, sc.r), i8_codes4_computed(hi, sc.r));
+    float f[8];
+    pc[i].get(f);
+    const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+    uint2 o = make_uint2(0, 0);
+    if (sc.finite) {
+      if constexpr (MODE == PLAIN || MODE == COPIES) o = make_uint2(i8_codes4<DT == B2Q_F32>(lo, sc.row), i8_codes4<DT == B2Q_F32>(hi, sc.row));
+      else o = make_uint2(i8_codes4_computed(lo, sc.r), i8_codes4_computed(hi, sc.r));
+    }
+    if constexpr (MODE == COPIES) {
+      for (int n = 0; n < p.to.k; ++n) {
+        const int32_t r = __shfl_sync(0xffffffffu, copy, n);
+        if (r >= 0 && c < n8) *reinterpret_cast<uint2*>(q + (int64_t)r * p.K + 8 * c) = o;
       }
-      if constexpr (MODE == COPIES) {
-        for (int n = 0; n < p.copies; ++n) {
-          const int32_t r = __ldcg(p.to + row * p.copies + n);
-          if (r >= 0) *reinterpret_cast<uint2*>(q + (int64_t)r * p.K + 8 * c) = o;
-        }
-      } else {
-        *reinterpret_cast<uint2*>(q + 8 * c) = o;
-      }
+    } else {
+      if (c < n8) *reinterpret_cast<uint2*>(q + 8 * c) = o;
     }
   }
 }
@@ -319,19 +324,21 @@ template <int MODE> static int run(const Params& p, int dt, bool vec, cudaStream
 static bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 }  // namespace i8q
 
-int quantize_i8_some(const void* x, int x_dtype, int64_t ldx, const int32_t* n_valid, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
+int quantize_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
   i8q::Params p{};
-  p.x = x; p.ldx = ldx; p.n_valid = n_valid; p.q = q; p.s = s; p.M = M; p.K = K;
+  p.x = x; p.ldx = ldx; p.q = q; p.s = s; p.M = M; p.K = K;
   return i8q::run<i8q::PLAIN>(p, x_dtype, aligned16(x) && i8q::aligned8(q) && ldx % 8 == 0, st);
 }
-int quantize_i8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
-  return quantize_i8_some(x, x_dtype, ldx, nullptr, q, s, M, K, st);
+int quantize_i8_computed(const float* x, const int32_t* n_valid, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
+  i8q::Params p{};
+  p.x = x; p.ldx = K; p.n_valid = n_valid; p.q = q; p.s = s; p.M = M; p.K = K;
+  return K <= 32768 ? i8q::run_vec<i8q::COMPUTED, B2Q_F32>(p, st) : i8q::run<i8q::PLAIN>(p, B2Q_F32, false, st);
 }
-int quantize_i8_copies(const void* x, bool bf16, const int32_t* to, int k, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
+int quantize_i8_copies(const void* x, bool bf16, const I8Copies& to, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {
   using namespace i8q;
   if (K > 32768) return B2Q_ERR_LIMIT;
   Params p{};
-  p.x = x; p.ldx = K; p.to = to; p.copies = k; p.q = q; p.s = s; p.M = M; p.K = K;
+  p.x = x; p.ldx = K; p.to = to; p.q = q; p.s = s; p.M = M; p.K = K;
   return bf16 ? run_vec<COPIES, B2Q_BF16>(p, st) : run_vec<COPIES, B2Q_F16>(p, st);
 }
 int silu_mul_quantize_i8(const void* gate_up, bool bf16, int64_t ldx, int8_t* q, float* s, int64_t M, int K, cudaStream_t st) {

@@ -23,6 +23,7 @@
 // Every wait is bounded; a warp that gives up still goes to the barriers where the others expect it.
 #include "arrivals.cuh"
 #include "i8.cuh"
+#include "i8_route.cuh"
 #include "sm100.cuh"
 #include "umma_gemm.cuh"
 
@@ -76,71 +77,15 @@ struct Route {
   __device__ __forceinline__ int chunk_pairs(int c) const { return min(XR, slot_first[chunk_slot[c] + 1] - chunk_first[c]); }
 };
 
-// Larger logits have larger keys, equal ones equal keys, none has key 0.
-__device__ __forceinline__ uint32_t logit_key(float v) {
-  const uint32_t u = __float_as_uint(v + 0.f);             // -0 becomes +0
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
-}
-
-// One warp: a token's logits, and the k largest of them, the lowest index first among equals; softmax over all or over the chosen.  A token whose logits
-// hold a NaN, or have no finite maximum, goes to no expert.
-template <int PER> __device__ __forceinline__ void load_logits(const Params& p, int tok, float (&v)[PER]) {
-  const int lane = threadIdx.x & 31;
-  const int64_t at = (int64_t)tok * p.E;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int e = lane + 32 * j;
-    v[j] = -INFINITY;
-    if (e < p.E)
-      v[j] = p.ldt == B2Q_F32 ? __ldcg(reinterpret_cast<const float*>(p.logits) + at + e)
-                              : scalar_from_raw(__ldcg(reinterpret_cast<const unsigned short*>(p.logits) + at + e), p.ldt);
-  }
-}
 template <int PER> __device__ __forceinline__ void route_token(const Params& p, int tok, const float (&v)[PER], Route& r) {
-  const int lane = threadIdx.x & 31;
-  uint32_t key[PER];
-  float mx = -INFINITY;
-  bool nan = false;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    mx = fmaxf(mx, v[j]);
-    nan = nan || v[j] != v[j];
-    key[j] = lane + 32 * j < p.E ? logit_key(v[j]) : 0u;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const bool none = __any_sync(0xffffffffu, nan) || !(fabsf(mx) < INFINITY);
-  float sum = 0.f;
-  if (!p.renorm) {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) sum += expf(v[j] - mx);  // absent experts: exp(-inf) = 0
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  }
-  float mine = 0.f, chosen = 0.f;
-  int id = -1;
-  for (int s = 0; s < p.k; ++s) {
-    uint32_t best = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) best = max(best, key[j]);
-    best = __reduce_max_sync(0xffffffffu, best);
-    uint32_t e = 0xFFFFu;
-#pragma unroll
-    for (int j = PER - 1; j >= 0; --j)
-      if (key[j] == best) e = lane + 32 * j;
-    e = __reduce_min_sync(0xffffffffu, e);
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (lane + 32 * j == (int)e) key[j] = 0;
-    const float l = __uint_as_float((best & 0x80000000u) ? best & 0x7FFFFFFFu : ~best), w = expf(l - mx);
-    chosen += w;
-    if (lane == s) { mine = w; id = (int)e; }
-  }
-  if (lane < p.k) {
-    const int pair = tok * p.k + lane;
-    r.expert[pair] = none ? -1 : (int16_t)id;
-    r.weight[pair] = none ? 0.f : mine / (p.renorm ? chosen : sum);
-    if (!none) {
+  int id;
+  float weight;
+  i8r::top_k<PER>(v, p.E, p.k, p.renorm != 0, id, weight);
+  if ((threadIdx.x & 31) < p.k) {
+    const int pair = tok * p.k + (threadIdx.x & 31);
+    r.expert[pair] = (int16_t)id;
+    r.weight[pair] = weight;
+    if (id >= 0) {
       atomicMin(&r.first[id], pair);
       r.place[pair] = (int16_t)atomicAdd(&r.count[id], 1);
     }
@@ -337,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_i8_kernel(const __grid_constan
   for (int i = threadIdx.x; i < 2 * PASS * p.T * 16; i += THREADS) sums[i] = 0;
   for (int i = threadIdx.x; i < p.E; i += THREADS) { rt.first[i] = pairs; rt.count[i] = 0; }
   float logits[PER];
-  if (warp < p.T) load_logits<PER>(p, warp, logits);
+  if (warp < p.T) i8r::load_logits<PER>(p.logits, p.ldt, p.E, warp, logits);
   // One or two tokens' codes are made alongside the routing; of more, only those that this CTA's columns need, behind it.
   const bool soon = p.T <= 2;
   I8TokenCodes<BF16, HELPERS, 6> tc(p.x, p.H, p.T, p.H);

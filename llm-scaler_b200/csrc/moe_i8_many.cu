@@ -1,0 +1,200 @@
+// What the int8 expert layer of many tokens has around its grouped GEMMs: the routing in one launch, and the weighted sum.
+//
+// Routing.  A CTA routes a run of tokens, a warp each in turn, and counts its pairs per expert in shared memory; the place a pair is counted at
+// is its place among the CTA's pairs of that expert.  The last CTA to finish (arrivals.cuh) turns the counts into where each CTA's pairs of an
+// expert begin in the sorted order, and lists the tiles.  Where a pair's row is then follows from its expert, its CTA and its place.  Which
+// of a CTA's pairs comes first is a matter of chance, and no result depends on it: a row of the sorted order does not see the others.
+// 4096 tokens, 128 experts, top-8: five launches of 27 us before (top-k, a stable sort in three, tiles).
+//
+// Weighted sum.  Memory-bound; a thread has eight columns of a token and requests eight experts' rows at a time.
+#include "arrivals.cuh"
+#include "i8.cuh"
+#include "i8_route.cuh"
+
+namespace b2q {
+
+namespace i8m {
+constexpr int THREADS = 512, WARPS = THREADS / 32, MAX_E = 1024;
+constexpr int CHUNKS = 4, SPANS = WARPS / CHUNKS, MAX_CTAS = 64, SPAN = MAX_CTAS / SPANS;      // of the last CTA's work: 128 experts at a time
+
+struct Params {
+  const void* logits; int dt;
+  int T, E, k, renorm, per_cta, tile;
+  float* weights; int32_t *ids, *place;                    // [T * k]
+  int32_t *base, *offsets, *tiles;                         // [CTAs, E], [E + 1], {n, pad, (expert, first row) ...}
+  Arrivals* count; Arrivals tag; const Arrivals* epoch;
+};
+
+__device__ __forceinline__ void enter() {
+  const bool few = gridDim.x <= 148;
+  if (few) grid_dep_release();
+  grid_dep_wait();
+  if (!few) grid_dep_release();
+}
+
+template <int PER>
+__global__ void __launch_bounds__(THREADS) moe_i8_route_kernel(const Params p) {
+  __shared__ int counts[MAX_E];
+  __shared__ int part[SPANS][CHUNKS][32];
+  __shared__ int last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < p.E; e += THREADS) counts[e] = 0;
+  __syncthreads();
+  enter();
+  if (threadIdx.x == 0) arrivals_open(p.count, p.tag, p.epoch);
+  const int t0 = blockIdx.x * p.per_cta, t1 = min(p.T, t0 + p.per_cta);
+  float v[PER];
+  if (t0 + warp < t1) i8r::load_logits<PER>(p.logits, p.dt, p.E, t0 + warp, v);
+  for (int t = t0 + warp; t < t1; t += WARPS) {
+    float now[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) now[j] = v[j];
+    if (t + WARPS < t1) i8r::load_logits<PER>(p.logits, p.dt, p.E, t + WARPS, v);
+    int id;
+    float w;
+    i8r::top_k<PER>(now, p.E, p.k, p.renorm != 0, id, w);
+    if (lane < p.k) {
+      const int64_t pair = (int64_t)t * p.k + lane;
+      p.weights[pair] = w;
+      p.ids[pair] = id;
+      p.place[pair] = id >= 0 ? atomicAdd(&counts[id], 1) : 0;
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += THREADS) p.base[(int64_t)blockIdx.x * p.E + e] = counts[e];
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last = arrivals_last(p.count, gridDim.x - 1);
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
+
+  // ---- the last CTA: where every expert and every CTA's part of it begins.  A warp has 32 experts and a span of CTAs ----
+  const int chunk = warp % CHUNKS, span = warp / CHUNKS, ctas = gridDim.x;
+  int before = 0, tiles_before = 0;                        // rows and tiles of the experts so far
+  int2* list = reinterpret_cast<int2*>(p.tiles + 4);
+  for (int e0 = 0; e0 < p.E; e0 += 32 * CHUNKS) {
+    const int e = e0 + 32 * chunk + lane;
+    int32_t* mine = p.base + (int64_t)span * SPAN * p.E + e;
+    int n[SPAN], sum = 0;
+#pragma unroll
+    for (int i = 0; i < SPAN; ++i) n[i] = e < p.E && span * SPAN + i < ctas ? __ldcg(mine + (int64_t)i * p.E) : 0;
+#pragma unroll
+    for (int i = 0; i < SPAN; ++i) sum += n[i];
+    part[span][chunk][lane] = sum;
+    __syncthreads();
+    int front = 0, all = 0, begin = before, first_tile = tiles_before;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      int of = 0;                                          // rows of this lane's expert of chunk c
+#pragma unroll
+      for (int s = 0; s < SPANS; ++s) {
+        const int v = part[s][c][lane];
+        of += v;
+        if (c == chunk && s < span) front += v;
+      }
+      const int nt = (of + p.tile - 1) / p.tile;
+      if (c == chunk) {
+        all = of;
+        int rows_upto = of, tiles_upto = nt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, rows_upto, o), y = __shfl_up_sync(0xffffffffu, tiles_upto, o);
+          if (lane >= o) { rows_upto += x; tiles_upto += y; }
+        }
+        begin = before + rows_upto - of;
+        first_tile = tiles_before + tiles_upto - nt;
+      }
+      before += __reduce_add_sync(0xffffffffu, of);
+      tiles_before += __reduce_add_sync(0xffffffffu, nt);
+    }
+    if (e < p.E) {
+      if (span == 0) p.offsets[e] = begin;
+      for (int i = span; i < (all + p.tile - 1) / p.tile; i += SPANS) list[first_tile + i] = make_int2(e, i * p.tile);
+      int at = begin + front;
+#pragma unroll
+      for (int i = 0; i < SPAN; ++i) {
+        if (span * SPAN + i < ctas) mine[(int64_t)i * p.E] = at;
+        at += n[i];
+      }
+    }
+    __syncthreads();                                       // part is used again
+  }
+  if (threadIdx.x == 0) { p.offsets[p.E] = before; p.tiles[0] = tiles_before; }
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(256) moe_i8_sum_kernel(const uint16_t* y, const float* weights, const int32_t* rows, uint16_t* out, int64_t total, int H8, int k) {
+  enter();
+  const int64_t H = (int64_t)H8 * 8;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t t = i / H8, c = (i - t * H8) * 8;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < k; s0 += 8) {
+      uint4 v[8];
+      float w[8];
+      int32_t r[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) r[s] = s0 + s < k ? __ldcg(rows + t * k + s0 + s) : -1;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        v[s] = r[s] >= 0 ? __ldcg(reinterpret_cast<const uint4*>(y + r[s] * H + c)) : make_uint4(0, 0, 0, 0);
+        w[s] = r[s] >= 0 ? __ldcg(weights + t * k + s0 + s) : 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        if (r[s] < 0) continue;
+        const uint32_t e[4] = {v[s].x, v[s].y, v[s].z, v[s].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float a, b;
+          unpack2<BF16>(e[j], a, b);
+          acc[2 * j] = fmaf(w[s], a, acc[2 * j]);
+          acc[2 * j + 1] = fmaf(w[s], b, acc[2 * j + 1]);
+        }
+      }
+    }
+    *reinterpret_cast<uint4*>(out + t * H + c) =
+        make_uint4(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]), pack2<BF16>(acc[4], acc[5]), pack2<BF16>(acc[6], acc[7]));
+  }
+}
+}  // namespace i8m
+
+int moe_i8_route_ctas(int64_t T) {
+  const int64_t n = (T + 15) / 16;
+  return (int)(n < i8m::MAX_CTAS ? n : i8m::MAX_CTAS);
+}
+
+int moe_i8_route(const void* logits, int dt, int64_t T, int E, int k, bool renorm, int tile, float* weights, int32_t* ids, int32_t* place, int32_t* base,
+                 int32_t* offsets, int32_t* tiles, void* count, cudaStream_t st) {
+  using namespace i8m;
+  Params p{};
+  p.logits = logits; p.dt = dt; p.T = (int)T; p.E = E; p.k = k; p.renorm = renorm; p.tile = tile;
+  p.weights = weights; p.ids = ids; p.place = place; p.base = base; p.offsets = offsets; p.tiles = tiles;
+  p.count = reinterpret_cast<Arrivals*>(count); p.tag = arrivals_tag(); p.epoch = arrivals_epoch();
+  if (!p.epoch) return B2Q_ERR_CUDA;
+  const int ctas = moe_i8_route_ctas(T);
+  p.per_cta = (int)((T + ctas - 1) / ctas);
+  auto go = [&](void (*kern)(const Params)) { launch_overlapped(kern, dim3(ctas), dim3(THREADS), 0, st, tls().overlap_mode > 0, p); };
+  if (E <= 128) go(moe_i8_route_kernel<4>);
+  else if (E <= 256) go(moe_i8_route_kernel<8>);
+  else go(moe_i8_route_kernel<32>);
+  note_launch("moe_i8_route");
+  return launch_status();
+}
+
+int moe_i8_sum(const void* y, const float* weights, const int32_t* rows, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st) {
+  const int64_t total = T * (H / 8);
+  const int64_t g = (total + 255) / 256;
+  const dim3 grid((unsigned)(g < 148 * 8 ? g : 148 * 8));
+  auto go = [&](auto kern) {
+    launch_overlapped(kern, grid, dim3(256), 0, st, tls().overlap_mode > 0, reinterpret_cast<const uint16_t*>(y), weights, rows, reinterpret_cast<uint16_t*>(out), total, H / 8, k);
+  };
+  if (bf16) go(i8m::moe_i8_sum_kernel<true>); else go(i8m::moe_i8_sum_kernel<false>);
+  note_launch("moe_i8_sum");
+  return launch_status();
+}
+
+}  // namespace b2q
