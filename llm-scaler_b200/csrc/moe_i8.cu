@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_i8_kernel(const __grid_constan
       if (g < nx && r < sr && sr * rg + r < rows) add_shared(down_sums + rt.list[first + g] * p.row_cap + sr * rg + r, acc[c >> 1][c & 1]);
     }
   }
-  if (!ok && lane == 0) drain_issued(full, p.stages, item);      // copies of this warp's may be on their way
+  if (!ok && lane == 0) drain_issued(full, p.stages, item + p.stages);      // the copies of this item, and of this warp's other stages
   __syncwarp();
   asm volatile("bar.sync 2, %0;" ::"n"(HELPERS) : "memory");
   // The last CTA that has seen all flags lowers them: a graph's replays have the same mark.  (What a CTA that gave up leaves raised, the
@@ -627,7 +627,7 @@ template <bool BF16, int PER> static int run(Params& p, cudaStream_t st) {
   at[0].id = cudaLaunchAttributeCooperative;
   at[0].val.cooperative = 1;
   cfg.attrs = at; cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, tu, td, p) != cudaSuccess) return B2Q_ERR_CUDA;
+  cudaLaunchKernelEx(&cfg, kern, tu, td, p);               // launch_status() reports
   note_launch("moe_i8");
   return launch_status();
 }

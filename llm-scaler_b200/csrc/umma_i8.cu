@@ -458,7 +458,7 @@ static int launch_form(const CUtensorMap& tx, const CUtensorMap& tw, Params& p, 
     ++n;
   }
   cfg.attrs = at; cfg.numAttrs = n;
-  if (cudaLaunchKernelEx(&cfg, kern, tx, tw, p) != cudaSuccess) return B2Q_ERR_CUDA;
+  cudaLaunchKernelEx(&cfg, kern, tx, tw, p);               // launch_status() reports
   note_launch(PAIR ? "umma_i8_pair" : (SPLIT ? "umma_i8_split" : "umma_i8"));
   return launch_status();
 }
