@@ -47,7 +47,7 @@ struct Params {
   int* status;
 };
 
-struct Tile { int tok0, rows, n0, cols, w0, w1, e; };      // cols: valid outputs; w0: first weight row in memory, w1: of the up half
+struct Tile { int tok0, rows, n0, cols, w0, w1; };         // cols: valid outputs; w0: first weight row in memory, w1: of the up half
 
 template <bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(const Params& p, int id) {
   Tile t;
@@ -55,7 +55,6 @@ template <bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(cons
     const int ti = id / p.n_strips, st = id - ti * p.n_strips;
     const int e = p.tiles[4 + 2 * ti], r0 = p.tiles[4 + 2 * ti + 1];
     const int width = GATED ? p.h / 2 : p.h;
-    t.e = e;
     t.tok0 = p.offsets[e] + r0;
     t.rows = min(p.tok_rows, p.offsets[e + 1] - t.tok0);
     t.n0 = st * width;
@@ -66,7 +65,6 @@ template <bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(cons
     // m_group token tiles against all strips before the next group: what runs at one time shares both operands in L2
     const int per = p.m_group * p.n_strips, gi = id / per, left = id - gi * per, m0 = gi * p.m_group;
     const int gm = min(p.m_group, p.m_tiles - m0), st = left / gm, mt = m0 + left - st * gm;
-    t.e = 0;
     t.tok0 = mt * p.tok_rows;
     t.rows = min(p.tok_rows, p.M - t.tok0);
     t.n0 = st * p.h;
@@ -253,6 +251,7 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
     const uint32_t stg = base + stg_off + (warp - FIRST_EPI) * 2048;
     if constexpr (!GROUPED) grid_dep_wait();
     int it = 0;
+    bool ok = true;                                        // a warp that has given up still goes to the barrier where the others expect it
     for (int id = first; id < total; id += step, ++it) {
       const Tile t = tile_at<GROUPED, GATED>(p, id);
       const int b = it & 1;
@@ -273,7 +272,8 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       const int trow = (PAIR ? (int)rank * 128 : 0) + quad * 32 + lane;      // this lane's token within the tile
       const float xs = trow < t.rows ? ld_f32(p.xs + t.tok0 + trow) : 0.f;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI) : "memory");
-      if (!mbar_wait_warp(acc_full + 8 * b, (it >> 1) & 1, abort_flag, p.status, ST_ACCFULL)) break;
+      ok = ok && mbar_wait_warp(acc_full + 8 * b, (it >> 1) & 1, abort_flag, p.status, ST_ACCFULL);
+      if (!ok) continue;
       tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + b * 256;
       const int row0 = (PAIR ? (int)rank * 128 : 0) + quad * 32;
