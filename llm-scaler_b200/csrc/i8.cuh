@@ -144,9 +144,14 @@ __device__ __forceinline__ uint32_t i8_codes4_computed(const float (&x)[4], floa
 // Never contracted, so that every kernel gives the same bits.
 __device__ __forceinline__ float i8_scaled(int sum, float scale, float wscale) { return __fmul_rn(__fmul_rn((float)sum, scale), wscale); }
 __device__ __forceinline__ float i8_output(int sum, float scale, float wscale, float bias) { return __fadd_rn(i8_scaled(sum, scale, wscale), bias); }
+__device__ __forceinline__ float rcp_f(float v) {      // of 1 and more: to a unit in the last place, zero beyond 2^126
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 // To within a few units in the last place: codes are made from it, and each that lands on the other side of a half is a step off (with the
 // fast exponential an fp16 layer of 14336 wide experts was off by 4.3e-4 of its norm instead of 2.1e-4).
-__device__ __forceinline__ float silu_mul_f(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
+__device__ __forceinline__ float silu_mul_f(float g, float u) { return g * rcp_f(1.f + expf(-g)) * u; }
 
 // Bytes between two tokens' codes in shared memory: 64 apart in the banks, so that a quarter warp reads two tokens' 64 bytes without a conflict.
 __host__ __device__ constexpr int i8_code_pitch(int K) { return (K + 127) / 128 * 128 + 64; }

@@ -5,7 +5,9 @@
 // 1 / rms: it cancels out of v w / max |v w|, so that one reduction gives both the sum of squares and the maximum.
 //
 // Memory-bound: a row is read once and stays in registers between the maximum and the codes.  Rows of up to 1024 values take a warp
-// each, longer ones a CTA with one barrier; what is not 16-byte aligned, or longer than 1024 threads hold, is read twice.
+// each, longer ones a CTA with one barrier; what is not 16-byte aligned, or longer than 1024 threads hold, is read twice.  The exponential
+// and the division of SiLU keep an SM busy for half as long as the bytes take: where a row fills it (2048 x 28672: 68 us for 45 of bytes) the two add
+// up.  A ring of bulk copies ahead of such rows took 59 us, but 20 % longer than this with two CTAs per SM.
 #include "i8.cuh"
 
 namespace b2q {
@@ -28,6 +30,18 @@ __device__ __forceinline__ void enter() {                  // as in moe_aux.cu: 
   if (!few) grid_dep_release();
 }
 
+// The largest magnitude, NaN above all: half an instruction per value (as integers two: norm of 2047 x 8192 19.6 us for 17.0, SiLU 18.2 for 17.6).
+__device__ __forceinline__ float abs_max(float m, float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t abs_max2(uint32_t m, uint32_t v) {      // of two packed values at a time
+  uint32_t r;
+  if constexpr (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(v & 0x7FFF7FFFu));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(v & 0x7FFF7FFFu));
+  return r;
+}
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }      // orders as |v|, NaN above all
 
 // What a row's codes are made with: a stored row's exactly (row), a computed one's by r = 127 / a.
@@ -93,7 +107,7 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
   constexpr bool BF16 = DT == B2Q_BF16;
   const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x) + row * p.ldx * (DT == B2Q_F32 ? 2 : 1);
   Piece<MODE, DT> pc[V];
-  uint32_t mx = 0;
+  float top = 0.f;
   float sum = 0.f;
   if constexpr (MODE == PLAIN || MODE == COPIES || MODE == COMPUTED) {
 #pragma unroll
@@ -108,12 +122,19 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
         pc[i].v = c < n8 ? ld_vec(x + 8 * c) : make_uint4(0, 0, 0, 0);
       }
     }
+    if constexpr (DT == B2Q_F32) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float f[8];
-      pc[i].get(f);
+      for (int i = 0; i < V; ++i) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mx = max(mx, abs_bits(f[j]));
+        for (int j = 0; j < 8; j += 2) top = abs_max(top, pc[i].f[j], pc[i].f[j + 1]);
+      }
+    } else {
+      uint32_t two = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) two = abs_max2<BF16>(abs_max2<BF16>(abs_max2<BF16>(abs_max2<BF16>(two, pc[i].v.x), pc[i].v.y), pc[i].v.z), pc[i].v.w);
+      float a, b;
+      unpack2<BF16>(two, a, b);
+      top = abs_max(0.f, a, b);
     }
   } else if constexpr (MODE == SILU) {
     uint4 g[V], u[V];
@@ -130,10 +151,9 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
       unpack8<DT>(g[i], a);
       unpack8<DT>(u[i], b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        pc[i].f[j] = silu_mul_f(a[j], b[j]);
-        mx = max(mx, abs_bits(pc[i].f[j]));
-      }
+      for (int j = 0; j < 8; ++j) pc[i].f[j] = silu_mul_f(a[j], b[j]);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) top = abs_max(top, pc[i].f[j], pc[i].f[j + 1]);
     }
   } else {
     const uint16_t* rs = reinterpret_cast<const uint16_t*>(p.residual) + row * p.K;
@@ -161,21 +181,20 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
             make_uint4(pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3]), pack2<BF16>(a[4], a[5]), pack2<BF16>(a[6], a[7]));
       unpack8<DT>(w[i], b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        pc[i].f[j] = a[j] * b[j];
-        mx = max(mx, abs_bits(pc[i].f[j]));
-      }
+      for (int j = 0; j < 8; ++j) pc[i].f[j] = a[j] * b[j];
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) top = abs_max(top, pc[i].f[j], pc[i].f[j + 1]);
     }
   }
-  mx = __reduce_max_sync(0xffffffffu, mx);
+  uint32_t mx = __reduce_max_sync(0xffffffffu, abs_bits(top));
   if constexpr (MODE == NORM) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
   if constexpr (!WARP) {                                   // every warp finishes the reduction itself: one barrier
+    const bool in = lane < (int)(blockDim.x >> 5);
     if (lane == 0) { red_max[warp] = mx; if constexpr (MODE == NORM) red_sum[warp] = sum; }
     __syncthreads();
-    const bool in = lane < (int)(blockDim.x >> 5);
     mx = __reduce_max_sync(0xffffffffu, in ? red_max[lane] : 0u);
     if constexpr (MODE == NORM) {
       sum = in ? red_sum[lane] : 0.f;
@@ -299,13 +318,16 @@ template <int MODE, int DT> static int run_vec(const Params& p, cudaStream_t st)
     if (n8 <= 2048) return launch(quantize_i8_kernel<MODE, DT, 2, false>, p.M, block(2), st, p);
     return launch(quantize_i8_kernel<MODE, DT, 4, false>, p.M, block(4), st, p);
   }
-  // Many rows: smaller CTAs with more in flight each.  Stored rows of 2047 x 8192 with two / four / eight pieces a thread 11.8 / 12.0 / 10.4 us (4.8
-  // TB/s), 2048 x 28672 with four / eight 52.5 / 33.4 (5.3 TB/s), 4096 x 2048 with one / two / eight 7.2 / 6.4 / 6.8; the other forms hold floats, and
-  // eight pieces of those do not fit the registers: norm 2047 x 8192 with two / four 21.5 / 19.7, 4096 x 5120 23.6 / 24.4, SiLU 20.1 / 18.8 and 22.7 / 22.4.
+  // Two CTAs per SM at most (256 x 8192, with two / four / eight pieces a thread: stored rows 2.4 / 2.5 / 2.7 us, SiLU 3.5 / 4.2; norm 3.5 / 3.3).
+  if (MODE != NORM && p.M <= 296 && n8 <= 2048) return launch(quantize_i8_kernel<MODE, DT, 2, false>, p.M, block(2), st, p);
+  // Many rows: smaller CTAs with more in flight each.  Two / four / eight pieces: stored rows of 16384 x 1536 17.6 / 17.9 / 17.6 us, 4096 x 5120 13.2 / 11.8 /
+  // 12.9, 2047 x 8192 11.1 / 10.0 / 9.7 (5.2 TB/s), 2048 x 28672 - / 44.8 / 35.2 (5.0 TB/s).  The other forms hold floats, and eight pieces of those do
+  // not fit the registers: SiLU 16384 x 1536 24.9 / 28.5, 4096 x 2048 9.3 / 9.4, 4096 x 5120 21.8 / 20.4, 2047 x 8192 19.7 / 17.2; norm 4096 x 2048
+  // 8.5 / 7.7, 4096 x 5120 23.3 / 21.5, 2047 x 8192 21.2 / 17.0.
+  if (n8 < 256) return launch(quantize_i8_kernel<MODE, DT, 2, false>, p.M, block(2), st, p);
   if constexpr (MODE == PLAIN || MODE == COPIES) {
-    if (n8 > 256) return launch(quantize_i8_kernel<MODE, DT, 8, false>, p.M, block(8), st, p);
+    if (n8 > 768) return launch(quantize_i8_kernel<MODE, DT, 8, false>, p.M, block(8), st, p);
   }
-  if (n8 <= 768) return launch(quantize_i8_kernel<MODE, DT, 2, false>, p.M, block(2), st, p);
   return launch(quantize_i8_kernel<MODE, DT, 4, false>, p.M, block(4), st, p);
 }
 
