@@ -126,7 +126,7 @@ extern "C" {
 
 size_t b2q_moe_forward_int8_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I) {
   if (T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || top_k > 32 || H <= 0 || I <= 0 || T > INT32_MAX / 32) return 0;
-  if (moe_i8_few_supported(T, E, top_k, H, I)) return moe_i8_few_bytes(T, top_k, I);
+  if (moe_i8_few_preferred(T, E, top_k, H, I)) return moe_i8_few_bytes(T, top_k, I);
   return moe_parts(nullptr, T, (int)E, (int)top_k, H, I).total;
 }
 
@@ -147,7 +147,7 @@ int b2q_moe_forward_int8(const b2q_moe_int8* m, void* workspace, size_t workspac
   cudaStream_t st = (cudaStream_t)stream;
   const bool bf16 = a.act_dtype == B2Q_BF16;
   const int E = (int)a.E, k = (int)a.top_k, H = (int)a.H, I = (int)a.I;
-  if (moe_i8_few_supported(a.T, E, k, H, I)) {
+  if (moe_i8_few_preferred(a.T, E, k, H, I)) {
     I8FewArgs f{};
     f.x = a.x; f.bf16 = bf16; f.logits = a.logits; f.logits_dtype = a.logits_dtype;
     f.w13 = a.w13; f.s13 = a.s13; f.s13_dtype = a.s13_dtype; f.w2 = a.w2; f.s2 = a.s2; f.s2_dtype = a.s2_dtype;

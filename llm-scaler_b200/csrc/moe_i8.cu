@@ -633,11 +633,15 @@ template <bool BF16, int PER> static int run(Params& p, cudaStream_t st) {
 }
 }  // namespace mi8
 
-bool moe_i8_few_supported(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
+// Every CTA makes all tokens' codes and fetches all pairs' codes of h, which grows with the tokens while the weights' bytes do not; the grouped GEMMs
+// pay six launches instead.  Over 18 layers of 3 to 1395 MB with 1 to 16 tokens the line below took 1.005 times as long as the better of the two
+// (always one kernel 1.10, never 1.12).  One kernel / grouped, us: 8 experts of 4096 x 14336, top-2, 1 / 2 / 16 tokens 87 / 91, 141 / 125, 379 / 232; 128 of 2048 x 768,
+// top-8, 1 / 4 / 8 / 16: 19 / 28, 43 / 48, 67 / 65, 98 / 86; 8 of 2048 x 2048, top-8, 4 / 16: 38 / 41, 91 / 42; 8 of 1024 x 512, top-2, 16: 21 / 24.
+bool moe_i8_few_preferred(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
   using namespace mi8;
   if (T > MAX_TOK || E > MAX_E || k > MAX_K || H > INT32_MAX / 64 || I > INT32_MAX / 64) return false;
   const int64_t cap = (H + grid_of(H) - 1) / grid_of(H);
-  return T * i8_code_pitch((int)H) <= CODES_MAX && T * k * cap * 4 <= TABLE_MAX;
+  return T * (2 * k * I + H) <= 81920 && T * i8_code_pitch((int)H) <= CODES_MAX && T * k * cap * 4 <= TABLE_MAX;
 }
 
 size_t moe_i8_few_bytes(int64_t T, int64_t k, int64_t I) {

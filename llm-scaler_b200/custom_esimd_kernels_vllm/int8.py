@@ -75,5 +75,5 @@ def moe_forward_int8(x, router_logits, gate_up_weight, gate_up_scale, down_weigh
 
     gate_up_weight int8 [E, 2I, H] (gate rows, then up), gate_up_scale [E, 2I], down_weight int8 [E, H, I], down_scale [E, H]; x and the
     intermediate rows are quantised to int8 per row.  Weights of the chosen experts are their softmax, renormalised over the chosen or
-    not.  Up to sixteen tokens take one kernel."""
+    not.  A few tokens take one kernel."""
     return _ops.moe_forward(x, router_logits, gate_up_weight, gate_up_scale, down_weight, down_scale, top_k, renormalize)

@@ -39,9 +39,9 @@ def on_gpu(a):
     return [t.to(DEV) for t in a]
 
 
-def one_kernel(T, H):
-    """Whether the tokens' codes fit the shared memory of the one-kernel form."""
-    return T <= 16 and T * ((H + 127) // 128 * 128 + 64) <= 68 * 1024
+def one_kernel(T, k, H, I):
+    """Whether the layer takes one kernel: little that every CTA has to fetch, and tokens whose codes fit the shared memory."""
+    return T <= 16 and T * (2 * k * I + H) <= 81920 and T * ((H + 127) // 128 * 128 + 64) <= 68 * 1024
 
 
 def experts_interval(h, w2, s2, dt, few):
@@ -60,7 +60,7 @@ def experts_interval(h, w2, s2, dt, few):
 
 def check(out, a, k, renorm=True):
     x, logits, w13, s13, w2, s2 = a
-    few, dt = one_kernel(*x.shape), x.dtype
+    few, dt = one_kernel(x.shape[0], k, x.shape[1], w2.shape[2]), x.dtype
     ids, w = int8.route(logits, k, renorm)
     codes, _, scale = int8.quantize_rows(x)
     lo, hi = torch.zeros(2, *out.shape, dtype=torch.float64)
@@ -80,6 +80,7 @@ def check(out, a, k, renorm=True):
 
 SHAPES = [(1, 8, 2, 64, 32), (1, 128, 8, 2048, 768), (2, 16, 1, 128, 48), (3, 8, 2, 4096, 1024), (5, 60, 4, 1008, 176), (7, 4, 4, 144, 400), (8, 256, 8, 512, 256), (13, 128, 8, 1040, 528),
           (16, 128, 8, 2048, 768), (16, 3, 2, 6400, 64), (16, 512, 10, 256, 128), (4, 1024, 32, 64, 64), (16, 8, 2, 5120, 128),
+          (5, 128, 8, 2048, 768), (13, 128, 4, 1040, 528), (16, 128, 2, 2048, 768), (15, 40, 1, 4240, 64), (16, 40, 1, 4240, 64), (1, 3, 2, 512, 14336), (2, 4, 2, 512, 14336),
           (17, 128, 8, 512, 256), (33, 8, 2, 272, 144), (64, 16, 4, 1024, 512), (100, 60, 4, 512, 400), (300, 8, 2, 512, 1040), (257, 300, 6, 128, 64), (700, 4, 1, 256, 128)]
 
 
@@ -90,7 +91,7 @@ def test_expert_layer(ops, T, E, k, H, I, dt):
     a = make(T, E, H, I, dt, T * E + k, sdt)
     out = ops.moe_forward_int8(*on_gpu(a), k)
     assert out.shape == (T, H) and out.dtype == dt
-    assert (ops.last_kernel() == "moe_i8") == one_kernel(T, H)
+    assert (ops.last_kernel() == "moe_i8") == one_kernel(T, k, H, I)
     check(out, a, k)
 
 
