@@ -40,6 +40,7 @@ struct I8FewArgs {
   void* out; int T, E, k, H, I; bool renorm;
   void* scratch;                                           // moe_i8_few_bytes(), 256-byte aligned
 };
+constexpr int I8_FEW_LOAD = 40960;                         // most of T (4 k I + H)
 bool moe_i8_few_preferred(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I);
 size_t moe_i8_few_bytes(int64_t T, int64_t k, int64_t I);
 int moe_i8_few(const I8FewArgs& a, cudaStream_t st);

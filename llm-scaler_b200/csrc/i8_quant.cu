@@ -98,7 +98,12 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int step = WARP ? 32 : blockDim.x, first = WARP ? lane : threadIdx.x;
   const int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : (int64_t)blockIdx.x;
-  enter();
+  if constexpr (MODE == COPIES) {                          // the grouped GEMM behind reads the routing's tile list as soon as it begins
+    grid_dep_wait();
+    grid_dep_release();
+  } else {
+    enter();
+  }
   if (row >= p.M) return;                                  // whole warps, or the whole CTA
   if constexpr (MODE == PLAIN || MODE == COMPUTED) {
     if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;

@@ -37,7 +37,7 @@ constexpr int WARPS = 8, WORKERS = 32 * WARPS;              // the warps that mu
 constexpr int THREADS = 512, W_WARP = 15;                  // and the one that fetches weights; all sixteen route
 constexpr int HELPERS = 32 * W_WARP;                       // threads that make the tokens' codes, fill tables and store
 constexpr int MAX_TOK = I8_STREAM_MAX_TOK, MAX_K = 32, MAX_PAIRS = MAX_TOK * MAX_K, MAX_E = 1024;
-constexpr int CODES_MAX = 68 * 1024;                       // bytes of the tokens' codes in shared memory
+static_assert(I8_FEW_LOAD + MAX_TOK * 192 <= 68 * 1024, "the tokens' codes leave the ring its shared memory");
 constexpr int PASS = 16;                                   // groups of eight columns whose sums are held at a time
 constexpr int TABLE_MAX = 24 * 1024;                       // bytes of the down part's sums, and of its scales
 constexpr int XR = 4;                                      // pairs of a down stage; an expert with more fetches its rows again, from L2
@@ -634,14 +634,15 @@ template <bool BF16, int PER> static int run(Params& p, cudaStream_t st) {
 }  // namespace mi8
 
 // Every CTA makes all tokens' codes and fetches all pairs' codes of h, which grows with the tokens while the weights' bytes do not; the grouped GEMMs
-// pay six launches instead.  Over 18 layers of 3 to 1395 MB with 1 to 16 tokens the line below took 1.005 times as long as the better of the two
-// (always one kernel 1.10, never 1.12).  One kernel / grouped, us: 8 experts of 4096 x 14336, top-2, 1 / 2 / 16 tokens 87 / 91, 141 / 125, 379 / 232; 128 of 2048 x 768,
-// top-8, 1 / 4 / 8 / 16: 19 / 28, 43 / 48, 67 / 65, 98 / 86; 8 of 2048 x 2048, top-8, 4 / 16: 38 / 41, 91 / 42; 8 of 1024 x 512, top-2, 16: 21 / 24.
+// pay six launches instead, four of them under the weights that a GEMM fetches in advance.  Over 18 layers of 3 to 1395 MB with 1 to 16 tokens the line
+// below took 1.003 times as long as the better of the two (always one kernel 1.18, never 1.013).  One kernel / grouped, us: 128 experts of 2048 x 768, top-8,
+// 1 / 2 / 4 / 16 tokens 19.3 / 21.7, 29.5 / 29.9, 43.2 / 40.8, 97.9 / 83.3; 16 of 4096 x 1024, top-1, 1 / 8: 16.0 / 19.6, 30.8 / 30.5; 8 of 4096 x 14336, top-2, 1 / 16:
+// 87.6 / 76.2, 416 / 229; 8 of 1024 x 512, top-2, 1 / 16: 15.6 / 16.3, 20.8 / 18.3; 8 of 2048 x 2048, top-8, 16: 91.3 / 36.6.
 bool moe_i8_few_preferred(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
   using namespace mi8;
   if (T > MAX_TOK || E > MAX_E || k > MAX_K || H > INT32_MAX / 64 || I > INT32_MAX / 64) return false;
   const int64_t cap = (H + grid_of(H) - 1) / grid_of(H);
-  return T * (2 * k * I + H) <= 81920 && T * i8_code_pitch((int)H) <= CODES_MAX && T * k * cap * 4 <= TABLE_MAX;
+  return T * (4 * k * I + H) <= I8_FEW_LOAD && T * k * cap * 4 <= TABLE_MAX;
 }
 
 size_t moe_i8_few_bytes(int64_t T, int64_t k, int64_t I) {

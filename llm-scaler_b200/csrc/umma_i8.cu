@@ -43,7 +43,7 @@ struct Params {
   int tok_rows, tok_box;                                   // tokens per tile; rows of the token box
   int stages, a_bytes, stage_bytes, split;
   const int32_t* tiles; const int32_t* offsets;            // grouped
-  int early;
+  int early;                                               // dense: weights may be read before the kernels in front are done
   int* status;
 };
 
@@ -53,10 +53,10 @@ template <bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(cons
   Tile t;
   if constexpr (GROUPED) {
     const int ti = id / p.n_strips, st = id - ti * p.n_strips;
-    const int e = p.tiles[4 + 2 * ti], r0 = p.tiles[4 + 2 * ti + 1];
+    const int e = __ldcg(p.tiles + 4 + 2 * ti), r0 = __ldcg(p.tiles + 4 + 2 * ti + 1);      // from L2: they may be read early
     const int width = GATED ? p.h / 2 : p.h;
-    t.tok0 = p.offsets[e] + r0;
-    t.rows = min(p.tok_rows, p.offsets[e + 1] - t.tok0);
+    t.tok0 = __ldcg(p.offsets + e) + r0;
+    t.rows = min(p.tok_rows, __ldcg(p.offsets + e + 1) - t.tok0);
     t.n0 = st * width;
     t.cols = min(width, p.N - t.n0);
     t.w0 = (GATED ? 2 : 1) * e * p.N + t.n0;
@@ -144,9 +144,10 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
   if constexpr (PAIR) cluster_sync_all();                  // both CTAs' barriers exist before anything is signalled across
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // the tile list comes from the kernels in front; a dense launch knows its tiles
-  if constexpr (GROUPED) grid_dep_wait();
-  const int total = GROUPED ? p.tiles[0] * p.n_strips : p.total;
+  // A dense launch knows its tiles.  A grouped one has their list, and its weights, as soon as it begins: that is when the tokens' codes are being made at
+  // the earliest, and the kernel that makes them lets it begin only once it has itself seen the routing, and so all that came before, done (COPIES in
+  // i8_quant.cu).  16 tokens, 8 experts of 4096 x 2048, top-2: 55 -> 50 us.
+  const int total = GROUPED ? __ldcg(p.tiles) * p.n_strips : p.total;
 
   if (warp == 0) {
     // ---- weights; boxes that begin beyond K read as zero ----
@@ -157,7 +158,6 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       int s = 0, issued = 0;
       uint32_t par = 1u;
       bool ok = true;
-      // a dense launch's weights do not depend on the kernels in front
       if (!GROUPED && !p.early) grid_dep_wait();
       for (int id = first; ok && id < total; id += step) {
         const Tile t = tile_at<GROUPED, GATED>(p, id);
@@ -191,7 +191,7 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       int s = 0, issued = 0;
       uint32_t par = 1u;
       bool ok = true;
-      if constexpr (!GROUPED) grid_dep_wait();
+      grid_dep_wait();
       for (int id = first; ok && id < total; id += step) {
         const Tile t = tile_at<GROUPED, GATED>(p, id);
         for (int ks = ks0; ks < ks1; ++ks) {
@@ -249,7 +249,7 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
     // ---- epilogue: lane quadrant = warp & 3 (tokens), column chunks of 32 shared by the two warps of a quadrant ----
     const int quad = warp & 3, half = (warp - FIRST_EPI) >> 2, etid = threadIdx.x - 32 * FIRST_EPI;
     const uint32_t stg = base + stg_off + (warp - FIRST_EPI) * 2048;
-    if constexpr (!GROUPED) grid_dep_wait();
+    grid_dep_wait();
     int it = 0;
     bool ok = true;                                        // a warp that has given up still goes to the barrier where the others expect it
     for (int id = first; id < total; id += step, ++it) {
@@ -557,7 +557,12 @@ int umma_i8_grouped(const I8GroupedArgs& a, cudaStream_t st) {
   p.tiles = a.tiles; p.offsets = a.offsets; p.split = 1;
   p.status = umma_status_ptr();
   if (!p.status) return B2Q_ERR_CUDA;
-  const int most = a.gated ? 128 : 256;                    // outputs of a tile
+  // Outputs of a tile: 128 gated, 256 otherwise, and half of that where there may be no more than two tiles per SM, which halves the last round
+  // (6 tokens, 8 experts of 2048 x 2048, top-8, 37.4 -> 34.5 us; 16, 16 of 1024 x 4096, top-8, 56.0 -> 53.2; 24, 16 of 2048 x 2048, top-4, 53.9 -> 50.4).  With
+  // more tiles it costs: 4096 tokens, 128 experts of 2048 x 768, top-8, 300 -> 392 us.
+  const int token_tiles = (a.rows + a.tile - 1) / a.tile, experts = a.E < a.rows ? a.E : a.rows, likely = token_tiles > experts ? token_tiles : experts;
+  int most = a.gated ? 128 : 256;
+  if ((int64_t)likely * ((a.N + most - 1) / most) <= 2 * sm_count()) most /= 2;
   p.n_strips = (a.N + most - 1) / most;
   const int width = round_up((a.N + p.n_strips - 1) / p.n_strips, 16);
   p.h = a.gated ? 2 * width : width;
