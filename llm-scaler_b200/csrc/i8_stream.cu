@@ -1,4 +1,4 @@
-// Int8 linear of up to sixteen tokens: out[m, n] = scale[m] wscale[n] sum_k codes[m, k] w[n, k] (+ bias[n]).
+// Int8 linear of up to sixteen tokens and 20 Mi weights: out[m, n] = scale[m] wscale[n] sum_k codes[m, k] w[n, k] (+ bias[n]).
 //
 // HBM-bound: the weights are read once and nothing else is large.  They go from global memory straight into the registers that
 // mma.sync m16n8k32 takes them from: with the k of a 64-byte piece permuted the same way on both sides, a lane's sixteen bytes of a weight
@@ -9,6 +9,9 @@
 // loads per lane (32 rows x 128 k, 16 x 256 or 8 x 512), an equal run of units each; the next unit's loads are on their way while a unit is
 // multiplied.  Integer sums are exact in any order, so warps that share rows add into shared memory by atomics and every result is
 // bit-identical whatever the division.
+//
+// 3 x 17408 x 5120 ran at 5.6 TB/s in umma_i8.cu, whose ring keeps more in flight per SM; below 20 Mi weights there is too little of that to matter, and
+// this starts sooner: 1 x 2048 x 2048 3.1 us, of which 0.65 are the bytes'.
 //
 // The 16-bit form quantises the tokens by itself: each CTA makes all codes in its shared memory while its first weights arrive.
 #include "i8.cuh"
