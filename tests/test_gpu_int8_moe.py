@@ -153,6 +153,24 @@ def test_few_tokens_take_one_kernel(ops):
     assert ops.launch_count() - before == 1 and ops.last_kernel() == "moe_i8"
 
 
+@pytest.mark.parametrize("mode", [0, 1])
+@pytest.mark.parametrize("T", [2, 16, 60, 300])
+def test_weights_written_right_before_the_layer(ops, T, mode):
+    """Only overlap mode 2 declares weights static: before it, a layer sees what the kernel in front of it has written."""
+    sets = [on_gpu(make(T, 16, 512, 256, torch.bfloat16, seed)) for seed in (7, 8)]
+    x, logits = sets[0][:2]
+    ops.set_overlap_mode(0)
+    refs = [ops.moe_forward_int8(x, logits, *a[2:], 4) for a in sets]
+    assert not torch.equal(*refs)
+    ops.set_overlap_mode(mode)
+    now = [t.clone() for t in sets[0][2:]]
+    for i in range(30):
+        for t, v in zip(now, sets[i % 2][2:]):
+            t.copy_(v)
+        assert torch.equal(ops.moe_forward_int8(x, logits, *now, 4), refs[i % 2])
+    ops.set_overlap_mode(1)
+
+
 @pytest.mark.parametrize("mode", [0, 1, 2])
 @pytest.mark.parametrize("T", [1, 16, 60])
 def test_layers_behind_one_another(ops, T, mode):
