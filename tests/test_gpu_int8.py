@@ -250,6 +250,25 @@ def test_empty_batches(ops):
     assert ops.silu_mul_quantize_int8(torch.empty(0, 64, dtype=torch.float16, device=DEV))[0].shape == (0, 32)
 
 
+def test_offsets_beyond_32_bits(ops):
+    """Rows and outputs of more than 2^31 elements: every block of rows like the first."""
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(1000, 32768, generator=g).bfloat16().to(DEV)
+    q, s = ops.quantize_int8(x)
+    many_q, many_s = ops.quantize_int8(x.repeat(70, 1))
+    assert many_q.numel() > 2 ** 31
+    assert (many_q.view(70, 1000, -1) == q).all() and (many_s.view(70, 1000) == s).all()
+    del many_q, many_s
+    many_q, many_s = ops.silu_mul_quantize_int8(x.repeat(135, 1))
+    q, s = ops.silu_mul_quantize_int8(x)
+    assert many_q.numel() > 2 ** 31 and (many_q.view(135, 1000, -1) == q).all() and (many_s.view(135, 1000) == s).all()
+    del many_q, many_s
+    codes, scale, w, ws, _ = [t.to(DEV) for t in make_linear(1000, 16384, 64, 3)]
+    out = ops.linear_int8(codes, scale, w, ws)
+    many = ops.linear_int8(codes.repeat(140, 1), scale.repeat(140), w, ws)
+    assert many.numel() > 2 ** 31 and (many.view(140, 1000, -1) == out).all()
+
+
 def test_refusals(ops):
     q, s = torch.zeros(4, 64, dtype=torch.int8, device=DEV), torch.ones(4, device=DEV)
     w, ws = torch.zeros(32, 64, dtype=torch.int8, device=DEV), torch.ones(32, device=DEV)

@@ -3,8 +3,8 @@
 No tolerance on the output: an interval that holds it is followed through the layer.  h is known to 2^-17 (SiLU's exponential is good to 10
 units of 2^-23 for |gate| <= 7, each fp32 step to 2^-24), routing weights to 2^-19.  Rounding is monotone, so the ends of h's interval, rounded
 as the layer rounds them, give the ends of its row's scale and of every code; nearly all codes have equal ends.  What the others can differ
-by, times |w2|, is the interval of an expert's output, which the remaining steps (rounded to 16 bits before the weighted sum, for more than
-sixteen tokens) map to the result's."""
+by, times |w2|, is the interval of an expert's output, which the remaining steps (rounded to 16 bits before the weighted sum, where the layer
+takes more than one kernel) map to the result's."""
 import math
 
 import pytest
@@ -151,6 +151,22 @@ def test_few_tokens_take_one_kernel(ops):
     before = ops.launch_count()
     ops.moe_forward_int8(*a, 8)
     assert ops.launch_count() - before == 1 and ops.last_kernel() == "moe_i8"
+
+
+@pytest.mark.parametrize("T", [2, 40])
+def test_weights_of_more_than_4_gb(ops, T):
+    E, H, I, used = 520, 2048, 2048, [3, 519]
+    a = make(T, 2, H, I, torch.bfloat16, T)
+    assert one_kernel(T, 2, H, I) == (T == 2)
+    whole = []
+    for t in a[2:]:
+        v = torch.zeros(E, *t.shape[1:], dtype=t.dtype, device=DEV)
+        v[used] = t.to(DEV)
+        whole.append(v)
+    assert whole[0].numel() > 2 ** 32
+    logits = torch.full((T, E), -50.0)
+    logits[:, used] = a[1]
+    check(ops.moe_forward_int8(a[0].to(DEV), logits.to(DEV), *whole, 2), a, 2)
 
 
 @pytest.mark.parametrize("mode", [0, 1])
