@@ -437,6 +437,8 @@ static int launch_form(const CUtensorMap& tx, const CUtensorMap& tw, Params& p, 
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   int bytes = p.stages * p.stage_bytes;
   if (SPLIT && bytes < (p.tok_box < 32 ? 32 : p.tok_box) * (p.h + 4) * 4) return B2Q_ERR_LIMIT;      // partial sums use the stages' room
+  // Never less than 165 KB (16 stages of 8 KB), so that no other CTA with tensor memory fits beside this one.  A kernel lets the next one begin before it has
+  // allocated its own; were both on an SM, it could wait for columns that the next one holds while that waits for it.
   const int smem = 1024 + bytes + over + TAIL;
   auto kern = umma_i8_kernel<KPS, PAIR, SPLIT, GROUPED, GATED>;
   static thread_local bool configured[16] = {false};
