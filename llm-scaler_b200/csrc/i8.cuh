@@ -28,7 +28,7 @@ int umma_i8_linear(const I8LinearArgs& a, cudaStream_t st);
 struct I8GroupedArgs {
   const int8_t* xq; const float* xs; const int8_t* w; const void* ws; int ws_dtype;
   const int32_t* offsets; const int32_t* tiles; int tile, tile_cap, E;      // tile list of this height (i8_grouped_tile)
-  void* out; bool out_bf16; int rows, N, K; bool gated;    // gated: out is fp32
+  void* out; bool out_bf16, out_f32; int rows, N, K; bool gated;      // gated: out is fp32 too
 };
 int i8_grouped_tile(int64_t rows, int E);
 int umma_i8_grouped(const I8GroupedArgs& a, cudaStream_t st);
@@ -66,7 +66,7 @@ int resadd_rmsnorm_quantize_i8(const void* hidden, const void* residual, const v
 int moe_i8_route_ctas(int64_t T);
 int moe_i8_route(const void* logits, int dt, int64_t T, int E, int k, bool renorm, int tile, float* weights, int32_t* ids, int32_t* place, int32_t* base,
                  int32_t* offsets, int32_t* tiles, void* count, cudaStream_t st);
-int moe_i8_sum(const void* y, const float* weights, const int32_t* rows, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st);
+int moe_i8_sum(const void* y, bool y_f32, const float* weights, const int32_t* rows, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st);
 
 #ifdef __CUDACC__
 // Ordinary loads, never by the read-only path: these kernels begin while the kernel that writes their inputs is still running.  Volatile

@@ -6,7 +6,7 @@
 // of a CTA's pairs comes first is a matter of chance, and no result depends on it: a row of the sorted order does not see the others.
 // 4096 tokens, 128 experts, top-8: five launches of 27 us before (top-k, a stable sort in three, tiles).
 //
-// Weighted sum.  Memory-bound; a thread has eight columns of a token and requests eight experts' rows at a time.
+// Weighted sum.  Memory-bound; a thread has eight columns of a token and requests eight experts' rows at a time, or four in fp32.
 #include "arrivals.cuh"
 #include "i8.cuh"
 #include "i8_route.cuh"
@@ -128,35 +128,44 @@ __global__ void __launch_bounds__(THREADS) moe_i8_route_kernel(const Params p) {
   if (threadIdx.x == 0) { p.offsets[p.E] = before; p.tiles[0] = tiles_before; }
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(256) moe_i8_sum_kernel(const uint16_t* y, const float* weights, const int32_t* rows, uint16_t* out, int64_t total, int H8, int k) {
+// F32: y is
+template <bool BF16, bool F32>
+__global__ void __launch_bounds__(256) moe_i8_sum_kernel(const void* y, const float* weights, const int32_t* rows, uint16_t* out, int64_t total, int H8, int k) {
+  constexpr int AT_ONCE = F32 ? 4 : 8;                     // experts whose rows are on their way together
   enter();
   const int64_t H = (int64_t)H8 * 8;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const int64_t t = i / H8, c = (i - t * H8) * 8;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < k; s0 += 8) {
-      uint4 v[8];
-      float w[8];
-      int32_t r[8];
+    for (int s0 = 0; s0 < k; s0 += AT_ONCE) {
+      uint4 v[AT_ONCE][F32 ? 2 : 1];
+      float w[AT_ONCE];
+      int32_t r[AT_ONCE];
 #pragma unroll
-      for (int s = 0; s < 8; ++s) r[s] = s0 + s < k ? __ldcg(rows + t * k + s0 + s) : -1;
+      for (int s = 0; s < AT_ONCE; ++s) r[s] = s0 + s < k ? __ldcg(rows + t * k + s0 + s) : -1;
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        v[s] = r[s] >= 0 ? __ldcg(reinterpret_cast<const uint4*>(y + r[s] * H + c)) : make_uint4(0, 0, 0, 0);
+      for (int s = 0; s < AT_ONCE; ++s) {
+        const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(y) + (r[s] * H + c) * (F32 ? 4 : 2));
+#pragma unroll
+        for (int h = 0; h < (F32 ? 2 : 1); ++h) v[s][h] = r[s] >= 0 ? __ldcg(from + h) : make_uint4(0, 0, 0, 0);
         w[s] = r[s] >= 0 ? __ldcg(weights + t * k + s0 + s) : 0.f;
       }
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
+      for (int s = 0; s < AT_ONCE; ++s) {
         if (r[s] < 0) continue;
-        const uint32_t e[4] = {v[s].x, v[s].y, v[s].z, v[s].w};
+        float f[8];
+        if constexpr (F32) {
+          const uint4 a = v[s][0], b = v[s][1];
+          const uint32_t e[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float a, b;
-          unpack2<BF16>(e[j], a, b);
-          acc[2 * j] = fmaf(w[s], a, acc[2 * j]);
-          acc[2 * j + 1] = fmaf(w[s], b, acc[2 * j + 1]);
+          for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(e[j]);
+        } else {
+          const uint32_t e[4] = {v[s][0].x, v[s][0].y, v[s][0].z, v[s][0].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) unpack2<BF16>(e[j], f[2 * j], f[2 * j + 1]);
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = fmaf(w[s], f[j], acc[j]);
       }
     }
     *reinterpret_cast<uint4*>(out + t * H + c) =
@@ -188,14 +197,13 @@ int moe_i8_route(const void* logits, int dt, int64_t T, int E, int k, bool renor
   return launch_status();
 }
 
-int moe_i8_sum(const void* y, const float* weights, const int32_t* rows, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st) {
+int moe_i8_sum(const void* y, bool y_f32, const float* weights, const int32_t* rows, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st) {
   const int64_t total = T * (H / 8);
   const int64_t g = (total + 255) / 256;
   const dim3 grid((unsigned)(g < 148 * 8 ? g : 148 * 8));
-  auto go = [&](auto kern) {
-    launch_overlapped(kern, grid, dim3(256), 0, st, tls().overlap_mode > 0, reinterpret_cast<const uint16_t*>(y), weights, rows, reinterpret_cast<uint16_t*>(out), total, H / 8, k);
-  };
-  if (bf16) go(i8m::moe_i8_sum_kernel<true>); else go(i8m::moe_i8_sum_kernel<false>);
+  auto go = [&](auto kern) { launch_overlapped(kern, grid, dim3(256), 0, st, tls().overlap_mode > 0, y, weights, rows, reinterpret_cast<uint16_t*>(out), total, H / 8, k); };
+  if (y_f32) { if (bf16) go(i8m::moe_i8_sum_kernel<true, true>); else go(i8m::moe_i8_sum_kernel<false, true>); }
+  else { if (bf16) go(i8m::moe_i8_sum_kernel<true, false>); else go(i8m::moe_i8_sum_kernel<false, false>); }
   note_launch("moe_i8_sum");
   return launch_status();
 }

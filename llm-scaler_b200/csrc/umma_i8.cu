@@ -39,6 +39,7 @@ constexpr int OVERREAD = 16384;                            // an MMA reads 128 t
 struct Params {
   const float* xs; const void* ws; int ws_dtype; const void* bias;
   uint16_t* out; int64_t ldo; int out_bf16, vec_out;
+  int out_f32;                                             // grouped, not gated
   int M, N;
   int nks;                                                 // stages that K takes
   int h;                                                   // weight rows (MMA columns) per tile
@@ -293,7 +294,7 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
             if (c + i < p.h) sts128(at + i * 4, r[i], r[i + 1], r[i + 2], r[i + 3]);
         }
       } else {
-        if constexpr (GATED) {
+        if (GATED || (GROUPED && p.out_f32)) {
           // sixteen outputs in fp32 at a time
           float* out = reinterpret_cast<float*>(p.out) + (int64_t)(t.tok0 + row0) * p.ldo + t.n0;
           const float* us = sc + p.h / 2;
@@ -301,7 +302,7 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
           uint32_t r[16], u[16], v[16];
           auto fetch = [&](int c) {
             tmem_ld16(acc + c, r);
-            tmem_ld16(acc + p.h / 2 + c, u);
+            if constexpr (GATED) tmem_ld16(acc + p.h / 2 + c, u);
           };
           if (half * 16 < end) fetch(half * 16);
           for (int c = half * 16; c < end; c += 32) {
@@ -310,11 +311,13 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
             const float4* u4 = reinterpret_cast<const float4*>(us + c);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float4 gs = g4[i], uv = u4[i];
+              const float4 gs = g4[i], uv = GATED ? u4[i] : gs;
               const float gv[4] = {gs.x, gs.y, gs.z, gs.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                v[4 * i + j] = __float_as_uint(silu_mul_f(i8_scaled((int)r[4 * i + j], xs, gv[j]), i8_scaled((int)u[4 * i + j], xs, uw[j])));
+              for (int j = 0; j < 4; ++j) {
+                const float y = i8_scaled((int)r[4 * i + j], xs, gv[j]);
+                v[4 * i + j] = __float_as_uint(GATED ? silu_mul_f(y, i8_scaled((int)u[4 * i + j], xs, uw[j])) : y);
+              }
             }
             if (c + 32 < end) fetch(c + 32);               // on its way while these are stored
             stage_rows(stg, lane, v);
@@ -558,6 +561,7 @@ int umma_i8_grouped(const I8GroupedArgs& a, cudaStream_t st) {
   Params p{};
   p.xs = a.xs; p.ws = a.ws; p.ws_dtype = a.ws_dtype;
   p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.N; p.out_bf16 = a.out_bf16; p.vec_out = aligned16(a.out) && a.N % 8 == 0;
+  p.out_f32 = a.out_f32;
   p.M = a.rows; p.N = a.N;
   p.tiles = a.tiles; p.offsets = a.offsets; p.split = 1;
   p.status = umma_status_ptr();

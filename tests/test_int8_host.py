@@ -105,7 +105,7 @@ def test_expert_layer_scratch(L, T, E, k, H, I):
     """Two buffers of h at least: fp32 and codes; with more tokens also each pair's codes of x and output."""
     rows, got = T * k, L.lib.b2q_moe_forward_int8_workspace_bytes(T, E, k, H, I)
     few = T <= 16 and T * (4 * k * I + H) <= 40960
-    least = rows * 5 * I + (0 if few else rows * 3 * H)
+    least = rows * 5 * I + (0 if few else rows * H * (5 if rows * H <= 1 << 19 else 3))
     assert least <= got <= least + 64 * rows + 300 * E + 8192
 
 
