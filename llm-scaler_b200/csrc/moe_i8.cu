@@ -25,6 +25,7 @@
 #include "arrivals.cuh"
 #include "i8.cuh"
 #include "i8_route.cuh"
+#include "moe_i8_sizes.h"
 #include "sm100.cuh"
 #include "umma_gemm.cuh"
 
@@ -34,17 +35,10 @@ using namespace sm100;
 
 namespace mi8 {
 enum { ST_EMPTY = 901, ST_UP_FULL = 902, ST_DOWN_FULL = 903, ST_FLAG = 904 };
-constexpr int WARPS = 8, WORKERS = 32 * WARPS;              // the warps that multiply
-constexpr int THREADS = 512, W_WARP = 15;                  // and the one that fetches weights; all sixteen route
+constexpr int THREADS = 512, W_WARP = 15;                  // the warp that fetches weights, beside those that multiply; all sixteen route
 constexpr int HELPERS = 32 * W_WARP;                       // threads that make the tokens' codes, fill tables and store
-constexpr int MAX_TOK = I8_STREAM_MAX_TOK, MAX_K = 32, MAX_PAIRS = MAX_TOK * MAX_K, MAX_E = 1024;
+static_assert(MAX_TOK == I8_STREAM_MAX_TOK, "");
 static_assert(I8_FEW_LOAD + MAX_TOK * 192 <= 68 * 1024, "the tokens' codes leave the ring its shared memory");
-constexpr int PASS = 16;                                   // groups of eight columns whose sums are held at a time
-constexpr int TABLE_MAX = 24 * 1024;                       // bytes of the down part's sums, and of its scales
-constexpr int XR = 4;                                      // pairs of a down stage; an expert with more fetches its rows again, from L2
-constexpr int PIECE = 2048;                                // longest k of a stage: 256 elements of eight bytes in a TMA box
-constexpr int MAX_STAGES = 32, BAR_BYTES = 16 * MAX_STAGES + 16;
-constexpr int SMEM_MAX = 232448 - 1024;                    // of a CTA, static part included
 
 struct Params {
   const uint16_t* x; const void* logits; int ldt;
@@ -77,6 +71,7 @@ struct Route {
   int slots, chunks;
   __device__ __forceinline__ int chunk_pairs(int c) const { return min(XR, slot_first[chunk_slot[c] + 1] - chunk_first[c]); }
 };
+static_assert(sizeof(Route) + sizeof(I8Tokens) + 4 * (WORKERS + MAX_PAIRS) <= STATIC_BYTES, "");
 
 template <int PER> __device__ __forceinline__ void route_token(const Params& p, int tok, const float (&v)[PER], Route& r) {
   int id;
@@ -212,13 +207,14 @@ __device__ __forceinline__ void multiply(int (&acc)[4], uint32_t w, uint32_t xa,
   for (int c = 0; c < 4; ++c) acc[c] += more[c];
 }
 
-// Sixteen weight rows, at u and v, against up to eight rows of codes at x.
-__device__ __forceinline__ void multiply16(int (&acc)[2][4], uint32_t u, uint32_t v, uint32_t x, bool has, int len) {
+// Nine to sixteen weight rows, at u and, where second says that the lane has one there, at v, against up to eight rows of codes at x.
+__device__ __forceinline__ void multiply16(int (&acc)[2][4], uint32_t u, uint32_t v, uint32_t x, bool has, bool second, int len) {
   const int t16 = 16 * (threadIdx.x & 3);
   int more[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
   auto step = [&](int k, bool in) {
     uint4 a = make_uint4(0, 0, 0, 0), b = a, c = a;
-    if (in) { b = lds(u + k); c = lds(v + k); }
+    if (in) b = lds(u + k);
+    if (in && second) c = lds(v + k);                      // a stage ends behind its own rows
     if (in && has) a = lds(x + k);
     mma_s8(acc[0], a.x, 0u, a.y, 0u, b.x, b.y);
     mma_s8(acc[1], a.x, 0u, a.y, 0u, c.x, c.y);
@@ -530,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_i8_kernel(const __grid_constan
     const uint32_t w = ring + stage * p.stage_bytes + g * p.down_piece + 16 * t, x = ring + stage * p.stage_bytes + sr * p.down_piece + g * (p.down_piece + 16) + 16 * t;
     const int len = min(p.down_piece, p.I - k0), left = rows - sr * rg;
     int acc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    if (sr > 8 && left > 8) multiply16(acc, w, w + 8 * p.down_piece, x, g < nx, len);
+    if (sr > 8 && left > 8) multiply16(acc, w, w + 8 * p.down_piece, x, g < nx, g + 8 < min(sr, left), len);
     else multiply(acc[0], w, x, 0, g < nx, false, len);
     if (k0 + len == p.I && rg == 0 && t == 0 && g < nx) {
       uint32_t v;
@@ -579,33 +575,13 @@ static int sm_count() {
 }
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 static int grid_of(int64_t H) { return (int)(sm_count() < H ? sm_count() : H); }
-static int room(int fixed) { return SMEM_MAX - (int)sizeof(Route) - (int)sizeof(I8Tokens) - 4 * (WORKERS + MAX_PAIRS) - 256 - fixed; }
-
-// k of a stage: the whole row where six stages of that fit, else what fits (a TMA box has 2048 bytes of a row at most)
-static int piece_of(int K, int rows, int more, int fixed) {
-  const int fits = (room(fixed) / 6 - more) / rows;
-  if (K <= fits && K <= PIECE) return K;
-  const int v = fits < PIECE ? fits : PIECE;
-  return v / 64 * 64;
-}
 
 template <bool BF16, int PER> static int run(Params& p, cudaStream_t st) {
-  const int grid = grid_of(p.H), pairs = p.T * p.k, xr = p.T < XR ? p.T : XR;
-  p.pitch = i8_code_pitch(p.H);
-  p.row_cap = (p.H + grid - 1) / grid;
-  const int tables = 2 * pairs * p.row_cap * 4;
-  p.front = (int)align256(p.T * p.pitch > tables ? p.T * p.pitch : tables);
-  const int fixed = p.front + 2 * PASS * p.T * 16 * 4 + BAR_BYTES;
-  p.up_piece = piece_of(p.H, 8, 0, fixed);
-  // up to sixteen rows that are one run of memory, if there are more than eight and they fit; else eight
-  const int most = p.row_cap < 16 ? p.row_cap : 16;
-  p.down_rows = p.row_cap > 8 && piece_of(p.I, most + xr, 16 * xr, fixed) == p.I ? most : 8;
-  p.down_piece = piece_of(p.I, p.down_rows + xr, 16 * xr, fixed);
-  const int up = 8 * p.up_piece, down = p.down_rows * p.down_piece + xr * (p.down_piece + 16);
-  p.stage_bytes = ((up > down ? up : down) + 127) / 128 * 128;
-  p.stages = room(fixed) / p.stage_bytes;
-  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-  const int smem = p.stages * p.stage_bytes + fixed;
+  const Sizes s = sizes_of(p.T, p.k, p.H, p.I, i8_code_pitch(p.H), sm_count());
+  const int grid = s.grid, smem = s.smem;
+  p.pitch = s.pitch; p.row_cap = s.row_cap; p.front = s.front;
+  p.up_piece = s.up_piece; p.down_piece = s.down_piece; p.down_rows = s.down_rows;
+  p.stages = s.stages; p.stage_bytes = s.stage_bytes;
   CUtensorMap tu{}, td{};
   int rc = B2Q_OK;
   if (p.up_piece < p.H)
