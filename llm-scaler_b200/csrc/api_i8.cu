@@ -104,7 +104,8 @@ int b2q_linear_int8_dynamic(const void* x, int act_dtype, int64_t ldx, const int
 namespace {
 // Workspace of an expert layer in its grouped form, part by part.
 // Each expert's output for each of its rows: in fp32 for decode batches, where it costs nothing (16 tokens, 128 experts of 2048 x 768, top-8: 85 us either way), so that
-// their results are the one-kernel form's, bit for bit; beyond, in 16 bits of act_dtype (256 tokens 127 us, in fp32 137).
+// their results are the one-kernel form's, bit for bit; beyond, in 16 bits of act_dtype (256 tokens 127 us, in fp32 137), but for outputs that those cannot hold, which
+// the weighted sum makes anew.
 bool moe_y_f32(size_t elements) { return elements <= (size_t)1 << 19; }
 
 struct MoeParts {
@@ -179,7 +180,8 @@ int b2q_moe_forward_int8(const b2q_moe_int8* m, void* workspace, size_t workspac
   if (!rc) rc = umma_i8_grouped(g, st);
   if (!rc) rc = quantize_i8_computed(reinterpret_cast<float*>(p.h), off + E, reinterpret_cast<int8_t*>(p.hq), reinterpret_cast<float*>(p.hs), rows, I, st);
   if (!rc) rc = umma_i8_grouped(d, st);
-  if (!rc) rc = moe_i8_sum(p.y, d.out_f32, reinterpret_cast<float*>(p.weights), out_rows, a.out, bf16, a.T, k, H, st);
+  const I8Outputs of{d.xq, d.xs, d.w, d.ws, d.ws_dtype, to.ids, I};
+  if (!rc) rc = moe_i8_sum(p.y, d.out_f32, reinterpret_cast<float*>(p.weights), out_rows, of, a.out, bf16, a.T, k, H, st);
   return rc;
 }
 

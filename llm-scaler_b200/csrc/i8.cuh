@@ -66,7 +66,10 @@ int resadd_rmsnorm_quantize_i8(const void* hidden, const void* residual, const v
 int moe_i8_route_ctas(int64_t T);
 int moe_i8_route(const void* logits, int dt, int64_t T, int E, int k, bool renorm, int tile, float* weights, int32_t* ids, int32_t* place, int32_t* base,
                  int32_t* offsets, int32_t* tiles, void* count, cudaStream_t st);
-int moe_i8_sum(const void* y, bool y_f32, const float* weights, const int32_t* rows, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st);
+struct I8Outputs {                                         // what the outputs are made of: codes and scales of h by row, the experts' matrices, the pairs' experts
+  const int8_t* q; const float* s; const int8_t* w; const void* ws; int ws_dt; const int32_t* ids; int I;
+};
+int moe_i8_sum(const void* y, bool y_f32, const float* weights, const int32_t* rows, const I8Outputs& of, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st);
 
 #ifdef __CUDACC__
 // Ordinary loads, never by the read-only path: these kernels begin while the kernel that writes their inputs is still running.  Volatile

@@ -6,7 +6,9 @@
 // of a CTA's pairs comes first is a matter of chance, and no result depends on it: a row of the sorted order does not see the others.
 // 4096 tokens, 128 experts, top-8: five launches of 27 us before (top-k, a stable sort in three, tiles).
 //
-// Weighted sum.  Memory-bound; a thread has eight columns of a token and requests eight experts' rows at a time, or four in fp32.
+// Weighted sum.  Memory-bound; a thread has eight columns of a token and requests eight experts' rows at a time, or four in fp32.  An expert's output
+// that its 16 bits cannot hold (fp16 beyond 65504) would make a sum infinite that is not: where a thread's sums are not finite, it adds
+// them up again and takes such outputs from the codes of h.
 #include "arrivals.cuh"
 #include "i8.cuh"
 #include "i8_route.cuh"
@@ -128,12 +130,41 @@ __global__ void __launch_bounds__(THREADS) moe_i8_route_kernel(const Params p) {
   if (threadIdx.x == 0) { p.offsets[p.E] = before; p.tiles[0] = tiles_before; }
 }
 
+// Eight columns c of token t once more, with every output that is infinite in y made anew.
+template <bool BF16> __device__ __forceinline__ void sum_again(const void* y, const float* weights, const int32_t* rows, const I8Outputs& of, int64_t t, int64_t c, int64_t H, int k, uint16_t* out) {
+#pragma unroll 1
+  for (int j = 0; j < 8; ++j) {
+    float acc = 0.f;
+#pragma unroll 1
+    for (int s = 0; s < k; ++s) {
+      const int64_t pair = t * k + s;
+      const int32_t r = __ldcg(rows + pair);
+      if (r < 0) continue;
+      float f = scalar_from_raw(__ldcg(reinterpret_cast<const unsigned short*>(y) + r * H + c + j), BF16 ? B2Q_BF16 : B2Q_F16);
+      if (fabsf(f) == INFINITY) {
+        const int64_t column = (int64_t)__ldcg(of.ids + pair) * H + c + j;
+        const int8_t *q = of.q + (int64_t)r * of.I, *m = of.w + column * of.I;
+        int sum = 0;
+#pragma unroll 1
+        for (int i = 0; i < of.I; i += 16) {
+          const uint4 a = ld_vec(q + i), b = ld_vec(m + i);
+          sum = __dp4a((int)a.w, (int)b.w, __dp4a((int)a.z, (int)b.z, __dp4a((int)a.y, (int)b.y, __dp4a((int)a.x, (int)b.x, sum))));
+        }
+        f = i8_scaled(sum, ld_f32(of.s + r), load_scalar(of.ws, column, of.ws_dt));
+      }
+      acc = fmaf(__ldcg(weights + pair), f, acc);
+    }
+    out[t * H + c + j] = (uint16_t)pack2<BF16>(acc, 0.f);
+  }
+}
+
 // F32: y is
 template <bool BF16, bool F32>
-__global__ void __launch_bounds__(256) moe_i8_sum_kernel(const void* y, const float* weights, const int32_t* rows, uint16_t* out, int64_t total, int H8, int k) {
+__global__ void __launch_bounds__(256) moe_i8_sum_kernel(const void* y, const float* weights, const int32_t* rows, uint16_t* out, int64_t total, int H8, int k, const I8Outputs of) {
   constexpr int AT_ONCE = F32 ? 4 : 8;                     // experts whose rows are on their way together
   enter();
   const int64_t H = (int64_t)H8 * 8;
+  float none = 0.f;                                        // NaN once a sum of this thread's was not finite (as their largest it cost 4 us of 282)
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const int64_t t = i / H8, c = (i - t * H8) * 8;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -168,8 +199,18 @@ __global__ void __launch_bounds__(256) moe_i8_sum_kernel(const void* y, const fl
         for (int j = 0; j < 8; ++j) acc[j] = fmaf(w[s], f[j], acc[j]);
       }
     }
+    if constexpr (!F32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) none = fmaf(acc[j], 0.f, none);
+    }
     *reinterpret_cast<uint4*>(out + t * H + c) =
         make_uint4(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]), pack2<BF16>(acc[4], acc[5]), pack2<BF16>(acc[6], acc[7]));
+  }
+  if constexpr (!F32) {
+    if (none != 0.f) {
+#pragma unroll 1
+      for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) sum_again<BF16>(y, weights, rows, of, i / H8, i % H8 * 8, H, k, out);
+    }
   }
 }
 }  // namespace i8m
@@ -197,11 +238,11 @@ int moe_i8_route(const void* logits, int dt, int64_t T, int E, int k, bool renor
   return launch_status();
 }
 
-int moe_i8_sum(const void* y, bool y_f32, const float* weights, const int32_t* rows, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st) {
+int moe_i8_sum(const void* y, bool y_f32, const float* weights, const int32_t* rows, const I8Outputs& of, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st) {
   const int64_t total = T * (H / 8);
   const int64_t g = (total + 255) / 256;
   const dim3 grid((unsigned)(g < 148 * 8 ? g : 148 * 8));
-  auto go = [&](auto kern) { launch_overlapped(kern, grid, dim3(256), 0, st, tls().overlap_mode > 0, y, weights, rows, reinterpret_cast<uint16_t*>(out), total, H / 8, k); };
+  auto go = [&](auto kern) { launch_overlapped(kern, grid, dim3(256), 0, st, tls().overlap_mode > 0, y, weights, rows, reinterpret_cast<uint16_t*>(out), total, H / 8, k, of); };
   if (y_f32) { if (bf16) go(i8m::moe_i8_sum_kernel<true, true>); else go(i8m::moe_i8_sum_kernel<false, true>); }
   else { if (bf16) go(i8m::moe_i8_sum_kernel<true, false>); else go(i8m::moe_i8_sum_kernel<false, false>); }
   note_launch("moe_i8_sum");
