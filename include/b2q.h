@@ -341,7 +341,7 @@ B2Q_API int b2q_quantize_int8(const void* x, int x_dtype, int64_t ldx, int8_t* q
 B2Q_API int b2q_silu_mul_quantize_int8(const void* gate_up, int act_dtype, int64_t ldx, int8_t* q, float* scale, int64_t M, int64_t K,
                                void* stream);
 /* The same of RMSNorm(v) * norm_weight with v = hidden + residual in fp32; residual_out <- v in act_dtype, and may be residual
- * itself.  All tensors contiguous [M, K].                                                                               */
+ * itself.  All tensors contiguous [M, K].  Finite rows of any size are normed, while every v * norm_weight is finite in fp32.  */
 B2Q_API int b2q_resadd_rmsnorm_quantize_int8(const void* hidden, const void* residual, const void* norm_weight, void* residual_out,
                                      int act_dtype, float eps, int8_t* q, float* scale, int64_t M, int64_t K, void* stream);
 

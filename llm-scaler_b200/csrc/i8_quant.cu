@@ -2,7 +2,8 @@
 // exactly (i8.cuh).  A row that holds an infinity or a NaN gets the scale NaN and zero codes, so that everything made from it is NaN.
 //
 // Three forms of x: a row of 16-bit (or fp32) values; silu(gate) * up; and the RMSNorm of hidden + residual, whose codes need no
-// 1 / rms: it cancels out of v w / max |v w|, so that one reduction gives both the sum of squares and the maximum.
+// 1 / rms: it cancels out of v w / max |v w|, so that one reduction gives both the sum of squares and the maximum.  Where that sum overflows (bf16
+// rows of rms above some 1e17) it is made again of 2^-80 v; other rows pay one test for it, behind the reduction.
 //
 // Memory-bound: a row is read once and stays in registers between the maximum and the codes.  Rows of up to 1024 values take a warp
 // each, longer ones a CTA with one barrier; what is not 16-byte aligned, or longer than 1024 threads hold, is read twice.  The exponential
@@ -65,6 +66,30 @@ template <int MODE> __device__ __forceinline__ Scale row_scale(uint32_t mx, floa
     if constexpr (MODE == PLAIN || MODE == COPIES) s.row = i8_row(a); else s.r = 127.f / a;
   }
   if (!s.finite) s.scale = __uint_as_float(0x7FC00000u);
+  return s;
+}
+
+constexpr float HUGE_UNIT = 8.271806125530277e-25f;        // 2^-80: 2^31 squares of it times the largest number add up to less than 2^128
+// Of a row of the NORM form whose sum of squares overflows, from each thread's sum of the squares of HUGE_UNIT v; eps is nothing beside them.
+template <bool WARP> __device__ __forceinline__ Scale huge_scale(float sum, uint32_t mx, int K, float* red) {
+  const int lane = threadIdx.x & 31;
+  auto add = [](float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  sum = add(sum);
+  if constexpr (!WARP) {
+    __syncthreads();                                       // red is being read
+    if (lane == 0) red[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    sum = add(lane < (int)(blockDim.x >> 5) ? red[lane] : 0.f);
+  }
+  const float a = __uint_as_float(mx), an = a * HUGE_UNIT * rsqrtf(sum / (float)K);
+  Scale s;
+  s.finite = abs_bits(an) < 0x7F800000u && mx < 0x7F800000u;
+  s.scale = s.finite ? fmaxf(an, I8_MIN_AMAX) / 127.f : __uint_as_float(0x7FC00000u);
+  s.r = 127.f / fmaxf(a, I8_MIN_AMAX / rsqrtf(sum / (float)K) / HUGE_UNIT);
   return s;
 }
 
@@ -244,6 +269,37 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
       if (c < n8) *reinterpret_cast<uint2*>(q + 8 * c) = o;
     }
   }
+  if constexpr (MODE == NORM && BF16) {
+    if (!(sum < INFINITY)) {                               // the same for the whole row; what was stored above is replaced
+      // In front of the codes, or out of line, this cost ordinary rows registers (4096 x 1024 up to 7.2 us for 5.7).  v is what is left of it: v w over w,
+      // and where w is 0 the rounded v that this thread has written.
+      sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = first + i * step;
+        float f[8];
+        pc[i].get(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (c >= n8) continue;
+          const float w = scalar_from_raw(ld_u16(reinterpret_cast<const uint16_t*>(p.nw) + 8 * c + j), DT);
+          const float v = w != 0.f ? __fdividef(f[j], w) : scalar_from_raw(ld_u16(reinterpret_cast<const uint16_t*>(p.residual_out) + row * p.K + 8 * c + j), DT);
+          sum = fmaf(v * HUGE_UNIT, v * HUGE_UNIT, sum);
+        }
+      }
+      __syncwarp();
+      const Scale huge = huge_scale<WARP>(sum, mx, p.K, red_sum);
+      if (first == 0) p.s[row] = huge.scale;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int c = first + i * step;
+        float f[8];
+        pc[i].get(f);
+        const float lo[4] = {f[0], f[1], f[2], f[3]}, hi[4] = {f[4], f[5], f[6], f[7]};
+        if (c < n8) *reinterpret_cast<uint2*>(q + 8 * c) = huge.finite ? make_uint2(i8_codes4_computed(lo, huge.r), i8_codes4_computed(hi, huge.r)) : make_uint2(0, 0);
+      }
+    }
+  }
 }
 
 // Any K, any alignment: element by element, the row read twice.
@@ -282,7 +338,18 @@ __global__ void __launch_bounds__(512) quantize_i8_any_kernel(const Params p) {
   sum = lane < 16 ? red_sum[lane] : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const Scale sc = row_scale<MODE>(mx, sum, p.K, p.eps);
+  Scale sc = row_scale<MODE>(mx, sum, p.K, p.eps);
+  if constexpr (MODE == NORM && DT == B2Q_BF16) {
+    if (!(sum < INFINITY)) {                               // the same for the whole row, and residual_out is not written yet
+      sum = 0.f;
+      for (int c = threadIdx.x; c < p.K; c += 512) {
+        const float v = (at(p.x, row * p.ldx + c) + at(p.residual, row * p.K + c)) * HUGE_UNIT;
+        sum = fmaf(v, v, sum);
+      }
+      __syncwarp();
+      sc = huge_scale<false>(sum, mx, p.K, red_sum);
+    }
+  }
   if (threadIdx.x == 0) p.s[row] = sc.scale;
   for (int c = threadIdx.x; c < p.K; c += 512) {
     float v = at(p.x, row * p.ldx + c);
