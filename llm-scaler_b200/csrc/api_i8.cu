@@ -8,6 +8,7 @@ bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t
 bool known(int dtype) { return dtype >= 0 && dtype <= 2; }
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 constexpr int64_t MAX_K = 131071;                          // 128 * 128 * K stays below 2^31
+constexpr int64_t MAX_COLUMNS = INT32_MAX - 512;           // of the quantisers, which count them in steps of 512
 
 int linear_check(const I8LinearArgs& a, int64_t M, int64_t N, int64_t K) {
   if (!a.w || !a.ws || !a.out) return B2Q_ERR_NULL;
@@ -28,7 +29,7 @@ int b2q_quantize_int8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float*
   if (!x || !q || !scale) return B2Q_ERR_NULL;
   if (!known(x_dtype)) return B2Q_ERR_DTYPE;
   if (M < 0 || K <= 0 || ldx < K) return B2Q_ERR_SHAPE;
-  if (M > INT32_MAX || K > INT32_MAX) return B2Q_ERR_LIMIT;
+  if (M > INT32_MAX || K > MAX_COLUMNS) return B2Q_ERR_LIMIT;
   if (!aligned_to(x, dtype_bytes(x_dtype)) || !aligned_to(scale, 4)) return B2Q_ERR_ALIGN;
   return quantize_i8(x, x_dtype, ldx, q, scale, M, (int)K, (cudaStream_t)stream);
 }
@@ -47,7 +48,7 @@ int b2q_resadd_rmsnorm_quantize_int8(const void* hidden, const void* residual, c
   if (!hidden || !residual || !norm_weight || !residual_out || !q || !scale) return B2Q_ERR_NULL;
   if (!is16(act_dtype)) return B2Q_ERR_DTYPE;
   if (M < 0 || K <= 0) return B2Q_ERR_SHAPE;
-  if (M > INT32_MAX || K > INT32_MAX) return B2Q_ERR_LIMIT;
+  if (M > INT32_MAX || K > MAX_COLUMNS) return B2Q_ERR_LIMIT;
   if (!aligned_to(hidden, 2) || !aligned_to(residual, 2) || !aligned_to(norm_weight, 2) || !aligned_to(residual_out, 2) || !aligned_to(scale, 4))
     return B2Q_ERR_ALIGN;
   return resadd_rmsnorm_quantize_i8(hidden, residual, norm_weight, residual_out, act_dtype == B2Q_BF16, eps, q, scale, M, (int)K,

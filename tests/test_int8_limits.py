@@ -1,0 +1,27 @@
+"""Sizes next to 2^31: the quantisers' columns are counted in steps of 512, the linears' rows in tiles, and neither count may pass the largest
+int.  Refused before any launch; no GPU needed."""
+import re
+import os
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llm-scaler_b200", "csrc")
+P = 1 << 20      # an address that nothing reads
+TOP = (1 << 31) - 1
+
+
+@pytest.fixture(scope="module")
+def L(lib_built):
+    from custom_esimd_kernels_vllm import _lib
+    return _lib
+
+
+@pytest.mark.parametrize("K", [TOP, TOP - 511])
+def test_quantisers_refuse_columns_whose_count_would_overflow(L, K):
+    with open(os.path.join(CSRC, "i8_quant.cu")) as f:
+        steps = set(re.findall(r"for \(int c = threadIdx\.x; c < p\.K; c \+= (\d+)\)", f.read()))
+    assert steps == {"512"}                                   # K - 1 + 512 is the last value of such a count
+    before = L.launch_count()
+    assert L.lib.b2q_quantize_int8(P, 0, K, P, P, 1, K, None) == -10
+    assert L.lib.b2q_resadd_rmsnorm_quantize_int8(P, P, P, P, 0, 1e-6, P, P, 1, K, None) == -10
+    assert L.launch_count() == before
