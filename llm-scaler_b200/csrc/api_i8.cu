@@ -8,13 +8,14 @@ bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t
 bool known(int dtype) { return dtype >= 0 && dtype <= 2; }
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 constexpr int64_t MAX_K = 131071;                          // 128 * 128 * K stays below 2^31
+constexpr int64_t MAX_ROWS = INT32_MAX - 4096;             // tokens and weight rows of a linear: rounded up to tiles and rounds of tiles, both below this
 constexpr int64_t MAX_COLUMNS = INT32_MAX - 512;           // of the quantisers, which count them in steps of 512
 
 int linear_check(const I8LinearArgs& a, int64_t M, int64_t N, int64_t K) {
   if (!a.w || !a.ws || !a.out) return B2Q_ERR_NULL;
   if (!known(a.ws_dtype)) return B2Q_ERR_DTYPE;
   if (M < 0 || N < 0 || K <= 0 || K % 16 != 0 || a.ldo < N) return B2Q_ERR_SHAPE;
-  if (M > INT32_MAX || N > INT32_MAX || K > MAX_K) return B2Q_ERR_LIMIT;
+  if (M > MAX_ROWS || N > MAX_ROWS || K > MAX_K) return B2Q_ERR_LIMIT;
   if (!aligned16(a.w) || !aligned_to(a.out, 2) || !aligned_to(a.bias, 2) || !aligned_to(a.ws, dtype_bytes(a.ws_dtype))) return B2Q_ERR_ALIGN;
   return B2Q_OK;
 }

@@ -507,7 +507,7 @@ static Plan plan(int M, int N, int K, int tok_box) {
     }
   }
   for (int h = 256; M > 128 && h >= 128; h -= 32) {        // a pair's columns come in 32s
-    const int rounds = ((M + 255) / 256 * ((N + h - 1) / h) + sms / 2 - 1) / (sms / 2);
+    const double rounds = ((int64_t)(M + 255) / 256 * ((N + h - 1) / h) + sms / 2 - 1) / (sms / 2);
     const double ns = fmax(dram, rounds * fmax(13.0 * h, nkb * (45 + 1.25 * h))) + 500.0 * (rounds - 1) + 13.0 * h;
     if (ns < least) { least = ns; best = Plan{h, 1, true}; }
   }

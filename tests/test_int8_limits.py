@@ -25,3 +25,13 @@ def test_quantisers_refuse_columns_whose_count_would_overflow(L, K):
     assert L.lib.b2q_quantize_int8(P, 0, K, P, P, 1, K, None) == -10
     assert L.lib.b2q_resadd_rmsnorm_quantize_int8(P, P, P, P, 0, 1e-6, P, P, 1, K, None) == -10
     assert L.launch_count() == before
+
+
+@pytest.mark.parametrize("size", [dict(M=TOP), dict(M=TOP - 4094), dict(N=TOP, ldo=TOP), dict(N=TOP - 4094, ldo=TOP)])
+def test_linears_refuse_rows_whose_tiles_would_overflow(L, size):
+    a = dict(M=1, N=32, K=32, ldo=32)
+    a.update(size)
+    before = L.launch_count()
+    assert L.lib.b2q_linear_int8(P, a["K"], P, P, P, 2, None, P, 0, a["ldo"], a["M"], a["N"], a["K"], None) == -10
+    assert L.lib.b2q_linear_int8_dynamic(P, 0, a["K"], P, P, 2, None, P, a["ldo"], a["M"], a["N"], a["K"], P, 1 << 50, None) == -10
+    assert L.launch_count() == before
