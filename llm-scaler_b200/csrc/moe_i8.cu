@@ -238,6 +238,7 @@ __device__ __forceinline__ int wait_flags(const Arrivals* flags, int from, int s
     if (slot < slots) asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(flags + slot) : "memory");
     const unsigned down = ~__ballot_sync(0xffffffffu, slot < slots && v == mark);
     if (!(down & 1u)) {
+      __syncwarp();                                        // the lane that copies is behind what the others have acquired
       asm volatile("fence.proxy.async;" ::: "memory");     // what the flags stand for was written by ordinary stores and is read by bulk copies
       return down ? __ffs(down) - 1 : 32;
     }
