@@ -105,9 +105,10 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b)
 }
 
 // What the codes of a row need of its largest value: rint(127 x / a), halves to even, decided exactly.  The quotient of y = 127 x by a is
-// corrected once by its remainder, which is exact in fp32; a quotient that is a half then comes out as one, and of 16-bit values no other
-// quotient is nearer to a half than 2^-13.  (A bf16 row has exact halves by the dozen: every value that is half its row's largest.  Deciding
-// the near ones in a branch of their own cost more than this: three of ten warps went there.)  Rows of huge values are taken 2^-40 of.
+// corrected once by its remainder, which is exact in fp32, and is good to about 2^-24 of itself then; a quotient that is a half comes out as one, and of
+// 16-bit values no other is nearer to a half than 2^-18.9 of it (by enumeration: fp16 a = 2047, x = 1910; bf16 2^-16.0; bf16 rows below the floor
+// 2^-14.3).  (A bf16 row has exact halves by the dozen: every value that is half its row's largest.  Deciding the near ones in a branch of their own
+// cost more than this: three of ten warps went there.)  Rows of huge values are taken 2^-40 of.
 struct I8Row {
   float c, a, ra;                                          // 127, a, 1 / a, or the first two 2^-40 times that
 };
