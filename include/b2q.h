@@ -366,11 +366,11 @@ B2Q_API int b2q_linear_int8_dynamic(const void* x, int act_dtype, int64_t ldx, c
  * A token whose logits hold a NaN, or none that is finite at the top, goes to no expert: its row of out is zero.
  * x [T, H], logits [T, E], out [T, H]; w13 int8 [E, 2I, H] (gate rows, then up), s13 [E, 2I], w2 int8 [E, H, I], s2 [E, H], all contiguous.
  * H % 16 == 0, I % 16 == 0, H <= 32768, I < 131072, E <= 1024, top_k <= 32.  h stays fp32 until its codes are made.  A few tokens (up to sixteen,
- * while T (4 top_k I + H) <= 40960) take one kernel, a cooperative launch; more are sorted by expert and go through grouped GEMMs.  An
- * expert's output is rounded to act_dtype before the weighted sum if T top_k H > 2^19, unless act_dtype cannot hold it: such an output (fp16 beyond
- * 65504) enters the sum in fp32, at the cost of being computed a second time.  Up to 2^19 a token's result does not depend on what else is in the
- * call.  workspace: 256-byte aligned, b2q_moe_forward_int8_workspace_bytes() bytes, the call's own until its last kernel has completed; what it holds
- * before does not matter.                                                                                                */
+ * while T (4 top_k I + H) <= 40960 and T top_k ceil(H / SMs) <= 6144) take one kernel, a cooperative launch; more are sorted by expert and go
+ * through grouped GEMMs.  Those round an expert's output to act_dtype before the weighted sum if T top_k H > 2^19, unless act_dtype cannot hold it:
+ * such an output (fp16 beyond 65504) enters the sum in fp32, at the cost of being computed a second time.  Up to 2^19 a token's result does not
+ * depend on what else is in the call.  workspace: 256-byte aligned, b2q_moe_forward_int8_workspace_bytes() bytes, the call's own until its last
+ * kernel has completed; what it holds before does not matter.                                                            */
 typedef struct b2q_moe_int8 {
   const void *x, *logits;
   const int8_t* w13; const void* s13; const int8_t* w2; const void* s2;

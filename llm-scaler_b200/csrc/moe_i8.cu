@@ -615,7 +615,8 @@ template <bool BF16, int PER> static int run(Params& p, cudaStream_t st) {
 // pay six launches instead, four of them under the weights that a GEMM fetches in advance.  Over 18 layers of 3 to 1395 MB with 1 to 16 tokens the line
 // below took 1.003 times as long as the better of the two (always one kernel 1.18, never 1.013).  One kernel / grouped, us: 128 experts of 2048 x 768, top-8,
 // 1 / 2 / 4 / 16 tokens 19.3 / 21.7, 29.5 / 29.9, 43.2 / 40.8, 97.9 / 83.3; 16 of 4096 x 1024, top-1, 1 / 8: 16.0 / 19.6, 30.8 / 30.5; 8 of 4096 x 14336, top-2, 1 / 16:
-// 87.6 / 76.2, 416 / 229; 8 of 1024 x 512, top-2, 1 / 16: 15.6 / 16.3, 20.8 / 18.3; 8 of 2048 x 2048, top-8, 16: 91.3 / 36.6.
+// 87.6 / 76.2, 416 / 229; 8 of 1024 x 512, top-2, 1 / 16: 15.6 / 16.3, 20.8 / 18.3; 8 of 2048 x 2048, top-8, 16: 91.3 / 36.6.  The second condition is room: a CTA's
+// sums of all pairs, and as many scales, take the place of the tokens' codes.
 bool moe_i8_few_preferred(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
   using namespace mi8;
   if (T > MAX_TOK || E > MAX_E || k > MAX_K || H > INT32_MAX / 64 || I > INT32_MAX / 64) return false;
