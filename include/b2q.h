@@ -337,11 +337,14 @@ B2Q_API int b2q_moe_gemm_fp8(const void* x, int act_dtype, int64_t ldx,
  * weight.  x bf16, fp16 or fp32 [M, K] with row pitch ldx (elements), any K >= 1, any alignment of the elements' own size; q is
  * contiguous [M, K].  Rows of 16-byte aligned 16-bit values with K % 8 == 0 are read once, others twice and more slowly.   */
 B2Q_API int b2q_quantize_int8(const void* x, int x_dtype, int64_t ldx, int8_t* q, float* scale, int64_t M, int64_t K, void* stream);
-/* The same of silu(x[:, :K]) * x[:, K:2K] in fp32, never rounded to 16 bits in between; ldx >= 2K, 16-bit types.        */
+/* The same of silu(x[:, :K]) * x[:, K:2K] in fp32, never rounded to 16 bits in between; ldx >= 2K, 16-bit types.  Values that are
+ * computed themselves are placed by one fp32 multiplication: a code is within half a step, and the value's own fp32 error, of
+ * 127 x / a.  A row's codes and scale do not depend on the other rows.                                                  */
 B2Q_API int b2q_silu_mul_quantize_int8(const void* gate_up, int act_dtype, int64_t ldx, int8_t* q, float* scale, int64_t M, int64_t K,
                                void* stream);
 /* The same of RMSNorm(v) * norm_weight with v = hidden + residual in fp32; residual_out <- v in act_dtype, and may be residual
- * itself.  All tensors contiguous [M, K].  Finite rows of any size are normed, while every v * norm_weight is finite in fp32.  */
+ * itself.  All tensors contiguous [M, K].  Finite rows of any size are normed, while every v * norm_weight is finite in fp32.  Codes as
+ * for SiLU; they do not depend on M, but the squares add up in an order that does, so that a scale may differ in its last bits.  */
 B2Q_API int b2q_resadd_rmsnorm_quantize_int8(const void* hidden, const void* residual, const void* norm_weight, void* residual_out,
                                      int act_dtype, float eps, int8_t* q, float* scale, int64_t M, int64_t K, void* stream);
 

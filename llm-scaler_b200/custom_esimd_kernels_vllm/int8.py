@@ -51,12 +51,14 @@ def quantize_int8(x):
 
 
 def silu_mul_quantize_int8(gate_up):
-    """quantize_int8 of silu(gate) * up, gate_up bf16 / fp16 [M, 2K]; the product is not rounded to 16 bits in between."""
+    """quantize_int8 of silu(gate) * up, gate_up bf16 / fp16 [M, 2K]; the product is not rounded to 16 bits in between.  Its codes are within half a
+    step and the product's own fp32 error."""
     return _ops.silu_mul_quantize(gate_up)
 
 
 def resadd_rmsnorm_quantize_int8(hidden, residual, norm_weight, eps, residual_out=None):
-    """v = hidden + residual; residual_out (residual itself by default) <- v; returns quantize_int8 of rmsnorm(v) * norm_weight."""
+    """v = hidden + residual; residual_out (residual itself by default) <- v; returns quantize_int8 of rmsnorm(v) * norm_weight, with codes within half a
+    step and the fp32 error.  The last bits of a scale may depend on the number of rows."""
     return _ops.resadd_rmsnorm_quantize(hidden, residual, norm_weight, eps, residual_out)
 
 
