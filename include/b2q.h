@@ -370,10 +370,12 @@ B2Q_API int b2q_linear_int8_dynamic(const void* x, int act_dtype, int64_t ldx, c
  * x [T, H], logits [T, E], out [T, H]; w13 int8 [E, 2I, H] (gate rows, then up), s13 [E, 2I], w2 int8 [E, H, I], s2 [E, H], all contiguous.
  * H % 16 == 0, I % 16 == 0, H <= 32768, I < 131072, E <= 1024, top_k <= 32.  h stays fp32 until its codes are made.  A few tokens (up to sixteen,
  * while T (4 top_k I + H) <= 40960 and T top_k ceil(H / SMs) <= 6144) take one kernel, a cooperative launch; more are sorted by expert and go
- * through grouped GEMMs.  Those round an expert's output to act_dtype before the weighted sum if T top_k H > 2^19, unless act_dtype cannot hold it:
- * such an output (fp16 beyond 65504) enters the sum in fp32, at the cost of being computed a second time.  Up to 2^19 a token's result does not
- * depend on what else is in the call.  workspace: 256-byte aligned, b2q_moe_forward_int8_workspace_bytes() bytes, the call's own until its last
- * kernel has completed; what it holds before does not matter.                                                            */
+ * through grouped GEMMs, as all do under b2q_set_force_kernel(2).  A GPU that cannot hold one CTA on each of its SMs at a time (a share of it
+ * given to other processes) refuses the cooperative launch: B2Q_ERR_CUDA, nothing has run, and the override is the way round.
+ * The grouped form rounds an expert's output to act_dtype before the weighted sum if T top_k H > 2^19, unless act_dtype cannot hold it: such an
+ * output (fp16 beyond 65504) enters the sum in fp32, at the cost of being computed a second time.  Up to 2^19 a token's result does not depend on
+ * what else is in the call.  workspace: 256-byte aligned, b2q_moe_forward_int8_workspace_bytes() bytes, the call's own until its last kernel has
+ * completed; what it holds before does not matter.                                                                       */
 typedef struct b2q_moe_int8 {
   const void *x, *logits;
   const int8_t* w13; const void* s13; const int8_t* w2; const void* s2;
@@ -520,7 +522,8 @@ B2Q_API int b2q_device_status_reset(void);
 B2Q_API int b2q_selftest_bounded_wait(int code, int* gave_up, void* stream);
 
 /* Kernel selection override for benchmarking: 0 = automatic, 1 = the mma.sync streaming kernel,
- * 2 = the tcgen05 kernel with 16-bit operands, 3 = the same without activation pre-pass,
+ * 2 = the tcgen05 kernel with 16-bit operands (8-bit integer operators: theirs, and an expert layer's grouped form; scratch
+ * is asked for while the override is set), 3 = the same without activation pre-pass,
  * 4 = the same with one CTA per strip (no strip cutting), 5 = INT4 decode on the int8 MMA (its scratch is asked for
  * while the override is set),
  * 6 = the CTA-pair (cta_group::2) variant of the W8A8 GEMM, 7 = the INT4 decode streaming kernel, 8 = the FP8 streaming

@@ -19,9 +19,10 @@ int linear_check(const I8LinearArgs& a, int64_t M, int64_t N, int64_t K) {
   if (!aligned16(a.w) || !aligned_to(a.out, 2) || !aligned_to(a.bias, 2) || !aligned_to(a.ws, dtype_bytes(a.ws_dtype))) return B2Q_ERR_ALIGN;
   return B2Q_OK;
 }
-// set_force_kernel(2): tcgen05 for everything
+// set_force_kernel(2): tcgen05 for everything, no cooperative launch
 bool use_stream(const I8LinearArgs& a) { return tls().force_kernel != 2 && i8_stream_preferred(a.M, a.N, a.K); }
 bool use_from16(int64_t M, int64_t N, int64_t K) { return tls().force_kernel != 2 && i8_stream_from16(M, N, K); }
+bool use_few(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) { return tls().force_kernel != 2 && moe_i8_few_preferred(T, E, k, H, I); }
 }  // namespace
 
 extern "C" {
@@ -133,7 +134,7 @@ extern "C" {
 
 size_t b2q_moe_forward_int8_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I) {
   if (T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || top_k > 32 || H <= 0 || I <= 0 || T > INT32_MAX / 32) return 0;
-  if (moe_i8_few_preferred(T, E, top_k, H, I)) return moe_i8_few_bytes(T, top_k, I);
+  if (use_few(T, E, top_k, H, I)) return moe_i8_few_bytes(T, top_k, I);
   return moe_parts(nullptr, T, (int)E, (int)top_k, H, I).total;
 }
 
@@ -154,7 +155,7 @@ int b2q_moe_forward_int8(const b2q_moe_int8* m, void* workspace, size_t workspac
   cudaStream_t st = (cudaStream_t)stream;
   const bool bf16 = a.act_dtype == B2Q_BF16;
   const int E = (int)a.E, k = (int)a.top_k, H = (int)a.H, I = (int)a.I;
-  if (moe_i8_few_preferred(a.T, E, k, H, I)) {
+  if (use_few(a.T, E, k, H, I)) {
     I8FewArgs f{};
     f.x = a.x; f.bf16 = bf16; f.logits = a.logits; f.logits_dtype = a.logits_dtype;
     f.w13 = a.w13; f.s13 = a.s13; f.s13_dtype = a.s13_dtype; f.w2 = a.w2; f.s2 = a.s2; f.s2_dtype = a.s2_dtype;

@@ -22,3 +22,16 @@ def test_documents_state_both(name):
     with open(os.path.join(ROOT, name)) as f:
         text = " ".join(re.sub(r"\n \*", "\n", f.read()).split())
     assert re.search(r"<= 40960`? and `?T top_k ceil\(H / SMs\) <= 6144", text)
+
+
+def test_scratch_of_the_grouped_form_on_request(lib_built):
+    from custom_esimd_kernels_vllm import _lib as L
+    f = L.lib.b2q_moe_forward_int8_workspace_bytes
+    shape = (1, 128, 8, 2048, 768)
+    few = f(*shape)
+    L.lib.b2q_set_force_kernel(2)
+    try:
+        assert f(*shape) >= few + 8 * 2048
+    finally:
+        L.lib.b2q_set_force_kernel(0)
+    assert f(*shape) == few
