@@ -15,6 +15,56 @@ if not os.path.exists(_PATH):
 torch.ops.load_library(_PATH)
 
 
+def _fakes():
+    """Outputs without data, for tracing: the sizes are checked as the ops check them, pointers and strides are not."""
+    fake, check, f32 = torch.library.register_fake, torch._check, torch.float32
+    half = (torch.bfloat16, torch.float16)
+
+    def codes(x, columns):
+        return x.new_empty((x.shape[0], columns), dtype=torch.int8), x.new_empty((x.shape[0],), dtype=f32)
+
+    @fake("b2q_int8::quantize")
+    def _(x):
+        check(x.dim() == 2 and x.dtype in half + (f32,), lambda: "x must be 2-D bf16, fp16 or fp32")
+        return codes(x, x.shape[1])
+
+    @fake("b2q_int8::silu_mul_quantize")
+    def _(gate_up):
+        check(gate_up.dim() == 2 and gate_up.dtype in half and gate_up.shape[1] % 2 == 0, lambda: "gate_up must be 2-D bf16 or fp16 with an even number of columns")
+        return codes(gate_up, gate_up.shape[1] // 2)
+
+    @fake("b2q_int8::resadd_rmsnorm_quantize")
+    def _(hidden, residual, norm_weight, eps, residual_out):
+        check(hidden.dim() == 2 and hidden.dtype in half and residual.shape == hidden.shape, lambda: "hidden and residual must be 2-D bf16 / fp16 of the same shape")
+        check(norm_weight.dim() == 1 and norm_weight.shape[0] == hidden.shape[1], lambda: "norm_weight must have K elements")
+        return codes(hidden, hidden.shape[1])
+
+    def linear(x, weight, weight_scale, dtype):
+        check(x.dim() == 2 and weight.dim() == 2 and weight.dtype == torch.int8 and weight.shape[1] == x.shape[1], lambda: "weight must be int8 [N, K]")
+        check(weight_scale.numel() == weight.shape[0], lambda: "weight_scale must have N elements")
+        check(dtype in half, lambda: "outputs are bf16 or fp16")
+        return x.new_empty((x.shape[0], weight.shape[0]), dtype=dtype)
+
+    @fake("b2q_int8::linear")
+    def _(codes, scale, weight, weight_scale, bias, out_dtype):
+        check(codes.dtype == torch.int8 and scale.numel() == codes.shape[0], lambda: "codes must be int8 and scale have M elements")
+        return linear(codes, weight, weight_scale, out_dtype)
+
+    @fake("b2q_int8::linear_dynamic")
+    def _(x, weight, weight_scale, bias):
+        return linear(x, weight, weight_scale, x.dtype)
+
+    @fake("b2q_int8::moe_forward")
+    def _(x, router_logits, gate_up_weight, gate_up_scale, down_weight, down_scale, top_k, renormalize):
+        check(x.dim() == 2 and x.dtype in half, lambda: "x must be a bf16 / fp16 [T, H] tensor")
+        check(router_logits.dim() == 2 and router_logits.shape[0] == x.shape[0], lambda: "router_logits must be a [T, E] tensor")
+        check(down_weight.dim() == 3 and down_weight.shape[1] == x.shape[1], lambda: "down_weight must be an int8 [E, H, I] tensor")
+        return x.new_empty(x.shape)
+
+
+_fakes()
+
+
 class _Ops:
     """The ops' only overloads, looked up once: a call is worth a few microseconds."""
 
