@@ -1,6 +1,20 @@
 // C ABI of the 8-bit integer operators: argument validation and kernel selection, as in api.cu.
 #include "i8.cuh"
 
+namespace b2q {
+int sm_count() {
+  static thread_local int sms[16] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 16) return 148;
+  if (!sms[dev]) {
+    cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    if (sms[dev] <= 0) sms[dev] = 148;
+  }
+  return sms[dev];
+}
+}  // namespace b2q
+
 using namespace b2q;
 
 namespace {

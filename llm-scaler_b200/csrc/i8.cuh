@@ -10,6 +10,8 @@ constexpr float I8_MIN_AMAX = 1e-12f;
 // up to this many tokens the streaming kernels serve a call: one m16n8k32 MMA takes sixteen rows of codes
 constexpr int I8_STREAM_MAX_TOK = 16;
 
+int sm_count();                                            // of the current device; 148 where there is none
+
 struct I8LinearArgs {
   const int8_t* xq; int64_t ldx; const float* xs;          // codes [M, ldx], scales [M]; or, with x16 set,
   const void* x16; int64_t ldx16; bool x_bf16;             // the 16-bit rows to be quantised first (streaming kernel only)
@@ -72,6 +74,14 @@ struct I8Outputs {                                         // what the outputs a
 int moe_i8_sum(const void* y, bool y_f32, const float* weights, const int32_t* rows, const I8Outputs& of, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st);
 
 #ifdef __CUDACC__
+// As in moe_aux.cu: a grid that fills the GPU lets the next one begin later.
+__device__ __forceinline__ void grid_dep_enter() {
+  const bool few = gridDim.x <= 148;
+  if (few) grid_dep_release();
+  grid_dep_wait();
+  if (!few) grid_dep_release();
+}
+
 // Ordinary loads, never by the read-only path: these kernels begin while the kernel that writes their inputs is still running.  Volatile
 // keeps them behind the wait for it; without a memory clobber several are on their way at a time.
 __device__ __forceinline__ uint4 ld_vec(const void* p) {

@@ -24,13 +24,6 @@ struct Params {
   int8_t* q; float* s; int64_t M; int K;
 };
 
-__device__ __forceinline__ void enter() {                  // as in moe_aux.cu: a grid that fills the GPU lets the next one begin later
-  const bool few = gridDim.x <= 148;
-  if (few) grid_dep_release();
-  grid_dep_wait();
-  if (!few) grid_dep_release();
-}
-
 // The largest magnitude, NaN above all: half an instruction per value (as integers two: norm of 2047 x 8192 19.6 us for 17.0, SiLU 18.2 for 17.6).
 __device__ __forceinline__ float abs_max(float m, float a, float b) {
   float r;
@@ -127,7 +120,7 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
     grid_dep_wait();
     grid_dep_release();
   } else {
-    enter();
+    grid_dep_enter();
   }
   if (row >= p.M) return;                                  // whole warps, or the whole CTA
   if constexpr (MODE == PLAIN || MODE == COMPUTED) {
@@ -309,7 +302,7 @@ __global__ void __launch_bounds__(512) quantize_i8_any_kernel(const Params p) {
   __shared__ float red_sum[16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x;
-  enter();
+  grid_dep_enter();
   if constexpr (MODE == PLAIN) {
     if (p.n_valid && row >= *reinterpret_cast<const volatile int32_t*>(p.n_valid)) return;
   }

@@ -135,17 +135,6 @@ __global__ void __launch_bounds__(THREADS, 2) i8_stream_kernel(const Params p) {
   }
 }
 
-static int sm_count() {
-  static thread_local int sms[16] = {0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 16) return 148;
-  if (!sms[dev]) {
-    cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
-    if (sms[dev] <= 0) sms[dev] = 148;
-  }
-  return sms[dev];
-}
 
 template <int R, bool FROM16, bool BF16> static int launch(Params& p, int grid, cudaStream_t st) {
   p.row_cap = (p.N + grid - 1) / grid;

@@ -563,17 +563,6 @@ __global__ void __launch_bounds__(THREADS, 1) moe_i8_kernel(const __grid_constan
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
-static int sm_count() {
-  static thread_local int sms[16] = {0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 16) return 148;
-  if (!sms[dev]) {
-    cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
-    if (sms[dev] <= 0) sms[dev] = 148;
-  }
-  return sms[dev];
-}
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 static int grid_of(int64_t H) { return (int)(sm_count() < H ? sm_count() : H); }
 

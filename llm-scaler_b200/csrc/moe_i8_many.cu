@@ -27,13 +27,6 @@ struct Params {
   Arrivals* count; Arrivals tag; const Arrivals* epoch;
 };
 
-__device__ __forceinline__ void enter() {
-  const bool few = gridDim.x <= 148;
-  if (few) grid_dep_release();
-  grid_dep_wait();
-  if (!few) grid_dep_release();
-}
-
 template <int PER>
 __global__ void __launch_bounds__(THREADS) moe_i8_route_kernel(const Params p) {
   __shared__ int counts[MAX_E];
@@ -42,7 +35,7 @@ __global__ void __launch_bounds__(THREADS) moe_i8_route_kernel(const Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < p.E; e += THREADS) counts[e] = 0;
   __syncthreads();
-  enter();
+  grid_dep_enter();
   const bool alone = gridDim.x == 1;                       // its counts need not leave the SM (16 tokens: 8.2 us otherwise, by itself)
   if (threadIdx.x == 0 && !alone) arrivals_open(p.count, p.tag, p.epoch);
   const int t0 = blockIdx.x * p.per_cta, t1 = min(p.T, t0 + p.per_cta);
@@ -162,7 +155,7 @@ template <bool BF16> __device__ __forceinline__ void sum_again(const void* y, co
 template <bool BF16, bool F32>
 __global__ void __launch_bounds__(256) moe_i8_sum_kernel(const void* y, const float* weights, const int32_t* rows, uint16_t* out, int64_t total, int H8, int k, const I8Outputs of) {
   constexpr int AT_ONCE = F32 ? 4 : 8;                     // experts whose rows are on their way together
-  enter();
+  grid_dep_enter();
   const int64_t H = (int64_t)H8 * 8;
   float none = 0.f;                                        // NaN once a sum of this thread's was not finite (as their largest it cost 4 us of 282)
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {

@@ -418,17 +418,6 @@ umma_i8_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
 // host side
 // ------------------------------------------------------------------------------------------------
 namespace ui8 {
-static int sm_count() {
-  static thread_local int sms[16] = {0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 16) return 148;
-  if (!sms[dev]) {
-    cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
-    if (sms[dev] <= 0) sms[dev] = 148;
-  }
-  return sms[dev];
-}
 static int round_up(int v, int a) { return (v + a - 1) / a * a; }
 
 template <int KPS, bool PAIR, bool SPLIT, bool GROUPED, bool GATED>
