@@ -10,9 +10,12 @@ import torch
 from . import _lib as L
 
 _PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libb2q_int8.so")
-if not os.path.exists(_PATH):
-    raise ImportError("b2q: %s is missing; build it with `python llm-scaler_b200/build.py`" % _PATH)
-torch.ops.load_library(_PATH)
+_MISSING = None if os.path.exists(_PATH) else "b2q: %s is missing; build it with `python llm-scaler_b200/build.py`" % _PATH
+_CHECK_STATUS = os.environ.get("B2Q_CHECK_STATUS") == "1"
+if _MISSING and os.environ.get("B2Q_PYTHON_DISPATCH") != "1" and not _CHECK_STATUS:
+    raise ImportError(_MISSING)      # under these two the other ops do without a C++ layer, so that only the operators here fail
+if not _MISSING:
+    torch.ops.load_library(_PATH)
 
 
 def _fakes():
@@ -62,7 +65,8 @@ def _fakes():
         return x.new_empty(x.shape)
 
 
-_fakes()
+if not _MISSING:
+    _fakes()
 
 
 class _Ops:
@@ -73,9 +77,14 @@ class _Ops:
             setattr(self, name, getattr(torch.ops.b2q_int8, name).default)
 
 
-_ops = _Ops()
+class _NoOps:
+    def __getattr__(self, name):
+        raise ImportError(_MISSING)
 
-if os.environ.get("B2Q_CHECK_STATUS") == "1":
+
+_ops = _NoOps() if _MISSING else _Ops()
+
+if _CHECK_STATUS and not _MISSING:
     # debugging, as for the other ops: every call synchronises and raises if a bounded device-side wait has expired
     class _Checked:
         def __getattr__(self, name):
