@@ -15,8 +15,8 @@
 // GATED (grouped, expert up projection): half of a tile's columns are gate rows, half the up rows of the same outputs, and the epilogue
 // stores silu(gate) * up.
 //
-// Bound by the MMA in prompts (4001 x 17408 x 5120 224 us, 3.18 PFLOP/s of int8, the power cap included; 2048 x 8192 x 28672 296 us), by HBM with few tokens (27 x
-// 17408 x 5120 16.1 us, 5.6 TB/s), where a split of k or half tiles keep all SMs loading.
+// Bound by the MMA in prompts: 4001 x 17408 x 5120 226 us in runs too short for the power cap, 3.15 PFLOP/s of int8, and 251 back to back for seconds, 2.84; 2048 x
+// 8192 x 28672 291 and 340.  By HBM with few tokens (27 x 17408 x 5120 16.6 us, 5.4 TB/s), where a split of k or half tiles keep all SMs loading.
 //
 // No multicast load; every mbarrier wait is bounded, as in the other tcgen05 kernels.
 #include "umma_gemm.cuh"
