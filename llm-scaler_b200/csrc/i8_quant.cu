@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(WARP ? 256 : (V == 8 ? 512 : 1024)) quantize_i
     if (!(sum < INFINITY)) {                               // the same for the whole row; what was stored above is replaced
       // In front of the codes, or out of line, this cost ordinary rows registers (4096 x 1024 up to 7.2 us for 5.7).  v is what is left of it: v w over w,
       // and where w is 0 the rounded v that this thread has written.
+      __syncwarp();                                        // those writes stay in front of the loads
       sum = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {

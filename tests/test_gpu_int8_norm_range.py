@@ -42,3 +42,28 @@ def test_rows_of_all_sizes_beside_one_another(ops, M, K):  # noqa: F811
     assert torch.isnan(s[2::4]).all() and (q[2::4] == 0).all()
     q, s = ops.resadd_rmsnorm_quantize_int8(h.to(DEV), r.to(DEV), w.to(DEV), 1e-5)
     assert torch.equal(q[3::4].cpu(), plain[0][3::4]) and torch.equal(s[3::4].cpu(), plain[1][3::4])
+
+
+@pytest.mark.parametrize("M,K", FORMS)
+def test_huge_rows_under_weights_of_zero(ops, M, K):  # noqa: F811
+    """Where the weight is 0, v enters the sum of squares as residual_out has it, in 16 bits; everything else in fp32."""
+    g = torch.Generator().manual_seed(K + 2)
+    h, r = ((torch.randn(M, K, generator=g) * 1e25).bfloat16() for _ in range(2))
+    w = (1 + 0.2 * torch.randn(K, generator=g)).bfloat16()
+    w[torch.randperm(K, generator=g)[:K // 3]] = 0
+    v = h.double() + r.double()
+    if K % 8 == 0 and K <= 32768:                            # the others are read twice, and exact
+        v = torch.where(w == 0, (h.float() + r.float()).bfloat16().double(), v)
+    n = v / torch.sqrt((v * v).mean(1, keepdim=True) + 1e-5) * w.double()
+    q, s = ops.resadd_rmsnorm_quantize_int8(h.to(DEV), r.to(DEV), w.to(DEV), 1e-5)
+    near(q, s, n, 127 * 8 * 2.0 ** -24, 64 * 2.0 ** -24)
+
+
+def test_the_values_written_are_read_back_behind_the_writes():
+    """What a thread reads back there goes by volatile loads, which the compiler orders among themselves only."""
+    import os
+    import re
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llm-scaler_b200", "csrc", "i8_quant.cu")
+    with open(src) as f:
+        body = re.sub(r"//[^\n]*", "", f.read()).split("if (!(sum < INFINITY)) {")[1].split("residual_out")[0]
+    assert "__syncwarp();" in body
