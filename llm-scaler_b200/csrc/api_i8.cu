@@ -121,8 +121,8 @@ int b2q_linear_int8_dynamic(const void* x, int act_dtype, int64_t ldx, const int
 namespace {
 // Workspace of an expert layer in its grouped form, part by part.
 // Each expert's output for each of its rows: in fp32 for decode batches, where it costs nothing (16 tokens, 128 experts of 2048 x 768, top-8: 85 us either way), so that
-// their results are the one-kernel form's, bit for bit; beyond, in 16 bits of act_dtype (256 tokens 127 us, in fp32 137), but for outputs that those cannot hold, which
-// the weighted sum makes anew.
+// their results are the one-kernel form's, bit for bit; beyond, in 16 bits of act_dtype (256 tokens 127 us, in fp32 137; bf16 error against
+// 64 bits 2.3e-3 of the norm, in fp32 1.7e-3), but for outputs that those cannot hold, which the weighted sum makes anew.
 bool moe_y_f32(size_t elements) { return elements <= (size_t)1 << 19; }
 
 struct MoeParts {
