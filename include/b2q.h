@@ -386,6 +386,52 @@ typedef struct b2q_moe_int8 {
 B2Q_API size_t b2q_moe_forward_int8_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I);
 B2Q_API int b2q_moe_forward_int8(const b2q_moe_int8* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- expert routing, and layers of 4-bit group-quantised weights ---------------------
+ * Checkpoints whose weights have a 4-bit code per value and a scale and zero point per group of 32, 64 or 128 values along k (GPTQ, AWQ), and the
+ * routing of mixtures of many experts.  The reference has group 128 without zero points and the softmax top-k alone; everything here is an addition.
+ *
+ * Routing.  l = logits of a token; p = softmax(l) over all E or sigmoid(l); an expert's key is l without a bias (both scores grow with it) and p + bias
+ * with one.  With num_groups > 1 the experts [i E / num_groups, ...) form groups, of which the top_groups with the largest group key stay: the largest key
+ * in it, or with B2Q_GROUP_TOP2 the sum of its two largest p (+ bias) (of its one, where groups have one).  ids = the top_k largest keys of what stays,
+ * in that order; equal keys, of experts and of groups, go to the lowest index first.  weights = scale * p, or scale * p / (sum of the chosen p) if
+ * renormalize, in fp32.  No rounding decides: sums of p and bias are compared in 64 bits.
+ * A logit of -inf, or a bias of -inf or NaN, takes an expert out of the choice; where fewer than top_k are left the last ids are -1 with the weight 0.  A token
+ * whose logits hold a NaN or +inf, or nothing above -inf, gets no expert at all.  logits [T, E] with row pitch ldl, bias [E], any of the three
+ * types each; weights, ids contiguous [T, top_k].  E <= 1024, num_groups <= 32 and a divisor of E, top_k <= 32 and <= top_groups * E / num_groups.   */
+#define B2Q_SCORE_SOFTMAX 0
+#define B2Q_SCORE_SIGMOID 1
+#define B2Q_GROUP_MAX  0
+#define B2Q_GROUP_TOP2 1
+B2Q_API int b2q_route_experts(const void* logits, int logits_dtype, int64_t ldl, const void* bias, int bias_dtype, float* weights, int32_t* ids,
+                      int64_t T, int64_t E, int64_t top_k, int scoring, int64_t num_groups, int64_t top_groups, int group_score,
+                      int renormalize, float scale, void* stream);
+
+/* out[m, n] = sum_k x[m, k] (q[n, k] - zero[k / group, n]) scale[k / group, n] (+ bias[n]), one rounding to act_dtype.  w holds q contiguous [N, K / 2], even k
+ * in the low half of a byte (as little-endian int32: eight values, lowest nibble first); scale [K / group, N] and zero [K / group, N] (uint8, any value;
+ * NULL: 8 everywhere) contiguous.  x [M, K] with row pitch ldx, scale, bias, out (row pitch ldo) in act_dtype (bf16 / fp16).  group 32, 64 or 128,
+ * K % group == 0, any M and N; w 16-byte aligned, the others to their elements (x rows that start on 16 bytes save a copy for many tokens).
+ * workspace: 256-byte aligned, b2q_linear_w4_workspace_bytes() bytes (0: may be NULL), the call's own until its last kernel has completed;
+ * what it holds before does not matter.                                                                                      */
+B2Q_API size_t b2q_linear_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t group);
+B2Q_API int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8_t* w, const void* scale, const uint8_t* zero, const void* bias, void* out,
+                  int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t group, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A whole expert layer on 4-bit experts for given routes: out[t] = sum over s of weights[t, s] y(ids[t, s], x[t]), y(e, x) = W2_e (silu(G_e x) * U_e x); ids outside
+ * [0, E) contribute nothing (an expert of another rank, padding), an expert named twice counts twice.  w13 [E, 2I, H / 2] (gate rows, then up), s13 and z13
+ * [E, H / group13, 2I], w2 [E, H, I / 2], s2 and z2 [E, I / group2, H], in the forms of b2q_linear_w4, all contiguous; z13, z2 may be NULL.  x, out
+ * contiguous [T, H] and scales in act_dtype, 16-byte aligned; weights fp32 and ids int32 contiguous [T, top_k].  E <= 1024, top_k <= 32.             */
+typedef struct b2q_moe_w4 {
+  const void* x;
+  const float* weights; const int32_t* ids;
+  const uint8_t* w13; const void* s13; const uint8_t* z13;
+  const uint8_t* w2; const void* s2; const uint8_t* z2;
+  void* out;
+  int64_t T, E, top_k, H, I, group13, group2;
+  int act_dtype;
+} b2q_moe_w4;
+B2Q_API size_t b2q_moe_forward_w4_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I);
+B2Q_API int b2q_moe_forward_w4(const b2q_moe_w4* args, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- sum of row-parallel partial results over the GPUs of one box ----------------------------
  * The exchange step behind a row-parallel linear (o_proj, down) of a tensor-parallel decoder layer; the
  * reference calls the serving framework's all-reduce there (vllm/patches/vllm_for_multi_arc.patch:10185,

@@ -19,6 +19,7 @@ OBJ = os.path.join(HERE, "build")
 OUT = os.path.join(HERE, "custom_esimd_kernels_vllm", "libb2q.so")
 OUT_TORCH = os.path.join(HERE, "custom_esimd_kernels_vllm", "libb2q_torch.so")
 OUT_INT8 = os.path.join(HERE, "custom_esimd_kernels_vllm", "libb2q_int8.so")
+OUT_W4 = os.path.join(HERE, "custom_esimd_kernels_vllm", "libb2q_w4.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC_FLAGS = [
@@ -74,13 +75,13 @@ def build(force=False, verbose=False):
         if r.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
     with cf.ThreadPoolExecutor() as ex:
-        list(ex.map(lambda a: build_torch_ops(force or bool(jobs), *a), ((OUT_TORCH, "torch_ops.cpp"), (OUT_INT8, "torch_int8.cpp"))))
+        list(ex.map(lambda a: build_torch_ops(force or bool(jobs), *a), ((OUT_TORCH, "torch_ops.cpp"), (OUT_INT8, "torch_int8.cpp"), (OUT_W4, "torch_w4.cpp"))))
     return OUT
 
 
 def build_torch_ops(force=False, out=OUT_TORCH, source="torch_ops.cpp"):
     """libb2q_torch.so: the C++ torch-op registration of the dense linears (csrc/torch_ops.cpp) over libb2q.so; libb2q_int8.so: that of
-    the 8-bit integer operators (csrc/torch_int8.cpp).
+    the 8-bit integer operators (csrc/torch_int8.cpp); libb2q_w4.so: that of expert routing and the 4-bit group-quantised layers (csrc/torch_w4.cpp).
     Host code only: compiled with g++ against the installed torch's headers and linked with its libraries."""
     src = os.path.join(CSRC, source)
     hdr = os.path.join(INCLUDE, "b2q.h")

@@ -25,6 +25,7 @@ from .int8 import (  # noqa: F401
     quantize_int8, silu_mul_quantize_int8, resadd_rmsnorm_quantize_int8, linear_int8, linear_int8_dynamic,
     moe_forward_int8,
 )
+from .w4 import route_experts, linear_w4, moe_forward_w4  # noqa: F401
 
 launch_count = _lib.launch_count
 last_kernel = _lib.last_kernel

@@ -42,6 +42,12 @@ class MoeInt8(C.Structure):
         + [(n, i32) for n in ("act_dtype", "logits_dtype", "s13_dtype", "s2_dtype", "renormalize")]
 
 
+class MoeW4(C.Structure):
+    """struct b2q_moe_w4"""
+    _fields_ = [(n, vp) for n in ("x", "weights", "ids", "w13", "s13", "z13", "w2", "s2", "z2", "out")] \
+        + [(n, i64) for n in ("T", "E", "top_k", "H", "I", "group13", "group2")] + [("act_dtype", i32)]
+
+
 _SIGS = {
     "b2q_strerror": (C.c_char_p, [i32]),
     "b2q_version": (i32, []),
@@ -89,6 +95,11 @@ _SIGS = {
     "b2q_linear_int8_dynamic": (i32, [vp, i32, i64, vp, vp, i32, vp, vp, i64, i64, i64, i64, vp, sz, vp]),
     "b2q_moe_forward_int8_workspace_bytes": (sz, [i64, i64, i64, i64, i64]),
     "b2q_moe_forward_int8": (i32, [C.POINTER(MoeInt8), vp, sz, vp]),
+    "b2q_route_experts": (i32, [vp, i32, i64, vp, i32, vp, vp, i64, i64, i64, i32, i64, i64, i32, i32, C.c_float, vp]),
+    "b2q_linear_w4_workspace_bytes": (sz, [i64, i64, i64, i64]),
+    "b2q_linear_w4": (i32, [vp, i32, i64, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, sz, vp]),
+    "b2q_moe_forward_w4_workspace_bytes": (sz, [i64, i64, i64, i64, i64]),
+    "b2q_moe_forward_w4": (i32, [C.POINTER(MoeW4), vp, sz, vp]),
     "b2q_comm_create": (i32, [i32, i32, i64, i64, vp, vp]),
     "b2q_comm_create_mode": (i32, [i32, i32, i64, i64, i32, vp, vp]),
     "b2q_comm_connect": (i32, [vp, vp]),
