@@ -32,8 +32,8 @@ int b2q_route_experts(const void* logits, int logits_dtype, int64_t ldl, const v
 }
 
 size_t b2q_linear_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t group) {
-  if (M <= 0 || N <= 0 || K <= 0 || !is_group(group)) return 0;
-  return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || !is_group(group) || M > MAX_ROWS || N > MAX_ROWS || K > MAX_K) return 0;
+  return g4_stream_fits((int)M, (int)N, (int)K, (int)group) ? g4_stream_bytes((int)M, (int)N, (int)K, (int)group) : 0;
 }
 
 int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8_t* w, const void* scale, const uint8_t* zero, const void* bias, void* out, int64_t ldo, int64_t M,
@@ -53,6 +53,7 @@ int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8_t* w, c
   G4LinearArgs a{};
   a.x = x; a.ldx = ldx; a.bf16 = act_dtype == B2Q_BF16; a.w = w; a.scale = scale; a.zero = zero; a.bias = bias; a.out = out; a.ldo = ldo;
   a.M = (int)M; a.N = (int)N; a.K = (int)K; a.G = (int)group;
+  if (g4_stream_fits(a.M, a.N, a.K, a.G)) return g4_stream_linear(a, workspace, (cudaStream_t)stream);
   return g4_tile_linear(a, (cudaStream_t)stream);
 }
 

@@ -23,6 +23,9 @@ struct G4LinearArgs {
   const void* bias; void* out; int64_t ldo;
   int M, N, K, G;
 };
+bool g4_stream_fits(int M, int N, int K, int G);           // up to sixteen tokens whose shares fit shared memory
+size_t g4_stream_bytes(int M, int N, int K, int G);
+int g4_stream_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st);
 int g4_tile_linear(const G4LinearArgs& a, cudaStream_t st);
 
 struct G4MoeArgs {

@@ -1,0 +1,363 @@
+// Linear of a few tokens on 4-bit group-quantised weights: out[m, n] = sum_g s[g, n] (sum_k x[m, k] q[n, k] - z[g, n] X[m, g]) (+ bias[n]).
+//
+// HBM-bound: the weights are read once, and there is little time to convert them (g4_stream.cuh has the mathematics and the layout).  A CTA per SM has rows of its own, dealt
+// out evenly.  Its units (16 RT rows of 128 k each) go to its sixteen warps in equal runs; a warp's next units are on their way while one is multiplied, and
+// nothing in the loop waits for another warp.  A warp leaves its sums of a tile of rows in a slot of shared memory; at the end they are added up in the
+// order of warps, so that results are the same every time.
+//
+// The tokens are scaled and permuted by each CTA for itself where that is one round of loads, else by a kernel in front, whose image of shared memory the CTAs
+// then fetch with one bulk copy, under the first weights.  Where the image does not fit, a cluster of two or four CTAs has rows together and a share of k each; their sums
+// meet in distributed shared memory.
+#include <algorithm>
+#include "sm100.cuh"
+#include "g4_stream.cuh"
+#include "umma_gemm.cuh"
+
+namespace b2q {
+namespace g4s {
+constexpr int WARPS = 16, THREADS = 32 * WARPS;
+constexpr int SELF = 4;                                    // eights that a thread prepares at most where a CTA prepares the tokens itself
+enum { ST_IMAGE = 901 };
+
+struct Params {
+  const uint16_t* x; int64_t ldx; int vec;
+  const uint8_t* image; const int* shifts;                 // of the kernel in front, or null
+  Matrix w; const uint16_t* bias; uint16_t* out; int64_t ldo;
+  int M, N, K, steps, cap;                                 // steps: of all K; cap: tiles of rows a CTA or cluster may have
+  int early;
+  int* status;
+};
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// One CTA per token: its row's image and shift.
+template <int G, int TT, bool BF16>
+__global__ void __launch_bounds__(256) g4_prep_kernel(const uint16_t* x, int64_t ldx, int vec, uint8_t* image, int* shifts, int M, int K, int steps) {
+  __shared__ uint32_t warp_max[8];
+  grid_dep_release();
+  grid_dep_wait();
+  constexpr int V = 8;
+  const int m = blockIdx.x, n = steps * (STEP / 8);
+  const uint16_t* row = x + m * ldx;
+  uint4 v[V];
+  uint32_t mx = 0;
+  for (int base = 0; base < n; base += V * 256) {
+#pragma unroll
+    for (int a = 0; a < V; ++a) {
+      const int c = base + a * 256 + threadIdx.x;
+      v[a] = 8 * c < K ? ld_eight(row + 8 * c, vec) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int a = 0; a < V; ++a) mx = max(mx, max_bits(v[a]));
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) mx = max(mx, warp_max[w]);
+  const int shift = row_shift<BF16>(mx);
+  const float f = pow2(shift);
+  if (threadIdx.x == 0) shifts[m] = shift;
+  for (int base = 0; base < n; base += V * 256) {
+    if (n > V * 256) {
+#pragma unroll
+      for (int a = 0; a < V; ++a) {
+        const int c = base + a * 256 + threadIdx.x;
+        v[a] = 8 * c < K ? ld_eight(row + 8 * c, vec) : make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < V; ++a) {
+      const int c = base + a * 256 + threadIdx.x;
+      if ((c & ~31) >= n) break;                           // whole warps
+      put_eight<G, TT, BF16>(image, M, m, c, v[a], f, c < n);
+    }
+  }
+}
+
+template <int VEC, int RT, int TT, bool BF16, bool PART>
+__global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
+  constexpr int G = 32 * VEC, GS = STEP / G, TOK = 8 * TT, ROWS = 16 * RT;      // GS: groups in a step
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint32_t row_max[TOK];
+  __shared__ int shifts[TOK];
+  __shared__ __align__(8) unsigned long long bar;
+  __shared__ int abort_flag;
+  uint32_t C;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(C));
+  const int rank = (int)sm100::cluster_ctarank();
+  const int cluster = blockIdx.x / C, clusters = gridDim.x / C;
+  const int s0 = rank * p.steps / (int)C, s1 = (rank + 1) * p.steps / (int)C, steps = s1 - s0;
+  const int sb = step_bytes(p.M, G, TT);
+  uint8_t* xs = smem + WARPS * RING<RT> * SLOT<RT>;            // [steps][step_bytes]
+  float* slots = reinterpret_cast<float*>(xs + (p.steps + C - 1) / C * sb);      // [tiles + WARPS][ROWS][TOK]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int r0 = (int)((int64_t)cluster * p.N / clusters), rows = (int)((int64_t)(cluster + 1) * p.N / clusters) - r0;
+  const int tiles = (rows + ROWS - 1) / ROWS, units = tiles * steps;
+  const int run = (units + WARPS - 1) / WARPS, u0 = min(units, warp * run), u1 = min(units, u0 + run);
+
+  grid_dep_release();
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    sm100::mbar_init(smem_addr(&bar), 1);
+    sm100::fence_barrier_init();
+  }
+  if (threadIdx.x < TOK) row_max[threadIdx.x] = 0;
+  if (!p.early) grid_dep_wait();
+  const Lane<VEC> ln;
+  const uint32_t ring = smem_addr(smem) + warp * RING<RT> * SLOT<RT>;
+  // Loads run ahead of the products: codes by RING - 1 steps, scales by two sets of four groups.  Sets begin anew with every tile.
+  Codes<RT, PART> codes;
+  Groups<RT> groups;
+  int uc = u0, us = u0, code_steps = 0, scale_steps = 0;   // the next units to load; steps left of their tiles
+  auto fetch_codes = [&](uint32_t slot) {
+    if (uc < u1) {
+      if (code_steps == 0) {
+        const int tile = uc / steps, s = uc - tile * steps;
+        codes.at(p.w, (s0 + s) * STEP, p.K, [&](int i) { return (int64_t)(r0 + min(ROWS * tile + g + 8 * i, rows - 1)); });
+        code_steps = min(u1 - uc, steps - s);
+      }
+      codes.copy(slot + ln.copy);
+      ++uc;
+      --code_steps;
+    }
+    copy_commit();
+  };
+  auto fetch_scales = [&](Scales<RT>& r) {
+    if (us < u1) {
+      if (scale_steps <= 0) {
+        const int tile = us / steps, s = us - tile * steps;
+        groups.at(p.w, r0, (s0 + s) * GS, p.K / G, [&](int i) { return min(ROWS * tile + g + 8 * i, rows - 1); });
+        scale_steps = min(u1 - us, steps - s);
+      }
+      groups.next(p.w, r);
+      const int n = min(4 / GS, scale_steps);
+      us += n;
+      scale_steps -= n;
+    }
+  };
+  Scales<RT> raw[2];
+#pragma unroll
+  for (int i = 0; i < RING<RT> - 1; ++i) fetch_codes(ring + i * SLOT<RT>);
+  fetch_scales(raw[0]);
+  fetch_scales(raw[1]);
+  if (p.early) grid_dep_wait();
+  __syncthreads();                                         // the barrier and the maxima
+  bool ok = true;
+  if (p.image) {
+    const uint32_t at = smem_addr(&bar);
+    if (threadIdx.x == 0) {
+      sm100::mbar_expect_tx(at, steps * sb);
+      for (int i = 0; i < steps * sb; i += 32768) sm100::bulk_load(smem_addr(xs) + i, p.image + (int64_t)s0 * sb + i, min(32768, steps * sb - i), at);
+    }
+    if (threadIdx.x < p.M) shifts[threadIdx.x] = __ldcg(p.shifts + threadIdx.x);
+    ok = sm100::mbar_wait_warp(at, 0, &abort_flag, p.status, ST_IMAGE);
+    if (!ok && threadIdx.x == 0) sm100::drain_issued(at, 1, 1);
+  } else {
+    const int per = steps * (STEP / 8), total = p.M * per;
+    const uint32_t inv = 0xFFFFFFFFu / (uint32_t)per + 1;  // i / per = i * inv >> 32 for i < 2^17, 1 < per < 2^14
+    uint4 v[SELF];
+    for (int i = threadIdx.x; i < steps * GS * TOK; i += THREADS) reinterpret_cast<float*>(xs + i / (GS * TOK) * sb + p.M * STEP * 2)[i % (GS * TOK)] = 0.f;
+#pragma unroll
+    for (int a = 0; a < SELF; ++a) {
+      const int i = a * THREADS + threadIdx.x, m = (int)__umulhi((uint32_t)i, inv), k = 8 * (i - m * per);
+      v[a] = i < total && k < p.K ? ld_eight(p.x + m * p.ldx + k, p.vec) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int a = 0; a < SELF; ++a) {
+      const int i = a * THREADS + threadIdx.x, m = (int)__umulhi((uint32_t)i, inv);
+      if ((i & ~31) >= total) break;                       // whole warps
+      uint32_t mx = max_bits(v[a]);                        // a half warp has one token, since `per` is a multiple of 16
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (i < total && (lane & 15) == 0) atomicMax(row_max + m, mx);
+    }
+    __syncthreads();
+    if (threadIdx.x < p.M) shifts[threadIdx.x] = row_shift<BF16>(row_max[threadIdx.x]);
+#pragma unroll
+    for (int a = 0; a < SELF; ++a) {
+      const int i = a * THREADS + threadIdx.x, m = (int)__umulhi((uint32_t)i, inv);
+      if ((i & ~31) >= total) break;
+      put_eight<G, TT, BF16>(xs, p.M, m, i - m * per, v[a], pow2(row_shift<BF16>(row_max[i < total ? m : 0])), i < total);
+    }
+  }
+  __syncthreads();
+
+  float sum[RT][TT][4];
+#pragma unroll
+  for (int h = 0; h < RT; ++h)
+#pragma unroll
+    for (int n = 0; n < TT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[h][n][i] = 0.f;
+  uint32_t token[TT];                                      // columns beyond M repeat the last: nobody looks at them
+#pragma unroll
+  for (int n = 0; n < TT; ++n) {
+    token[n] = smem_addr(xs) + min(8 * n + g, p.M - 1) * STEP * 2;
+  }
+  const uint32_t xg = smem_addr(xs) + p.M * STEP * 2 + 8 * t;
+  uint32_t packed[2 * RT], slot = ring;
+  int tile = steps ? u0 / steps : 0, s = u0 - tile * steps, used = 4;      // used: groups of the set
+  for (int u = u0; ok && u < u1; ++u) {
+    copy_wait<RING<RT> - 2>();
+    __syncwarp();                                          // other lanes' pieces are there, and all have read the slot that is filled next
+    fetch_codes(slot == ring ? ring + (RING<RT> - 1) * SLOT<RT> : slot - SLOT<RT>);
+    if (used == 4) {
+#pragma unroll
+      for (int i = 0; i < 2 * RT; ++i) packed[i] = pack_scale(raw[0].s[i], raw[0].z[i]);
+      raw[0] = raw[1];
+      fetch_scales(raw[1]);
+      used = 0;
+    }
+    uint32_t at[TT];
+#pragma unroll
+    for (int n = 0; n < TT; ++n) at[n] = token[n] + s * sb;
+    multiply<VEC, RT, TT, BF16>(sum, slot, ln, at, xg + s * sb, packed, used, rows - ROWS * tile > 16 ? 2 : 1);
+    used += GS;
+    slot = slot == ring + (RING<RT> - 1) * SLOT<RT> ? ring : slot + SLOT<RT>;
+    if (++s == steps || u + 1 == u1) {
+      flush<RT, TT>(sum, slots + (tile + warp) * ROWS * TOK);
+      ++tile;
+      s = 0;
+      used = 4;
+    }
+  }
+  copy_wait<0>();
+  __syncthreads();
+
+  // this CTA's sums, tile by tile, of warps in their order; sixteen lanes have consecutive rows
+  auto put = [&](int m, int r, float v) {
+    if (p.bias) v += half_f<BF16>(p.bias[r0 + r]);
+    p.out[m * p.ldo + r0 + r] = to_half<BF16>(v);
+  };
+  float* part = reinterpret_cast<float*>(smem);            // [M][rows], where the rings and the tokens were
+  const bool alone = C == 1;
+  for (int h = warp; h < tiles * RT; h += WARPS) {         // sixteens of rows
+    const int tl = h / RT, first = tl * steps / run, last = ((tl + 1) * steps - 1) / run, r = 16 * h + (lane & 15);      // warps that have units of it
+    for (int m = lane >> 4; m < p.M; m += 2) {
+      const float* from = slots + (tl * ROWS + r - ROWS * tl) * TOK + m;
+      float v = 0.f;
+      for (int w = first; w <= last; ++w) v += from[w * ROWS * TOK];
+      v = unshift(v, shifts[m]);
+      if (r < rows) {
+        if (alone) put(m, r, v);
+        else part[m * rows + r] = v;
+      }
+    }
+  }
+  if (!alone) {
+    sm100::cluster_sync_all();
+    const uint32_t from = smem_addr(part);
+    for (int r = rank * 32 + lane; r < rows; r += C * 32) {
+      for (int m = warp; m < p.M; m += WARPS) {
+        float v = 0.f;
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c)
+          if (c < C) v += ld_cluster_f32(sm100::map_to_cta(from + (m * rows + r) * 4, c));
+        put(m, r, v);
+      }
+    }
+    sm100::cluster_sync_all();                             // nobody leaves while its sums may be read
+  }
+}
+
+// ---- host ----
+constexpr int SMEM = 220 * 1024;
+struct Plan { int C, clusters, cap, smem, tt, rt, steps; bool self; };
+// Clusters of four that the SMs hold at a time: not all of them can be in one.
+static int resident(int C) { return C == 4 ? sm_count() * 7 / 32 : sm_count() / C; }
+static Plan plan(int M, int N, int K, int G) {
+  Plan q{};
+  q.steps = (K + STEP - 1) / STEP;
+  q.tt = M <= 8 ? 1 : 2;
+  q.self = M * q.steps * (STEP / 8) <= SELF * THREADS;
+  for (q.C = 1; q.C <= 4; q.C *= 2) {
+    if (q.C > 1 && (q.self || q.C > q.steps)) break;
+    q.clusters = resident(q.C);
+    if (q.clusters > (N + 7) / 8) q.clusters = (N + 7) / 8;
+    const int rows = (N + q.clusters - 1) / q.clusters, most = (q.steps + q.C - 1) / q.C;
+    q.rt = rows > 16 ? 2 : 1;
+    q.cap = (rows + 16 * q.rt - 1) / (16 * q.rt);
+    const int64_t front = (int64_t)WARPS * (q.rt == 2 ? RING<2> * SLOT<2> : RING<1> * SLOT<1>) + (int64_t)most * step_bytes(M, G, q.tt);
+    const int64_t smem = front + (int64_t)(q.cap + WARPS) * 16 * q.rt * 8 * q.tt * 4;
+    if (smem <= SMEM && (q.C == 1 || (int64_t)M * rows * 4 <= front)) { q.smem = (int)smem; return q; }
+  }
+  return q;
+}
+
+template <int VEC, int RT, int TT, bool BF16, bool PART> static int launch(Params& p, const Plan& q, cudaStream_t st) {
+  p.cap = q.cap;
+  const bool overlap = tls().overlap_mode > 0;
+  if (p.image) {
+    launch_overlapped(g4_prep_kernel<32 * VEC, TT, BF16>, dim3(p.M), dim3(256), 0, st, overlap, p.x, p.ldx, p.vec, const_cast<uint8_t*>(p.image), const_cast<int*>(p.shifts), p.M, p.K, p.steps);
+    note_launch("g4_prep");
+  }
+  auto kern = g4_stream_kernel<VEC, RT, TT, BF16, PART>;
+  static thread_local bool configured[16] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 16 || !configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return B2Q_ERR_CUDA;
+    if (dev < 16) configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(q.clusters * q.C); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = q.smem; cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (q.C > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = q.C; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (overlap) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at; cfg.numAttrs = n;
+  cudaLaunchKernelEx(&cfg, kern, p);                       // launch_status() reports
+  note_launch("g4_stream");
+  return launch_status();
+}
+template <int VEC, bool BF16, bool PART> static int by_size(Params& p, const Plan& q, cudaStream_t st) {
+  if (q.rt == 1) return q.tt == 1 ? launch<VEC, 1, 1, BF16, PART>(p, q, st) : launch<VEC, 1, 2, BF16, PART>(p, q, st);
+  return q.tt == 1 ? launch<VEC, 2, 1, BF16, PART>(p, q, st) : launch<VEC, 2, 2, BF16, PART>(p, q, st);
+}
+template <int VEC, bool PART> static int by_type(Params& p, bool bf16, const Plan& q, cudaStream_t st) {
+  return bf16 ? by_size<VEC, true, PART>(p, q, st) : by_size<VEC, false, PART>(p, q, st);
+}
+}  // namespace g4s
+
+bool g4_stream_fits(int M, int N, int K, int G) { return M <= 16 && g4s::plan(M, N, K, G).smem > 0; }
+
+size_t g4_stream_bytes(int M, int N, int K, int G) {
+  const g4s::Plan q = g4s::plan(M, N, K, G);
+  return q.self ? 0 : (size_t)q.steps * g4s::step_bytes(M, G, q.tt) + 16 * sizeof(int);
+}
+
+int g4_stream_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st) {
+  using namespace g4s;
+  const Plan q = plan(a.M, a.N, a.K, a.G);
+  if (!q.smem) return B2Q_ERR_LIMIT;
+  Params p{};
+  p.x = reinterpret_cast<const uint16_t*>(a.x); p.ldx = a.ldx; p.vec = ((reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(2 * a.ldx)) & 15u) == 0;
+  p.w = Matrix{a.w, reinterpret_cast<const uint16_t*>(a.scale), a.zero, a.K / 2, a.N};
+  p.bias = reinterpret_cast<const uint16_t*>(a.bias); p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.ldo;
+  p.M = a.M; p.N = a.N; p.K = a.K; p.steps = q.steps; p.early = tls().overlap_mode == 2;
+  p.status = umma_status_ptr();
+  if (!p.status) return B2Q_ERR_CUDA;
+  if (!q.self) {
+    p.image = reinterpret_cast<const uint8_t*>(scratch);
+    p.shifts = reinterpret_cast<const int*>(p.image + (size_t)q.steps * step_bytes(a.M, a.G, q.tt));
+  }
+  const bool part = a.K % STEP != 0;                       // groups of 128 leave no part of a step
+  if (a.G == 128) return by_type<4, false>(p, a.bf16, q, st);
+  if (a.G == 64) return part ? by_type<2, true>(p, a.bf16, q, st) : by_type<2, false>(p, a.bf16, q, st);
+  return part ? by_type<1, true>(p, a.bf16, q, st) : by_type<1, false>(p, a.bf16, q, st);
+}
+}  // namespace b2q
