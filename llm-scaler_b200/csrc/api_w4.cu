@@ -33,7 +33,8 @@ int b2q_route_experts(const void* logits, int logits_dtype, int64_t ldl, const v
 
 size_t b2q_linear_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t group) {
   if (M <= 0 || N <= 0 || K <= 0 || !is_group(group) || M > MAX_ROWS || N > MAX_ROWS || K > MAX_K) return 0;
-  return g4_stream_fits((int)M, (int)N, (int)K, (int)group) ? g4_stream_bytes((int)M, (int)N, (int)K, (int)group) : 0;
+  if (g4_stream_fits((int)M, (int)N, (int)K, (int)group)) return g4_stream_bytes((int)M, (int)N, (int)K, (int)group);
+  return umma_g4_bytes(nullptr, 0, (int)M, (int)N, (int)K, (int)group);
 }
 
 int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8_t* w, const void* scale, const uint8_t* zero, const void* bias, void* out, int64_t ldo, int64_t M,
@@ -54,14 +55,14 @@ int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8_t* w, c
   a.x = x; a.ldx = ldx; a.bf16 = act_dtype == B2Q_BF16; a.w = w; a.scale = scale; a.zero = zero; a.bias = bias; a.out = out; a.ldo = ldo;
   a.M = (int)M; a.N = (int)N; a.K = (int)K; a.G = (int)group;
   if (g4_stream_fits(a.M, a.N, a.K, a.G)) return g4_stream_linear(a, workspace, (cudaStream_t)stream);
-  return g4_tile_linear(a, (cudaStream_t)stream);
+  return umma_g4_linear(a, workspace, (cudaStream_t)stream);
 }
 
 size_t b2q_moe_forward_w4_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I) {
   if (T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || top_k > 32 || H <= 0 || I <= 0 || T > INT32_MAX / 32) return 0;
   G4MoeArgs g{};
   g.T = (int)T; g.E = (int)E; g.k = (int)top_k; g.H = (int)H; g.I = (int)I;
-  return g4_tile_moe_bytes(g);
+  return moe_g4_many_bytes(g);
 }
 
 int b2q_moe_forward_w4(const b2q_moe_w4* m, void* workspace, size_t workspace_bytes, void* stream) {
@@ -81,7 +82,7 @@ int b2q_moe_forward_w4(const b2q_moe_w4* m, void* workspace, size_t workspace_by
   G4MoeArgs g{};
   g.x = a.x; g.bf16 = a.act_dtype == B2Q_BF16; g.weights = a.weights; g.ids = a.ids; g.w13 = a.w13; g.s13 = a.s13; g.z13 = a.z13; g.w2 = a.w2; g.s2 = a.s2; g.z2 = a.z2;
   g.out = a.out; g.T = (int)a.T; g.E = (int)a.E; g.k = (int)a.top_k; g.H = (int)a.H; g.I = (int)a.I; g.G13 = (int)a.group13; g.G2 = (int)a.group2;
-  return g4_tile_moe(g, workspace, (cudaStream_t)stream);
+  return moe_g4_many(g, workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -26,7 +26,20 @@ struct G4LinearArgs {
 bool g4_stream_fits(int M, int N, int K, int G);           // up to sixteen tokens whose shares fit shared memory
 size_t g4_stream_bytes(int M, int N, int K, int G);
 int g4_stream_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st);
-int g4_tile_linear(const G4LinearArgs& a, cudaStream_t st);
+
+// Many tokens, on tcgen05.  out_w: grouped, what every row of the output is multiplied by.
+struct G4GroupedArgs {
+  const void* x; bool bf16;                                // rows sorted by expert, k permuted in eights (g4_position)
+  const uint8_t* w; const void* scale; const uint8_t* zero;      // [E, N (gated: 2 N), K / 2], [E, K / G, N (2 N)]
+  const int32_t* offsets; const int32_t* tiles; int tile, tile_cap, E;      // tile list of this height (g4_grouped_tile)
+  const float* out_w; void* out; int rows, N, K, G; bool gated;      // gated: out is silu(gate) * up, its columns permuted in eights
+};
+size_t umma_g4_bytes(const void* x, int64_t ldx, int M, int N, int K, int G);      // x null: the most that any x takes
+int umma_g4_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st);
+int g4_grouped_tile(int64_t rows, int E);
+int umma_g4_grouped(const G4GroupedArgs& a, cudaStream_t st);
+// Where value k of eight is kept for the grouped kernel: its masks take the codes of a word in the order 0, 4, 1, 5, 2, 6, 3, 7.
+__host__ __device__ constexpr int g4_position(int k) { return (k & ~7) | (k & 3) << 1 | (k >> 2 & 1); }
 
 struct G4MoeArgs {
   const void* x; bool bf16;
@@ -36,7 +49,7 @@ struct G4MoeArgs {
   void* out;
   int T, E, k, H, I, G13, G2;
 };
-size_t g4_tile_moe_bytes(const G4MoeArgs& a);
-int g4_tile_moe(const G4MoeArgs& a, void* scratch, cudaStream_t st);
+size_t moe_g4_many_bytes(const G4MoeArgs& a);
+int moe_g4_many(const G4MoeArgs& a, void* scratch, cudaStream_t st);
 
 }  // namespace b2q

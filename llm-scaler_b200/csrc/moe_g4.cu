@@ -1,0 +1,116 @@
+// The 4-bit expert layer of many tokens for given routes: the pairs (token, expert) sorted by expert, the tokens' rows copied into that order, a grouped GEMM with SiLU * mul
+// in its epilogue, a grouped GEMM whose outputs are multiplied by the routes' weights, the sum of each token's rows.
+//
+// h and the weighted outputs have 16 bits in between: h because it is the second product's operand; the outputs, one rounding each before the sum of top_k of them,
+// because they are read and written once (67 M values for 4096 tokens, top-8, H = 2048).
+#include "i8.cuh"
+#include "g4.cuh"
+
+namespace b2q {
+namespace g4m {
+struct Copies {
+  const int32_t *ids, *place, *base; const float* weights;
+  int32_t* rows; float* row_w;                             // of pairs; of rows
+  int k, E, run;
+};
+
+// A CTA per token: its row to the row of each of its pairs, the values of every eight in the order that the grouped kernel wants.
+__global__ void __launch_bounds__(256) g4_copies_kernel(const uint4* x, uint4* to, int per, const Copies c) {
+  __shared__ int rows[32];
+  grid_dep_enter();
+  const int t = blockIdx.x;
+  if (threadIdx.x < c.k) {
+    const int64_t pair = (int64_t)t * c.k + threadIdx.x;
+    const int id = __ldcg(c.ids + pair);
+    int row = -1;
+    if ((uint32_t)id < (uint32_t)c.E) {
+      row = __ldcg(c.base + (int64_t)(t / c.run) * c.E + id) + __ldcg(c.place + pair);
+      c.row_w[row] = __ldcg(c.weights + pair);
+    }
+    c.rows[pair] = row;
+    rows[threadIdx.x] = row;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < per; i += 256) {
+    const uint4 v = ld_vec(x + (int64_t)t * per + i);
+    const uint4 o = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+    for (int s = 0; s < c.k; ++s)
+      if (rows[s] >= 0) to[(int64_t)rows[s] * per + i] = o;
+  }
+}
+
+template <bool BF16> __global__ void __launch_bounds__(256) g4_sum_kernel(const uint4* y, const int32_t* rows, uint4* out, int64_t total, int per, int k) {
+  constexpr int AT_ONCE = 8;
+  grid_dep_enter();
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t t = i / per, c = i - t * per;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < k; s0 += AT_ONCE) {
+      uint4 v[AT_ONCE];
+      int32_t r[AT_ONCE];
+#pragma unroll
+      for (int s = 0; s < AT_ONCE; ++s) r[s] = s0 + s < k ? __ldcg(rows + t * k + s0 + s) : -1;
+#pragma unroll
+      for (int s = 0; s < AT_ONCE; ++s) v[s] = r[s] >= 0 ? __ldcg(y + (int64_t)r[s] * per + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int s = 0; s < AT_ONCE; ++s) {
+        const uint32_t e[4] = {v[s].x, v[s].y, v[s].z, v[s].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float a, b;
+          unpack2<BF16>(e[j], a, b);
+          acc[2 * j] += a;
+          acc[2 * j + 1] += b;
+        }
+      }
+    }
+    out[i] = make_uint4(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]), pack2<BF16>(acc[4], acc[5]), pack2<BF16>(acc[6], acc[7]));
+  }
+}
+
+struct Parts { uint8_t *place, *rows, *row_w, *base, *offsets, *count, *tiles, *x, *h, *y; size_t total; };
+static Parts parts_of(void* ws, const G4MoeArgs& a) {
+  Parts p{};
+  uint8_t* base = reinterpret_cast<uint8_t*>(ws);
+  size_t at = 0;
+  auto take = [&](size_t bytes) { uint8_t* q = base + at; at += (bytes + 255) / 256 * 256; return q; };
+  const size_t rows = (size_t)a.T * a.k;
+  p.place = take(rows * 4); p.rows = take(rows * 4); p.row_w = take(rows * 4);
+  p.base = take((size_t)moe_i8_route_ctas(a.T) * a.E * 4); p.offsets = take((size_t)(a.E + 1) * 4); p.count = take(8);
+  p.tiles = take(16 + 8 * (rows / 32 + 1 + a.E));
+  p.x = take(rows * a.H * 2); p.h = take(rows * a.I * 2); p.y = take(rows * a.H * 2);
+  p.total = at;
+  return p;
+}
+}  // namespace g4m
+
+size_t moe_g4_many_bytes(const G4MoeArgs& a) { return g4m::parts_of(nullptr, a).total; }
+
+int moe_g4_many(const G4MoeArgs& a, void* scratch, cudaStream_t st) {
+  using namespace g4m;
+  const Parts p = parts_of(scratch, a);
+  const int64_t rows = (int64_t)a.T * a.k;
+  const int tile = g4_grouped_tile(rows, a.E), ctas = moe_i8_route_ctas(a.T);
+  const bool overlap = tls().overlap_mode > 0;
+  int32_t *off = reinterpret_cast<int32_t*>(p.offsets), *tiles = reinterpret_cast<int32_t*>(p.tiles), *out_rows = reinterpret_cast<int32_t*>(p.rows);
+  int rc = moe_route_given(a.ids, a.T, a.E, a.k, tile, reinterpret_cast<int32_t*>(p.place), reinterpret_cast<int32_t*>(p.base), off, tiles, p.count, st);
+  if (rc) return rc;
+  Copies c{};
+  c.ids = a.ids; c.place = reinterpret_cast<int32_t*>(p.place); c.base = reinterpret_cast<int32_t*>(p.base); c.weights = a.weights;
+  c.rows = out_rows; c.row_w = reinterpret_cast<float*>(p.row_w); c.k = a.k; c.E = a.E; c.run = (a.T + ctas - 1) / ctas;
+  launch_overlapped(g4_copies_kernel, dim3(a.T), dim3(256), 0, st, overlap, reinterpret_cast<const uint4*>(a.x), reinterpret_cast<uint4*>(p.x), a.H / 8, c);
+  note_launch("g4_copies");
+  G4GroupedArgs g{};
+  g.x = p.x; g.bf16 = a.bf16; g.w = a.w13; g.scale = a.s13; g.zero = a.z13; g.offsets = off; g.tiles = tiles; g.tile = tile; g.tile_cap = (int)((rows + tile - 1) / tile + a.E); g.E = a.E;
+  g.out = p.h; g.rows = (int)rows; g.N = a.I; g.K = a.H; g.G = a.G13; g.gated = true;
+  rc = umma_g4_grouped(g, st);
+  g.x = p.h; g.w = a.w2; g.scale = a.s2; g.zero = a.z2; g.out_w = c.row_w; g.out = p.y; g.N = a.H; g.K = a.I; g.G = a.G2; g.gated = false;
+  if (!rc) rc = umma_g4_grouped(g, st);
+  if (rc) return rc;
+  const int64_t total = (int64_t)a.T * (a.H / 8), n = (total + 255) / 256;
+  launch_overlapped(a.bf16 ? g4_sum_kernel<true> : g4_sum_kernel<false>, dim3((unsigned)(n < 148 * 8 ? n : 148 * 8)), dim3(256), 0, st, overlap, reinterpret_cast<const uint4*>(p.y),
+                    (const int32_t*)out_rows, reinterpret_cast<uint4*>(a.out), total, a.H / 8, a.k);
+  note_launch("g4_sum");
+  return launch_status();
+}
+}  // namespace b2q

@@ -27,7 +27,8 @@ struct Params {
   Arrivals* count; Arrivals tag; const Arrivals* epoch;
 };
 
-template <int PER>
+// GIVEN: the experts of every token are there already (ids outside [0, E): none), and only their pairs are sorted.
+template <int PER, bool GIVEN>
 __global__ void __launch_bounds__(THREADS) moe_i8_route_kernel(const Params p) {
   __shared__ int counts[MAX_E];
   __shared__ int part[SPANS][CHUNKS][32];
@@ -39,9 +40,15 @@ __global__ void __launch_bounds__(THREADS) moe_i8_route_kernel(const Params p) {
   const bool alone = gridDim.x == 1;                       // its counts need not leave the SM (16 tokens: 8.2 us otherwise, by itself)
   if (threadIdx.x == 0 && !alone) arrivals_open(p.count, p.tag, p.epoch);
   const int t0 = blockIdx.x * p.per_cta, t1 = min(p.T, t0 + p.per_cta);
+  if constexpr (GIVEN) {
+    for (int64_t pair = (int64_t)t0 * p.k + threadIdx.x; pair < (int64_t)t1 * p.k; pair += THREADS) {
+      const int id = __ldcg(p.ids + pair);
+      p.place[pair] = (uint32_t)id < (uint32_t)p.E ? atomicAdd(&counts[id], 1) : 0;
+    }
+  }
   float v[PER];
-  if (t0 + warp < t1) i8r::load_logits<PER>(p.logits, p.dt, p.E, t0 + warp, v);
-  for (int t = t0 + warp; t < t1; t += WARPS) {
+  if (!GIVEN && t0 + warp < t1) i8r::load_logits<PER>(p.logits, p.dt, p.E, t0 + warp, v);
+  for (int t = t0 + warp; !GIVEN && t < t1; t += WARPS) {
     float now[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) now[j] = v[j];
@@ -213,22 +220,33 @@ int moe_i8_route_ctas(int64_t T) {
   return (int)(n < i8m::MAX_CTAS ? n : i8m::MAX_CTAS);
 }
 
-int moe_i8_route(const void* logits, int dt, int64_t T, int E, int k, bool renorm, int tile, float* weights, int32_t* ids, int32_t* place, int32_t* base,
-                 int32_t* offsets, int32_t* tiles, void* count, cudaStream_t st) {
+static int route(i8m::Params& p, int64_t T, int E, int k, int tile, int32_t* ids, int32_t* place, int32_t* base, int32_t* offsets, int32_t* tiles, void* count, bool given, cudaStream_t st) {
   using namespace i8m;
-  Params p{};
-  p.logits = logits; p.dt = dt; p.T = (int)T; p.E = E; p.k = k; p.renorm = renorm; p.tile = tile;
-  p.weights = weights; p.ids = ids; p.place = place; p.base = base; p.offsets = offsets; p.tiles = tiles;
+  p.T = (int)T; p.E = E; p.k = k; p.tile = tile;
+  p.ids = ids; p.place = place; p.base = base; p.offsets = offsets; p.tiles = tiles;
   p.count = reinterpret_cast<Arrivals*>(count); p.tag = arrivals_tag(); p.epoch = arrivals_epoch();
   if (!p.epoch) return B2Q_ERR_CUDA;
   const int ctas = moe_i8_route_ctas(T);
   p.per_cta = (int)((T + ctas - 1) / ctas);
   auto go = [&](void (*kern)(const Params)) { launch_overlapped(kern, dim3(ctas), dim3(THREADS), 0, st, tls().overlap_mode > 0, p); };
-  if (E <= 128) go(moe_i8_route_kernel<4>);
-  else if (E <= 256) go(moe_i8_route_kernel<8>);
-  else go(moe_i8_route_kernel<32>);
+  if (given) go(moe_i8_route_kernel<1, true>);
+  else if (E <= 128) go(moe_i8_route_kernel<4, false>);
+  else if (E <= 256) go(moe_i8_route_kernel<8, false>);
+  else go(moe_i8_route_kernel<32, false>);
   note_launch("moe_i8_route");
   return launch_status();
+}
+
+int moe_i8_route(const void* logits, int dt, int64_t T, int E, int k, bool renorm, int tile, float* weights, int32_t* ids, int32_t* place, int32_t* base,
+                 int32_t* offsets, int32_t* tiles, void* count, cudaStream_t st) {
+  i8m::Params p{};
+  p.logits = logits; p.dt = dt; p.renorm = renorm; p.weights = weights;
+  return route(p, T, E, k, tile, ids, place, base, offsets, tiles, count, false, st);
+}
+
+int moe_route_given(const int32_t* ids, int64_t T, int E, int k, int tile, int32_t* place, int32_t* base, int32_t* offsets, int32_t* tiles, void* count, cudaStream_t st) {
+  i8m::Params p{};
+  return route(p, T, E, k, tile, const_cast<int32_t*>(ids), place, base, offsets, tiles, count, true, st);      // read only
 }
 
 int moe_i8_sum(const void* y, bool y_f32, const float* weights, const int32_t* rows, const I8Outputs& of, void* out, bool bf16, int64_t T, int k, int H, cudaStream_t st) {

@@ -308,6 +308,15 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uin
       : "memory");
 }
 
+// The same over a pair of CTAs: 256 rows, each CTA's 128 in its own tensor memory.
+__device__ __forceinline__ void mma_f16_ts_pair(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // ---- descriptors ----------------------------------------------------------------------------
 // K-major operand tile stored as rows of 128 bytes with the 128-byte swizzle (16-byte chunk c of
 // row r lives at chunk c ^ (r & 7)); 8-row groups are 1024 bytes apart.  The tile base must be

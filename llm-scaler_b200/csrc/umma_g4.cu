@@ -1,0 +1,706 @@
+// GEMM of many tokens on 4-bit group-quantised weights by tcgen05: out[m, n] = sum_k x[m, k] w[n, k] (+ bias[n]), w = (q - z) s rounded once to the activations' type;
+// dense where g4_stream.cu does not serve, and grouped by expert.
+//
+// 128 weight rows are the MMA's rows, a tile of NT tokens its columns.  Raw codes come by TMA; transform warps turn them into 16-bit values, a thread a row, and write
+// them straight into tensor memory as the MMA's A operand; tokens come by TMA.  q - z is exact (the code is put below a power of two and that power plus z
+// subtracted), times s is the one rounding; it is of the size of the output's own.
+//
+// A persistent CTA has separate warps for the weights' copies, the tokens' copies, the MMA, the epilogue and the transform, so that nothing of one tile stops the stream
+// of the next.  An operand stage is 128 k; each ring stage stays with one group of four transform warps, since a parity wait cannot tell a phase from the one
+// before the last.
+//
+//  * PAIR: two CTAs share a tile of 256 rows (cta_group::2), each with its own 128 rows in tensor memory and half of the tokens in shared memory.  A CTA alone would pull
+//    64 bytes of tokens per cycle of MMA through L2, a pair's 32.
+//  * Where strips of 128 rows are fewer than SMs, k is cut into pieces; whoever delivers the last of a strip's partial sums adds them up in order (arrivals.cuh).
+//  * GATED (expert up projection): a warp's 32 rows are 16 gate and 16 up rows of the same outputs, and the epilogue stores silu(gate) * up.
+//
+// No multicast load; every mbarrier wait is bounded, as in the other tcgen05 kernels.
+#include "umma_gemm.cuh"
+#include "sm100.cuh"
+#include "arrivals.cuh"
+#include "g4.cuh"
+
+namespace b2q {
+
+using namespace sm100;
+
+namespace ug4 {
+enum { ST_RAWEMPTY = 951, ST_RAWFULL = 952, ST_AEMPTY = 953, ST_AFULL = 954, ST_XEMPTY = 955, ST_XFULL = 956, ST_ACCEMPTY = 957, ST_ACCFULL = 958 };
+
+template <int NT, bool PAIR> struct Cfg {
+  static constexpr int DG = NT <= 64 ? 4 : 2;                // transform groups
+  static constexpr int EW = NT <= 64 ? 4 : 8;                // epilogue warps
+  static constexpr int FIRST_EPI = 4, FIRST_DEQ = FIRST_EPI + EW, THREADS = 32 * (FIRST_DEQ + 4 * DG);
+  static constexpr int COLS = NT < 32 ? 32 : NT;             // of an accumulator
+  static constexpr int NBUF = NT <= 128 ? 2 : 1;
+  static constexpr int A_COL0 = NBUF * COLS;
+  static constexpr int S = (512 - A_COL0) / 64 / DG * DG;    // operand stages of 128 k
+  static constexpr int TOK = PAIR ? NT / 2 : NT;             // tokens that a CTA loads
+  static constexpr int X_BYTES = TOK * 256, RAW_BYTES = 8192;
+  static constexpr int XS = NT == 256 ? (PAIR ? 4 : 2) : (NT == 128 ? 4 : 6);
+  static constexpr int RS = NT <= 64 ? 8 : 6;                // raw stages, a multiple of DG
+  static constexpr int STG = EW * 2048;                      // 32 tokens x 32 columns for every epilogue warp
+  static constexpr int USED = XS * X_BYTES + RS * RAW_BYTES + STG + 1024;
+  static constexpr int SMEM = 1024 + (USED < 170 * 1024 ? 170 * 1024 : USED);      // one CTA with tensor memory on an SM: see umma_i8.cu
+  static_assert(RS % DG == 0 && S % DG == 0 && S > 0 && SMEM <= 232448, "rings");
+};
+
+struct Params {
+  const uint16_t* s; const uint8_t* z; int64_t s_expert; int s_rows;      // scales [groups][s_rows]
+  const uint16_t* bias; const float* out_w;
+  uint16_t* out; int64_t ldo; int vec_out;
+  int M, N, K, groups, nks;                                // nks: stages that K takes
+  int n_strips, m_tiles, m_group, pieces, total;           // total: tiles of a dense launch
+  float* partials; Arrivals* arrivals; Arrivals tag; const Arrivals* epoch;
+  const int32_t* tiles; const int32_t* offsets;            // grouped
+  int early;
+  int* status;
+};
+
+struct Tile { int tok0, rows, n0, w0, ks0, ks1, piece, strip, e; };      // n0: first output column of the CTA or pair; w0: first weight row in memory (of an expert's gate half)
+
+template <int NT, bool PAIR, bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(const Params& p, int id) {
+  constexpr int WIDTH = (PAIR ? 256 : 128) / (GATED ? 2 : 1);      // output columns of a strip
+  Tile t;
+  t.piece = 0; t.ks0 = 0; t.ks1 = p.nks; t.e = 0;
+  if constexpr (GROUPED) {
+    const int ti = id / p.n_strips, st = id - ti * p.n_strips;
+    const int e = __ldcg(p.tiles + 4 + 2 * ti), r0 = __ldcg(p.tiles + 4 + 2 * ti + 1);
+    t.tok0 = __ldcg(p.offsets + e) + r0;
+    t.rows = min(NT, __ldcg(p.offsets + e + 1) - t.tok0);
+    t.n0 = st * WIDTH;
+    t.w0 = (GATED ? 2 : 1) * e * p.N + t.n0;
+    t.strip = 0;
+    t.e = e;
+  } else {
+    if (p.pieces > 1) {
+      t.strip = id / p.pieces;
+      t.piece = id - t.strip * p.pieces;
+      t.ks0 = (int)((int64_t)t.piece * p.nks / p.pieces);
+      t.ks1 = (int)((int64_t)(t.piece + 1) * p.nks / p.pieces);
+      id = t.strip;
+    }
+    const int per = p.m_group * p.n_strips, gi = id / per, left = id - gi * per, m0 = gi * p.m_group;
+    const int gm = min(p.m_group, p.m_tiles - m0), st = left / gm, mt = m0 + left - st * gm;
+    t.tok0 = mt * NT;
+    t.rows = min(NT, p.M - t.tok0);
+    t.n0 = st * WIDTH;
+    t.w0 = t.n0;
+  }
+  return t;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(v) : "memory"); }
+__device__ __forceinline__ uint32_t ld_u16(const uint16_t* p) { uint32_t v; asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p)); return v; }
+__device__ __forceinline__ uint32_t ld_u8(const uint8_t* p) { uint32_t v; asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(v) : "l"(p)); return v; }
+
+// Two 16-bit values at a time.
+template <bool BF16> __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma2_f16(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
+// Eight codes of a word -> four registers of two values (q - z) s.  PERM: in the order 0, 4, 1, 5, 2, 6, 3, 7, else as they come.  zc: the power of two plus z, twice (fp16 and
+// PERM: and -(64 + z) in zh); more: bf16, what z has beyond 127, for 128 + z has to fit eight bits.
+template <bool BF16, bool PERM> __device__ __forceinline__ void decode(uint32_t w, uint32_t s2, uint32_t zc, uint32_t zh, uint32_t more, bool has_more, uint32_t* o) {
+  constexpr uint32_t MASK = 0x000F000Fu, MAGIC = BF16 ? 0x43004300u : 0x64006400u;
+  if constexpr (PERM && !BF16) {
+    const uint32_t w8 = w >> 8;
+    o[0] = sub2<false>((w & MASK) | MAGIC, zc);
+    o[2] = sub2<false>((w8 & MASK) | MAGIC, zc);
+    o[1] = fma2_f16((w & 0x00F000F0u) | MAGIC, 0x2C002C00u, zh);      // 2^-4 (1024 + 16 q) - (64 + z)
+    o[3] = fma2_f16((w8 & 0x00F000F0u) | MAGIC, 0x2C002C00u, zh);
+  } else if constexpr (PERM) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = sub2<true>(((w >> 4 * i) & MASK) | MAGIC, zc);
+  } else {
+    const uint32_t w4 = w >> 4;
+    o[0] = sub2<BF16>((__byte_perm(w, w4, 0x4400) & MASK) | MAGIC, zc);
+    o[1] = sub2<BF16>((__byte_perm(w, w4, 0x5511) & MASK) | MAGIC, zc);
+    o[2] = sub2<BF16>((__byte_perm(w, w4, 0x6622) & MASK) | MAGIC, zc);
+    o[3] = sub2<BF16>((__byte_perm(w, w4, 0x7733) & MASK) | MAGIC, zc);
+  }
+  if (BF16 && has_more) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = sub2<true>(o[i], more);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = mul2<BF16>(o[i], s2);
+}
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (BF16) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool BF16> __device__ __forceinline__ float half_f(uint32_t raw) { return BF16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half((unsigned short)raw)); }
+
+// Sixteen tokens' values of a warp's rows (a lane has one row, tokens 2 i and 2 i + 1 in o[i]) through shared memory to out: rows of 32 consecutive columns.  cols, rows: how
+// many there are.
+__device__ __forceinline__ void store16(uint32_t stg, const uint32_t (&o)[8], uint16_t* out, int64_t ldo, int rows, int cols, bool vec) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    sts16(stg + (2 * i) * 64 + lane * 2, (uint16_t)o[i]);
+    sts16(stg + (2 * i + 1) * 64 + lane * 2, (uint16_t)(o[i] >> 16));
+  }
+  __syncwarp();
+  if (vec && cols % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int tk = i * 8 + (lane >> 2), c = (lane & 3) * 8;
+      const uint4 v = lds128(stg + tk * 64 + c * 2);
+      if (tk < rows && c < cols) *reinterpret_cast<uint4*>(out + tk * ldo + c) = v;
+    }
+  } else {
+    for (int tk = 0; tk < 16 && tk < rows; ++tk) {
+      uint16_t v;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(stg + tk * 64 + lane * 2) : "memory");
+      if (lane < cols) out[tk * ldo + lane] = v;
+    }
+  }
+}
+}  // namespace ug4
+
+template <bool BF16, int G, int NT, bool PAIR, bool GROUPED, bool GATED>
+__global__ void __launch_bounds__(ug4::Cfg<NT, PAIR>::THREADS, 1)
+umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const ug4::Params p) {
+  using namespace ug4;
+  using C = Cfg<NT, PAIR>;
+  constexpr bool PERM = GROUPED;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  // [token stages] [raw stages] [staging] [barriers]
+  const uint32_t raw0 = base + C::XS * C::X_BYTES, stg0 = raw0 + C::RS * C::RAW_BYTES, bar = stg0 + C::STG;
+  const uint32_t x_full = bar, x_empty = x_full + 8 * C::XS, raw_full = x_empty + 8 * C::XS, raw_empty = raw_full + 8 * C::RS, a_full = raw_empty + 8 * C::RS, a_empty = a_full + 8 * C::S,
+                 acc_full = a_empty + 8 * C::S, acc_empty = acc_full + 16, tail = acc_empty + 16;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + (tail - base));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + (tail + 4 - base));
+  volatile int* last_flag = reinterpret_cast<volatile int*>(gen + (tail + 8 - base));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+  const int first = (int)blockIdx.x / (PAIR ? 2 : 1), step = (int)gridDim.x / (PAIR ? 2 : 1);
+
+  grid_dep_release();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::XS; ++i) { mbar_init(x_full + 8 * i, 1); mbar_init(x_empty + 8 * i, 1); }
+    for (int i = 0; i < C::RS; ++i) { mbar_init(raw_full + 8 * i, 1); mbar_init(raw_empty + 8 * i, 4); }
+    for (int i = 0; i < C::S; ++i) { mbar_init(a_full + 8 * i, PAIR ? 8 : 4); mbar_init(a_empty + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, PAIR ? 2 * C::EW : C::EW); }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) { tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512); tmem_relinquish_pair(); }
+    else { tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512); tmem_relinquish(); }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (GROUPED) grid_dep_wait();                            // the tile list is made by the kernels in front
+  const int total = GROUPED ? __ldcg(p.tiles) * p.n_strips : p.total;
+
+  if (warp == 0) {
+    // ---- raw codes ----
+    if (elect_one()) {
+      tma_prefetch_desc(&tm_w);
+      if (!GROUPED && !p.early) grid_dep_wait();
+      int s = 0, issued = 0;
+      uint32_t par = 1u;
+      bool ok = true;
+      for (int id = first; ok && id < total; id += step) {
+        const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+        const int w = t.w0 + (int)rank * (GATED ? 64 : 128);
+        for (int ks = t.ks0; ks < t.ks1; ++ks) {
+          ok = mbar_wait(raw_empty + 8 * s, par, abort_flag, p.status, ST_RAWEMPTY);
+          if (!ok) break;
+          mbar_expect_tx(raw_full + 8 * s, C::RAW_BYTES);
+          const uint32_t dst = raw0 + s * C::RAW_BYTES;
+          tma_load_2d(dst, &tm_w, ks * 64, w, raw_full + 8 * s);
+          if constexpr (GATED) tma_load_2d(dst + C::RAW_BYTES / 2, &tm_w, ks * 64, w + p.N, raw_full + 8 * s);
+          ++issued;
+          if (++s == C::RS) { s = 0; par ^= 1u; }
+        }
+      }
+      if (!ok) drain_issued(raw_full, C::RS, issued);
+    }
+  } else if (warp == 2) {
+    // ---- tokens ----
+    if (elect_one()) {
+      tma_prefetch_desc(&tm_x);
+      grid_dep_wait();
+      int s = 0, issued = 0;
+      uint32_t par = 1u;
+      bool ok = true;
+      for (int id = first; ok && id < total; id += step) {
+        const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+        for (int ks = t.ks0; ks < t.ks1; ++ks) {
+          ok = mbar_wait(x_empty + 8 * s, par, abort_flag, p.status, ST_XEMPTY);
+          if (!ok) break;
+          const uint32_t dst = base + s * C::X_BYTES;
+          if (rank == 0) mbar_expect_tx(x_full + 8 * s, C::X_BYTES * (PAIR ? 2 : 1));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if constexpr (PAIR) tma_load_2d_pair(dst + i * C::TOK * 128, &tm_x, ks * 128 + i * 64, t.tok0 + (int)rank * C::TOK, map_to_cta(x_full + 8 * s, 0));
+            else tma_load_2d(dst + i * C::TOK * 128, &tm_x, ks * 128 + i * 64, t.tok0, x_full + 8 * s);
+          }
+          ++issued;
+          if (++s == C::XS) { s = 0; par ^= 1u; }
+        }
+      }
+      if (!ok && rank == 0) drain_issued(x_full, C::XS, issued);
+    }
+  } else if (warp == 1) {
+    if ((!PAIR || rank == 0) && elect_one()) {
+      const uint32_t idesc = instr_desc(BF16 ? 1u : 0u, BF16 ? 1u : 0u, PAIR ? 256u : 128u, (uint32_t)NT);
+      int xs = 0, as = 0, it = 0;
+      uint32_t xpar = 0u, apar = 0u;
+      bool ok = true;
+      for (int id = first; ok && id < total; id += step, ++it) {
+        const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+        const int b = it % C::NBUF;
+        if (it >= C::NBUF) ok = mbar_wait(acc_empty + 8 * b, (it / C::NBUF - 1) & 1, abort_flag, p.status, ST_ACCEMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + b * C::COLS;
+        for (int ks = t.ks0; ks < t.ks1; ++ks) {
+          ok = mbar_wait(x_full + 8 * xs, xpar, abort_flag, p.status, ST_XFULL) && mbar_wait(a_full + 8 * as, apar, abort_flag, p.status, ST_AFULL);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a = tmem + C::A_COL0 + as * 64;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint64_t db = smem_desc_sw128(base + xs * C::X_BYTES + i * C::TOK * 128);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if constexpr (PAIR) mma_f16_ts_pair(d, a + 32 * i + 8 * j, db + 2 * j, idesc, ks > t.ks0 || i > 0 || j > 0);
+              else mma_f16_ts(d, a + 32 * i + 8 * j, db + 2 * j, idesc, ks > t.ks0 || i > 0 || j > 0);
+            }
+          }
+          if constexpr (PAIR) { tc_commit_pair(x_empty + 8 * xs, 3); tc_commit_pair(a_empty + 8 * as, 3); }
+          else { tc_commit(x_empty + 8 * xs); tc_commit(a_empty + 8 * as); }
+          if (++xs == C::XS) { xs = 0; xpar ^= 1u; }
+          if (++as == C::S) { as = 0; apar ^= 1u; }
+        }
+        if (!ok) break;
+        if constexpr (PAIR) tc_commit_pair(acc_full + 8 * b, 3); else tc_commit(acc_full + 8 * b);
+      }
+    }
+  } else if (warp >= C::FIRST_DEQ) {
+    // ---- transform: group g of four warps has every DG-th stage, a thread a row ----
+    const int grp = (warp - C::FIRST_DEQ) >> 2, quad = warp & 3;
+    const int raw_row = GATED ? (lane < 16 ? 16 * quad + lane : 48 + 16 * quad + lane) : 32 * quad + lane;      // 64 + 16 quad + lane - 16
+    const uint32_t row_at = raw_row * 64, f = (raw_row >> 1) & 3;      // 64-byte swizzle of the raw box
+    constexpr int GS = 128 / G;
+    if (!GROUPED && !p.early) grid_dep_wait();
+    int it = 0;                                            // stages so far
+    bool ok = true;
+    uint32_t sc[GS], zc[GS];
+    for (int id = first; ok && id < total; id += step) {
+      const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+      // this thread's row among the scales' rows; beyond the last it repeats it, and nobody looks at the sums
+      int row;
+      if constexpr (GATED) { const int h = min(t.n0 + (int)rank * 64 + 16 * quad + (lane & 15), p.N - 1); row = lane < 16 ? h : p.N + h; }
+      else row = min(t.n0 + (int)rank * 128 + 32 * quad + lane, p.N - 1);
+      const int64_t at0 = (int64_t)t.e * p.s_expert + row;
+      const int n = t.ks1 - t.ks0, mine0 = (grp - it % C::DG + C::DG) % C::DG;      // the tile's first stage that is this group's
+      auto fetch = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < GS; ++i) {
+          const int64_t at = at0 + (int64_t)min((t.ks0 + j) * GS + i, p.groups - 1) * p.s_rows;
+          sc[i] = ld_u16(p.s + at);
+          zc[i] = p.z ? ld_u8(p.z + at) : 8u;
+        }
+      };
+      if (mine0 < n) fetch(mine0);
+      for (int j = mine0; j < n; j += C::DG) {
+        const int now = it + j, rs = now % C::RS, as = now % C::S;
+        uint32_t s2[GS], z2[GS], zh[GS], more[GS];
+        bool has_more = false;
+#pragma unroll
+        for (int i = 0; i < GS; ++i) {
+          s2[i] = sc[i] * 0x00010001u;
+          const uint32_t z = zc[i];
+          if (BF16) {
+            const uint32_t low = min(z, 127u);
+            z2[i] = 0x43004300u | low * 0x00010001u;
+            more[i] = __float_as_uint((float)(z - low)) >> 16;
+            more[i] |= more[i] << 16;
+            has_more = has_more || z > 127u;
+            zh[i] = 0;
+          } else {
+            z2[i] = 0x64006400u | z * 0x00010001u;
+            zh[i] = __half_as_ushort(__float2half_rn(-64.f - (float)z)) * 0x00010001u;
+            more[i] = 0;
+          }
+        }
+        has_more = BF16 && __any_sync(0xffffffffu, has_more);
+        if (j + C::DG < n) fetch(j + C::DG);
+        ok = mbar_wait_warp(raw_full + 8 * rs, (now / C::RS) & 1, abort_flag, p.status, ST_RAWFULL);
+        if (!ok) break;
+        uint4 raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = lds128(raw0 + rs * C::RAW_BYTES + row_at + ((i ^ f) << 4));
+        if (now >= C::S) ok = mbar_wait_warp(a_empty + 8 * as, (now / C::S - 1) & 1, abort_flag, p.status, ST_AEMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t a = tmem + C::A_COL0 + as * 64 + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint4 r = raw[2 * h + i];
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const int grp_of = (h * 64 + i * 32 + v * 8) / G;
+              decode<BF16, PERM>(w[v], s2[grp_of], z2[grp_of], zh[grp_of], more[grp_of], has_more, o + 16 * i + 4 * v);
+            }
+          }
+          tmem_st32(a + 32 * h, o);
+        }
+        mbar_arrive_read(raw_empty + 8 * rs);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(a_full + 8 * as, 0));
+          else mbar_arrive(a_full + 8 * as);
+        }
+        __syncwarp();
+      }
+      it += n;
+    }
+  } else if (warp >= C::FIRST_EPI) {
+    // ---- epilogue: lane quadrant = warp & 3 (weight rows); tokens shared by the warps of a quadrant ----
+    const int quad = warp & 3, half = (warp - C::FIRST_EPI) >> 2;
+    constexpr int HALVES = C::EW / 4, MINE = NT / HALVES;  // tokens of a warp
+    constexpr int CH = MINE < 32 ? 16 : 32;
+    const uint32_t stg = stg0 + (warp - C::FIRST_EPI) * 2048;
+    grid_dep_wait();
+    int it = 0;
+    bool ok = true;
+    for (int id = first; id < total; id += step, ++it) {
+      const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+      const int b = it % C::NBUF;
+      ok = ok && mbar_wait_warp(acc_full + 8 * b, (it / C::NBUF) & 1, abort_flag, p.status, ST_ACCFULL);
+      if (!ok) {
+        if (!GROUPED && p.pieces > 1) { asm volatile("bar.sync 1, %0;" ::"n"(32 * C::EW) : "memory"); asm volatile("bar.sync 1, %0;" ::"n"(32 * C::EW) : "memory"); }
+        continue;
+      }
+      tc_fence_after();
+      const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + b * C::COLS;
+      const int c0 = t.n0 + (int)rank * (GATED ? 64 : 128) + quad * (GATED ? 16 : 32);      // this warp's first output column
+      const int cols = p.N - c0;
+      const int row = c0 + lane;
+      float bias = 0.f;
+      if (!GROUPED && p.bias && row < p.N) bias = half_f<BF16>(p.bias[row]);
+      auto free_acc = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(acc_empty + 8 * b, 0));
+          else mbar_arrive(acc_empty + 8 * b);
+        }
+        __syncwarp();
+      };
+      if (!GROUPED && p.pieces > 1) {
+        // partial sums [strip][piece][token][128 rows]; the last to deliver adds them up
+        float* mine = p.partials + ((int64_t)t.strip * p.pieces + t.piece) * NT * 128 + quad * 32 + lane;
+        if (threadIdx.x == 32 * C::FIRST_EPI) arrivals_open(p.arrivals + t.strip, p.tag, p.epoch);
+        for (int c = half * MINE; c < (half + 1) * MINE && c < t.rows; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(acc + c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c + i < t.rows) __stcg(mine + (int64_t)(c + i) * 128, __uint_as_float(r[i]));
+        }
+        free_acc();
+        __threadfence();
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * C::EW) : "memory");
+        if (threadIdx.x == 32 * C::FIRST_EPI) {
+          *last_flag = arrivals_last(p.arrivals + t.strip, p.pieces - 1);
+          __threadfence();
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * C::EW) : "memory");
+        if (*last_flag) {
+          const float* from = p.partials + (int64_t)t.strip * p.pieces * NT * 128 + quad * 32 + lane;
+          for (int c = half * MINE; c < (half + 1) * MINE && c < t.rows; c += 16) {
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              float v[2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                v[k] = bias;
+                if (c + i + k < t.rows)
+                  for (int q = 0; q < p.pieces; ++q) v[k] += __ldcg(from + ((int64_t)q * NT + c + i + k) * 128);
+              }
+              o[i / 2] = pack2<BF16>(v[0], v[1]);
+            }
+            if (cols > 0) store16(stg, o, p.out + (int64_t)(t.tok0 + c) * p.ldo + c0, p.ldo, t.rows - c, min(cols, 32), p.vec_out);
+          }
+        }
+        continue;
+      }
+      if constexpr (GATED) {
+        const bool upper = lane >= 16;
+        for (int c = half * MINE; c < (half + 1) * MINE && c < t.rows; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(acc + c, r);
+          tmem_ld_wait();
+          uint16_t h[16];                                  // of token 2 i (lower lanes) or 2 i + 1
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float a = __uint_as_float(r[2 * i]), d = __uint_as_float(r[2 * i + 1]);
+            const float got = __shfl_xor_sync(0xffffffffu, upper ? a : d, 16);
+            const float gate = upper ? got : a, up = upper ? d : got;
+            h[i] = (uint16_t)pack2<BF16>(gate / (1.f + expf(-gate)) * up, 0.f);
+          }
+          // through shared memory: [32 tokens][16 columns], the columns permuted in eights
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sts16(stg + (2 * i + upper) * 32 + g4_position(lane & 15) * 2, h[i]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int tk = i * 16 + (lane >> 1), cc = (lane & 1) * 8;
+            const uint4 v = lds128(stg + tk * 32 + cc * 2);
+            if (c + tk < t.rows && cc < cols) *reinterpret_cast<uint4*>(p.out + (int64_t)(t.tok0 + c + tk) * p.ldo + c0 + cc) = v;
+          }
+        }
+        free_acc();
+      } else {
+        // all of a warp's values first where the accumulator is the only one, so that the next tile can begin
+        constexpr int KEEP = C::NBUF == 1 ? MINE : CH;
+        for (int c1 = half * MINE; c1 < (half + 1) * MINE && c1 < t.rows; c1 += KEEP) {
+          uint32_t o[KEEP / 2];
+#pragma unroll
+          for (int c = 0; c < KEEP; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(acc + c1 + c, r);
+            float w = 1.f;
+            if (GROUPED) w = c1 + c + (lane & 15) < t.rows ? __ldcg(p.out_w + t.tok0 + c1 + c + (lane & 15)) : 0.f;
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float a = __uint_as_float(r[2 * i]) + bias, d = __uint_as_float(r[2 * i + 1]) + bias;
+              if (GROUPED) { a *= __shfl_sync(0xffffffffu, w, 2 * i); d *= __shfl_sync(0xffffffffu, w, 2 * i + 1); }
+              o[c / 2 + i] = pack2<BF16>(a, d);
+            }
+          }
+          if (C::NBUF == 1) free_acc();
+          if (cols > 0) {
+#pragma unroll
+            for (int c = 0; c < KEEP; c += 16) {
+              if (c1 + c < t.rows) {
+                uint32_t part[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) part[i] = o[c / 2 + i];
+                store16(stg, part, p.out + (int64_t)(t.tok0 + c1 + c) * p.ldo + c0, p.ldo, t.rows - c1 - c, min(cols, 32), p.vec_out);
+              }
+            }
+          }
+        }
+        if (C::NBUF > 1 || half * MINE >= t.rows) free_acc();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync_all();                  // nobody leaves while the partner may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, 512); else tmem_dealloc(tmem, 512);
+  }
+}
+
+// Rows of x to rows of aligned pitch: TMA wants rows that start on 16 bytes.
+__global__ void __launch_bounds__(256) g4_align_rows_kernel(const uint16_t* x, int64_t ldx, uint16_t* to, int K) {
+  grid_dep_release();
+  grid_dep_wait();
+  const uint16_t* from = x + blockIdx.x * ldx;
+  for (int k = threadIdx.x; k < K; k += 256) to[(int64_t)blockIdx.x * K + k] = __ldcg(from + k);
+}
+
+// ---- host ----
+namespace ug4 {
+template <bool BF16, int G, int NT, bool PAIR, bool GROUPED, bool GATED>
+static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const Params& p, int grid, cudaStream_t st) {
+  using C = Cfg<NT, PAIR>;
+  auto kern = umma_g4_kernel<BF16, G, NT, PAIR, GROUPED, GATED>;
+  static thread_local bool configured[16] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 16 || !configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return B2Q_ERR_CUDA;
+    if (dev < 16) configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid); cfg.blockDim = dim3(C::THREADS); cfg.dynamicSmemBytes = C::SMEM; cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (PAIR) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = 2; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (tls().overlap_mode > 0) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at; cfg.numAttrs = n;
+  cudaLaunchKernelEx(&cfg, kern, tx, tw, p);               // launch_status() reports
+  note_launch(PAIR ? "umma_g4_pair" : "umma_g4");
+  return launch_status();
+}
+template <int NT, bool PAIR, bool GROUPED, bool GATED>
+static int by_type(bool bf16, int G, const CUtensorMap& tx, const CUtensorMap& tw, const Params& p, int grid, cudaStream_t st) {
+  if (bf16) {
+    if (G == 128) return launch<true, 128, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
+    if (G == 64) return launch<true, 64, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
+    return launch<true, 32, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
+  }
+  if (G == 128) return launch<false, 128, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
+  if (G == 64) return launch<false, 64, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
+  return launch<false, 32, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
+}
+static size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+struct Plan { int nt, pieces, m_tiles, n_strips; bool pair; };
+static Plan plan(int M, int N, int K) {
+  Plan q{};
+  q.nt = M <= 32 ? 32 : (M <= 64 ? 64 : (M <= 128 ? 128 : 256));
+  q.pair = q.nt == 256;
+  q.m_tiles = (M + q.nt - 1) / q.nt;
+  q.n_strips = (N + (q.pair ? 255 : 127)) / (q.pair ? 256 : 128);
+  q.pieces = 1;
+  if (!q.pair) {
+    const int tiles = q.m_tiles * q.n_strips, nks = (K + 127) / 128;
+    q.pieces = sm_count() / tiles;
+    if (q.pieces > nks / 4) q.pieces = nks / 4;
+    if (q.pieces > 8) q.pieces = 8;
+    if (q.pieces < 1) q.pieces = 1;
+  }
+  return q;
+}
+static bool needs_copy(const void* x, int64_t ldx) { return !x || ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(2 * ldx)) & 15u); }
+}  // namespace ug4
+
+size_t umma_g4_bytes(const void* x, int64_t ldx, int M, int N, int K, int G) {
+  using namespace ug4;
+  const Plan q = plan(M, N, K);
+  size_t n = needs_copy(x, ldx) ? align_up((size_t)M * K * 2, 256) : 0;
+  if (q.pieces > 1) n += align_up((size_t)q.m_tiles * q.n_strips * q.pieces * q.nt * 128 * 4, 256) + align_up((size_t)q.m_tiles * q.n_strips * sizeof(Arrivals), 256);
+  return n;
+}
+
+int umma_g4_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st) {
+  using namespace ug4;
+  if (!tensor_map_encoder()) return B2Q_ERR_CUDA;
+  const Plan q = plan(a.M, a.N, a.K);
+  uint8_t* at = reinterpret_cast<uint8_t*>(scratch);
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x);
+  int64_t ldx = a.ldx;
+  if (needs_copy(a.x, a.ldx)) {
+    uint16_t* to = reinterpret_cast<uint16_t*>(at);
+    launch_overlapped(g4_align_rows_kernel, dim3(a.M), dim3(256), 0, st, tls().overlap_mode > 0, x, a.ldx, to, a.K);
+    note_launch("g4_align_rows");
+    at += align_up((size_t)a.M * a.K * 2, 256);
+    x = to;
+    ldx = a.K;
+  }
+  Params p{};
+  p.s = reinterpret_cast<const uint16_t*>(a.scale); p.z = a.zero; p.s_rows = a.N;
+  p.bias = reinterpret_cast<const uint16_t*>(a.bias); p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.ldo; p.vec_out = aligned16(a.out) && a.ldo % 8 == 0;
+  p.M = a.M; p.N = a.N; p.K = a.K; p.groups = a.K / a.G; p.nks = (a.K + 127) / 128;
+  p.n_strips = q.n_strips; p.m_tiles = q.m_tiles; p.m_group = q.m_tiles < 16 ? q.m_tiles : 16; p.pieces = q.pieces;
+  if ((int64_t)q.n_strips * q.m_tiles * q.pieces > INT32_MAX / 8) return B2Q_ERR_LIMIT;
+  p.total = q.n_strips * q.m_tiles * q.pieces;
+  if (q.pieces > 1) {
+    p.partials = reinterpret_cast<float*>(at);
+    p.arrivals = reinterpret_cast<Arrivals*>(at + align_up((size_t)q.m_tiles * q.n_strips * q.pieces * q.nt * 128 * 4, 256));
+    p.tag = arrivals_tag();
+    p.epoch = arrivals_epoch();
+    if (!p.epoch) return B2Q_ERR_CUDA;
+  }
+  p.early = tls().overlap_mode == 2;
+  p.status = umma_status_ptr();
+  if (!p.status) return B2Q_ERR_CUDA;
+  CUtensorMap tx, tw;
+  int rc = make_tmap_2d(&tx, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, a.M, a.K, (uint64_t)ldx * 2, q.pair ? q.nt / 2 : q.nt, 64,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.N, a.K / 2, (uint64_t)a.K / 2, 128, 64, CU_TENSOR_MAP_SWIZZLE_64B);
+  if (rc) return rc;
+  const int sms = sm_count();
+  if (q.pair) return by_type<256, true, false, false>(a.bf16, a.G, tx, tw, p, 2 * (p.total < sms / 2 ? p.total : sms / 2), st);
+  const int grid = p.total < sms ? p.total : sms;
+  if (q.nt == 32) return by_type<32, false, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  if (q.nt == 64) return by_type<64, false, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  return by_type<128, false, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
+}
+
+// Token height of the tiles, from the mean rows per expert.
+int g4_grouped_tile(int64_t rows, int E) {
+  const int64_t avg = (rows + E - 1) / E;
+  return avg <= 24 ? 32 : (avg <= 48 ? 64 : 128);
+}
+
+int umma_g4_grouped(const G4GroupedArgs& a, cudaStream_t st) {
+  using namespace ug4;
+  if (!tensor_map_encoder()) return B2Q_ERR_CUDA;
+  const bool pair = a.tile == 128;
+  Params p{};
+  p.s = reinterpret_cast<const uint16_t*>(a.scale); p.z = a.zero;
+  p.s_rows = a.gated ? 2 * a.N : a.N; p.groups = a.K / a.G; p.s_expert = (int64_t)p.groups * p.s_rows;
+  p.out_w = a.out_w; p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.N; p.vec_out = aligned16(a.out) && a.N % 8 == 0;
+  p.M = a.rows; p.N = a.N; p.K = a.K; p.nks = (a.K + 127) / 128; p.pieces = 1;
+  const int width = (pair ? 256 : 128) / (a.gated ? 2 : 1);
+  p.n_strips = (a.N + width - 1) / width;
+  p.tiles = a.tiles; p.offsets = a.offsets;
+  p.status = umma_status_ptr();
+  if (!p.status) return B2Q_ERR_CUDA;
+  const int64_t w_rows = (int64_t)a.E * p.s_rows;
+  if (w_rows > INT32_MAX || (int64_t)a.tile_cap * p.n_strips > INT32_MAX / 2) return B2Q_ERR_LIMIT;
+  CUtensorMap tx, tw;
+  int rc = make_tmap_2d(&tx, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.x, a.rows, a.K, (uint64_t)a.K * 2, pair ? a.tile / 2 : a.tile, 64,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, w_rows, a.K / 2, (uint64_t)a.K / 2, a.gated ? 64 : 128, 64, CU_TENSOR_MAP_SWIZZLE_64B);
+  if (rc) return rc;
+  const int sms = sm_count(), most = a.tile_cap * p.n_strips;
+  if (pair) {
+    const int grid = 2 * (most < sms / 2 ? most : sms / 2);
+    return a.gated ? by_type<128, true, true, true>(a.bf16, a.G, tx, tw, p, grid, st) : by_type<128, true, true, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  }
+  const int grid = most < sms ? most : sms;
+  if (a.tile == 32) return a.gated ? by_type<32, false, true, true>(a.bf16, a.G, tx, tw, p, grid, st) : by_type<32, false, true, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  return a.gated ? by_type<64, false, true, true>(a.bf16, a.G, tx, tw, p, grid, st) : by_type<64, false, true, false>(a.bf16, a.G, tx, tw, p, grid, st);
+}
+
+}  // namespace b2q
