@@ -57,14 +57,21 @@ struct Params {
   int* status;
 };
 
-struct Tile { int tok0, rows, n0, w0, ks0, ks1, piece, strip, e; };      // n0: first output column of the CTA or pair; w0: first weight row in memory (of an expert's gate half)
+// n0: first output column of the CTA or pair; w0: first weight row in memory (of an expert's gate half); k is walked from stage ks0 + turn on and round to it, since CTAs that all
+// begin at the same k ask the same L2 lines for the tokens at the same time.
+struct Tile {
+  int tok0, rows, n0, w0, ks0, n, turn, piece, strip, e;
+  __device__ __forceinline__ int stage(int j) const { const int i = j + turn; return ks0 + (i >= n ? i - n : i); }
+};
 
 template <int NT, bool PAIR, bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(const Params& p, int id) {
   constexpr int WIDTH = (PAIR ? 256 : 128) / (GATED ? 2 : 1);      // output columns of a strip
   Tile t;
-  t.piece = 0; t.ks0 = 0; t.ks1 = p.nks; t.e = 0;
+  t.piece = 0; t.ks0 = 0; t.n = p.nks; t.e = 0;
+  int st;
   if constexpr (GROUPED) {
-    const int ti = id / p.n_strips, st = id - ti * p.n_strips;
+    const int ti = id / p.n_strips;
+    st = id - ti * p.n_strips;
     const int e = __ldcg(p.tiles + 4 + 2 * ti), r0 = __ldcg(p.tiles + 4 + 2 * ti + 1);
     t.tok0 = __ldcg(p.offsets + e) + r0;
     t.rows = min(NT, __ldcg(p.offsets + e + 1) - t.tok0);
@@ -77,16 +84,19 @@ template <int NT, bool PAIR, bool GROUPED, bool GATED> __device__ __forceinline_
       t.strip = id / p.pieces;
       t.piece = id - t.strip * p.pieces;
       t.ks0 = (int)((int64_t)t.piece * p.nks / p.pieces);
-      t.ks1 = (int)((int64_t)(t.piece + 1) * p.nks / p.pieces);
+      t.n = (int)((int64_t)(t.piece + 1) * p.nks / p.pieces) - t.ks0;
       id = t.strip;
     }
     const int per = p.m_group * p.n_strips, gi = id / per, left = id - gi * per, m0 = gi * p.m_group;
-    const int gm = min(p.m_group, p.m_tiles - m0), st = left / gm, mt = m0 + left - st * gm;
+    const int gm = min(p.m_group, p.m_tiles - m0);
+    st = left / gm;
+    const int mt = m0 + left - st * gm;
     t.tok0 = mt * NT;
     t.rows = min(NT, p.M - t.tok0);
     t.n0 = st * WIDTH;
     t.w0 = t.n0;
   }
+  t.turn = (int)((int64_t)st * t.n / p.n_strips);
   return t;
 }
 
@@ -234,7 +244,8 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       for (int id = first; ok && id < total; id += step) {
         const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
         const int w = t.w0 + (int)rank * (GATED ? 64 : 128);
-        for (int ks = t.ks0; ks < t.ks1; ++ks) {
+        for (int j = 0; j < t.n; ++j) {
+          const int ks = t.stage(j);
           ok = mbar_wait(raw_empty + 8 * s, par, abort_flag, p.status, ST_RAWEMPTY);
           if (!ok) break;
           mbar_expect_tx(raw_full + 8 * s, C::RAW_BYTES);
@@ -257,7 +268,8 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       bool ok = true;
       for (int id = first; ok && id < total; id += step) {
         const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
-        for (int ks = t.ks0; ks < t.ks1; ++ks) {
+        for (int j = 0; j < t.n; ++j) {
+          const int ks = t.stage(j);
           ok = mbar_wait(x_empty + 8 * s, par, abort_flag, p.status, ST_XEMPTY);
           if (!ok) break;
           const uint32_t dst = base + s * C::X_BYTES;
@@ -286,7 +298,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + b * C::COLS;
-        for (int ks = t.ks0; ks < t.ks1; ++ks) {
+        for (int ks = 0; ks < t.n; ++ks) {
           ok = mbar_wait(x_full + 8 * xs, xpar, abort_flag, p.status, ST_XFULL) && mbar_wait(a_full + 8 * as, apar, abort_flag, p.status, ST_AFULL);
           if (!ok) break;
           tc_fence_after();
@@ -296,8 +308,8 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
             const uint64_t db = smem_desc_sw128(base + xs * C::X_BYTES + i * C::TOK * 128);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              if constexpr (PAIR) mma_f16_ts_pair(d, a + 32 * i + 8 * j, db + 2 * j, idesc, ks > t.ks0 || i > 0 || j > 0);
-              else mma_f16_ts(d, a + 32 * i + 8 * j, db + 2 * j, idesc, ks > t.ks0 || i > 0 || j > 0);
+              if constexpr (PAIR) mma_f16_ts_pair(d, a + 32 * i + 8 * j, db + 2 * j, idesc, ks > 0 || i > 0 || j > 0);
+              else mma_f16_ts(d, a + 32 * i + 8 * j, db + 2 * j, idesc, ks > 0 || i > 0 || j > 0);
             }
           }
           if constexpr (PAIR) { tc_commit_pair(x_empty + 8 * xs, 3); tc_commit_pair(a_empty + 8 * as, 3); }
@@ -326,11 +338,11 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       if constexpr (GATED) { const int h = min(t.n0 + (int)rank * 64 + 16 * quad + (lane & 15), p.N - 1); row = lane < 16 ? h : p.N + h; }
       else row = min(t.n0 + (int)rank * 128 + 32 * quad + lane, p.N - 1);
       const int64_t at0 = (int64_t)t.e * p.s_expert + row;
-      const int n = t.ks1 - t.ks0, mine0 = (grp - it % C::DG + C::DG) % C::DG;      // the tile's first stage that is this group's
+      const int n = t.n, mine0 = (grp - it % C::DG + C::DG) % C::DG;      // the tile's first stage that is this group's
       auto fetch = [&](int j) {
 #pragma unroll
         for (int i = 0; i < GS; ++i) {
-          const int64_t at = at0 + (int64_t)min((t.ks0 + j) * GS + i, p.groups - 1) * p.s_rows;
+          const int64_t at = at0 + (int64_t)min(t.stage(j) * GS + i, p.groups - 1) * p.s_rows;
           sc[i] = ld_u16(p.s + at);
           zc[i] = p.z ? ld_u8(p.z + at) : 8u;
         }
@@ -388,7 +400,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(a_full + 8 * as, 0));
+          if constexpr (PAIR) mbar_arrive_cluster_relaxed(map_to_cta(a_full + 8 * as, 0));
           else mbar_arrive(a_full + 8 * as);
         }
         __syncwarp();
@@ -423,7 +435,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(acc_empty + 8 * b, 0));
+          if constexpr (PAIR) mbar_arrive_cluster_relaxed(map_to_cta(acc_empty + 8 * b, 0));
           else mbar_arrive(acc_empty + 8 * b);
         }
         __syncwarp();
