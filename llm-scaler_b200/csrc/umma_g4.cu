@@ -5,16 +5,18 @@
 // them straight into tensor memory as the MMA's A operand; tokens come by TMA.  q - z is exact (the code is put below a power of two and that power plus z
 // subtracted), times s is the one rounding; it is of the size of the output's own.
 //
-// A persistent CTA has separate warps for the weights' copies, the tokens' copies, the MMA, the epilogue and the transform, so that nothing of one tile stops the stream
-// of the next.  An operand stage is 128 k; each ring stage stays with one group of four transform warps, since a parity wait cannot tell a phase from the one
-// before the last.
+// Two CTAs share a tile of 256 rows (cta_group::2), each with its own 128 rows in tensor memory and half of the tokens in shared memory: a CTA alone would pull twice the
+// tokens through L2, which at 9 TB/s is what bounds narrow tiles too (64 x 17408 x 5120: 97 MB of tokens beside 46 of weights).
 //
-//  * PAIR: two CTAs share a tile of 256 rows (cta_group::2), each with its own 128 rows in tensor memory and half of the tokens in shared memory.  A CTA alone would pull
-//    64 bytes of tokens per cycle of MMA through L2, a pair's 32.
-//  * Where strips of 128 rows are fewer than SMs, k is cut into pieces; whoever delivers the last of a strip's partial sums adds them up in order (arrivals.cuh).
+// A persistent CTA has separate warps for the weights' copies, the tokens' copies, the MMA, the epilogue and the transform, so that nothing of one tile stops the stream of the
+// next.  An operand stage is 128 k; each ring stage stays with one group of four transform warps, since a parity wait cannot tell a phase from the one before the
+// last.
+//
+//  * Where strips of 256 rows are fewer than pairs of SMs, k is cut into pieces; whoever delivers the last of a strip's partial sums adds them up in order (arrivals.cuh).
 //  * GATED (expert up projection): a warp's 32 rows are 16 gate and 16 up rows of the same outputs, and the epilogue stores silu(gate) * up.
 //
 // No multicast load; every mbarrier wait is bounded, as in the other tcgen05 kernels.
+#include <type_traits>
 #include "umma_gemm.cuh"
 #include "sm100.cuh"
 #include "arrivals.cuh"
@@ -25,22 +27,22 @@ namespace b2q {
 using namespace sm100;
 
 namespace ug4 {
-enum { ST_RAWEMPTY = 951, ST_RAWFULL = 952, ST_AEMPTY = 953, ST_AFULL = 954, ST_XEMPTY = 955, ST_XFULL = 956, ST_ACCEMPTY = 957, ST_ACCFULL = 958 };
+enum { ST_RAWEMPTY = 951, ST_RAWFULL = 952, ST_AEMPTY = 953, ST_FULL = 954, ST_XEMPTY = 955, ST_ACCEMPTY = 957, ST_ACCFULL = 958 };
 
-template <int NT, bool PAIR> struct Cfg {
-  static constexpr int DG = NT <= 64 ? 4 : 2;                // transform groups
+template <int NT> struct Cfg {
+  static constexpr int NBUF = NT <= 128 ? 2 : 1;             // accumulators
+  static constexpr int COLS = NT, A_COL0 = NBUF * COLS;
+  static constexpr int S = (512 - A_COL0) / 64 > 6 ? 6 : (512 - A_COL0) / 64;      // stages of 128 k: operand columns and tokens
+  // Transform groups.  Two slots a group hide its waits where tensor memory has room for them; the accumulators of 128 tokens leave four slots, and four groups with one each
+  // do better than two with two.
+  static constexpr int DG = NT == 256 ? 2 : (NT == 128 ? 4 : 3);
   static constexpr int EW = NT <= 64 ? 4 : 8;                // epilogue warps
   static constexpr int FIRST_EPI = 4, FIRST_DEQ = FIRST_EPI + EW, THREADS = 32 * (FIRST_DEQ + 4 * DG);
-  static constexpr int COLS = NT < 32 ? 32 : NT;             // of an accumulator
-  static constexpr int NBUF = NT <= 128 ? 2 : 1;
-  static constexpr int A_COL0 = NBUF * COLS;
-  static constexpr int S = (512 - A_COL0) / 64 / DG * DG;    // operand stages of 128 k
-  static constexpr int TOK = PAIR ? NT / 2 : NT;             // tokens that a CTA loads
+  static constexpr int TOK = NT / 2;                         // tokens that a CTA loads
   static constexpr int X_BYTES = TOK * 256, RAW_BYTES = 8192;
-  static constexpr int XS = NT == 256 ? (PAIR ? 4 : 2) : (NT == 128 ? 4 : 6);
-  static constexpr int RS = NT <= 64 ? 8 : 6;                // raw stages, a multiple of DG
+  static constexpr int RS = NT == 256 ? 6 : (NT == 128 ? 8 : 9);      // raw stages, a multiple of DG
   static constexpr int STG = EW * 2048;                      // 32 tokens x 32 columns for every epilogue warp
-  static constexpr int USED = XS * X_BYTES + RS * RAW_BYTES + STG + 1024;
+  static constexpr int USED = S * X_BYTES + RS * RAW_BYTES + STG + 1024;
   static constexpr int SMEM = 1024 + (USED < 170 * 1024 ? 170 * 1024 : USED);      // one CTA with tensor memory on an SM: see umma_i8.cu
   static_assert(RS % DG == 0 && S % DG == 0 && S > 0 && SMEM <= 232448, "rings");
 };
@@ -64,8 +66,8 @@ struct Tile {
   __device__ __forceinline__ int stage(int j) const { const int i = j + turn; return ks0 + (i >= n ? i - n : i); }
 };
 
-template <int NT, bool PAIR, bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(const Params& p, int id) {
-  constexpr int WIDTH = (PAIR ? 256 : 128) / (GATED ? 2 : 1);      // output columns of a strip
+template <int NT, bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(const Params& p, int id) {
+  constexpr int WIDTH = GATED ? 128 : 256;                 // output columns of a strip
   Tile t;
   t.piece = 0; t.ks0 = 0; t.n = p.nks; t.e = 0;
   int st;
@@ -129,8 +131,8 @@ __device__ __forceinline__ uint32_t fma2_f16(uint32_t a, uint32_t b, uint32_t c)
 }
 
 // Eight codes of a word -> four registers of two values (q - z) s.  PERM: in the order 0, 4, 1, 5, 2, 6, 3, 7, else as they come.  zc: the power of two plus z, twice (fp16 and
-// PERM: and -(64 + z) in zh); more: bf16, what z has beyond 127, for 128 + z has to fit eight bits.
-template <bool BF16, bool PERM> __device__ __forceinline__ void decode(uint32_t w, uint32_t s2, uint32_t zc, uint32_t zh, uint32_t more, bool has_more, uint32_t* o) {
+// PERM: and -(64 + z) in zh); MORE: bf16, with what z has beyond 127 in more, for 128 + z has to fit eight bits.
+template <bool BF16, bool PERM, bool MORE> __device__ __forceinline__ void decode(uint32_t w, uint32_t s2, uint32_t zc, uint32_t zh, uint32_t more, uint32_t* o) {
   constexpr uint32_t MASK = 0x000F000Fu, MAGIC = BF16 ? 0x43004300u : 0x64006400u;
   if constexpr (PERM && !BF16) {
     const uint32_t w8 = w >> 8;
@@ -148,7 +150,7 @@ template <bool BF16, bool PERM> __device__ __forceinline__ void decode(uint32_t 
     o[2] = sub2<BF16>((__byte_perm(w, w4, 0x6622) & MASK) | MAGIC, zc);
     o[3] = sub2<BF16>((__byte_perm(w, w4, 0x7733) & MASK) | MAGIC, zc);
   }
-  if (BF16 && has_more) {
+  if constexpr (MORE) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = sub2<true>(o[i], more);
   }
@@ -191,43 +193,44 @@ __device__ __forceinline__ void store16(uint32_t stg, const uint32_t (&o)[8], ui
 }
 }  // namespace ug4
 
-template <bool BF16, int G, int NT, bool PAIR, bool GROUPED, bool GATED>
-__global__ void __launch_bounds__(ug4::Cfg<NT, PAIR>::THREADS, 1)
+template <bool BF16, int G, int NT, bool GROUPED, bool GATED>
+__global__ void __launch_bounds__(ug4::Cfg<NT>::THREADS, 1)
 umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, const ug4::Params p) {
   using namespace ug4;
-  using C = Cfg<NT, PAIR>;
+  using C = Cfg<NT>;
   constexpr bool PERM = GROUPED;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   // [token stages] [raw stages] [staging] [barriers]
-  const uint32_t raw0 = base + C::XS * C::X_BYTES, stg0 = raw0 + C::RS * C::RAW_BYTES, bar = stg0 + C::STG;
-  const uint32_t x_full = bar, x_empty = x_full + 8 * C::XS, raw_full = x_empty + 8 * C::XS, raw_empty = raw_full + 8 * C::RS, a_full = raw_empty + 8 * C::RS, a_empty = a_full + 8 * C::S,
-                 acc_full = a_empty + 8 * C::S, acc_empty = acc_full + 16, tail = acc_empty + 16;
+  const uint32_t raw0 = base + C::S * C::X_BYTES, stg0 = raw0 + C::RS * C::RAW_BYTES, bar = stg0 + C::STG;
+  // A stage is full when its tokens have landed and both CTAs' operands are written; one barrier for both, since a wait costs the issuing thread some 125 cycles even when it is
+  // over, and a commit 90.
+  const uint32_t full = bar, empty = full + 8 * C::S, raw_full = empty + 8 * C::S, raw_empty = raw_full + 8 * C::RS, acc_full = raw_empty + 8 * C::RS, acc_empty = acc_full + 16,
+                 tail = acc_empty + 16;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen + (tail - base));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + (tail + 4 - base));
   volatile int* last_flag = reinterpret_cast<volatile int*>(gen + (tail + 8 - base));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
-  const int first = (int)blockIdx.x / (PAIR ? 2 : 1), step = (int)gridDim.x / (PAIR ? 2 : 1);
+  const uint32_t rank = cluster_ctarank();
+  const int first = (int)blockIdx.x / 2, step = (int)gridDim.x / 2;
 
   grid_dep_release();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::XS; ++i) { mbar_init(x_full + 8 * i, 1); mbar_init(x_empty + 8 * i, 1); }
+    for (int i = 0; i < C::S; ++i) { mbar_init(full + 8 * i, 9); mbar_init(empty + 8 * i, 1); }
     for (int i = 0; i < C::RS; ++i) { mbar_init(raw_full + 8 * i, 1); mbar_init(raw_empty + 8 * i, 4); }
-    for (int i = 0; i < C::S; ++i) { mbar_init(a_full + 8 * i, PAIR ? 8 : 4); mbar_init(a_empty + 8 * i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, PAIR ? 2 * C::EW : C::EW); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, 2 * C::EW); }
     *abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
-    if constexpr (PAIR) { tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512); tmem_relinquish_pair(); }
-    else { tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512); tmem_relinquish(); }
+    tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync_all();
+  cluster_sync_all();                                      // both CTAs' barriers exist before anything is signalled across
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (GROUPED) grid_dep_wait();                            // the tile list is made by the kernels in front
@@ -242,7 +245,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       uint32_t par = 1u;
       bool ok = true;
       for (int id = first; ok && id < total; id += step) {
-        const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+        const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
         const int w = t.w0 + (int)rank * (GATED ? 64 : 128);
         for (int j = 0; j < t.n; ++j) {
           const int ks = t.stage(j);
@@ -267,58 +270,54 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       uint32_t par = 1u;
       bool ok = true;
       for (int id = first; ok && id < total; id += step) {
-        const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+        const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
         for (int j = 0; j < t.n; ++j) {
           const int ks = t.stage(j);
-          ok = mbar_wait(x_empty + 8 * s, par, abort_flag, p.status, ST_XEMPTY);
+          ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_XEMPTY);
           if (!ok) break;
           const uint32_t dst = base + s * C::X_BYTES;
-          if (rank == 0) mbar_expect_tx(x_full + 8 * s, C::X_BYTES * (PAIR ? 2 : 1));
+          if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * C::X_BYTES);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            if constexpr (PAIR) tma_load_2d_pair(dst + i * C::TOK * 128, &tm_x, ks * 128 + i * 64, t.tok0 + (int)rank * C::TOK, map_to_cta(x_full + 8 * s, 0));
-            else tma_load_2d(dst + i * C::TOK * 128, &tm_x, ks * 128 + i * 64, t.tok0, x_full + 8 * s);
+            tma_load_2d_pair(dst + i * C::TOK * 128, &tm_x, ks * 128 + i * 64, t.tok0 + (int)rank * C::TOK, map_to_cta(full + 8 * s, 0));
           }
           ++issued;
-          if (++s == C::XS) { s = 0; par ^= 1u; }
+          if (++s == C::S) { s = 0; par ^= 1u; }
         }
       }
-      if (!ok && rank == 0) drain_issued(x_full, C::XS, issued);
+      if (!ok && rank == 0) drain_issued(full, C::S, issued);
     }
   } else if (warp == 1) {
-    if ((!PAIR || rank == 0) && elect_one()) {
-      const uint32_t idesc = instr_desc(BF16 ? 1u : 0u, BF16 ? 1u : 0u, PAIR ? 256u : 128u, (uint32_t)NT);
-      int xs = 0, as = 0, it = 0;
-      uint32_t xpar = 0u, apar = 0u;
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = instr_desc(BF16 ? 1u : 0u, BF16 ? 1u : 0u, 256u, (uint32_t)NT);
+      int s = 0, it = 0;
+      uint32_t par = 0u;
       bool ok = true;
       for (int id = first; ok && id < total; id += step, ++it) {
-        const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+        const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
         const int b = it % C::NBUF;
         if (it >= C::NBUF) ok = mbar_wait(acc_empty + 8 * b, (it / C::NBUF - 1) & 1, abort_flag, p.status, ST_ACCEMPTY);
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + b * C::COLS;
         for (int ks = 0; ks < t.n; ++ks) {
-          ok = mbar_wait(x_full + 8 * xs, xpar, abort_flag, p.status, ST_XFULL) && mbar_wait(a_full + 8 * as, apar, abort_flag, p.status, ST_AFULL);
+          ok = mbar_wait(full + 8 * s, par, abort_flag, p.status, ST_FULL);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t a = tmem + C::A_COL0 + as * 64;
+          const uint32_t a = tmem + C::A_COL0 + s * 64;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint64_t db = smem_desc_sw128(base + xs * C::X_BYTES + i * C::TOK * 128);
+            const uint64_t db = smem_desc_sw128(base + s * C::X_BYTES + i * C::TOK * 128);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              if constexpr (PAIR) mma_f16_ts_pair(d, a + 32 * i + 8 * j, db + 2 * j, idesc, ks > 0 || i > 0 || j > 0);
-              else mma_f16_ts(d, a + 32 * i + 8 * j, db + 2 * j, idesc, ks > 0 || i > 0 || j > 0);
+              mma_f16_ts_pair(d, a + 32 * i + 8 * j, db + 2 * j, idesc, ks > 0 || i > 0 || j > 0);
             }
           }
-          if constexpr (PAIR) { tc_commit_pair(x_empty + 8 * xs, 3); tc_commit_pair(a_empty + 8 * as, 3); }
-          else { tc_commit(x_empty + 8 * xs); tc_commit(a_empty + 8 * as); }
-          if (++xs == C::XS) { xs = 0; xpar ^= 1u; }
-          if (++as == C::S) { as = 0; apar ^= 1u; }
+          tc_commit_pair(empty + 8 * s, 3);
+          if (++s == C::S) { s = 0; par ^= 1u; }
         }
         if (!ok) break;
-        if constexpr (PAIR) tc_commit_pair(acc_full + 8 * b, 3); else tc_commit(acc_full + 8 * b);
+        tc_commit_pair(acc_full + 8 * b, 3);
       }
     }
   } else if (warp >= C::FIRST_DEQ) {
@@ -330,32 +329,36 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
     if (!GROUPED && !p.early) grid_dep_wait();
     int it = 0;                                            // stages so far
     bool ok = true;
-    uint32_t sc[GS], zc[GS];
+    uint32_t sc[2][GS], zc[2][GS];                         // of this group's next two stages
     for (int id = first; ok && id < total; id += step) {
-      const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+      const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
       // this thread's row among the scales' rows; beyond the last it repeats it, and nobody looks at the sums
       int row;
       if constexpr (GATED) { const int h = min(t.n0 + (int)rank * 64 + 16 * quad + (lane & 15), p.N - 1); row = lane < 16 ? h : p.N + h; }
       else row = min(t.n0 + (int)rank * 128 + 32 * quad + lane, p.N - 1);
       const int64_t at0 = (int64_t)t.e * p.s_expert + row;
       const int n = t.n, mine0 = (grp - it % C::DG + C::DG) % C::DG;      // the tile's first stage that is this group's
-      auto fetch = [&](int j) {
+      auto fetch = [&](int j, uint32_t (&s)[GS], uint32_t (&z)[GS]) {
+        if (j >= n) return;
 #pragma unroll
         for (int i = 0; i < GS; ++i) {
           const int64_t at = at0 + (int64_t)min(t.stage(j) * GS + i, p.groups - 1) * p.s_rows;
-          sc[i] = ld_u16(p.s + at);
-          zc[i] = p.z ? ld_u8(p.z + at) : 8u;
+          s[i] = ld_u16(p.s + at);
+          z[i] = p.z ? ld_u8(p.z + at) : 8u;
         }
       };
-      if (mine0 < n) fetch(mine0);
+      fetch(mine0, sc[0], zc[0]);
+      fetch(mine0 + C::DG, sc[1], zc[1]);
       for (int j = mine0; j < n; j += C::DG) {
         const int now = it + j, rs = now % C::RS, as = now % C::S;
         uint32_t s2[GS], z2[GS], zh[GS], more[GS];
         bool has_more = false;
 #pragma unroll
         for (int i = 0; i < GS; ++i) {
-          s2[i] = sc[i] * 0x00010001u;
-          const uint32_t z = zc[i];
+          s2[i] = sc[0][i] * 0x00010001u;
+          const uint32_t z = zc[0][i];
+          sc[0][i] = sc[1][i];
+          zc[0][i] = zc[1][i];
           if (BF16) {
             const uint32_t low = min(z, 127u);
             z2[i] = 0x43004300u | low * 0x00010001u;
@@ -370,39 +373,40 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
           }
         }
         has_more = BF16 && __any_sync(0xffffffffu, has_more);
-        if (j + C::DG < n) fetch(j + C::DG);
+        fetch(j + 2 * C::DG, sc[1], zc[1]);
         ok = mbar_wait_warp(raw_full + 8 * rs, (now / C::RS) & 1, abort_flag, p.status, ST_RAWFULL);
         if (!ok) break;
         uint4 raw[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) raw[i] = lds128(raw0 + rs * C::RAW_BYTES + row_at + ((i ^ f) << 4));
-        if (now >= C::S) ok = mbar_wait_warp(a_empty + 8 * as, (now / C::S - 1) & 1, abort_flag, p.status, ST_AEMPTY);
+        if (now >= C::S) ok = mbar_wait_warp(empty + 8 * as, (now / C::S - 1) & 1, abort_flag, p.status, ST_AEMPTY);
         if (!ok) break;
         tc_fence_after();
         const uint32_t a = tmem + C::A_COL0 + as * 64 + ((uint32_t)(quad * 32) << 16);
+        auto convert = [&](auto with_more) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t o[32];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t o[32];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint4 r = raw[2 * h + i];
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+            for (int i = 0; i < 2; ++i) {
+              const uint4 r = raw[2 * h + i];
+              const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const int grp_of = (h * 64 + i * 32 + v * 8) / G;
-              decode<BF16, PERM>(w[v], s2[grp_of], z2[grp_of], zh[grp_of], more[grp_of], has_more, o + 16 * i + 4 * v);
+              for (int v = 0; v < 4; ++v) {
+                const int of = (h * 64 + i * 32 + v * 8) / G;
+                decode<BF16, PERM, decltype(with_more)::value>(w[v], s2[of], z2[of], zh[of], more[of], o + 16 * i + 4 * v);
+              }
             }
+            tmem_st32(a + 32 * h, o);
           }
-          tmem_st32(a + 32 * h, o);
-        }
+        };
+        if (has_more) convert(std::true_type{});
+        else convert(std::false_type{});
         mbar_arrive_read(raw_empty + 8 * rs);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_cluster_relaxed(map_to_cta(a_full + 8 * as, 0));
-          else mbar_arrive(a_full + 8 * as);
-        }
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(full + 8 * as, 0));
         __syncwarp();
       }
       it += n;
@@ -417,7 +421,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
     int it = 0;
     bool ok = true;
     for (int id = first; id < total; id += step, ++it) {
-      const Tile t = tile_at<NT, PAIR, GROUPED, GATED>(p, id);
+      const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
       const int b = it % C::NBUF;
       ok = ok && mbar_wait_warp(acc_full + 8 * b, (it / C::NBUF) & 1, abort_flag, p.status, ST_ACCFULL);
       if (!ok) {
@@ -434,16 +438,14 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       auto free_acc = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_cluster_relaxed(map_to_cta(acc_empty + 8 * b, 0));
-          else mbar_arrive(acc_empty + 8 * b);
-        }
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(acc_empty + 8 * b, 0));
         __syncwarp();
       };
       if (!GROUPED && p.pieces > 1) {
-        // partial sums [strip][piece][token][128 rows]; the last to deliver adds them up
-        float* mine = p.partials + ((int64_t)t.strip * p.pieces + t.piece) * NT * 128 + quad * 32 + lane;
-        if (threadIdx.x == 32 * C::FIRST_EPI) arrivals_open(p.arrivals + t.strip, p.tag, p.epoch);
+        // partial sums [strip][rank][piece][token][128 rows]; the last to deliver adds them up
+        const int64_t at = 2 * t.strip + (int)rank;
+        float* mine = p.partials + (at * p.pieces + t.piece) * NT * 128 + quad * 32 + lane;
+        if (threadIdx.x == 32 * C::FIRST_EPI) arrivals_open(p.arrivals + at, p.tag, p.epoch);
         for (int c = half * MINE; c < (half + 1) * MINE && c < t.rows; c += 16) {
           uint32_t r[16];
           tmem_ld16(acc + c, r);
@@ -456,25 +458,27 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         __threadfence();
         asm volatile("bar.sync 1, %0;" ::"n"(32 * C::EW) : "memory");
         if (threadIdx.x == 32 * C::FIRST_EPI) {
-          *last_flag = arrivals_last(p.arrivals + t.strip, p.pieces - 1);
+          *last_flag = arrivals_last(p.arrivals + at, p.pieces - 1);
           __threadfence();
         }
         asm volatile("bar.sync 1, %0;" ::"n"(32 * C::EW) : "memory");
         if (*last_flag) {
-          const float* from = p.partials + (int64_t)t.strip * p.pieces * NT * 128 + quad * 32 + lane;
+          const float* from = p.partials + at * p.pieces * NT * 128 + quad * 32 + lane;
           for (int c = half * MINE; c < (half + 1) * MINE && c < t.rows; c += 16) {
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = bias;
+#pragma unroll 2
+            for (int q = 0; q < p.pieces; ++q) {           // tokens beyond the last are read and not looked at
+              float w[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = __ldcg(from + ((int64_t)q * NT + c + i) * 128);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] += w[i];
+            }
             uint32_t o[8];
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float v[2];
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                v[k] = bias;
-                if (c + i + k < t.rows)
-                  for (int q = 0; q < p.pieces; ++q) v[k] += __ldcg(from + ((int64_t)q * NT + c + i + k) * 128);
-              }
-              o[i / 2] = pack2<BF16>(v[0], v[1]);
-            }
+            for (int i = 0; i < 8; ++i) o[i] = pack2<BF16>(v[2 * i], v[2 * i + 1]);
             if (cols > 0) store16(stg, o, p.out + (int64_t)(t.tok0 + c) * p.ldo + c0, p.ldo, t.rows - c, min(cols, 32), p.vec_out);
           }
         }
@@ -545,10 +549,10 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync_all();                  // nobody leaves while the partner may still signal it
+  cluster_sync_all();                                      // nobody leaves while the partner may still signal it
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (PAIR) tmem_dealloc_pair(tmem, 512); else tmem_dealloc(tmem, 512);
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -562,10 +566,10 @@ __global__ void __launch_bounds__(256) g4_align_rows_kernel(const uint16_t* x, i
 
 // ---- host ----
 namespace ug4 {
-template <bool BF16, int G, int NT, bool PAIR, bool GROUPED, bool GATED>
+template <bool BF16, int G, int NT, bool GROUPED, bool GATED>
 static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const Params& p, int grid, cudaStream_t st) {
-  using C = Cfg<NT, PAIR>;
-  auto kern = umma_g4_kernel<BF16, G, NT, PAIR, GROUPED, GATED>;
+  using C = Cfg<NT>;
+  auto kern = umma_g4_kernel<BF16, G, NT, GROUPED, GATED>;
   static thread_local bool configured[16] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -577,11 +581,9 @@ static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const Params& p,
   cfg.gridDim = dim3(grid); cfg.blockDim = dim3(C::THREADS); cfg.dynamicSmemBytes = C::SMEM; cfg.stream = st;
   cudaLaunchAttribute at[2];
   int n = 0;
-  if (PAIR) {
-    at[n].id = cudaLaunchAttributeClusterDimension;
-    at[n].val.clusterDim.x = 2; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
-    ++n;
-  }
+  at[n].id = cudaLaunchAttributeClusterDimension;
+  at[n].val.clusterDim.x = 2; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
+  ++n;
   if (tls().overlap_mode > 0) {
     at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[n].val.programmaticStreamSerializationAllowed = 1;
@@ -589,39 +591,37 @@ static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const Params& p,
   }
   cfg.attrs = at; cfg.numAttrs = n;
   cudaLaunchKernelEx(&cfg, kern, tx, tw, p);               // launch_status() reports
-  note_launch(PAIR ? "umma_g4_pair" : "umma_g4");
+  note_launch("umma_g4");
   return launch_status();
 }
-template <int NT, bool PAIR, bool GROUPED, bool GATED>
+template <int NT, bool GROUPED, bool GATED>
 static int by_type(bool bf16, int G, const CUtensorMap& tx, const CUtensorMap& tw, const Params& p, int grid, cudaStream_t st) {
   if (bf16) {
-    if (G == 128) return launch<true, 128, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
-    if (G == 64) return launch<true, 64, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
-    return launch<true, 32, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
+    if (G == 128) return launch<true, 128, NT, GROUPED, GATED>(tx, tw, p, grid, st);
+    if (G == 64) return launch<true, 64, NT, GROUPED, GATED>(tx, tw, p, grid, st);
+    return launch<true, 32, NT, GROUPED, GATED>(tx, tw, p, grid, st);
   }
-  if (G == 128) return launch<false, 128, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
-  if (G == 64) return launch<false, 64, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
-  return launch<false, 32, NT, PAIR, GROUPED, GATED>(tx, tw, p, grid, st);
+  if (G == 128) return launch<false, 128, NT, GROUPED, GATED>(tx, tw, p, grid, st);
+  if (G == 64) return launch<false, 64, NT, GROUPED, GATED>(tx, tw, p, grid, st);
+  return launch<false, 32, NT, GROUPED, GATED>(tx, tw, p, grid, st);
 }
 static size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
-struct Plan { int nt, pieces, m_tiles, n_strips; bool pair; };
+struct Plan { int nt, pieces, m_tiles, n_strips; };
 static Plan plan(int M, int N, int K) {
   Plan q{};
   q.nt = M <= 32 ? 32 : (M <= 64 ? 64 : (M <= 128 ? 128 : 256));
-  q.pair = q.nt == 256;
   q.m_tiles = (M + q.nt - 1) / q.nt;
-  q.n_strips = (N + (q.pair ? 255 : 127)) / (q.pair ? 256 : 128);
-  q.pieces = 1;
-  if (!q.pair) {
-    const int tiles = q.m_tiles * q.n_strips, nks = (K + 127) / 128;
-    q.pieces = sm_count() / tiles;
-    if (q.pieces > nks / 4) q.pieces = nks / 4;
-    if (q.pieces > 8) q.pieces = 8;
-    if (q.pieces < 1) q.pieces = 1;
-  }
+  q.n_strips = (N + 255) / 256;
+  const int64_t tiles = (int64_t)q.m_tiles * q.n_strips, pairs = sm_count() / 2;
+  const int nks = (K + 127) / 128;
+  q.pieces = tiles >= pairs ? 1 : (int)(pairs / tiles);
+  if (q.pieces > nks / 4) q.pieces = nks / 4;
+  if (q.pieces > 8) q.pieces = 8;
+  if (q.pieces < 1) q.pieces = 1;
   return q;
 }
+static size_t partial_bytes(const Plan& q) { return align_up((size_t)q.m_tiles * q.n_strips * 2 * q.pieces * q.nt * 128 * 4, 256); }
 static bool needs_copy(const void* x, int64_t ldx) { return !x || ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(2 * ldx)) & 15u); }
 }  // namespace ug4
 
@@ -629,7 +629,7 @@ size_t umma_g4_bytes(const void* x, int64_t ldx, int M, int N, int K, int G) {
   using namespace ug4;
   const Plan q = plan(M, N, K);
   size_t n = needs_copy(x, ldx) ? align_up((size_t)M * K * 2, 256) : 0;
-  if (q.pieces > 1) n += align_up((size_t)q.m_tiles * q.n_strips * q.pieces * q.nt * 128 * 4, 256) + align_up((size_t)q.m_tiles * q.n_strips * sizeof(Arrivals), 256);
+  if (q.pieces > 1) n += partial_bytes(q) + align_up((size_t)q.m_tiles * q.n_strips * 2 * sizeof(Arrivals), 256);
   return n;
 }
 
@@ -657,7 +657,7 @@ int umma_g4_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st) {
   p.total = q.n_strips * q.m_tiles * q.pieces;
   if (q.pieces > 1) {
     p.partials = reinterpret_cast<float*>(at);
-    p.arrivals = reinterpret_cast<Arrivals*>(at + align_up((size_t)q.m_tiles * q.n_strips * q.pieces * q.nt * 128 * 4, 256));
+    p.arrivals = reinterpret_cast<Arrivals*>(at + partial_bytes(q));
     p.tag = arrivals_tag();
     p.epoch = arrivals_epoch();
     if (!p.epoch) return B2Q_ERR_CUDA;
@@ -666,16 +666,15 @@ int umma_g4_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st) {
   p.status = umma_status_ptr();
   if (!p.status) return B2Q_ERR_CUDA;
   CUtensorMap tx, tw;
-  int rc = make_tmap_2d(&tx, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, a.M, a.K, (uint64_t)ldx * 2, q.pair ? q.nt / 2 : q.nt, 64,
+  int rc = make_tmap_2d(&tx, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, a.M, a.K, (uint64_t)ldx * 2, q.nt / 2, 64,
                         CU_TENSOR_MAP_SWIZZLE_128B);
   if (!rc) rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.N, a.K / 2, (uint64_t)a.K / 2, 128, 64, CU_TENSOR_MAP_SWIZZLE_64B);
   if (rc) return rc;
-  const int sms = sm_count();
-  if (q.pair) return by_type<256, true, false, false>(a.bf16, a.G, tx, tw, p, 2 * (p.total < sms / 2 ? p.total : sms / 2), st);
-  const int grid = p.total < sms ? p.total : sms;
-  if (q.nt == 32) return by_type<32, false, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
-  if (q.nt == 64) return by_type<64, false, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
-  return by_type<128, false, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  const int pairs = sm_count() / 2, grid = 2 * (p.total < pairs ? p.total : pairs);
+  if (q.nt == 32) return by_type<32, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  if (q.nt == 64) return by_type<64, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  if (q.nt == 128) return by_type<128, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  return by_type<256, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
 }
 
 // Token height of the tiles, from the mean rows per expert.
@@ -687,13 +686,12 @@ int g4_grouped_tile(int64_t rows, int E) {
 int umma_g4_grouped(const G4GroupedArgs& a, cudaStream_t st) {
   using namespace ug4;
   if (!tensor_map_encoder()) return B2Q_ERR_CUDA;
-  const bool pair = a.tile == 128;
   Params p{};
   p.s = reinterpret_cast<const uint16_t*>(a.scale); p.z = a.zero;
   p.s_rows = a.gated ? 2 * a.N : a.N; p.groups = a.K / a.G; p.s_expert = (int64_t)p.groups * p.s_rows;
   p.out_w = a.out_w; p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.N; p.vec_out = aligned16(a.out) && a.N % 8 == 0;
   p.M = a.rows; p.N = a.N; p.K = a.K; p.nks = (a.K + 127) / 128; p.pieces = 1;
-  const int width = (pair ? 256 : 128) / (a.gated ? 2 : 1);
+  const int width = a.gated ? 128 : 256;
   p.n_strips = (a.N + width - 1) / width;
   p.tiles = a.tiles; p.offsets = a.offsets;
   p.status = umma_status_ptr();
@@ -701,18 +699,14 @@ int umma_g4_grouped(const G4GroupedArgs& a, cudaStream_t st) {
   const int64_t w_rows = (int64_t)a.E * p.s_rows;
   if (w_rows > INT32_MAX || (int64_t)a.tile_cap * p.n_strips > INT32_MAX / 2) return B2Q_ERR_LIMIT;
   CUtensorMap tx, tw;
-  int rc = make_tmap_2d(&tx, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.x, a.rows, a.K, (uint64_t)a.K * 2, pair ? a.tile / 2 : a.tile, 64,
+  int rc = make_tmap_2d(&tx, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.x, a.rows, a.K, (uint64_t)a.K * 2, a.tile / 2, 64,
                         CU_TENSOR_MAP_SWIZZLE_128B);
   if (!rc) rc = make_tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, w_rows, a.K / 2, (uint64_t)a.K / 2, a.gated ? 64 : 128, 64, CU_TENSOR_MAP_SWIZZLE_64B);
   if (rc) return rc;
-  const int sms = sm_count(), most = a.tile_cap * p.n_strips;
-  if (pair) {
-    const int grid = 2 * (most < sms / 2 ? most : sms / 2);
-    return a.gated ? by_type<128, true, true, true>(a.bf16, a.G, tx, tw, p, grid, st) : by_type<128, true, true, false>(a.bf16, a.G, tx, tw, p, grid, st);
-  }
-  const int grid = most < sms ? most : sms;
-  if (a.tile == 32) return a.gated ? by_type<32, false, true, true>(a.bf16, a.G, tx, tw, p, grid, st) : by_type<32, false, true, false>(a.bf16, a.G, tx, tw, p, grid, st);
-  return a.gated ? by_type<64, false, true, true>(a.bf16, a.G, tx, tw, p, grid, st) : by_type<64, false, true, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  const int pairs = sm_count() / 2, most = a.tile_cap * p.n_strips, grid = 2 * (most < pairs ? most : pairs);
+  if (a.tile == 32) return a.gated ? by_type<32, true, true>(a.bf16, a.G, tx, tw, p, grid, st) : by_type<32, true, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  if (a.tile == 64) return a.gated ? by_type<64, true, true>(a.bf16, a.G, tx, tw, p, grid, st) : by_type<64, true, false>(a.bf16, a.G, tx, tw, p, grid, st);
+  return a.gated ? by_type<128, true, true>(a.bf16, a.G, tx, tw, p, grid, st) : by_type<128, true, false>(a.bf16, a.G, tx, tw, p, grid, st);
 }
 
 }  // namespace b2q
