@@ -62,7 +62,8 @@ size_t b2q_moe_forward_w4_workspace_bytes(int64_t T, int64_t E, int64_t top_k, i
   if (T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || top_k > 32 || H <= 0 || I <= 0 || T > INT32_MAX / 32) return 0;
   G4MoeArgs g{};
   g.T = (int)T; g.E = (int)E; g.k = (int)top_k; g.H = (int)H; g.I = (int)I;
-  return moe_g4_many_bytes(g);
+  const size_t few = moe_g4_few_bytes(g), many = moe_g4_many_bytes(g);      // which form it will be depends on the groups too
+  return few > many ? few : many;
 }
 
 int b2q_moe_forward_w4(const b2q_moe_w4* m, void* workspace, size_t workspace_bytes, void* stream) {
@@ -82,6 +83,7 @@ int b2q_moe_forward_w4(const b2q_moe_w4* m, void* workspace, size_t workspace_by
   G4MoeArgs g{};
   g.x = a.x; g.bf16 = a.act_dtype == B2Q_BF16; g.weights = a.weights; g.ids = a.ids; g.w13 = a.w13; g.s13 = a.s13; g.z13 = a.z13; g.w2 = a.w2; g.s2 = a.s2; g.z2 = a.z2;
   g.out = a.out; g.T = (int)a.T; g.E = (int)a.E; g.k = (int)a.top_k; g.H = (int)a.H; g.I = (int)a.I; g.G13 = (int)a.group13; g.G2 = (int)a.group2;
+  if (moe_g4_few_preferred(g)) return moe_g4_few(g, workspace, (cudaStream_t)stream);
   return moe_g4_many(g, workspace, (cudaStream_t)stream);
 }
 

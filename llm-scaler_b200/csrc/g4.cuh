@@ -49,6 +49,9 @@ struct G4MoeArgs {
   void* out;
   int T, E, k, H, I, G13, G2;
 };
+bool moe_g4_few_preferred(const G4MoeArgs& a);
+size_t moe_g4_few_bytes(const G4MoeArgs& a);
+int moe_g4_few(const G4MoeArgs& a, void* scratch, cudaStream_t st);
 size_t moe_g4_many_bytes(const G4MoeArgs& a);
 int moe_g4_many(const G4MoeArgs& a, void* scratch, cudaStream_t st);
 

@@ -203,6 +203,39 @@ __device__ __forceinline__ void multiply(float (&sum)[RT][TT][4], uint32_t slot,
   }
 }
 
+// The same for 16 rows and eight tokens whose columns lie apart: xs is this lane's at the step, its eights exchanged by `flip` (64, if its parity is not that of g); xg of the two
+// columns whose sums this lane has.
+template <int VEC, bool BF16>
+__device__ __forceinline__ void multiply_column(float (&sum)[4], uint32_t slot, const Lane<VEC>& ln, uint32_t xs, uint32_t flip, uint32_t xg0, uint32_t xg1, const uint32_t (&packed)[2], int t0) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 4 / VEC; ++j) {
+    uint32_t wa[VEC], wb[VEC];
+    lds_words<VEC>(slot + ln.word[j], wa);
+    lds_words<VEC>(slot + ln.word[j] + 512, wb);
+    const int from = (lane & ~3) + t0 + j;
+    const uint32_t qa = __shfl_sync(0xffffffffu, packed[0], from), qb = __shfl_sync(0xffffffffu, packed[1], from);
+    float d[4];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      uint32_t x[4];
+      lds_words<4>(xs + (ln.x[VEC * j + v] ^ flip), x);
+      const uint32_t a = wa[v], b = wb[v], a8 = a >> 8, b8 = b >> 8;
+      if (v == 0) mma_first(d, a & 0x000F000Fu, b & 0x000F000Fu, a8 & 0x000F000Fu, b8 & 0x000F000Fu, x[0], x[1]);
+      else mma(d, a & 0x000F000Fu, b & 0x000F000Fu, a8 & 0x000F000Fu, b8 & 0x000F000Fu, x[0], x[1]);
+      mma(d, a & 0x00F000F0u, b & 0x00F000F0u, a8 & 0x00F000F0u, b8 & 0x00F000F0u, x[2], x[3]);
+    }
+    uint32_t X0, X1;
+    lds_words<1>(xg0 + 4 * j, &X0);
+    lds_words<1>(xg1 + 4 * j, &X1);
+    const float sa = half_f<BF16>(qa), sb = half_f<BF16>(qb), za = __uint_as_float(qa & 0xFFFF0000u), zb = __uint_as_float(qb & 0xFFFF0000u);
+    sum[0] = fmaf(sa, fmaf(-za, __uint_as_float(X0), d[0]), sum[0]);
+    sum[1] = fmaf(sa, fmaf(-za, __uint_as_float(X1), d[1]), sum[1]);
+    sum[2] = fmaf(sb, fmaf(-zb, __uint_as_float(X0), d[2]), sum[2]);
+    sum[3] = fmaf(sb, fmaf(-zb, __uint_as_float(X1), d[3]), sum[3]);
+  }
+}
+
 // A tile's sums to [16 RT rows][8 TT], and zero.
 template <int RT, int TT> __device__ __forceinline__ void flush(float (&sum)[RT][TT][4], float* to) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
