@@ -1,7 +1,7 @@
 // Linear of a few tokens on 4-bit group-quantised weights: out[m, n] = sum_g s[g, n] (sum_k x[m, k] q[n, k] - z[g, n] X[m, g]) (+ bias[n]).
 //
 // HBM-bound: the weights are read once, and there is little time to convert them (g4_stream.cuh has the mathematics and the layout).  A CTA per SM has rows of its own, dealt
-// out evenly.  Its units (16 RT rows of 128 k each) go to its sixteen warps in equal runs; a warp's next units are on their way while one is multiplied, and
+// out evenly.  Its units (32 rows of 128 k each) go to its twelve warps in equal runs; a warp's next units are on their way while one is multiplied, and
 // nothing in the loop waits for another warp.  A warp leaves its sums of a tile of rows in a slot of shared memory; at the end they are added up in the
 // order of warps, so that results are the same every time.
 //
@@ -15,7 +15,7 @@
 
 namespace b2q {
 namespace g4s {
-constexpr int WARPS = 16, THREADS = 32 * WARPS;
+constexpr int WARPS = 12, THREADS = 32 * WARPS;
 constexpr int SELF = 4;                                    // eights that a thread prepares at most where a CTA prepares the tokens itself
 enum { ST_IMAGE = 901 };
 
@@ -79,9 +79,9 @@ __global__ void __launch_bounds__(256) g4_prep_kernel(const uint16_t* x, int64_t
   }
 }
 
-template <int VEC, int RT, int TT, bool BF16, bool PART>
+template <int VEC, int TT, bool BF16, bool PART>
 __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
-  constexpr int G = 32 * VEC, GS = STEP / G, TOK = 8 * TT, ROWS = 16 * RT;      // GS: groups in a step
+  constexpr int G = 32 * VEC, GS = STEP / G, TOK = 8 * TT;      // GS: groups in a step
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t row_max[TOK];
   __shared__ int shifts[TOK];
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
   const int cluster = blockIdx.x / C, clusters = gridDim.x / C;
   const int s0 = rank * p.steps / (int)C, s1 = (rank + 1) * p.steps / (int)C, steps = s1 - s0;
   const int sb = step_bytes(p.M, G, TT);
-  uint8_t* xs = smem + WARPS * RING<RT> * SLOT<RT>;            // [steps][step_bytes]
+  uint8_t* xs = smem + WARPS * WARP_BYTES;                 // [steps][step_bytes]
   float* slots = reinterpret_cast<float*>(xs + (p.steps + C - 1) / C * sb);      // [tiles + WARPS][ROWS][TOK]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -109,43 +109,23 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
   }
   if (threadIdx.x < TOK) row_max[threadIdx.x] = 0;
   if (!p.early) grid_dep_wait();
-  const Lane<VEC> ln;
-  const uint32_t ring = smem_addr(smem) + warp * RING<RT> * SLOT<RT>;
-  // Loads run ahead of the products: codes by RING - 1 steps, scales by two sets of four groups.  Sets begin anew with every tile.
-  Codes<RT, PART> codes;
-  Groups<RT> groups;
-  int uc = u0, us = u0, code_steps = 0, scale_steps = 0;   // the next units to load; steps left of their tiles
-  auto fetch_codes = [&](uint32_t slot) {
-    if (uc < u1) {
-      if (code_steps == 0) {
-        const int tile = uc / steps, s = uc - tile * steps;
-        codes.at(p.w, (s0 + s) * STEP, p.K, [&](int i) { return (int64_t)(r0 + min(ROWS * tile + g + 8 * i, rows - 1)); });
-        code_steps = min(u1 - uc, steps - s);
-      }
-      codes.copy(slot + ln.copy);
-      ++uc;
-      --code_steps;
-    }
-    copy_commit();
-  };
-  auto fetch_scales = [&](Scales<RT>& r) {
-    if (us < u1) {
-      if (scale_steps <= 0) {
-        const int tile = us / steps, s = us - tile * steps;
-        groups.at(p.w, r0, (s0 + s) * GS, p.K / G, [&](int i) { return min(ROWS * tile + g + 8 * i, rows - 1); });
-        scale_steps = min(u1 - us, steps - s);
-      }
-      groups.next(p.w, r);
-      const int n = min(4 / GS, scale_steps);
-      us += n;
-      scale_steps -= n;
-    }
-  };
-  Scales<RT> raw[2];
+  struct Tiles {
+    int r0, nrows, g, t, M; uint32_t xs;
+    __device__ __forceinline__ int rows(int tile, int64_t (&row)[4], int (&off)[4], int64_t& base) const {
+      base = r0;
 #pragma unroll
-  for (int i = 0; i < RING<RT> - 1; ++i) fetch_codes(ring + i * SLOT<RT>);
-  fetch_scales(raw[0]);
-  fetch_scales(raw[1]);
+      for (int i = 0; i < 4; ++i) { off[i] = min(ROWS * tile + g + 8 * i, nrows - 1); row[i] = r0 + off[i]; }
+      return nrows - ROWS * tile > 16 ? 2 : 1;
+    }
+    __device__ __forceinline__ void columns(int, uint32_t (&at)[TT], uint32_t& xg) const {
+#pragma unroll
+      for (int n = 0; n < TT; ++n) at[n] = xs + min(8 * n + g, M - 1) * STEP * 2;      // columns beyond M repeat the last: nobody looks at them
+      xg = xs + M * STEP * 2 + 8 * t;
+    }
+  } of{r0, rows, g, t, p.M, smem_addr(xs)};
+  const uint32_t ring = smem_addr(smem) + warp * WARP_BYTES;
+  Stream<VEC, TT, BF16, PART, Tiles> stream(p.w, of, p.K, steps, s0, u0, u1, ring);
+  stream.load(ring);
   if (p.early) grid_dep_wait();
   __syncthreads();                                         // the barrier and the maxima
   bool ok = true;
@@ -188,45 +168,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
   }
   __syncthreads();
 
-  float sum[RT][TT][4];
-#pragma unroll
-  for (int h = 0; h < RT; ++h)
-#pragma unroll
-    for (int n = 0; n < TT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum[h][n][i] = 0.f;
-  uint32_t token[TT];                                      // columns beyond M repeat the last: nobody looks at them
-#pragma unroll
-  for (int n = 0; n < TT; ++n) {
-    token[n] = smem_addr(xs) + min(8 * n + g, p.M - 1) * STEP * 2;
-  }
-  const uint32_t xg = smem_addr(xs) + p.M * STEP * 2 + 8 * t;
-  uint32_t packed[2 * RT], slot = ring;
-  int tile = steps ? u0 / steps : 0, s = u0 - tile * steps, used = 4;      // used: groups of the set
-  for (int u = u0; ok && u < u1; ++u) {
-    copy_wait<RING<RT> - 2>();
-    __syncwarp();                                          // other lanes' pieces are there, and all have read the slot that is filled next
-    fetch_codes(slot == ring ? ring + (RING<RT> - 1) * SLOT<RT> : slot - SLOT<RT>);
-    if (used == 4) {
-#pragma unroll
-      for (int i = 0; i < 2 * RT; ++i) packed[i] = pack_scale(raw[0].s[i], raw[0].z[i]);
-      raw[0] = raw[1];
-      fetch_scales(raw[1]);
-      used = 0;
-    }
-    uint32_t at[TT];
-#pragma unroll
-    for (int n = 0; n < TT; ++n) at[n] = token[n] + s * sb;
-    multiply<VEC, RT, TT, BF16>(sum, slot, ln, at, xg + s * sb, packed, used, rows - ROWS * tile > 16 ? 2 : 1);
-    used += GS;
-    slot = slot == ring + (RING<RT> - 1) * SLOT<RT> ? ring : slot + SLOT<RT>;
-    if (++s == steps || u + 1 == u1) {
-      flush<RT, TT>(sum, slots + (tile + warp) * ROWS * TOK);
-      ++tile;
-      s = 0;
-      used = 4;
-    }
-  }
+  if (ok) stream.run(sb, sb, slots, warp);
   copy_wait<0>();
   __syncthreads();
 
@@ -237,8 +179,8 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
   };
   float* part = reinterpret_cast<float*>(smem);            // [M][rows], where the rings and the tokens were
   const bool alone = C == 1;
-  for (int h = warp; h < tiles * RT; h += WARPS) {         // sixteens of rows
-    const int tl = h / RT, first = tl * steps / run, last = ((tl + 1) * steps - 1) / run, r = 16 * h + (lane & 15);      // warps that have units of it
+  for (int h = warp; h < tiles * 2; h += WARPS) {          // sixteens of rows
+    const int tl = h / 2, first = tl * steps / run, last = ((tl + 1) * steps - 1) / run, r = 16 * h + (lane & 15);      // warps that have units of it
     for (int m = lane >> 4; m < p.M; m += 2) {
       const float* from = slots + (tl * ROWS + r - ROWS * tl) * TOK + m;
       float v = 0.f;
@@ -268,7 +210,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
 
 // ---- host ----
 constexpr int SMEM = 220 * 1024;
-struct Plan { int C, clusters, cap, smem, tt, rt, steps; bool self; };
+struct Plan { int C, clusters, cap, smem, tt, steps; bool self; };
 // Clusters of four that the SMs hold at a time: not all of them can be in one.
 static int resident(int C) { return C == 4 ? sm_count() * 7 / 32 : sm_count() / C; }
 static Plan plan(int M, int N, int K, int G) {
@@ -281,23 +223,22 @@ static Plan plan(int M, int N, int K, int G) {
     q.clusters = resident(q.C);
     if (q.clusters > (N + 7) / 8) q.clusters = (N + 7) / 8;
     const int rows = (N + q.clusters - 1) / q.clusters, most = (q.steps + q.C - 1) / q.C;
-    q.rt = rows > 16 ? 2 : 1;
-    q.cap = (rows + 16 * q.rt - 1) / (16 * q.rt);
-    const int64_t front = (int64_t)WARPS * (q.rt == 2 ? RING<2> * SLOT<2> : RING<1> * SLOT<1>) + (int64_t)most * step_bytes(M, G, q.tt);
-    const int64_t smem = front + (int64_t)(q.cap + WARPS) * 16 * q.rt * 8 * q.tt * 4;
+    q.cap = (rows + ROWS - 1) / ROWS;
+    const int64_t front = (int64_t)WARPS * WARP_BYTES + (int64_t)most * step_bytes(M, G, q.tt);
+    const int64_t smem = front + (int64_t)(q.cap + WARPS) * ROWS * 8 * q.tt * 4;
     if (smem <= SMEM && (q.C == 1 || (int64_t)M * rows * 4 <= front)) { q.smem = (int)smem; return q; }
   }
   return q;
 }
 
-template <int VEC, int RT, int TT, bool BF16, bool PART> static int launch(Params& p, const Plan& q, cudaStream_t st) {
+template <int VEC, int TT, bool BF16, bool PART> static int launch(Params& p, const Plan& q, cudaStream_t st) {
   p.cap = q.cap;
   const bool overlap = tls().overlap_mode > 0;
   if (p.image) {
     launch_overlapped(g4_prep_kernel<32 * VEC, TT, BF16>, dim3(p.M), dim3(256), 0, st, overlap, p.x, p.ldx, p.vec, const_cast<uint8_t*>(p.image), const_cast<int*>(p.shifts), p.M, p.K, p.steps);
     note_launch("g4_prep");
   }
-  auto kern = g4_stream_kernel<VEC, RT, TT, BF16, PART>;
+  auto kern = g4_stream_kernel<VEC, TT, BF16, PART>;
   static thread_local bool configured[16] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -325,8 +266,7 @@ template <int VEC, int RT, int TT, bool BF16, bool PART> static int launch(Param
   return launch_status();
 }
 template <int VEC, bool BF16, bool PART> static int by_size(Params& p, const Plan& q, cudaStream_t st) {
-  if (q.rt == 1) return q.tt == 1 ? launch<VEC, 1, 1, BF16, PART>(p, q, st) : launch<VEC, 1, 2, BF16, PART>(p, q, st);
-  return q.tt == 1 ? launch<VEC, 2, 1, BF16, PART>(p, q, st) : launch<VEC, 2, 2, BF16, PART>(p, q, st);
+  return q.tt == 1 ? launch<VEC, 1, BF16, PART>(p, q, st) : launch<VEC, 2, BF16, PART>(p, q, st);
 }
 template <int VEC, bool PART> static int by_type(Params& p, bool bf16, const Plan& q, cudaStream_t st) {
   return bf16 ? by_size<VEC, true, PART>(p, q, st) : by_size<VEC, false, PART>(p, q, st);

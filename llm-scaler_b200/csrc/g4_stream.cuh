@@ -8,7 +8,7 @@
 // [2^14, 2^15): bf16 and fp16 values down to 2^-24 of that stay exact, and smaller ones are off by no more than 2^-35 of it.
 //
 // Issue slots and the integer pipe are what bounds such a kernel before memory does: a warp takes 32 rows at a time, so that the activations are read half
-// as often (1 x 28672 x 8192: 29.0 us, 36 with 16 rows).  Codes by cp.async and not straight into registers, where a wait for one load was a wait for
+// as often (1 x 28672 x 8192: 29.0 us, 36 with 16 rows), and two steps at a time.  Codes by cp.async and not straight into registers, where a wait for one load was a wait for
 // younger ones too (43 us).  An 8-bit mma.sync of e4m3, for which the bytes q need no more than masks, took 43 us where this took 36 at the time: half
 // again as many instructions.
 //
@@ -76,17 +76,14 @@ template <bool BF16> __device__ __forceinline__ uint16_t to_half(float v) { retu
 // One matrix: codes [N, K / 2], scales and zero points [K / G, N].
 struct Matrix { const uint8_t* w; const uint16_t* s; const uint8_t* z; int64_t half; int64_t n; };      // half: K / 2, n: rows of the scales' pitch
 
-// A warp takes its tiles of 16 RT rows step by step.  Codes go by cp.async, a row's 64 bytes of a step by four lanes, into a ring of the warp's own in shared
-// memory; the 16-byte pieces of a slot are permuted so that the words are read without bank conflicts, whatever the group.
-template <int RT> constexpr int RING = RT == 2 ? 3 : 4;
-template <int RT> constexpr int SLOT = 16 * RT * STEP / 2;
+// A warp takes its tiles of 32 rows two steps at a time.  Codes go by cp.async, a row's 64 bytes of a step by four lanes, into one of two slots of the warp's own in shared
+// memory, the next two steps' while these are multiplied; the 16-byte pieces of a slot are permuted so that the words are read without bank conflicts,
+// whatever the group.
+constexpr int ROWS = 32, PART_BYTES = ROWS * STEP / 2, SLOT = 2 * PART_BYTES, WARP_BYTES = 2 * SLOT;
 __device__ __forceinline__ int slot_piece(int row, int piece) {      // byte offset in a slot; row < 8
   const int f = (row >> 1 & 1) << 1 | (row >> 2 & 1);
   return row * 64 + ((piece ^ f) << 4);
 }
-
-// Rows of a lane in a tile: g + 8 i, i < 2 RT.  Scales and zero points of four groups: lane t of a quad has those of group t.
-template <int RT> struct Scales { uint32_t s[2 * RT], z[2 * RT]; };
 
 template <int VEC> struct Lane {                           // what stays the same throughout
   uint32_t copy;                                           // where this lane's piece of its first row goes in a slot; the next rows 512 further each
@@ -105,50 +102,6 @@ template <int VEC> struct Lane {                           // what stays the sam
   }
 };
 
-// Where a lane copies from: its 16 bytes of its rows, step by step.  Rows beyond the last repeat it, and nobody looks at their sums; codes beyond K are zeros.
-template <int RT, bool PART> struct Codes {                // PART: K is no multiple of 128
-  const uint8_t* p[2 * RT];
-  int left;                                                // PART: values from this lane's to the end of the row
-  template <typename RowAt> __device__ __forceinline__ void at(const Matrix& m, int k0, int K, RowAt row) {      // row(i): of the matrix
-    const int t = threadIdx.x & 3;
-#pragma unroll
-    for (int i = 0; i < 2 * RT; ++i) p[i] = m.w + row(i) * m.half + (k0 >> 1) + 16 * t;
-    left = K - k0 - 32 * t;
-  }
-  __device__ __forceinline__ void copy(uint32_t to) {
-    const uint32_t n = !PART || left > 0 ? 16 : 0;
-#pragma unroll
-    for (int i = 0; i < 2 * RT; ++i) {
-      if (PART) copy16(to + 512 * i, p[i], n);
-      else copy16(to + 512 * i, p[i]);
-      p[i] += STEP / 2;
-    }
-    left -= STEP;
-  }
-};
-// The same for scales and zero points, four groups at a time, of which those beyond K repeat the last: their activations are zero.
-template <int RT> struct Groups {
-  int64_t first; int off[2 * RT], left;                    // element of the first row at the next group; from it to the rows; groups left
-  template <typename RowAt> __device__ __forceinline__ void at(const Matrix& m, int64_t base, int g0, int groups, RowAt row) {      // row(i): in the scales' rows from base
-    first = g0 * m.n + base;
-#pragma unroll
-    for (int i = 0; i < 2 * RT; ++i) off[i] = (int)row(i);
-    left = groups - g0;
-  }
-  __device__ __forceinline__ void next(const Matrix& m, Scales<RT>& r) {
-    const int64_t at = first + min((int)(threadIdx.x & 3), left - 1) * m.n;
-#pragma unroll
-    for (int i = 0; i < 2 * RT; ++i) r.s[i] = ld_scale(m.s + at + off[i]);
-#pragma unroll
-    for (int i = 0; i < 2 * RT; ++i) r.z[i] = 8;
-    if (m.z) {
-#pragma unroll
-      for (int i = 0; i < 2 * RT; ++i) r.z[i] = ld_zero(m.z + at + off[i]);
-    }
-    first += 4 * m.n;
-    left -= 4;
-  }
-};
 // Scale in the low half as it is, zero point in the upper half as bf16, which holds every byte.
 __device__ __forceinline__ uint32_t pack_scale(uint32_t s, uint32_t z) {
   return (__float_as_uint(__uint_as_float(0x4B000000u | z) - 8388608.f) & 0xFFFF0000u) | s;
@@ -156,8 +109,8 @@ __device__ __forceinline__ uint32_t pack_scale(uint32_t s, uint32_t z) {
 
 // sum += a step's share, in units of 2^-24.  slot: the codes; xs: shared address of this lane's token (of each eight of tokens) at the step; xg: of the group sums at the
 // step's first group and this lane's columns; packed: scales, of which the step's first group is in lane t0 of a quad; halves: sixteens of rows there are.
-template <int VEC, int RT, int TT, bool BF16>
-__device__ __forceinline__ void multiply(float (&sum)[RT][TT][4], uint32_t slot, const Lane<VEC>& ln, const uint32_t (&xs)[TT], uint32_t xg, const uint32_t (&packed)[2 * RT], int t0,
+template <int VEC, int TT, bool BF16>
+__device__ __forceinline__ void multiply(float (&sum)[2][TT][4], uint32_t slot, const Lane<VEC>& ln, const uint32_t (&xs)[TT], uint32_t xg, const uint32_t (&packed)[4], int t0,
                                          int halves) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -172,8 +125,8 @@ __device__ __forceinline__ void multiply(float (&sum)[RT][TT][4], uint32_t slot,
     for (int n = 0; n < TT; ++n) X[n] = lds64f(xg + (j * 8 * TT + 8 * n) * 4);
     const int from = (lane & ~3) + t0 + j;
 #pragma unroll
-    for (int h = 0; h < RT; ++h) {
-      if (h > 0 && h >= halves) break;
+    for (int h = 0; h < 2; ++h) {
+      if (h == 1 && halves == 1) break;
       uint32_t wa[VEC], wb[VEC];
       lds_words<VEC>(slot + ln.word[j] + 1024 * h, wa);
       lds_words<VEC>(slot + ln.word[j] + 1024 * h + 512, wb);
@@ -203,44 +156,11 @@ __device__ __forceinline__ void multiply(float (&sum)[RT][TT][4], uint32_t slot,
   }
 }
 
-// The same for 16 rows and eight tokens whose columns lie apart: xs is this lane's at the step, its eights exchanged by `flip` (64, if its parity is not that of g); xg of the two
-// columns whose sums this lane has.
-template <int VEC, bool BF16>
-__device__ __forceinline__ void multiply_column(float (&sum)[4], uint32_t slot, const Lane<VEC>& ln, uint32_t xs, uint32_t flip, uint32_t xg0, uint32_t xg1, const uint32_t (&packed)[2], int t0) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int j = 0; j < 4 / VEC; ++j) {
-    uint32_t wa[VEC], wb[VEC];
-    lds_words<VEC>(slot + ln.word[j], wa);
-    lds_words<VEC>(slot + ln.word[j] + 512, wb);
-    const int from = (lane & ~3) + t0 + j;
-    const uint32_t qa = __shfl_sync(0xffffffffu, packed[0], from), qb = __shfl_sync(0xffffffffu, packed[1], from);
-    float d[4];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      uint32_t x[4];
-      lds_words<4>(xs + (ln.x[VEC * j + v] ^ flip), x);
-      const uint32_t a = wa[v], b = wb[v], a8 = a >> 8, b8 = b >> 8;
-      if (v == 0) mma_first(d, a & 0x000F000Fu, b & 0x000F000Fu, a8 & 0x000F000Fu, b8 & 0x000F000Fu, x[0], x[1]);
-      else mma(d, a & 0x000F000Fu, b & 0x000F000Fu, a8 & 0x000F000Fu, b8 & 0x000F000Fu, x[0], x[1]);
-      mma(d, a & 0x00F000F0u, b & 0x00F000F0u, a8 & 0x00F000F0u, b8 & 0x00F000F0u, x[2], x[3]);
-    }
-    uint32_t X0, X1;
-    lds_words<1>(xg0 + 4 * j, &X0);
-    lds_words<1>(xg1 + 4 * j, &X1);
-    const float sa = half_f<BF16>(qa), sb = half_f<BF16>(qb), za = __uint_as_float(qa & 0xFFFF0000u), zb = __uint_as_float(qb & 0xFFFF0000u);
-    sum[0] = fmaf(sa, fmaf(-za, __uint_as_float(X0), d[0]), sum[0]);
-    sum[1] = fmaf(sa, fmaf(-za, __uint_as_float(X1), d[1]), sum[1]);
-    sum[2] = fmaf(sb, fmaf(-zb, __uint_as_float(X0), d[2]), sum[2]);
-    sum[3] = fmaf(sb, fmaf(-zb, __uint_as_float(X1), d[3]), sum[3]);
-  }
-}
-
-// A tile's sums to [16 RT rows][8 TT], and zero.
-template <int RT, int TT> __device__ __forceinline__ void flush(float (&sum)[RT][TT][4], float* to) {
+// A tile's sums to [32 rows][8 TT], and zero.
+template <int TT> __device__ __forceinline__ void flush(float (&sum)[2][TT][4], float* to) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int h = 0; h < RT; ++h)
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int n = 0; n < TT; ++n) {
       float* at = to + (16 * h + g) * 8 * TT + 8 * n + 2 * t;
@@ -250,6 +170,129 @@ template <int RT, int TT> __device__ __forceinline__ void flush(float (&sum)[RT]
       for (int i = 0; i < 4; ++i) sum[h][n][i] = 0.f;
     }
 }
+
+// A warp's run of units (a tile's step each): [u0, u1) of tiles with `steps` steps, the matrix's steps s0 on.  Tiles::rows(tile, row, off, base) gives the lane's four rows (of the
+// codes), their scales' offsets from base, and how many sixteens of rows there are; Tiles::columns(tile, xs, xg) where its tokens and their group sums begin.
+template <int VEC, int TT, bool BF16, bool PART, typename Tiles> struct Stream {      // PART: K is no multiple of 128
+  static constexpr int G = 32 * VEC, GS = STEP / G;        // groups in a step
+  static constexpr int SETS = GS == 4 ? 2 : 1;             // fours of groups in two steps
+  const Matrix& m;
+  Tiles& tiles;
+  const Lane<VEC> ln;
+  int K, steps, s0, u, u1;                                 // u: the next unit to load
+  uint32_t ring;
+  // of the two steps that are loaded next: where this lane copies from, and its scales
+  const uint8_t* p[4];
+  int64_t base; int off[4], tile, s, n, halves;
+  uint32_t raw_s[SETS][4], raw_z[SETS][4];
+
+  __device__ __forceinline__ Stream(const Matrix& m_, Tiles& tiles_, int K_, int steps_, int s0_, int u0_, int u1_, uint32_t ring_)
+      : m(m_), tiles(tiles_), K(K_), steps(steps_), s0(s0_), u(u0_), u1(u1_), ring(ring_) {
+    tile = steps ? u / steps : 0;
+    s = u - tile * steps;
+    n = 0;
+    if (u < u1) enter();
+  }
+  __device__ __forceinline__ void enter() {                // the tile's rows, from step s on
+    const int t = threadIdx.x & 3;
+    int64_t row[4];
+    halves = tiles.rows(tile, row, off, base);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = m.w + row[i] * m.half + (s0 + s) * (STEP / 2) + 16 * t;
+    n = min(2, min(steps - s, u1 - u));
+  }
+  // Loads two steps, or what is left of the tile, into the slot.  Rows beyond the last repeat it, and nobody looks at their sums; codes beyond K are zeros, and groups beyond K repeat
+  // the last: their activations are zero.
+  __device__ __forceinline__ void load(uint32_t slot) {
+    if (u < u1) {
+      const int t = threadIdx.x & 3, k0 = (s0 + s) * STEP;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j == 1 && n == 1) break;
+        const uint32_t to = slot + ln.copy + j * PART_BYTES, bytes = !PART || k0 + j * STEP + 32 * t < K ? 16 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (i == 2 && halves == 1) break;
+          if (PART) copy16(to + 512 * i, p[i] + j * (STEP / 2), bytes);
+          else copy16(to + 512 * i, p[i] + j * (STEP / 2));
+        }
+      }
+      const int g0 = (s0 + s) * GS, last = min(K / G - 1 - g0, n * GS - 1);
+#pragma unroll
+      for (int q = 0; q < SETS; ++q) {
+        const int64_t at = base + (int64_t)(g0 + min(4 * q + t, last)) * m.n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw_s[q][i] = ld_scale(m.s + at + off[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw_z[q][i] = 8;
+        if (m.z) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) raw_z[q][i] = ld_zero(m.z + at + off[i]);
+        }
+      }
+    }
+    copy_commit();
+  }
+  __device__ __forceinline__ void advance() {              // behind load()
+    u += n;
+    s += n;
+    if (s == steps) {
+      s = 0;
+      ++tile;
+      if (u < u1) enter();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] += STEP;
+      n = min(2, min(steps - s, u1 - u));
+    }
+  }
+  // Everything, behind load() of the first slot and the staging of the tokens.  A tile's sums go to slots[tile + warp].
+  __device__ __forceinline__ void run(uint32_t x_stride, uint32_t xg_stride, float* slots, int warp) {
+    float sum[2][TT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[h][i][j] = 0.f;
+    uint32_t at[TT], xg = 0, slot = ring;
+    bool fresh = true;
+    while (u < u1) {
+      const int now_tile = tile, now_s = s, now_n = n, now_halves = halves;
+      uint32_t packed[SETS][4];
+#pragma unroll
+      for (int q = 0; q < SETS; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) packed[q][i] = pack_scale(raw_s[q][i], raw_z[q][i]);
+      advance();
+      load(2 * ring + SLOT - slot);
+      if (fresh) {
+        tiles.columns(now_tile, at, xg);
+#pragma unroll
+        for (int i = 0; i < TT; ++i) at[i] += now_s * x_stride;
+        xg += now_s * xg_stride;
+        fresh = false;
+      }
+      copy_wait<1>();
+      __syncwarp();                                        // other lanes' pieces are there
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j == 1 && now_n == 1) break;
+        multiply<VEC, TT, BF16>(sum, slot + j * PART_BYTES, ln, at, xg, packed[j * GS / 4], j * GS % 4, now_halves);
+#pragma unroll
+        for (int i = 0; i < TT; ++i) at[i] += x_stride;
+        xg += xg_stride;
+      }
+      if (u >= u1 || tile != now_tile) {
+        flush<TT>(sum, slots + (now_tile + warp) * ROWS * 8 * TT);
+        fresh = true;
+      }
+      __syncwarp();                                        // all have read what the copies after the next replace
+      slot = 2 * ring + SLOT - slot;
+    }
+    copy_wait<0>();
+  }
+};
 
 // ---- tokens ----
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }      // |k| < 127

@@ -2,9 +2,9 @@
 // tokens are more than a handful.
 //
 // HBM-bound for a batch, a chain of latencies for one token.  Every CTA sorts the routes by itself, in shared memory: the pairs (token, slot) of an expert form groups of
-// up to eight, whose tokens are the columns of one MMA.  A tile is 16 weight rows of one group; CTAs have equal runs of the tiles of all groups, and their sixteen
+// up to eight, whose tokens are the columns of one MMA.  A tile is 32 weight rows of one group; CTAs have equal runs of the tiles of all groups, and their twelve
 // warps equal runs of the tiles' steps of 128 k, as in the linear.
-//  * up: a tile has eight gate rows and the eight up rows of the same outputs; h = silu(gate) * up goes out in 16 bits, with its largest magnitude per tile, from which the
+//  * up: a tile has sixteen gate rows and the sixteen up rows of the same outputs; h = silu(gate) * up goes out in 16 bits, with its largest magnitude per tile, from which the
 //    second kernel takes the power of two that it scales a row of h by.
 //  * down, OWN: a CTA has rows of its own, for all groups; it adds the weighted outputs of a token's experts up by itself.  While all pairs' h fit its shared memory.
 //  * down otherwise: weighted outputs of each pair in fp32, which a third kernel adds up in the order of the slots.
@@ -15,19 +15,17 @@
 namespace b2q {
 namespace g4f {
 using namespace g4s;
-constexpr int WARPS = 16, THREADS = 32 * WARPS, MAX_PAIRS = 512, MAX_E = 1024, TOK = 8;
-constexpr int CAP = 64;                                    // tiles that are summed up at a time
-constexpr int SLOT1 = SLOT<1>, RING1 = RING<1>;
+constexpr int WARPS = 12, THREADS = 32 * WARPS, MAX_PAIRS = THREADS, MAX_E = 1024, PER = (MAX_E + THREADS - 1) / THREADS, TOK = 8;
+constexpr int CAP = 24;                                    // tiles that are summed up at a time
 constexpr int SMEM = 208 * 1024;                           // beside the routes'
 
 struct Params {
   const uint16_t* x; const int32_t* ids; const float* weights;      // x: tokens, or h by pair
-  Matrix w; int64_t w_expert, s_expert;                    // bytes, elements of an expert
-  uint16_t* h; uint32_t* h_max;                            // [pairs, I], [pairs, I / 8]
+  Matrix w; int64_t w_rows, s_expert;                      // rows, scales of an expert
+  uint16_t* h; uint32_t* h_max;                            // [pairs, I], [pairs, I / 16]
   float* y; uint16_t* out;                                 // [pairs, N], [T, N]
   int T, E, k, N, K, steps;                                // N: outputs (I, H)
-  int columns;                                             // that there is room for
-  int early;
+  int columns, groups;                                     // that there is room for
 };
 
 struct Group { int16_t expert, first, count; };            // first, count: of the sorted pairs
@@ -41,6 +39,7 @@ struct alignas(16) Shared {
   int warp_sum[WARPS][2];
   int n_groups;
   uint32_t max[MAX_PAIRS];                                 // of a staged column's row
+  struct { int16_t group, strip, first, last; } tiles[CAP];      // of a batch; warps that have units of it
 };
 
 // The routes' pairs sorted by expert, those of an expert by their number: all CTAs of both kernels have to agree on which group a pair is in.
@@ -62,11 +61,16 @@ __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
       at += (v.x == id) + (v.y == id && j + 1 < (int)threadIdx.x) + (v.z == id && j + 2 < (int)threadIdx.x) + (v.w == id && j + 3 < (int)threadIdx.x);
     }
   }
-  // a thread has two experts
-  const int e0 = 2 * threadIdx.x;
-  const int c0 = e0 < p.E ? sh.count[e0] : 0, c1 = e0 + 1 < p.E ? sh.count[e0 + 1] : 0;
-  const int g0 = (c0 + TOK - 1) / TOK, g1 = (c1 + TOK - 1) / TOK;
-  int pairs = c0 + c1, groups = g0 + g1;
+  // a thread has PER experts
+  const int e0 = PER * threadIdx.x;
+  int c[PER], pairs = 0, groups = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    c[i] = e0 + i < p.E ? sh.count[e0 + i] : 0;
+    pairs += c[i];
+    groups += (c[i] + TOK - 1) / TOK;
+  }
+  const int own_pairs = pairs, own_groups = groups;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int a = __shfl_up_sync(0xffffffffu, pairs, o), b = __shfl_up_sync(0xffffffffu, groups, o);
@@ -74,14 +78,15 @@ __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
   }
   if (lane == 31) { sh.warp_sum[warp][0] = pairs; sh.warp_sum[warp][1] = groups; }
   __syncthreads();
-  int before = 0, gbefore = 0;
-  for (int w = 0; w < warp; ++w) { before += sh.warp_sum[w][0]; gbefore += sh.warp_sum[w][1]; }
-  int first = before + pairs - c0 - c1, g = gbefore + groups - g0 - g1;
-  if (threadIdx.x == THREADS - 1) sh.n_groups = gbefore + groups;
-  if (e0 < p.E) sh.count[e0] = first;
-  if (e0 + 1 < p.E) sh.count[e0 + 1] = first + c0;
-  for (int i = 0; i < c0; i += TOK) sh.groups[g++] = Group{(int16_t)e0, (int16_t)(first + i), (int16_t)min(TOK, c0 - i)};
-  for (int i = 0; i < c1; i += TOK) sh.groups[g++] = Group{(int16_t)(e0 + 1), (int16_t)(first + c0 + i), (int16_t)min(TOK, c1 - i)};
+  for (int w = 0; w < warp; ++w) { pairs += sh.warp_sum[w][0]; groups += sh.warp_sum[w][1]; }
+  if (threadIdx.x == THREADS - 1) sh.n_groups = groups;
+  int first = pairs - own_pairs, to_group = groups - own_groups;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (e0 + i < p.E) sh.count[e0 + i] = first;
+    for (int j = 0; j < c[i]; j += TOK) sh.groups[to_group++] = Group{(int16_t)(e0 + i), (int16_t)(first + j), (int16_t)min(TOK, c[i] - j)};
+    first += c[i];
+  }
   __syncthreads();
   if (threadIdx.x < n) {
     const int to = id >= 0 ? sh.count[id] + at : -1;
@@ -96,31 +101,30 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
   constexpr int G = 32 * VEC, GS = STEP / G;               // groups of k in a step
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Shared sh;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int steps = p.steps;
-  uint8_t* xs = smem + WARPS * RING1 * SLOT1;              // [columns][steps][256], then [columns][groups]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int steps = p.steps, group_xg = steps * GS * TOK;  // group sums of a group's columns: [steps * GS][8]
+  uint8_t* xs = smem + WARPS * WARP_BYTES;                 // [columns][steps][256], then [groups][group_xg]
   float* xg = reinterpret_cast<float*>(xs + (size_t)p.columns * steps * 256);
-  float* slots = xg + (p.columns * steps * GS + 3) / 4 * 4;      // [CAP + WARPS][16][TOK]
+  float* slots = xg + p.groups * group_xg;                 // [CAP + WARPS][ROWS][TOK]
 
   grid_dep_wait();
   // Only now: the next kernel may then read the routes, and begin with its weights, before this one is done.
   grid_dep_release();
   sort_routes(sh, p);
 
-  // this CTA's tiles: strip by strip of every group in turn.  OWN: rows of its own, in strips of sixteen, for all groups
-  constexpr int STRIP = UP ? 8 : 16;                       // outputs of a tile
+  // this CTA's tiles: strip by strip of every group in turn.  OWN: rows of its own, in strips of 32, for all groups
+  constexpr int STRIP = UP ? 16 : 32;                      // outputs of a tile
   const int own0 = OWN ? (int)((int64_t)blockIdx.x * p.N / gridDim.x) : 0, own = OWN ? (int)((int64_t)(blockIdx.x + 1) * p.N / gridDim.x) - own0 : p.N;
   const int strips = (own + STRIP - 1) / STRIP, all = sh.n_groups * strips;
   const int begin = OWN ? 0 : (int)((int64_t)blockIdx.x * all / gridDim.x), end = OWN ? all : (int)((int64_t)(blockIdx.x + 1) * all / gridDim.x);
-  const Lane<VEC> ln;
-  const uint32_t ring = smem_addr(smem) + warp * RING1 * SLOT1;
+  const uint32_t ring = smem_addr(smem) + warp * WARP_BYTES;
 
   for (int b0 = begin; b0 < end;) {
     // a batch: tiles whose groups' columns and sums fit
     const int ga = b0 / strips;
     int gb = ga + 1, columns = sh.groups[ga].count;
     int b1 = min(min(end, gb * strips), b0 + CAP);
-    while (b1 == gb * strips && b1 < end && b1 - b0 < CAP && columns + sh.groups[gb].count <= p.columns) {
+    while (b1 == gb * strips && b1 < end && b1 - b0 < CAP && columns + sh.groups[gb].count <= p.columns && gb - ga < p.groups) {
       columns += sh.groups[gb].count;
       ++gb;
       b1 = min(min(end, gb * strips), b0 + CAP);
@@ -128,54 +132,34 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
     const int pair0 = sh.groups[ga].first;                 // columns are the sorted pairs from here on
     const int tiles = b1 - b0, units = tiles * steps, run = (units + WARPS - 1) / WARPS, u0 = min(units, warp * run), u1 = min(units, u0 + run);
 
-    // ---- loads of weights run ahead ----
-    Codes<1, PART> codes;
-    Groups<1> groups;
-    int uc = u0, us = u0, code_steps = 0, scale_steps = 0;
-    auto rows_of = [&](int tile, int& expert, int& r0, int& rows) {      // rows r0 .. of the matrix that the tile's outputs begin at
-      const int id = b0 + tile, gi = id / strips, st = id - gi * strips;
-      expert = sh.groups[gi].expert;
-      r0 = own0 + STRIP * st;
-      rows = min(STRIP, own - STRIP * st);
-    };
-    auto row_at = [&](int i, int r0, int rows) { return UP ? r0 + min(g, rows - 1) + i * p.N : r0 + min(g + 8 * i, rows - 1); };      // up rows lie N behind the gate rows
-    auto fetch_codes = [&](uint32_t slot) {
-      if (uc < u1) {
-        if (code_steps == 0) {
-          const int tile = uc / steps, s = uc - tile * steps;
-          int e, r0, rows;
-          rows_of(tile, e, r0, rows);
-          Matrix m = p.w;
-          m.w += e * p.w_expert;
-          codes.at(m, s * STEP, p.K, [&](int i) { return (int64_t)row_at(i, r0, rows); });
-          code_steps = min(u1 - uc, steps - s);
-        }
-        codes.copy(slot + ln.copy);
-        ++uc;
-        --code_steps;
-      }
-      copy_commit();
-    };
-    auto fetch_scales = [&](Scales<1>& r) {
-      if (us < u1) {
-        if (scale_steps <= 0) {
-          const int tile = us / steps, s = us - tile * steps;
-          int e, r0, rows;
-          rows_of(tile, e, r0, rows);
-          groups.at(p.w, e * p.s_expert, s * GS, p.K / G, [&](int i) { return row_at(i, r0, rows); });
-          scale_steps = min(u1 - us, steps - s);
-        }
-        groups.next(p.w, r);
-        const int n = min(4 / GS, scale_steps);
-        us += n;
-        scale_steps -= n;
-      }
-    };
-    Scales<1> raw[2];
+    if (threadIdx.x < tiles) {
+      const int id = b0 + threadIdx.x, gi = id / strips;
+      sh.tiles[threadIdx.x] = {(int16_t)gi, (int16_t)(id - gi * strips), (int16_t)(threadIdx.x * steps / run), (int16_t)(((threadIdx.x + 1) * steps - 1) / run)};
+    }
+    __syncthreads();
+    struct Tiles {
+      const Shared& sh; const Params& p; int own0, own, ga, pair0, group_xg; uint32_t xs, xg;
+      __device__ __forceinline__ int rows(int tile, int64_t (&row)[4], int (&off)[4], int64_t& base) const {
+        const int e = sh.groups[sh.tiles[tile].group].expert, r = STRIP * sh.tiles[tile].strip, g = (threadIdx.x & 31) >> 2, left = own - r;
+        const int64_t first = (int64_t)e * p.w_rows;
+        base = e * p.s_expert;
 #pragma unroll
-    for (int i = 0; i < RING1 - 1; ++i) fetch_codes(ring + i * SLOT1);
-    fetch_scales(raw[0]);
-    fetch_scales(raw[1]);
+        for (int i = 0; i < 4; ++i) {
+          // up: rows 0 to 15 of the tile are gate rows, 16 to 31 up rows, which lie N behind them
+          off[i] = UP ? r + g + 8 * (i & 1) + (i >> 1) * p.N : own0 + r + min(g + 8 * i, left - 1);
+          row[i] = first + off[i];
+        }
+        return UP || left > 16 ? 2 : 1;
+      }
+      __device__ __forceinline__ void columns(int tile, uint32_t (&at)[1], uint32_t& x) const {
+        const int gi = sh.tiles[tile].group, lane = threadIdx.x & 31;
+        const Group gr = sh.groups[gi];
+        at[0] = xs + (gr.first - pair0 + min(lane >> 2, gr.count - 1)) * (p.steps * 256);      // columns beyond the group's repeat its last: nobody looks at them
+        x = xg + (gi - ga) * group_xg * 4 + 8 * (lane & 3);
+      }
+    } of{sh, p, own0, own, ga, pair0, group_xg, smem_addr(xs), smem_addr(xg)};
+    Stream<VEC, 1, BF16, PART, Tiles> stream(p.w, of, p.K, steps, 0, u0, u1, ring);
+    stream.load(ring);
 
     // ---- columns ----
     auto source = [&](int c) {
@@ -209,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
         }
       }
     } else {
-      const int n = p.K / 8;
+      const int n = p.K / 16;
       for (int c = warp; c < columns; c += WARPS) {
         const uint32_t* from = p.h_max + (int64_t)sh.pairs[pair0 + c] * n;
         uint32_t mx = 0;
@@ -227,92 +211,53 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
         const int i = base + a * THREADS + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv), at = i - c * per;
         if ((i & ~31) >= total) break;
         float sum = 0.f;
-        if (i < total)
-          *reinterpret_cast<uint4*>(xs + ((size_t)c * steps + (at >> 4)) * 256 + eight_at(at & 15, c)) = scaled_eight<BF16>(v[a], pow2(row_shift<BF16>(sh.max[c])), sum);
+        int local = 0, gi = ga;                            // the column's place in its group
+        if (i < total) {
+          while (gi + 1 < gb && pair0 + c >= sh.groups[gi + 1].first) ++gi;
+          local = pair0 + c - sh.groups[gi].first;
+          *reinterpret_cast<uint4*>(xs + ((size_t)c * steps + (at >> 4)) * 256 + eight_at(at & 15, local)) = scaled_eight<BF16>(v[a], pow2(row_shift<BF16>(sh.max[c])), sum);
+        }
 #pragma unroll
         for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (i < total && at % (G / 8) == 0) xg[c * steps * GS + at / (G / 8)] = sum * 5.9604644775390625e-8f;      // 2^-24
+        if (i < total && at % (G / 8) == 0) xg[(gi - ga) * group_xg + at / (G / 8) * TOK + local] = sum * 5.9604644775390625e-8f;      // 2^-24
       }
     }
     __syncthreads();
 
     // ---- products ----
-    float sum[1][1][4] = {{{0.f, 0.f, 0.f, 0.f}}};
-    uint32_t packed[2], slot = ring, column = 0, xg_at[2] = {0, 0};
-    int tile = u0 / steps, s = u0 - tile * steps, used = 4;
-    bool fresh = true;                                     // a new tile
-    for (int u = u0; u < u1; ++u) {
-      if (fresh) {
-        const Group gr = sh.groups[(b0 + tile) / strips];
-        const int c0 = gr.first - pair0, c = c0 + min(g, gr.count - 1);      // columns beyond the group's repeat its last: nobody looks at them
-        column = smem_addr(xs) + c * steps * 256;
-        for (int i = 0; i < 2; ++i) xg_at[i] = smem_addr(xg) + (c0 + min(2 * t + i, gr.count - 1)) * steps * GS * 4;
-        column |= (uint32_t)(c & 1);                       // parity of the column, by which its eights are permuted
-        fresh = false;
-      }
-      copy_wait<RING1 - 2>();
-      __syncwarp();
-      fetch_codes(slot == ring ? ring + (RING1 - 1) * SLOT1 : slot - SLOT1);
-      if (used == 4) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) packed[i] = pack_scale(raw[0].s[i], raw[0].z[i]);
-        raw[0] = raw[1];
-        fetch_scales(raw[1]);
-        used = 0;
-      }
-      multiply_column<VEC, BF16>(sum[0][0], slot, ln, (column & ~1u) + s * 256, ((column ^ (uint32_t)g) & 1u) << 6, xg_at[0] + s * GS * 4, xg_at[1] + s * GS * 4, packed, used);
-      used += GS;
-      slot = slot == ring + (RING1 - 1) * SLOT1 ? ring : slot + SLOT1;
-      if (++s == steps || u + 1 == u1) {
-        flush<1, 1>(sum, slots + (tile + warp) * 16 * TOK);
-        ++tile;
-        s = 0;
-        used = 4;
-        fresh = true;
-      }
-    }
-    copy_wait<0>();
+    stream.run(256, GS * TOK * 4, slots, warp);
     __syncthreads();
 
     // ---- sums of warps in their order ----
     auto total_of = [&](int tl, int r, int c) {            // row r of tile tl, column c of its group
-      const int first = tl * steps / run, last = ((tl + 1) * steps - 1) / run;
-      const float* from = slots + (tl * 16 + r) * TOK + c;
+      const float* from = slots + (tl * ROWS + r) * TOK + c;
       float f = 0.f;
-      for (int w = first; w <= last; ++w) f += from[w * 16 * TOK];
+      for (int w = sh.tiles[tl].first; w <= sh.tiles[tl].last; ++w) f += from[w * ROWS * TOK];
       return f;
     };
     if constexpr (UP) {
-      // eight lanes a column: its outputs in this tile
-      for (int i = threadIdx.x; i < tiles * 64; i += THREADS) {
-        const int tl = i >> 6, c = (i >> 3) & 7, r = i & 7, id = b0 + tl, gi = id / strips, st = id - gi * strips;
-        const Group gr = sh.groups[gi];
-        float hv = 0.f;
-        const bool valid = c < gr.count;
-        int pair = 0;
-        if (valid) {
-          pair = sh.pairs[gr.first + c];
-          const int shift = row_shift<BF16>(sh.max[gr.first - pair0 + c]);
-          const float gate = unshift(total_of(tl, r, c), shift), up = unshift(total_of(tl, r + 8, c), shift);
-          hv = gate / (1.f + expf(-gate)) * up;
-        }
-        const uint16_t bits = to_half<BF16>(hv);
+      // sixteen lanes a column: its outputs in this tile
+      for (int i = threadIdx.x; i < tiles * 128; i += THREADS) {
+        const int tl = i >> 7, c = (i >> 4) & 7, r = i & 15;
+        const Group gr = sh.groups[sh.tiles[tl].group];
+        if (c >= gr.count) continue;                       // whole half warps
+        const int pair = sh.pairs[gr.first + c], shift = row_shift<BF16>(sh.max[gr.first - pair0 + c]), st = sh.tiles[tl].strip;
+        const float gate = unshift(total_of(tl, r, c), shift), up = unshift(total_of(tl, r + 16, c), shift);
+        const uint16_t bits = to_half<BF16>(gate / (1.f + expf(-gate)) * up);
         uint32_t mx = bits & 0x7FFFu;
+        const uint32_t half = 0xFFFFu << (lane & 16);
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (valid) {
-          p.h[(int64_t)pair * p.N + 8 * st + r] = bits;
-          if (r == 0) p.h_max[(int64_t)pair * (p.N / 8) + st] = mx;
-        }
+        for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(half, mx, o));
+        p.h[(int64_t)pair * p.N + 16 * st + r] = bits;
+        if (r == 0) p.h_max[(int64_t)pair * (p.N / 16) + st] = mx;
       }
     } else if constexpr (!OWN) {
-      for (int i = threadIdx.x; i < tiles * 128; i += THREADS) {
-        const int tl = i >> 7, c = (i >> 4) & 7, r = i & 15, id = b0 + tl, gi = id / strips, st = id - gi * strips;
-        const Group gr = sh.groups[gi];
-        if (c < gr.count && 16 * st + r < p.N) {
-          const int pair = sh.pairs[gr.first + c];
-          p.y[(int64_t)pair * p.N + 16 * st + r] = __ldcg(p.weights + pair) * unshift(total_of(tl, r, c), row_shift<BF16>(sh.max[gr.first - pair0 + c]));
-        }
+      for (int i = threadIdx.x; i < tiles * 256; i += THREADS) {
+        const int tl = i >> 8, c = (i >> 5) & 7, r = i & 31, n = 32 * sh.tiles[tl].strip + r;
+        const Group gr = sh.groups[sh.tiles[tl].group];
+        if (c >= gr.count || n >= p.N) continue;
+        const int pair = sh.pairs[gr.first + c];
+        p.y[(int64_t)pair * p.N + n] = __ldcg(p.weights + pair) * unshift(total_of(tl, r, c), row_shift<BF16>(sh.max[gr.first - pair0 + c]));
       }
     } else {
       for (int i = threadIdx.x; i < p.T * own; i += THREADS) {
@@ -326,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
             const int mid = (lo + hi) / 2;
             if (sh.groups[mid].first <= at) lo = gi = mid; else hi = mid;
           }
-          f = fmaf(__ldcg(p.weights + pair), unshift(total_of(gi * strips + (r >> 4), r & 15, at - sh.groups[gi].first), row_shift<BF16>(sh.max[at])), f);
+          f = fmaf(__ldcg(p.weights + pair), unshift(total_of(gi * strips + (r >> 5), r & 31, at - sh.groups[gi].first), row_shift<BF16>(sh.max[at])), f);
         }
         p.out[(int64_t)m * p.N + own0 + r] = to_half<BF16>(f);
       }
@@ -353,19 +298,25 @@ template <bool BF16> __global__ void __launch_bounds__(256) g4_pairs_sum_kernel(
 
 // ---- host ----
 struct Plan { int up_columns, down_columns, smem_up, smem_down; bool own, fits; };
-static int column_bytes(int K, int G) { const int steps = (K + STEP - 1) / STEP; return steps * (256 + STEP / G * 4); }
+// Columns and groups that shared memory has room for, one group for two columns and one more.
+static int groups_of(int columns) { return columns / 2 + 1; }
+static int bytes_of(int columns, int K, int G) { const int steps = (K + STEP - 1) / STEP; return columns * steps * 256 + groups_of(columns) * steps * (STEP / G) * TOK * 4; }
+static int room_for(int most, int K, int G, int room) {
+  int n = most;
+  while (n > 0 && bytes_of(n, K, G) > room) --n;
+  return n;
+}
 static Plan plan(const G4MoeArgs& a) {
   Plan q{};
-  const int fixed = WARPS * RING1 * SLOT1 + (CAP + WARPS) * 16 * TOK * 4 + 16, room = SMEM - fixed;
-  const int pairs = a.T * a.k;
-  q.up_columns = std::min(room / column_bytes(a.H, a.G13), pairs);
-  q.down_columns = std::min(room / column_bytes(a.I, a.G2), pairs);
-  // a column's index and its eights stay below 2^17
-  q.fits = pairs <= MAX_PAIRS && std::min(pairs, TOK) <= q.up_columns && std::min(pairs, TOK) <= q.down_columns && a.H % 8 == 0;
-  const int strips = ((a.H + sm_count() - 1) / sm_count() + 15) / 16;
-  q.own = q.down_columns == pairs && pairs * strips <= CAP && (int64_t)pairs * a.I <= 16384;
-  q.smem_up = fixed + q.up_columns * column_bytes(a.H, a.G13);
-  q.smem_down = fixed + q.down_columns * column_bytes(a.I, a.G2);
+  const int fixed = WARPS * WARP_BYTES + (CAP + WARPS) * ROWS * TOK * 4, room = SMEM - fixed, pairs = a.T * a.k;
+  if (pairs > MAX_PAIRS) return q;
+  q.up_columns = room_for(pairs, a.H, a.G13, room);
+  q.down_columns = room_for(pairs, a.I, a.G2, room);
+  q.fits = std::min(pairs, TOK) <= q.up_columns && std::min(pairs, TOK) <= q.down_columns;
+  const int strips = ((a.H + sm_count() - 1) / sm_count() + ROWS - 1) / ROWS;
+  q.own = q.down_columns == pairs && groups_of(pairs) >= pairs && pairs * strips <= CAP && (int64_t)pairs * a.I <= 16384;
+  q.smem_up = fixed + bytes_of(q.up_columns, a.H, a.G13);
+  q.smem_down = fixed + bytes_of(q.down_columns, a.I, a.G2);
   return q;
 }
 template <int VEC, bool BF16, bool UP, bool OWN, bool PART> static int launch(const Params& p, int smem, cudaStream_t st) {
@@ -399,7 +350,7 @@ bool moe_g4_few_preferred(const G4MoeArgs& a) { return g4f::plan(a).fits && a.T 
 
 size_t moe_g4_few_bytes(const G4MoeArgs& a) {
   const size_t pairs = (size_t)a.T * a.k;
-  return g4f::align_up(pairs * a.I * 2) + g4f::align_up(pairs * (a.I / 8) * 4) + g4f::align_up(pairs * a.H * 4);
+  return g4f::align_up(pairs * a.I * 2) + g4f::align_up(pairs * (a.I / 16) * 4) + g4f::align_up(pairs * a.H * 4);
 }
 
 int moe_g4_few(const G4MoeArgs& a, void* scratch, cudaStream_t st) {
@@ -410,20 +361,19 @@ int moe_g4_few(const G4MoeArgs& a, void* scratch, cudaStream_t st) {
   Params p{};
   p.ids = a.ids; p.weights = a.weights; p.T = a.T; p.E = a.E; p.k = a.k;
   p.h = reinterpret_cast<uint16_t*>(at); at += align_up(pairs * a.I * 2);
-  p.h_max = reinterpret_cast<uint32_t*>(at); at += align_up(pairs * (a.I / 8) * 4);
+  p.h_max = reinterpret_cast<uint32_t*>(at); at += align_up(pairs * (a.I / 16) * 4);
   p.y = reinterpret_cast<float*>(at);
   p.out = reinterpret_cast<uint16_t*>(a.out);
-  p.early = tls().overlap_mode == 2;
   p.x = reinterpret_cast<const uint16_t*>(a.x);
   p.w = Matrix{a.w13, reinterpret_cast<const uint16_t*>(a.s13), a.z13, a.H / 2, 2 * (int64_t)a.I};
-  p.w_expert = (int64_t)a.I * a.H; p.s_expert = (int64_t)(a.H / a.G13) * 2 * a.I;
-  p.N = a.I; p.K = a.H; p.steps = (a.H + STEP - 1) / STEP; p.columns = q.up_columns;
+  p.w_rows = 2 * (int64_t)a.I; p.s_expert = (int64_t)(a.H / a.G13) * 2 * a.I;
+  p.N = a.I; p.K = a.H; p.steps = (a.H + STEP - 1) / STEP; p.columns = q.up_columns; p.groups = groups_of(q.up_columns);
   int rc = by_type<true, false>(p, a.bf16, a.G13, q.smem_up, st);
   if (rc) return rc;
   p.x = p.h;
   p.w = Matrix{a.w2, reinterpret_cast<const uint16_t*>(a.s2), a.z2, a.I / 2, a.H};
-  p.w_expert = (int64_t)a.H * a.I / 2; p.s_expert = (int64_t)(a.I / a.G2) * a.H;
-  p.N = a.H; p.K = a.I; p.steps = (a.I + STEP - 1) / STEP; p.columns = q.down_columns;
+  p.w_rows = a.H; p.s_expert = (int64_t)(a.I / a.G2) * a.H;
+  p.N = a.H; p.K = a.I; p.steps = (a.I + STEP - 1) / STEP; p.columns = q.down_columns; p.groups = groups_of(q.down_columns);
   if (q.own) return by_type<false, true>(p, a.bf16, a.G2, q.smem_down, st);
   rc = by_type<false, false>(p, a.bf16, a.G2, q.smem_down, st);
   if (rc) return rc;
