@@ -1,7 +1,7 @@
 // Linear of a few tokens on 4-bit group-quantised weights: out[m, n] = sum_g s[g, n] (sum_k x[m, k] q[n, k] - z[g, n] X[m, g]) (+ bias[n]).
 //
 // HBM-bound: the weights are read once, and there is little time to convert them (g4_stream.cuh has the mathematics and the layout).  A CTA per SM has rows of its own, dealt
-// out evenly.  Its units (32 rows of 128 k each) go to its twelve warps in equal runs; a warp's next units are on their way while one is multiplied, and
+// out evenly.  Its units (32 rows of 128 k each) go to its warps in equal runs; a warp's next units are on their way while one is multiplied, and
 // nothing in the loop waits for another warp.  A warp leaves its sums of a tile of rows in a slot of shared memory; at the end they are added up in the
 // order of warps, so that results are the same every time.
 //
@@ -15,7 +15,7 @@
 
 namespace b2q {
 namespace g4s {
-constexpr int WARPS = 12, THREADS = 32 * WARPS;
+constexpr int MOST_WARPS = 16, THREADS = 32 * MOST_WARPS;      // sixteen warps, or twelve where that many tokens leave no room for more
 constexpr int SELF = 4;                                    // eights that a thread prepares at most where a CTA prepares the tokens itself
 enum { ST_IMAGE = 901 };
 
@@ -93,10 +93,10 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
   const int cluster = blockIdx.x / C, clusters = gridDim.x / C;
   const int s0 = rank * p.steps / (int)C, s1 = (rank + 1) * p.steps / (int)C, steps = s1 - s0;
   const int sb = step_bytes(p.M, G, TT);
-  uint8_t* xs = smem + WARPS * WARP_BYTES;                 // [steps][step_bytes]
+  uint8_t* xs = smem + blockDim.x / 32 * WARP_BYTES;       // [steps][step_bytes]
   float* slots = reinterpret_cast<float*>(xs + (p.steps + C - 1) / C * sb);      // [tiles + WARPS][ROWS][TOK]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int WARPS = blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int r0 = (int)((int64_t)cluster * p.N / clusters), rows = (int)((int64_t)(cluster + 1) * p.N / clusters) - r0;
   const int tiles = (rows + ROWS - 1) / ROWS, units = tiles * steps;
   const int run = (units + WARPS - 1) / WARPS, u0 = min(units, warp * run), u1 = min(units, u0 + run);
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
   if (!p.early) grid_dep_wait();
   struct Tiles {
     int r0, nrows, g, t, M; uint32_t xs;
-    __device__ __forceinline__ int rows(int tile, int64_t (&row)[4], int (&off)[4], int64_t& base) const {
+    __device__ __forceinline__ int rows(int tile, int64_t (&row)[4], uint32_t (&off)[4], int64_t& base) const {
       base = r0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) { off[i] = min(ROWS * tile + g + 8 * i, nrows - 1); row[i] = r0 + off[i]; }
@@ -142,15 +142,15 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
     const int per = steps * (STEP / 8), total = p.M * per;
     const uint32_t inv = 0xFFFFFFFFu / (uint32_t)per + 1;  // i / per = i * inv >> 32 for i < 2^17, 1 < per < 2^14
     uint4 v[SELF];
-    for (int i = threadIdx.x; i < steps * GS * TOK; i += THREADS) reinterpret_cast<float*>(xs + i / (GS * TOK) * sb + p.M * STEP * 2)[i % (GS * TOK)] = 0.f;
+    for (int i = threadIdx.x; i < steps * GS * TOK; i += blockDim.x) reinterpret_cast<float*>(xs + i / (GS * TOK) * sb + p.M * STEP * 2)[i % (GS * TOK)] = 0.f;
 #pragma unroll
     for (int a = 0; a < SELF; ++a) {
-      const int i = a * THREADS + threadIdx.x, m = (int)__umulhi((uint32_t)i, inv), k = 8 * (i - m * per);
+      const int i = a * blockDim.x + threadIdx.x, m = (int)__umulhi((uint32_t)i, inv), k = 8 * (i - m * per);
       v[a] = i < total && k < p.K ? ld_eight(p.x + m * p.ldx + k, p.vec) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int a = 0; a < SELF; ++a) {
-      const int i = a * THREADS + threadIdx.x, m = (int)__umulhi((uint32_t)i, inv);
+      const int i = a * blockDim.x + threadIdx.x, m = (int)__umulhi((uint32_t)i, inv);
       if ((i & ~31) >= total) break;                       // whole warps
       uint32_t mx = max_bits(v[a]);                        // a half warp has one token, since `per` is a multiple of 16
 #pragma unroll
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
     if (threadIdx.x < p.M) shifts[threadIdx.x] = row_shift<BF16>(row_max[threadIdx.x]);
 #pragma unroll
     for (int a = 0; a < SELF; ++a) {
-      const int i = a * THREADS + threadIdx.x, m = (int)__umulhi((uint32_t)i, inv);
+      const int i = a * blockDim.x + threadIdx.x, m = (int)__umulhi((uint32_t)i, inv);
       if ((i & ~31) >= total) break;
       put_eight<G, TT, BF16>(xs, p.M, m, i - m * per, v[a], pow2(row_shift<BF16>(row_max[i < total ? m : 0])), i < total);
     }
@@ -210,23 +210,27 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
 
 // ---- host ----
 constexpr int SMEM = 220 * 1024;
-struct Plan { int C, clusters, cap, smem, tt, steps; bool self; };
+struct Plan { int C, clusters, cap, smem, tt, steps, warps; bool self; };
 // Clusters of four that the SMs hold at a time: not all of them can be in one.
 static int resident(int C) { return C == 4 ? sm_count() * 7 / 32 : sm_count() / C; }
 static Plan plan(int M, int N, int K, int G) {
   Plan q{};
   q.steps = (K + STEP - 1) / STEP;
   q.tt = M <= 8 ? 1 : 2;
-  q.self = M * q.steps * (STEP / 8) <= SELF * THREADS;
   for (q.C = 1; q.C <= 4; q.C *= 2) {
-    if (q.C > 1 && (q.self || q.C > q.steps)) break;
+    if (q.C > q.steps) break;
     q.clusters = resident(q.C);
     if (q.clusters > (N + 7) / 8) q.clusters = (N + 7) / 8;
     const int rows = (N + q.clusters - 1) / q.clusters, most = (q.steps + q.C - 1) / q.C;
     q.cap = (rows + ROWS - 1) / ROWS;
-    const int64_t front = (int64_t)WARPS * WARP_BYTES + (int64_t)most * step_bytes(M, G, q.tt);
-    const int64_t smem = front + (int64_t)(q.cap + WARPS) * ROWS * 8 * q.tt * 4;
-    if (smem <= SMEM && (q.C == 1 || (int64_t)M * rows * 4 <= front)) { q.smem = (int)smem; return q; }
+    // (fewer where there is little for each to do: 1 x 2048 x 2048 4.6 us with sixteen, 4.15 with twelve; 1 x 28672 x 8192 28.1 and 30.4)
+    for (q.warps = q.cap * most >= 4 * MOST_WARPS ? MOST_WARPS : 12; q.warps >= 12; q.warps -= 4) {
+      const int64_t front = (int64_t)q.warps * WARP_BYTES + (int64_t)most * step_bytes(M, G, q.tt);
+      const int64_t smem = front + (int64_t)(q.cap + q.warps) * ROWS * 8 * q.tt * 4;
+      q.self = M * q.steps * (STEP / 8) <= SELF * 32 * q.warps;
+      if (q.self && q.C > 1) break;
+      if (smem <= SMEM && (q.C == 1 || (int64_t)M * rows * 4 <= front)) { q.smem = (int)smem; return q; }
+    }
   }
   return q;
 }
@@ -247,7 +251,7 @@ template <int VEC, int TT, bool BF16, bool PART> static int launch(Params& p, co
     if (dev < 16) configured[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(q.clusters * q.C); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = q.smem; cfg.stream = st;
+  cfg.gridDim = dim3(q.clusters * q.C); cfg.blockDim = dim3(32 * q.warps); cfg.dynamicSmemBytes = q.smem; cfg.stream = st;
   cudaLaunchAttribute at[2];
   int n = 0;
   if (q.C > 1) {

@@ -183,7 +183,8 @@ template <int VEC, int TT, bool BF16, bool PART, typename Tiles> struct Stream {
   uint32_t ring;
   // of the two steps that are loaded next: where this lane copies from, and its scales
   const uint8_t* p[4];
-  int64_t base; int off[4], tile, s, n, halves;
+  const uint16_t* scales; const uint8_t* zeros; uint32_t off[4];
+  int tile, s, n, halves;
   uint32_t raw_s[SETS][4], raw_z[SETS][4];
 
   __device__ __forceinline__ Stream(const Matrix& m_, Tiles& tiles_, int K_, int steps_, int s0_, int u0_, int u1_, uint32_t ring_)
@@ -195,8 +196,10 @@ template <int VEC, int TT, bool BF16, bool PART, typename Tiles> struct Stream {
   }
   __device__ __forceinline__ void enter() {                // the tile's rows, from step s on
     const int t = threadIdx.x & 3;
-    int64_t row[4];
+    int64_t row[4], base;
     halves = tiles.rows(tile, row, off, base);
+    scales = m.s + base;
+    zeros = m.z + base;
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[i] = m.w + row[i] * m.half + (s0 + s) * (STEP / 2) + 16 * t;
     n = min(2, min(steps - s, u1 - u));
@@ -220,14 +223,14 @@ template <int VEC, int TT, bool BF16, bool PART, typename Tiles> struct Stream {
       const int g0 = (s0 + s) * GS, last = min(K / G - 1 - g0, n * GS - 1);
 #pragma unroll
       for (int q = 0; q < SETS; ++q) {
-        const int64_t at = base + (int64_t)(g0 + min(4 * q + t, last)) * m.n;
+        const uint32_t at = (uint32_t)(g0 + min(4 * q + t, last)) * (uint32_t)m.n;      // within a matrix's scales, below 2^31
 #pragma unroll
-        for (int i = 0; i < 4; ++i) raw_s[q][i] = ld_scale(m.s + at + off[i]);
+        for (int i = 0; i < 4; ++i) raw_s[q][i] = ld_scale(scales + (at + off[i]));
 #pragma unroll
         for (int i = 0; i < 4; ++i) raw_z[q][i] = 8;
         if (m.z) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) raw_z[q][i] = ld_zero(m.z + at + off[i]);
+          for (int i = 0; i < 4; ++i) raw_z[q][i] = ld_zero(zeros + (at + off[i]));
         }
       }
     }

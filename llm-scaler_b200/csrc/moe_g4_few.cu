@@ -2,7 +2,7 @@
 // tokens are more than a handful.
 //
 // HBM-bound for a batch, a chain of latencies for one token.  Every CTA sorts the routes by itself, in shared memory: the pairs (token, slot) of an expert form groups of
-// up to eight, whose tokens are the columns of one MMA.  A tile is 32 weight rows of one group; CTAs have equal runs of the tiles of all groups, and their twelve
+// up to eight, whose tokens are the columns of one MMA.  A tile is 32 weight rows of one group; CTAs have equal runs of the tiles of all groups, and their
 // warps equal runs of the tiles' steps of 128 k, as in the linear.
 //  * up: a tile has sixteen gate rows and the sixteen up rows of the same outputs; h = silu(gate) * up goes out in 16 bits, with its largest magnitude per tile, from which the
 //    second kernel takes the power of two that it scales a row of h by.
@@ -15,7 +15,8 @@
 namespace b2q {
 namespace g4f {
 using namespace g4s;
-constexpr int WARPS = 12, THREADS = 32 * WARPS, MAX_PAIRS = THREADS, MAX_E = 1024, PER = (MAX_E + THREADS - 1) / THREADS, TOK = 8;
+constexpr int MOST_WARPS = 16, LEAST_WARPS = 12, THREADS = 32 * MOST_WARPS;      // as many as leave room for the columns
+constexpr int MAX_PAIRS = 32 * LEAST_WARPS, MAX_E = 1024, PER = (MAX_E + 32 * LEAST_WARPS - 1) / (32 * LEAST_WARPS), TOK = 8;
 constexpr int CAP = 24;                                    // tiles that are summed up at a time
 constexpr int SMEM = 208 * 1024;                           // beside the routes'
 
@@ -36,7 +37,7 @@ struct alignas(16) Shared {
   int16_t pairs[MAX_PAIRS];                                // sorted by expert
   int16_t place[MAX_PAIRS];                                // of a pair among the sorted; -1: no expert
   Group groups[MAX_PAIRS];
-  int warp_sum[WARPS][2];
+  int warp_sum[MOST_WARPS][2];
   int n_groups;
   uint32_t max[MAX_PAIRS];                                 // of a staged column's row
   struct { int16_t group, strip, first, last; } tiles[CAP];      // of a batch; warps that have units of it
@@ -45,7 +46,7 @@ struct alignas(16) Shared {
 // The routes' pairs sorted by expert, those of an expert by their number: all CTAs of both kernels have to agree on which group a pair is in.
 __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
   const int n = p.T * p.k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e < p.E; e += THREADS) sh.count[e] = 0;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) sh.count[e] = 0;
   __syncthreads();
   int id = -1, at = 0;
   if (threadIdx.x < n) {
@@ -53,7 +54,7 @@ __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
     if ((uint32_t)id >= (uint32_t)p.E) id = -1;
     if (id >= 0) atomicAdd(&sh.count[id], 1);
   }
-  sh.ids[threadIdx.x] = id;
+  if (threadIdx.x < MAX_PAIRS) sh.ids[threadIdx.x] = id;
   __syncthreads();
   if (id >= 0) {
     for (int j = 0; j < (int)threadIdx.x; j += 4) {
@@ -79,7 +80,7 @@ __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
   if (lane == 31) { sh.warp_sum[warp][0] = pairs; sh.warp_sum[warp][1] = groups; }
   __syncthreads();
   for (int w = 0; w < warp; ++w) { pairs += sh.warp_sum[w][0]; groups += sh.warp_sum[w][1]; }
-  if (threadIdx.x == THREADS - 1) sh.n_groups = groups;
+  if (threadIdx.x == blockDim.x - 1) sh.n_groups = groups;
   int first = pairs - own_pairs, to_group = groups - own_groups;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
   constexpr int G = 32 * VEC, GS = STEP / G;               // groups of k in a step
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Shared sh;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int WARPS = blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int steps = p.steps, group_xg = steps * GS * TOK;  // group sums of a group's columns: [steps * GS][8]
   uint8_t* xs = smem + WARPS * WARP_BYTES;                 // [columns][steps][256], then [groups][group_xg]
   float* xg = reinterpret_cast<float*>(xs + (size_t)p.columns * steps * 256);
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
     __syncthreads();
     struct Tiles {
       const Shared& sh; const Params& p; int own0, own, ga, pair0, group_xg; uint32_t xs, xg;
-      __device__ __forceinline__ int rows(int tile, int64_t (&row)[4], int (&off)[4], int64_t& base) const {
+      __device__ __forceinline__ int rows(int tile, int64_t (&row)[4], uint32_t (&off)[4], int64_t& base) const {
         const int e = sh.groups[sh.tiles[tile].group].expert, r = STRIP * sh.tiles[tile].strip, g = (threadIdx.x & 31) >> 2, left = own - r;
         const int64_t first = (int64_t)e * p.w_rows;
         base = e * p.s_expert;
@@ -173,18 +174,18 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
     auto fetch_x = [&](int base) {
 #pragma unroll
       for (int a = 0; a < V; ++a) {
-        const int i = base + a * THREADS + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv), at = 8 * (i - c * per);
+        const int i = base + a * blockDim.x + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv), at = 8 * (i - c * per);
         v[a] = i < total && at < p.K ? ld_eight(source(c) + at, true) : make_uint4(0, 0, 0, 0);
       }
     };
     if (UP) {
-      for (int c = threadIdx.x; c < columns; c += THREADS) sh.max[c] = 0;
+      for (int c = threadIdx.x; c < columns; c += blockDim.x) sh.max[c] = 0;
       __syncthreads();
-      for (int base = 0; base < total; base += V * THREADS) {
+      for (int base = 0; base < total; base += V * blockDim.x) {
         fetch_x(base);
 #pragma unroll
         for (int a = 0; a < V; ++a) {
-          const int i = base + a * THREADS + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv);
+          const int i = base + a * blockDim.x + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv);
           if ((i & ~31) >= total) break;                   // whole warps
           uint32_t mx = max_bits(v[a]);                    // a half warp has one column, since `per` is a multiple of 16
 #pragma unroll
@@ -201,14 +202,14 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
         mx = __reduce_max_sync(0xffffffffu, mx);
         if (lane == 0) sh.max[c] = mx;
       }
-      if (total <= V * THREADS) fetch_x(0);
+      if (total <= V * blockDim.x) fetch_x(0);
     }
     __syncthreads();
-    for (int base = 0; base < total; base += V * THREADS) {
-      if (total > V * THREADS) fetch_x(base);
+    for (int base = 0; base < total; base += V * blockDim.x) {
+      if (total > V * blockDim.x) fetch_x(base);
 #pragma unroll
       for (int a = 0; a < V; ++a) {
-        const int i = base + a * THREADS + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv), at = i - c * per;
+        const int i = base + a * blockDim.x + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv), at = i - c * per;
         if ((i & ~31) >= total) break;
         float sum = 0.f;
         int local = 0, gi = ga;                            // the column's place in its group
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
     };
     if constexpr (UP) {
       // sixteen lanes a column: its outputs in this tile
-      for (int i = threadIdx.x; i < tiles * 128; i += THREADS) {
+      for (int i = threadIdx.x; i < tiles * 128; i += blockDim.x) {
         const int tl = i >> 7, c = (i >> 4) & 7, r = i & 15;
         const Group gr = sh.groups[sh.tiles[tl].group];
         if (c >= gr.count) continue;                       // whole half warps
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
         if (r == 0) p.h_max[(int64_t)pair * (p.N / 16) + st] = mx;
       }
     } else if constexpr (!OWN) {
-      for (int i = threadIdx.x; i < tiles * 256; i += THREADS) {
+      for (int i = threadIdx.x; i < tiles * 256; i += blockDim.x) {
         const int tl = i >> 8, c = (i >> 5) & 7, r = i & 31, n = 32 * sh.tiles[tl].strip + r;
         const Group gr = sh.groups[sh.tiles[tl].group];
         if (c >= gr.count || n >= p.N) continue;
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
         p.y[(int64_t)pair * p.N + n] = __ldcg(p.weights + pair) * unshift(total_of(tl, r, c), row_shift<BF16>(sh.max[gr.first - pair0 + c]));
       }
     } else {
-      for (int i = threadIdx.x; i < p.T * own; i += THREADS) {
+      for (int i = threadIdx.x; i < p.T * own; i += blockDim.x) {
         const int m = i / own, r = i - m * own;
         float f = 0.f;
         for (int q = 0; q < p.k; ++q) {
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
     b0 = b1;
   }
   if (OWN && sh.n_groups == 0) {                           // nobody has an expert
-    for (int i = threadIdx.x; i < p.T * own; i += THREADS) p.out[(int64_t)(i / own) * p.N + own0 + i % own] = 0;
+    for (int i = threadIdx.x; i < p.T * own; i += blockDim.x) p.out[(int64_t)(i / own) * p.N + own0 + i % own] = 0;
   }
 }
 
@@ -297,7 +298,7 @@ template <bool BF16> __global__ void __launch_bounds__(256) g4_pairs_sum_kernel(
 }
 
 // ---- host ----
-struct Plan { int up_columns, down_columns, smem_up, smem_down; bool own, fits; };
+struct Plan { int warps, up_columns, down_columns, smem_up, smem_down; bool own, fits; };
 // Columns and groups that shared memory has room for, one group for two columns and one more.
 static int groups_of(int columns) { return columns / 2 + 1; }
 static int bytes_of(int columns, int K, int G) { const int steps = (K + STEP - 1) / STEP; return columns * steps * 256 + groups_of(columns) * steps * (STEP / G) * TOK * 4; }
@@ -308,18 +309,23 @@ static int room_for(int most, int K, int G, int room) {
 }
 static Plan plan(const G4MoeArgs& a) {
   Plan q{};
-  const int fixed = WARPS * WARP_BYTES + (CAP + WARPS) * ROWS * TOK * 4, room = SMEM - fixed, pairs = a.T * a.k;
+  const int pairs = a.T * a.k, most = std::min(pairs, TOK);
   if (pairs > MAX_PAIRS) return q;
-  q.up_columns = room_for(pairs, a.H, a.G13, room);
-  q.down_columns = room_for(pairs, a.I, a.G2, room);
-  q.fits = std::min(pairs, TOK) <= q.up_columns && std::min(pairs, TOK) <= q.down_columns;
+  int fixed = 0;
+  for (q.warps = MOST_WARPS; q.warps >= LEAST_WARPS && !q.fits; q.warps -= 4) {
+    fixed = q.warps * WARP_BYTES + (CAP + q.warps) * ROWS * TOK * 4;
+    q.up_columns = room_for(pairs, a.H, a.G13, SMEM - fixed);
+    q.down_columns = room_for(pairs, a.I, a.G2, SMEM - fixed);
+    q.fits = most <= q.up_columns && most <= q.down_columns;
+  }
+  q.warps += 4;
   const int strips = ((a.H + sm_count() - 1) / sm_count() + ROWS - 1) / ROWS;
   q.own = q.down_columns == pairs && groups_of(pairs) >= pairs && pairs * strips <= CAP && (int64_t)pairs * a.I <= 16384;
   q.smem_up = fixed + bytes_of(q.up_columns, a.H, a.G13);
   q.smem_down = fixed + bytes_of(q.down_columns, a.I, a.G2);
   return q;
 }
-template <int VEC, bool BF16, bool UP, bool OWN, bool PART> static int launch(const Params& p, int smem, cudaStream_t st) {
+template <int VEC, bool BF16, bool UP, bool OWN, bool PART> static int launch(const Params& p, int warps, int smem, cudaStream_t st) {
   auto kern = g4_experts_kernel<VEC, BF16, UP, OWN, PART>;
   static thread_local bool configured[16] = {false};
   int dev = 0;
@@ -329,19 +335,19 @@ template <int VEC, bool BF16, bool UP, bool OWN, bool PART> static int launch(co
     if (dev < 16) configured[dev] = true;
   }
   const int grid = OWN ? std::min(sm_count(), p.N) : sm_count();
-  launch_overlapped(kern, dim3(grid), dim3(THREADS), smem, st, tls().overlap_mode > 0, p);
+  launch_overlapped(kern, dim3(grid), dim3(32 * warps), smem, st, tls().overlap_mode > 0, p);
   note_launch(UP ? "g4_experts_up" : "g4_experts_down");
   return launch_status();
 }
-template <bool UP, bool OWN> static int by_type(const Params& p, bool bf16, int G, int smem, cudaStream_t st) {
+template <bool UP, bool OWN> static int by_type(const Params& p, bool bf16, int G, int warps, int smem, cudaStream_t st) {
   const bool part = p.K % STEP != 0;                       // groups of 128 leave no part of a step
-  if (G == 128) return bf16 ? launch<4, true, UP, OWN, false>(p, smem, st) : launch<4, false, UP, OWN, false>(p, smem, st);
+  if (G == 128) return bf16 ? launch<4, true, UP, OWN, false>(p, warps, smem, st) : launch<4, false, UP, OWN, false>(p, warps, smem, st);
   if (G == 64) {
-    if (part) return bf16 ? launch<2, true, UP, OWN, true>(p, smem, st) : launch<2, false, UP, OWN, true>(p, smem, st);
-    return bf16 ? launch<2, true, UP, OWN, false>(p, smem, st) : launch<2, false, UP, OWN, false>(p, smem, st);
+    if (part) return bf16 ? launch<2, true, UP, OWN, true>(p, warps, smem, st) : launch<2, false, UP, OWN, true>(p, warps, smem, st);
+    return bf16 ? launch<2, true, UP, OWN, false>(p, warps, smem, st) : launch<2, false, UP, OWN, false>(p, warps, smem, st);
   }
-  if (part) return bf16 ? launch<1, true, UP, OWN, true>(p, smem, st) : launch<1, false, UP, OWN, true>(p, smem, st);
-  return bf16 ? launch<1, true, UP, OWN, false>(p, smem, st) : launch<1, false, UP, OWN, false>(p, smem, st);
+  if (part) return bf16 ? launch<1, true, UP, OWN, true>(p, warps, smem, st) : launch<1, false, UP, OWN, true>(p, warps, smem, st);
+  return bf16 ? launch<1, true, UP, OWN, false>(p, warps, smem, st) : launch<1, false, UP, OWN, false>(p, warps, smem, st);
 }
 static size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 }  // namespace g4f
@@ -368,14 +374,14 @@ int moe_g4_few(const G4MoeArgs& a, void* scratch, cudaStream_t st) {
   p.w = Matrix{a.w13, reinterpret_cast<const uint16_t*>(a.s13), a.z13, a.H / 2, 2 * (int64_t)a.I};
   p.w_rows = 2 * (int64_t)a.I; p.s_expert = (int64_t)(a.H / a.G13) * 2 * a.I;
   p.N = a.I; p.K = a.H; p.steps = (a.H + STEP - 1) / STEP; p.columns = q.up_columns; p.groups = groups_of(q.up_columns);
-  int rc = by_type<true, false>(p, a.bf16, a.G13, q.smem_up, st);
+  int rc = by_type<true, false>(p, a.bf16, a.G13, q.warps, q.smem_up, st);
   if (rc) return rc;
   p.x = p.h;
   p.w = Matrix{a.w2, reinterpret_cast<const uint16_t*>(a.s2), a.z2, a.I / 2, a.H};
   p.w_rows = a.H; p.s_expert = (int64_t)(a.I / a.G2) * a.H;
   p.N = a.H; p.K = a.I; p.steps = (a.I + STEP - 1) / STEP; p.columns = q.down_columns; p.groups = groups_of(q.down_columns);
-  if (q.own) return by_type<false, true>(p, a.bf16, a.G2, q.smem_down, st);
-  rc = by_type<false, false>(p, a.bf16, a.G2, q.smem_down, st);
+  if (q.own) return by_type<false, true>(p, a.bf16, a.G2, q.warps, q.smem_down, st);
+  rc = by_type<false, false>(p, a.bf16, a.G2, q.warps, q.smem_down, st);
   if (rc) return rc;
   const int64_t total = (int64_t)a.T * a.H, n = (total + 255) / 256;
   launch_overlapped(a.bf16 ? g4_pairs_sum_kernel<true> : g4_pairs_sum_kernel<false>, dim3((unsigned)std::min<int64_t>(n, 1184)), dim3(256), 0, st, tls().overlap_mode > 0, (const float*)p.y,

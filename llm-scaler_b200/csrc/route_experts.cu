@@ -5,7 +5,9 @@
 // the scores that a group's two best add up to.  So no rounding of the scores decides between two experts, and equal keys go to the lowest index.
 // Weights are fp32, of the scores without the bias.
 //
-// Latency-bound: a warp per token, its logits in registers, k rounds of a warp-wide maximum.
+// Latency-bound: a warp per token, its logits in registers, k rounds of a warp-wide maximum.  Scores are made in fp32 first, good to EPS; where no two
+// that the choice depends on are nearer to each other than their errors, it is the one of 64 bits, and only the other tokens are done again in those (in 64
+// bits throughout: 4093 tokens of 256 experts 24 us; see the table of cases for now).
 #include "g4.cuh"
 
 namespace b2q {
@@ -36,6 +38,183 @@ __device__ __forceinline__ double value_of(Key k) {        // of a key that is n
   return __longlong_as_double((long long)((k >> 63) ? k & ~(1ull << 63) : ~k));
 }
 
+// fp32 values as keys of 32 bits, in the same order; those of -inf and NaN are 0.
+__device__ __forceinline__ uint32_t key32(float v) {
+  if (!(v > -INFINITY)) return 0;
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value32(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7FFFFFFFu : ~k); }      // of a key that is not 0
+__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ Key as_key(double v, Key) { return key_of(v); }
+__device__ __forceinline__ uint32_t as_key(float v, uint32_t) { return key32(v); }
+__device__ __forceinline__ double value(Key k) { return value_of(k); }
+__device__ __forceinline__ float value(uint32_t k) { return value32(k); }
+
+// How far the fp32 keys may be off, relative to the larger of 1 and the key.  __expf is good to 2 + 1.17 |x| units of 2^-23, so that a sigmoid's p (1 - p) |x| of it is below 2^-23, the
+// quotient's two units are another 2^-23 at most, and the sums with 1 and with the bias are rounded to 2^-24.  A softmax has 2^-22 of its exponential and as much
+// of the sum of all, and 2^-21 at most of that sum's roundings.
+template <bool SIGMOID> constexpr float EPS = SIGMOID ? 4.76837158203125e-7f : 9.5367431640625e-7f;      // 2^-21, 2^-20
+
+// Values of experts lane + 32 j; `beyond` from E on.
+template <int PER> __device__ __forceinline__ void load_row(float (&v)[PER], const void* from, int64_t at, int dt, int E, float beyond) {
+  const int lane = threadIdx.x & 31;
+  if (dt == B2Q_F32) {
+    const float* q = reinterpret_cast<const float*>(from) + at;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v[j] = lane + 32 * j < E ? __ldcg(q + lane + 32 * j) : beyond;
+  } else {
+    const unsigned short* q = reinterpret_cast<const unsigned short*>(from) + at;
+    uint32_t raw[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) raw[j] = lane + 32 * j < E ? __ldcg(q + lane + 32 * j) : 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v[j] = lane + 32 * j < E ? scalar_from_raw(raw[j], dt) : beyond;
+  }
+}
+// exp and 1 / x of the two precisions; the fp32 ones are good to 2^-22, more or less.
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float exp_of(float x) { return __expf(x); }
+__device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
+__device__ __forceinline__ float inverse(float x) { return __fdividef(1.f, x); }
+
+// The choice of lane i < k, -1 where there is none, from keys (key: of experts lane + 32 j; gkey: what groups add up, with TOP2).  CHECK: returns false where keys that the choice
+// depends on are too near to each other.
+template <int PER, bool SIGMOID, bool GROUPS, bool TOP2, bool CHECK, typename K>
+__device__ __forceinline__ bool choose(K (&key)[PER], const K (&gkey)[TOP2 ? PER : 1], const Params& p, int& id) {
+  const int lane = threadIdx.x & 31;
+  bool sure = true;
+  auto apart = [](K a, K b, float times) {                 // a >= b, both there
+    const float x = (float)value(a), y = (float)value(b);
+    return x - y > times * EPS<SIGMOID> * fmaxf(1.f, fmaxf(fabsf(x), fabsf(y)));
+  };
+  if constexpr (GROUPS) {
+    K mine = 0;                                            // lane g: of group g
+    auto of_group = [&](K a, K b) {                        // the two largest of each lane
+      K best = warp_max(a);
+      if (TOP2 && p.size > 1) {
+        const uint32_t who = __ballot_sync(0xffffffffu, a == best);
+        if (lane == __ffs(who) - 1) a = b;
+        const K second = warp_max(a);
+        best = best && second ? as_key(value(best) + value(second), K{}) : 0;
+      }
+      return best;
+    };
+    if (p.size == 32) {                                    // a register each
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const K best = of_group(TOP2 ? gkey[TOP2 ? j : 0] : key[j], 0);
+        if (lane == j) mine = best;
+      }
+    } else {
+      for (int g = 0; g < p.groups; ++g) {
+        const int lo = g * p.size, hi = lo + p.size;
+        K a = 0, b = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const int e = lane + 32 * j;
+          const K c = e >= lo && e < hi ? (TOP2 ? gkey[TOP2 ? j : 0] : key[j]) : 0;
+          if (TOP2) b = max(b, min(a, c));
+          a = max(a, c);
+        }
+        const K best = of_group(a, b);
+        if (lane == g) mine = best;
+      }
+    }
+    uint32_t keep = 0;
+    K last = 0;
+    for (int i = 0; i < p.top_groups; ++i) {
+      const K best = warp_max(mine);
+      if (best == 0) break;
+      last = best;
+      const int g = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
+      keep |= 1u << g;
+      if (lane == g) mine = 0;
+    }
+    if (CHECK) {
+      const K next = warp_max(mine);
+      if (next) sure = apart(last, next, TOP2 ? 4.f : 2.f);
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int e = lane + 32 * j, g = p.size == 32 ? j : e / p.size;
+      if (e < p.E && !(keep >> g & 1u)) key[j] = 0;
+    }
+  }
+  id = -1;
+  K mine = 0;                                              // lane i: the key of its choice; lane k: of the best that is left
+  for (int i = 0; i < p.k + (CHECK ? 1 : 0); ++i) {
+    K best = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) best = max(best, key[j]);
+    best = warp_max(best);
+    if (best == 0) break;
+    if (CHECK && (lane == i || (i == 32 && lane == 31))) {
+      if (i == 32) sure = sure && apart(mine, best, 2.f);
+      else mine = best;
+    }
+    if (i == p.k) break;
+    uint32_t e = 0xFFFFu;
+#pragma unroll
+    for (int j = PER - 1; j >= 0; --j)
+      if (key[j] == best) e = lane + 32 * j;
+    e = __reduce_min_sync(0xffffffffu, e);
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (lane + 32 * j == (int)e) key[j] = 0;
+    if (lane == i) id = (int)e;
+  }
+  if (CHECK) {
+    const K next = __shfl_down_sync(0xffffffffu, mine, 1);
+    if (lane < 31 && mine && next) sure = sure && apart(mine, next, 2.f);
+  }
+  return sure;
+}
+
+// Scores in F, plus bias, of experts lane + 32 j.
+template <int PER, bool SIGMOID, bool BIAS, typename F> __device__ __forceinline__ void scores(F (&s)[PER], const float (&v)[PER], float mx, const Params& p) {
+  F sum = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (SIGMOID) s[j] = inverse((F)1 + exp_of(-(F)v[j]));
+    else { s[j] = exp_of((F)v[j] - (F)mx); sum += s[j]; }
+  }
+  if (!SIGMOID) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const F inv = (F)1 / sum;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) s[j] *= inv;
+  }
+  if (BIAS) {
+    float b[PER];
+    load_row<PER>(b, p.bias, 0, p.bias_dt, p.E, 0.f);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) s[j] += (F)b[j];
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (v[j] == -INFINITY) s[j] = -INFINITY;               // an expert that is masked out
+}
+template <int PER, bool SIGMOID, bool BIAS, bool GROUPS, bool TOP2, bool CHECK, typename F, typename K>
+__device__ __forceinline__ bool choose_by_scores(const float (&v)[PER], float mx, const Params& p, int& id) {
+  F s[PER];
+  scores<PER, SIGMOID, BIAS, F>(s, v, mx, p);
+  K key[PER], gkey[TOP2 ? PER : 1];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const K of_score = as_key(s[j], K{});
+    if (TOP2) gkey[TOP2 ? j : 0] = of_score;
+    key[j] = BIAS ? of_score : as_key((F)v[j], K{});
+  }
+  return choose<PER, SIGMOID, GROUPS, TOP2, CHECK, K>(key, gkey, p, id);
+}
+template <int PER, bool SIGMOID, bool BIAS, bool GROUPS, bool TOP2> __device__ __noinline__ int choose_exactly(const float (&v)[PER], float mx, const Params& p) {
+  int id;
+  choose_by_scores<PER, SIGMOID, BIAS, GROUPS, TOP2, false, double, Key>(v, mx, p, id);
+  return id;
+}
+
 template <int PER, bool SIGMOID, bool BIAS, bool GROUPS, bool TOP2>
 __global__ void __launch_bounds__(32 * WARPS) route_experts_kernel(const Params p) {
   const int lane = threadIdx.x & 31, t = blockIdx.x * WARPS + (threadIdx.x >> 5);
@@ -44,11 +223,7 @@ __global__ void __launch_bounds__(32 * WARPS) route_experts_kernel(const Params 
   if (t >= p.T) return;
   const int64_t row = (int64_t)t * p.ldl;
   float v[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int e = lane + 32 * j;
-    v[j] = e < p.E ? load_scalar(p.logits, row + e, p.dt) : -INFINITY;
-  }
+  load_row<PER>(v, p.logits, row, p.dt, p.E, -INFINITY);
   float mx = -INFINITY;
   bool bad = false;
 #pragma unroll
@@ -60,86 +235,19 @@ __global__ void __launch_bounds__(32 * WARPS) route_experts_kernel(const Params 
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   bad = __any_sync(0xffffffffu, bad) || mx == -INFINITY;
 
-  constexpr bool SCORES = BIAS || (GROUPS && TOP2);
-  double s[SCORES ? PER : 1];
-  if constexpr (SCORES) {
-    double sum = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (SIGMOID) s[j] = 1.0 / (1.0 + exp(-(double)v[j]));
-      else { s[j] = exp((double)v[j] - (double)mx); sum += s[j]; }
-    }
-    if (!SIGMOID) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) s[j] /= sum;
-    }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int e = lane + 32 * j;
-      if (BIAS && e < p.E) s[j] += (double)load_scalar(p.bias, e, p.bias_dt);
-      if (v[j] == -INFINITY) s[j] = -INFINITY;             // an expert that is masked out
-    }
-  }
-  Key key[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) key[j] = key_of(BIAS ? s[j] : (double)v[j]);
-
-  if constexpr (GROUPS) {
-    Key mine = 0;                                          // lane g: of group g
-    for (int g = 0; g < p.groups; ++g) {
-      const int lo = g * p.size, hi = lo + p.size;
-      Key a = 0, b = 0;                                    // the two largest
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int e = lane + 32 * j;
-        Key c = e >= lo && e < hi ? (TOP2 ? key_of(s[j]) : key[j]) : 0;
-        b = max(b, min(a, c));
-        a = max(a, c);
-      }
-      Key best = warp_max(a);
-      if (TOP2 && p.size > 1) {
-        const uint32_t who = __ballot_sync(0xffffffffu, a == best);
-        if (lane == __ffs(who) - 1) a = b;
-        const Key second = warp_max(a);
-        best = best && second ? key_of(value_of(best) + value_of(second)) : 0;
-      }
-      if (lane == g) mine = best;
-    }
-    uint32_t keep = 0;
-    for (int i = 0; i < p.top_groups; ++i) {
-      const Key best = warp_max(mine);
-      if (best == 0) break;
-      const int g = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
-      keep |= 1u << g;
-      if (lane == g) mine = 0;
-    }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int e = lane + 32 * j;
-      if (e < p.E && !(keep >> (e / p.size) & 1u)) key[j] = 0;
-    }
-  }
-
   int id = -1;
-  for (int i = 0; i < p.k; ++i) {
-    Key best = 0;
+  if constexpr (BIAS || (GROUPS && TOP2)) {
+    if (!bad) {
+      const bool sure = choose_by_scores<PER, SIGMOID, BIAS, GROUPS, TOP2, true, float, uint32_t>(v, mx, p, id);
+      if (!__all_sync(0xffffffffu, sure)) id = choose_exactly<PER, SIGMOID, BIAS, GROUPS, TOP2>(v, mx, p);
+    }
+  } else if (!bad) {
+    uint32_t key[PER];
+    const uint32_t none[1] = {0};
 #pragma unroll
-    for (int j = 0; j < PER; ++j) best = max(best, key[j]);
-    best = warp_max(best);
-    if (best == 0) break;
-    uint32_t e = 0xFFFFu;
-#pragma unroll
-    for (int j = PER - 1; j >= 0; --j)
-      if (key[j] == best) e = lane + 32 * j;
-    e = __reduce_min_sync(0xffffffffu, e);
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (lane + 32 * j == (int)e) key[j] = 0;
-    if (lane == i) id = (int)e;
+    for (int j = 0; j < PER; ++j) key[j] = key32(v[j]);
+    choose<PER, SIGMOID, GROUPS, false, false, uint32_t>(key, none, p, id);
   }
-  if (bad) id = -1;
 
   // Scores of the chosen.  Renormalised, they are taken relative to the largest where that is below a half, so that logits far below zero do not all
   // become zero.

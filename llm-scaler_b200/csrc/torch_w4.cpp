@@ -68,14 +68,15 @@ Weight weight_of(const char* name, const Tensor& x, const Tensor& w, const Tenso
   return r;
 }
 
-std::tuple<Tensor, Tensor> route_experts(const Tensor& logits, int64_t top_k, c10::string_view scoring, const OptTensor& bias, int64_t num_groups, int64_t top_groups,
-                                         c10::string_view group_score, bool renormalize, double scale) {
+// scoring, group_score: B2Q_SCORE_*, B2Q_GROUP_* (a string takes longer through the dispatcher than a small call)
+std::tuple<Tensor, Tensor> route_experts(const Tensor& logits, int64_t top_k, int64_t scoring, const OptTensor& bias, int64_t num_groups, int64_t top_groups,
+                                         int64_t group_score, bool renormalize, double scale) {
   same_device({&logits});
   check_rows(logits, "logits");
   const int dt = dtype_of(logits);
   const int64_t T = logits.size(0), E = logits.size(1);
-  TORCH_CHECK(scoring == "softmax" || scoring == "sigmoid", "scoring must be \"softmax\" or \"sigmoid\"");
-  TORCH_CHECK(group_score == "max" || group_score == "top2", "group_score must be \"max\" or \"top2\"");
+  TORCH_CHECK(scoring == B2Q_SCORE_SOFTMAX || scoring == B2Q_SCORE_SIGMOID, "scoring must be 0 (softmax) or 1 (sigmoid)");
+  TORCH_CHECK(group_score == B2Q_GROUP_MAX || group_score == B2Q_GROUP_TOP2, "group_score must be 0 (max) or 1 (top2)");
   TORCH_CHECK(E > 0 && num_groups > 0 && E % num_groups == 0, "num_groups must divide the number of experts");
   TORCH_CHECK(top_groups > 0 && top_groups <= num_groups, "top_groups must be between 1 and num_groups");
   TORCH_CHECK(top_k > 0 && top_k <= E / num_groups * top_groups, "top_k must be between 1 and the number of experts in top_groups groups");
@@ -87,8 +88,7 @@ std::tuple<Tensor, Tensor> route_experts(const Tensor& logits, int64_t top_k, c1
   Tensor w = fresh(logits, {T, top_k}, at::kFloat), ids = fresh(logits, {T, top_k}, at::kInt);
   if (T > 0)
     check(b2q_route_experts(logits.data_ptr(), dt, pitch(logits), bias.has_value() ? bias->data_ptr() : nullptr, bias.has_value() ? dtype_of(*bias) : 0, w.data_ptr<float>(),
-                            ids.data_ptr<int32_t>(), T, E, top_k, scoring == "sigmoid" ? B2Q_SCORE_SIGMOID : B2Q_SCORE_SOFTMAX, num_groups, top_groups,
-                            group_score == "top2" ? B2Q_GROUP_TOP2 : B2Q_GROUP_MAX, renormalize, (float)scale, stream_of(logits)));
+                            ids.data_ptr<int32_t>(), T, E, top_k, (int)scoring, num_groups, top_groups, (int)group_score, renormalize, (float)scale, stream_of(logits)));
   return {w, ids};
 }
 
@@ -145,7 +145,7 @@ Tensor moe_forward(const Tensor& x, const Tensor& topk_weights, const Tensor& to
 }  // namespace
 
 TORCH_LIBRARY(b2q_w4, m) {
-  m.def("route_experts(Tensor logits, int top_k, str scoring, Tensor? bias, int num_groups, int top_groups, str group_score, bool renormalize, float scale) -> (Tensor, Tensor)");
+  m.def("route_experts(Tensor logits, int top_k, int scoring, Tensor? bias, int num_groups, int top_groups, int group_score, bool renormalize, float scale) -> (Tensor, Tensor)");
   m.def("linear(Tensor x, Tensor weight, Tensor scale, Tensor? zero, Tensor? bias) -> Tensor");
   m.def("moe_forward(Tensor x, Tensor topk_weights, Tensor topk_ids, Tensor gate_up_weight, Tensor gate_up_scale, Tensor down_weight, Tensor down_scale, "
         "Tensor? gate_up_zero, Tensor? down_zero) -> Tensor");

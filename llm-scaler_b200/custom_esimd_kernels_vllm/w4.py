@@ -81,6 +81,9 @@ else:
     _ops = _Checked() if _CHECK_STATUS else _Ops()
 
 
+_SCORING, _GROUP_SCORE = {"softmax": 0, "sigmoid": 1}, {"max": 0, "top2": 1}      # B2Q_SCORE_*, B2Q_GROUP_*
+
+
 def route_experts(logits, top_k, scoring="softmax", bias=None, num_groups=1, top_groups=1, group_score="max", renormalize=True, scale=1.0):
     """Router logits [T, E] -> weights fp32 [T, top_k], ids int32 [T, top_k], the best expert first, the lowest index first among equals.
 
@@ -88,7 +91,10 @@ def route_experts(logits, top_k, scoring="softmax", bias=None, num_groups=1, top
     top_groups best groups can be chosen; a group counts by its best expert ("max") or the sum of its two best ("top2").  Weights are the chosen scores,
     divided by their sum if `renormalize`, times `scale`.  Choices are exact.  Where no expert is left (masked by -inf, or the token's logits hold a
     NaN or +inf) the id is -1 and the weight 0."""
-    return _ops.route_experts(logits, top_k, scoring, bias, num_groups, top_groups, group_score, renormalize, scale)
+    try:
+        return _ops.route_experts(logits, top_k, _SCORING[scoring], bias, num_groups, top_groups, _GROUP_SCORE[group_score], renormalize, scale)
+    except KeyError as unknown:
+        raise RuntimeError("b2q: scoring is \"softmax\" or \"sigmoid\" and group_score \"max\" or \"top2\", not %s" % unknown) from None
 
 
 def linear_w4(x, weight, scale, zero=None, bias=None):
