@@ -42,7 +42,8 @@ template <int NT> struct Cfg {
   static constexpr int X_BYTES = TOK * 256, RAW_BYTES = 8192;
   static constexpr int RS = NT == 256 ? 6 : (NT == 128 ? 8 : 9);      // raw stages, a multiple of DG
   static constexpr int STG = EW * 2048;                      // 32 tokens x 32 columns for every epilogue warp
-  static constexpr int USED = S * X_BYTES + RS * RAW_BYTES + STG + 1024;
+  static constexpr int TABLE = 48;                           // tiles of a grouped launch that every role finds in shared memory
+  static constexpr int USED = S * X_BYTES + RS * RAW_BYTES + STG + TABLE * 16 + 1024;
   static constexpr int SMEM = 1024 + (USED < 170 * 1024 ? 170 * 1024 : USED);      // one CTA with tensor memory on an SM: see umma_i8.cu
   static_assert(RS % DG == 0 && S % DG == 0 && S > 0 && SMEM <= 232448, "rings");
 };
@@ -56,6 +57,7 @@ struct Params {
   float* partials; Arrivals* arrivals; Arrivals tag; const Arrivals* epoch;
   const int32_t* tiles; const int32_t* offsets;            // grouped
   int early;
+  uint32_t mask, magic;                                    // of the decode: as constants they take an operation each
   int* status;
 };
 
@@ -66,21 +68,27 @@ struct Tile {
   __device__ __forceinline__ int stage(int j) const { const int i = j + turn; return ks0 + (i >= n ? i - n : i); }
 };
 
-template <int NT, bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(const Params& p, int id) {
+// table: {first token, tokens, expert, strip} of this CTA's tiles, of which it has `known`; id is the n-th of them.
+template <int NT, bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile_at(const Params& p, int id, const int4* table, int n, int known) {
   constexpr int WIDTH = GATED ? 128 : 256;                 // output columns of a strip
   Tile t;
   t.piece = 0; t.ks0 = 0; t.n = p.nks; t.e = 0;
   int st;
   if constexpr (GROUPED) {
-    const int ti = id / p.n_strips;
-    st = id - ti * p.n_strips;
-    const int e = __ldcg(p.tiles + 4 + 2 * ti), r0 = __ldcg(p.tiles + 4 + 2 * ti + 1);
-    t.tok0 = __ldcg(p.offsets + e) + r0;
-    t.rows = min(NT, __ldcg(p.offsets + e + 1) - t.tok0);
+    int4 v;
+    if (n < known) {
+      v = table[n];
+    } else {
+      const int ti = id / p.n_strips, e = __ldcg(p.tiles + 4 + 2 * ti), tok0 = __ldcg(p.offsets + e) + __ldcg(p.tiles + 4 + 2 * ti + 1);
+      v = make_int4(tok0, min(NT, __ldcg(p.offsets + e + 1) - tok0), e, id - ti * p.n_strips);
+    }
+    st = v.w;
+    t.tok0 = v.x;
+    t.rows = v.y;
     t.n0 = st * WIDTH;
-    t.w0 = (GATED ? 2 : 1) * e * p.N + t.n0;
+    t.w0 = (GATED ? 2 : 1) * v.z * p.N + t.n0;
     t.strip = 0;
-    t.e = e;
+    t.e = v.z;
   } else {
     if (p.pieces > 1) {
       t.strip = id / p.pieces;
@@ -132,14 +140,13 @@ __device__ __forceinline__ uint32_t fma2_f16(uint32_t a, uint32_t b, uint32_t c)
 
 // Eight codes of a word -> four registers of two values (q - z) s.  PERM: in the order 0, 4, 1, 5, 2, 6, 3, 7, else as they come.  zc: the power of two plus z, twice (fp16 and
 // PERM: and -(64 + z) in zh); MORE: bf16, with what z has beyond 127 in more, for 128 + z has to fit eight bits.
-template <bool BF16, bool PERM, bool MORE> __device__ __forceinline__ void decode(uint32_t w, uint32_t s2, uint32_t zc, uint32_t zh, uint32_t more, uint32_t* o) {
-  constexpr uint32_t MASK = 0x000F000Fu, MAGIC = BF16 ? 0x43004300u : 0x64006400u;
+template <bool BF16, bool PERM, bool MORE> __device__ __forceinline__ void decode(uint32_t w, uint32_t s2, uint32_t zc, uint32_t zh, uint32_t more, uint32_t MASK, uint32_t MAGIC, uint32_t* o) {
   if constexpr (PERM && !BF16) {
     const uint32_t w8 = w >> 8;
     o[0] = sub2<false>((w & MASK) | MAGIC, zc);
     o[2] = sub2<false>((w8 & MASK) | MAGIC, zc);
-    o[1] = fma2_f16((w & 0x00F000F0u) | MAGIC, 0x2C002C00u, zh);      // 2^-4 (1024 + 16 q) - (64 + z)
-    o[3] = fma2_f16((w8 & 0x00F000F0u) | MAGIC, 0x2C002C00u, zh);
+    o[1] = fma2_f16((w & (MASK << 4)) | MAGIC, 0x2C002C00u, zh);      // 2^-4 (1024 + 16 q) - (64 + z)
+    o[3] = fma2_f16((w8 & (MASK << 4)) | MAGIC, 0x2C002C00u, zh);
   } else if constexpr (PERM) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = sub2<true>(((w >> 4 * i) & MASK) | MAGIC, zc);
@@ -202,8 +209,9 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-  // [token stages] [raw stages] [staging] [barriers]
-  const uint32_t raw0 = base + C::S * C::X_BYTES, stg0 = raw0 + C::RS * C::RAW_BYTES, bar = stg0 + C::STG;
+  // [token stages] [raw stages] [staging] [tiles] [barriers]
+  const uint32_t raw0 = base + C::S * C::X_BYTES, stg0 = raw0 + C::RS * C::RAW_BYTES, tab0 = stg0 + C::STG, bar = tab0 + C::TABLE * 16;
+  int4* table = reinterpret_cast<int4*>(gen + (tab0 - base));
   // A stage is full when its tokens have landed and both CTAs' operands are written; one barrier for both, since a wait costs the issuing thread some 125 cycles even when it is
   // over, and a commit 90.
   const uint32_t full = bar, empty = full + 8 * C::S, raw_full = empty + 8 * C::S, raw_empty = raw_full + 8 * C::RS, acc_full = raw_empty + 8 * C::RS, acc_empty = acc_full + 16,
@@ -233,8 +241,19 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
   cluster_sync_all();                                      // both CTAs' barriers exist before anything is signalled across
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (GROUPED) grid_dep_wait();                            // the tile list is made by the kernels in front
-  const int total = GROUPED ? __ldcg(p.tiles) * p.n_strips : p.total;
+  int total = p.total, known = 0;
+  if constexpr (GROUPED) {
+    grid_dep_wait();                                       // the tile list is made by the kernels in front
+    total = __ldcg(p.tiles) * p.n_strips;
+    const int mine = first < total ? (total - first + step - 1) / step : 0;
+    known = min(mine, C::TABLE);
+    // looked up once, all at a time: two loads that follow each other are 1500 cycles of every role at every tile
+    if (threadIdx.x < known) {
+      const Tile t = tile_at<NT, GROUPED, GATED>(p, first + threadIdx.x * step, table, 0, 0);
+      table[threadIdx.x] = make_int4(t.tok0, t.rows, t.e, t.n0 / (GATED ? 128 : 256));
+    }
+    __syncthreads();
+  }
 
   if (warp == 0) {
     // ---- raw codes ----
@@ -244,8 +263,8 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       int s = 0, issued = 0;
       uint32_t par = 1u;
       bool ok = true;
-      for (int id = first; ok && id < total; id += step) {
-        const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
+      for (int id = first, i = 0; ok && id < total; id += step, ++i) {
+        const Tile t = tile_at<NT, GROUPED, GATED>(p, id, table, i, known);
         const int w = t.w0 + (int)rank * (GATED ? 64 : 128);
         for (int j = 0; j < t.n; ++j) {
           const int ks = t.stage(j);
@@ -269,8 +288,8 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       int s = 0, issued = 0;
       uint32_t par = 1u;
       bool ok = true;
-      for (int id = first; ok && id < total; id += step) {
-        const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
+      for (int id = first, q = 0; ok && id < total; id += step, ++q) {
+        const Tile t = tile_at<NT, GROUPED, GATED>(p, id, table, q, known);
         for (int j = 0; j < t.n; ++j) {
           const int ks = t.stage(j);
           ok = mbar_wait(empty + 8 * s, par, abort_flag, p.status, ST_XEMPTY);
@@ -294,7 +313,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
       uint32_t par = 0u;
       bool ok = true;
       for (int id = first; ok && id < total; id += step, ++it) {
-        const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
+        const Tile t = tile_at<NT, GROUPED, GATED>(p, id, table, it, known);
         const int b = it % C::NBUF;
         if (it >= C::NBUF) ok = mbar_wait(acc_empty + 8 * b, (it / C::NBUF - 1) & 1, abort_flag, p.status, ST_ACCEMPTY);
         if (!ok) break;
@@ -327,30 +346,50 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
     const uint32_t row_at = raw_row * 64, f = (raw_row >> 1) & 3;      // 64-byte swizzle of the raw box
     constexpr int GS = 128 / G;
     if (!GROUPED && !p.early) grid_dep_wait();
-    int it = 0;                                            // stages so far
+    // This group's stages one after the other, whatever tile they are of.  All tiles of a CTA have the same number of stages: where k is cut into pieces, it has one tile.
     bool ok = true;
     uint32_t sc[2][GS], zc[2][GS];                         // of this group's next two stages
-    for (int id = first; ok && id < total; id += step) {
-      const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
+    struct Ahead { int id, q, j; Tile t; int64_t at; } ahead;      // of the stage whose scales are fetched next
+    auto enter = [&]() {
+      if (ahead.id >= total) return;
+      const Tile t = ahead.t = tile_at<NT, GROUPED, GATED>(p, ahead.id, table, ahead.q, known);
       // this thread's row among the scales' rows; beyond the last it repeats it, and nobody looks at the sums
       int row;
       if constexpr (GATED) { const int h = min(t.n0 + (int)rank * 64 + 16 * quad + (lane & 15), p.N - 1); row = lane < 16 ? h : p.N + h; }
       else row = min(t.n0 + (int)rank * 128 + 32 * quad + lane, p.N - 1);
-      const int64_t at0 = (int64_t)t.e * p.s_expert + row;
-      const int n = t.n, mine0 = (grp - it % C::DG + C::DG) % C::DG;      // the tile's first stage that is this group's
-      auto fetch = [&](int j, uint32_t (&s)[GS], uint32_t (&z)[GS]) {
-        if (j >= n) return;
+      ahead.at = (int64_t)t.e * p.s_expert + row;
+    };
+    ahead.id = first;
+    ahead.q = 0;
+    ahead.j = grp;
+    enter();
+    const int n = first < total ? ahead.t.n : 1;
+    auto pass = [&]() {                                    // tiles that end before this group's next stage
+      while (ahead.j >= n && ahead.id < total) {
+        ahead.j -= n;
+        ahead.id += step;
+        ++ahead.q;
+        enter();
+      }
+    };
+    pass();
+    auto fetch = [&](uint32_t (&s)[GS], uint32_t (&z)[GS]) {
+      if (ahead.id >= total) return;
 #pragma unroll
-        for (int i = 0; i < GS; ++i) {
-          const int64_t at = at0 + (int64_t)min(t.stage(j) * GS + i, p.groups - 1) * p.s_rows;
-          s[i] = ld_u16(p.s + at);
-          z[i] = p.z ? ld_u8(p.z + at) : 8u;
-        }
-      };
-      fetch(mine0, sc[0], zc[0]);
-      fetch(mine0 + C::DG, sc[1], zc[1]);
-      for (int j = mine0; j < n; j += C::DG) {
-        const int now = it + j, rs = now % C::RS, as = now % C::S;
+      for (int i = 0; i < GS; ++i) {
+        const int64_t at = ahead.at + (int64_t)min(ahead.t.stage(ahead.j) * GS + i, p.groups - 1) * p.s_rows;
+        s[i] = ld_u16(p.s + at);
+        z[i] = p.z ? ld_u8(p.z + at) : 8u;
+      }
+      ahead.j += C::DG;
+      pass();
+    };
+    fetch(sc[0], zc[0]);
+    fetch(sc[1], zc[1]);
+    const int tiles = first < total ? (total - first + step - 1) / step : 0, end = tiles * n;
+    {
+      for (int now = grp; now < end; now += C::DG) {
+        const int rs = now % C::RS, as = now % C::S;
         uint32_t s2[GS], z2[GS], zh[GS], more[GS];
         bool has_more = false;
 #pragma unroll
@@ -373,7 +412,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
           }
         }
         has_more = BF16 && __any_sync(0xffffffffu, has_more);
-        fetch(j + 2 * C::DG, sc[1], zc[1]);
+        fetch(sc[1], zc[1]);
         ok = mbar_wait_warp(raw_full + 8 * rs, (now / C::RS) & 1, abort_flag, p.status, ST_RAWFULL);
         if (!ok) break;
         uint4 raw[4];
@@ -394,7 +433,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
 #pragma unroll
               for (int v = 0; v < 4; ++v) {
                 const int of = (h * 64 + i * 32 + v * 8) / G;
-                decode<BF16, PERM, decltype(with_more)::value>(w[v], s2[of], z2[of], zh[of], more[of], o + 16 * i + 4 * v);
+                decode<BF16, PERM, decltype(with_more)::value>(w[v], s2[of], z2[of], zh[of], more[of], p.mask, p.magic, o + 16 * i + 4 * v);
               }
             }
             tmem_st32(a + 32 * h, o);
@@ -409,7 +448,6 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(full + 8 * as, 0));
         __syncwarp();
       }
-      it += n;
     }
   } else if (warp >= C::FIRST_EPI) {
     // ---- epilogue: lane quadrant = warp & 3 (weight rows); tokens shared by the warps of a quadrant ----
@@ -421,7 +459,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
     int it = 0;
     bool ok = true;
     for (int id = first; id < total; id += step, ++it) {
-      const Tile t = tile_at<NT, GROUPED, GATED>(p, id);
+      const Tile t = tile_at<NT, GROUPED, GATED>(p, id, table, it, known);
       const int b = it % C::NBUF;
       ok = ok && mbar_wait_warp(acc_full + 8 * b, (it / C::NBUF) & 1, abort_flag, p.status, ST_ACCFULL);
       if (!ok) {
@@ -566,6 +604,8 @@ __global__ void __launch_bounds__(256) g4_align_rows_kernel(const uint16_t* x, i
 
 // ---- host ----
 namespace ug4 {
+constexpr uint32_t MASK = 0x000F000Fu, MAGIC_BF16 = 0x43004300u, MAGIC_F16 = 0x64006400u;      // 128 and 1024, whose lowest bits a code takes
+
 template <bool BF16, int G, int NT, bool GROUPED, bool GATED>
 static int launch(const CUtensorMap& tx, const CUtensorMap& tw, const Params& p, int grid, cudaStream_t st) {
   using C = Cfg<NT>;
@@ -663,6 +703,7 @@ int umma_g4_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st) {
     if (!p.epoch) return B2Q_ERR_CUDA;
   }
   p.early = tls().overlap_mode == 2;
+  p.mask = MASK; p.magic = a.bf16 ? MAGIC_BF16 : MAGIC_F16;
   p.status = umma_status_ptr();
   if (!p.status) return B2Q_ERR_CUDA;
   CUtensorMap tx, tw;
@@ -694,6 +735,7 @@ int umma_g4_grouped(const G4GroupedArgs& a, cudaStream_t st) {
   const int width = a.gated ? 128 : 256;
   p.n_strips = (a.N + width - 1) / width;
   p.tiles = a.tiles; p.offsets = a.offsets;
+  p.mask = MASK; p.magic = a.bf16 ? MAGIC_BF16 : MAGIC_F16;
   p.status = umma_status_ptr();
   if (!p.status) return B2Q_ERR_CUDA;
   const int64_t w_rows = (int64_t)a.E * p.s_rows;
