@@ -17,7 +17,7 @@ namespace b2q {
 namespace g4s {
 constexpr int MOST_WARPS = 16, THREADS = 32 * MOST_WARPS;      // sixteen warps, or twelve where that many tokens leave no room for more
 constexpr int SELF = 4;                                    // eights that a thread prepares at most where a CTA prepares the tokens itself
-enum { ST_IMAGE = 901 };
+enum { ST_IMAGE = 961 };
 
 struct Params {
   const uint16_t* x; int64_t ldx; int vec;
