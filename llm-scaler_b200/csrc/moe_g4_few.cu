@@ -6,8 +6,7 @@
 // warps equal runs of the tiles' steps of 128 k, as in the linear.
 //  * up: a tile has sixteen gate rows and the sixteen up rows of the same outputs; h = silu(gate) * up goes out in 16 bits, with its largest magnitude per tile, from which the
 //    second kernel takes the power of two that it scales a row of h by.
-//  * down, OWN: a CTA has rows of its own, for all groups; it adds the weighted outputs of a token's experts up by itself.  While all pairs' h fit its shared memory.
-//  * down otherwise: weighted outputs of each pair in fp32, which a third kernel adds up in the order of the slots.
+//  * down: weighted outputs of each pair in fp32, which a third kernel adds up in the order of the slots.  Its weights are on their way before the first kernel is done.
 #include <algorithm>
 #include "i8.cuh"
 #include "g4_stream.cuh"
@@ -15,10 +14,10 @@
 namespace b2q {
 namespace g4f {
 using namespace g4s;
-constexpr int MOST_WARPS = 16, LEAST_WARPS = 12, THREADS = 32 * MOST_WARPS;      // as many as leave room for the columns
-constexpr int MAX_PAIRS = 32 * LEAST_WARPS, MAX_E = 1024, PER = (MAX_E + 32 * LEAST_WARPS - 1) / (32 * LEAST_WARPS), TOK = 8;
-constexpr int CAP = 24;                                    // tiles that are summed up at a time
-constexpr int SMEM = 208 * 1024;                           // beside the routes'
+// Twelve warps: sixteen were as fast, and leave less room for the columns.
+constexpr int WARPS = 12, THREADS = 32 * WARPS, MAX_PAIRS = THREADS, MAX_E = 1024, PER = (MAX_E + THREADS - 1) / THREADS, TOK = 8;
+constexpr int MAX_TILES = 64;                              // that are summed up at a time
+constexpr int SMEM = 214 * 1024;                           // beside the routes'
 
 struct Params {
   const uint16_t* x; const int32_t* ids; const float* weights;      // x: tokens, or h by pair
@@ -26,7 +25,8 @@ struct Params {
   uint16_t* h; uint32_t* h_max;                            // [pairs, I], [pairs, I / 16]
   float* y; uint16_t* out;                                 // [pairs, N], [T, N]
   int T, E, k, N, K, steps;                                // N: outputs (I, H)
-  int columns, groups;                                     // that there is room for
+  int columns, groups, cap;                                // columns, groups and tiles that there is room for
+  int early;
 };
 
 struct Group { int16_t expert, first, count; };            // first, count: of the sorted pairs
@@ -37,16 +37,16 @@ struct alignas(16) Shared {
   int16_t pairs[MAX_PAIRS];                                // sorted by expert
   int16_t place[MAX_PAIRS];                                // of a pair among the sorted; -1: no expert
   Group groups[MAX_PAIRS];
-  int warp_sum[MOST_WARPS][2];
+  int warp_sum[WARPS][2];
   int n_groups;
   uint32_t max[MAX_PAIRS];                                 // of a staged column's row
-  struct { int16_t group, strip, first, last; } tiles[CAP];      // of a batch; warps that have units of it
+  struct { int16_t group, strip, first, last; } tiles[MAX_TILES];      // of a batch; warps that have units of it
 };
 
 // The routes' pairs sorted by expert, those of an expert by their number: all CTAs of both kernels have to agree on which group a pair is in.
 __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
   const int n = p.T * p.k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) sh.count[e] = 0;
+  for (int e = threadIdx.x; e < p.E; e += THREADS) sh.count[e] = 0;
   __syncthreads();
   int id = -1, at = 0;
   if (threadIdx.x < n) {
@@ -54,7 +54,7 @@ __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
     if ((uint32_t)id >= (uint32_t)p.E) id = -1;
     if (id >= 0) atomicAdd(&sh.count[id], 1);
   }
-  if (threadIdx.x < MAX_PAIRS) sh.ids[threadIdx.x] = id;
+  sh.ids[threadIdx.x] = id;
   __syncthreads();
   if (id >= 0) {
     for (int j = 0; j < (int)threadIdx.x; j += 4) {
@@ -80,7 +80,7 @@ __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
   if (lane == 31) { sh.warp_sum[warp][0] = pairs; sh.warp_sum[warp][1] = groups; }
   __syncthreads();
   for (int w = 0; w < warp; ++w) { pairs += sh.warp_sum[w][0]; groups += sh.warp_sum[w][1]; }
-  if (threadIdx.x == blockDim.x - 1) sh.n_groups = groups;
+  if (threadIdx.x == THREADS - 1) sh.n_groups = groups;
   int first = pairs - own_pairs, to_group = groups - own_groups;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -97,41 +97,42 @@ __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
   __syncthreads();
 }
 
-template <int VEC, bool BF16, bool UP, bool OWN, bool PART>
+template <int VEC, bool BF16, bool UP, bool PART>
 __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) {
   constexpr int G = 32 * VEC, GS = STEP / G;               // groups of k in a step
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Shared sh;
-  const int WARPS = blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int steps = p.steps, group_xg = steps * GS * TOK;  // group sums of a group's columns: [steps * GS][8]
   uint8_t* xs = smem + WARPS * WARP_BYTES;                 // [columns][steps][256], then [groups][group_xg]
   float* xg = reinterpret_cast<float*>(xs + (size_t)p.columns * steps * 256);
-  float* slots = xg + p.groups * group_xg;                 // [CAP + WARPS][ROWS][TOK]
+  float* slots = xg + p.groups * group_xg;                 // [cap + WARPS][ROWS][TOK]
 
-  grid_dep_wait();
-  // Only now: the next kernel may then read the routes, and begin with its weights, before this one is done.
+  // up lets the next kernel begin only when it has itself seen that all before it is done: that one may then read the routes, and its weights, while up runs
+  bool waited = UP || !p.early;
+  if (waited) grid_dep_wait();
   grid_dep_release();
   sort_routes(sh, p);
 
-  // this CTA's tiles: strip by strip of every group in turn.  OWN: rows of its own, in strips of 32, for all groups
+  // this CTA's tiles: strip by strip of every group in turn
   constexpr int STRIP = UP ? 16 : 32;                      // outputs of a tile
-  const int own0 = OWN ? (int)((int64_t)blockIdx.x * p.N / gridDim.x) : 0, own = OWN ? (int)((int64_t)(blockIdx.x + 1) * p.N / gridDim.x) - own0 : p.N;
-  const int strips = (own + STRIP - 1) / STRIP, all = sh.n_groups * strips;
-  const int begin = OWN ? 0 : (int)((int64_t)blockIdx.x * all / gridDim.x), end = OWN ? all : (int)((int64_t)(blockIdx.x + 1) * all / gridDim.x);
+  const int strips = (p.N + STRIP - 1) / STRIP, all = sh.n_groups * strips;
+  const int begin = (int)((int64_t)blockIdx.x * all / gridDim.x), end = (int)((int64_t)(blockIdx.x + 1) * all / gridDim.x);
+  const int batches = (end - begin + p.cap - 1) / p.cap, cap = batches ? (end - begin + batches - 1) / batches : 0;
   const uint32_t ring = smem_addr(smem) + warp * WARP_BYTES;
 
   for (int b0 = begin; b0 < end;) {
     // a batch: tiles whose groups' columns and sums fit
     const int ga = b0 / strips;
     int gb = ga + 1, columns = sh.groups[ga].count;
-    int b1 = min(min(end, gb * strips), b0 + CAP);
-    while (b1 == gb * strips && b1 < end && b1 - b0 < CAP && columns + sh.groups[gb].count <= p.columns && gb - ga < p.groups) {
+    int b1 = min(min(end, gb * strips), b0 + cap);
+    while (b1 == gb * strips && b1 < end && b1 - b0 < cap && columns + sh.groups[gb].count <= p.columns && gb - ga < p.groups) {
       columns += sh.groups[gb].count;
       ++gb;
-      b1 = min(min(end, gb * strips), b0 + CAP);
+      b1 = min(min(end, gb * strips), b0 + cap);
     }
     const int pair0 = sh.groups[ga].first;                 // columns are the sorted pairs from here on
-    const int tiles = b1 - b0, units = tiles * steps, run = (units + WARPS - 1) / WARPS, u0 = min(units, warp * run), u1 = min(units, u0 + run);
+    const int tiles = b1 - b0, units = tiles * steps, even = (units + WARPS - 1) / WARPS, run = even > 6 ? (even + 1) / 2 * 2 : even, u0 = min(units, warp * run), u1 = min(units, u0 + run);
 
     if (threadIdx.x < tiles) {
       const int id = b0 + threadIdx.x, gi = id / strips;
@@ -139,15 +140,15 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
     }
     __syncthreads();
     struct Tiles {
-      const Shared& sh; const Params& p; int own0, own, ga, pair0, group_xg; uint32_t xs, xg;
+      const Shared& sh; const Params& p; int ga, pair0, group_xg; uint32_t xs, xg;
       __device__ __forceinline__ int rows(int tile, int64_t (&row)[4], uint32_t (&off)[4], int64_t& base) const {
-        const int e = sh.groups[sh.tiles[tile].group].expert, r = STRIP * sh.tiles[tile].strip, g = (threadIdx.x & 31) >> 2, left = own - r;
+        const int e = sh.groups[sh.tiles[tile].group].expert, r = STRIP * sh.tiles[tile].strip, g = (threadIdx.x & 31) >> 2, left = p.N - r;
         const int64_t first = (int64_t)e * p.w_rows;
         base = e * p.s_expert;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           // up: rows 0 to 15 of the tile are gate rows, 16 to 31 up rows, which lie N behind them
-          off[i] = UP ? r + g + 8 * (i & 1) + (i >> 1) * p.N : own0 + r + min(g + 8 * i, left - 1);
+          off[i] = UP ? r + g + 8 * (i & 1) + (i >> 1) * p.N : r + min(g + 8 * i, left - 1);
           row[i] = first + off[i];
         }
         return UP || left > 16 ? 2 : 1;
@@ -158,9 +159,10 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
         at[0] = xs + (gr.first - pair0 + min(lane >> 2, gr.count - 1)) * (p.steps * 256);      // columns beyond the group's repeat its last: nobody looks at them
         x = xg + (gi - ga) * group_xg * 4 + 8 * (lane & 3);
       }
-    } of{sh, p, own0, own, ga, pair0, group_xg, smem_addr(xs), smem_addr(xg)};
+    } of{sh, p, ga, pair0, group_xg, smem_addr(xs), smem_addr(xg)};
     Stream<VEC, 1, BF16, PART, Tiles> stream(p.w, of, p.K, steps, 0, u0, u1, ring);
     stream.load(ring);
+    if (!waited) { grid_dep_wait(); waited = true; }
 
     // ---- columns ----
     auto source = [&](int c) {
@@ -174,18 +176,18 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
     auto fetch_x = [&](int base) {
 #pragma unroll
       for (int a = 0; a < V; ++a) {
-        const int i = base + a * blockDim.x + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv), at = 8 * (i - c * per);
+        const int i = base + a * THREADS + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv), at = 8 * (i - c * per);
         v[a] = i < total && at < p.K ? ld_eight(source(c) + at, true) : make_uint4(0, 0, 0, 0);
       }
     };
     if (UP) {
-      for (int c = threadIdx.x; c < columns; c += blockDim.x) sh.max[c] = 0;
+      for (int c = threadIdx.x; c < columns; c += THREADS) sh.max[c] = 0;
       __syncthreads();
-      for (int base = 0; base < total; base += V * blockDim.x) {
+      for (int base = 0; base < total; base += V * THREADS) {
         fetch_x(base);
 #pragma unroll
         for (int a = 0; a < V; ++a) {
-          const int i = base + a * blockDim.x + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv);
+          const int i = base + a * THREADS + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv);
           if ((i & ~31) >= total) break;                   // whole warps
           uint32_t mx = max_bits(v[a]);                    // a half warp has one column, since `per` is a multiple of 16
 #pragma unroll
@@ -202,14 +204,14 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
         mx = __reduce_max_sync(0xffffffffu, mx);
         if (lane == 0) sh.max[c] = mx;
       }
-      if (total <= V * blockDim.x) fetch_x(0);
+      if (total <= V * THREADS) fetch_x(0);
     }
     __syncthreads();
-    for (int base = 0; base < total; base += V * blockDim.x) {
-      if (total > V * blockDim.x) fetch_x(base);
+    for (int base = 0; base < total; base += V * THREADS) {
+      if (total > V * THREADS) fetch_x(base);
 #pragma unroll
       for (int a = 0; a < V; ++a) {
-        const int i = base + a * blockDim.x + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv), at = i - c * per;
+        const int i = base + a * THREADS + threadIdx.x, c = (int)__umulhi((uint32_t)i, inv), at = i - c * per;
         if ((i & ~31) >= total) break;
         float sum = 0.f;
         int local = 0, gi = ga;                            // the column's place in its group
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
     };
     if constexpr (UP) {
       // sixteen lanes a column: its outputs in this tile
-      for (int i = threadIdx.x; i < tiles * 128; i += blockDim.x) {
+      for (int i = threadIdx.x; i < tiles * 128; i += THREADS) {
         const int tl = i >> 7, c = (i >> 4) & 7, r = i & 15;
         const Group gr = sh.groups[sh.tiles[tl].group];
         if (c >= gr.count) continue;                       // whole half warps
@@ -252,37 +254,19 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
         p.h[(int64_t)pair * p.N + 16 * st + r] = bits;
         if (r == 0) p.h_max[(int64_t)pair * (p.N / 16) + st] = mx;
       }
-    } else if constexpr (!OWN) {
-      for (int i = threadIdx.x; i < tiles * 256; i += blockDim.x) {
+    } else {
+      for (int i = threadIdx.x; i < tiles * 256; i += THREADS) {
         const int tl = i >> 8, c = (i >> 5) & 7, r = i & 31, n = 32 * sh.tiles[tl].strip + r;
         const Group gr = sh.groups[sh.tiles[tl].group];
         if (c >= gr.count || n >= p.N) continue;
         const int pair = sh.pairs[gr.first + c];
         p.y[(int64_t)pair * p.N + n] = __ldcg(p.weights + pair) * unshift(total_of(tl, r, c), row_shift<BF16>(sh.max[gr.first - pair0 + c]));
       }
-    } else {
-      for (int i = threadIdx.x; i < p.T * own; i += blockDim.x) {
-        const int m = i / own, r = i - m * own;
-        float f = 0.f;
-        for (int q = 0; q < p.k; ++q) {
-          const int pair = m * p.k + q, at = sh.place[pair];
-          if (at < 0) continue;
-          int gi = 0;                                      // the pair's group
-          for (int lo = 0, hi = sh.n_groups; hi - lo > 1;) {
-            const int mid = (lo + hi) / 2;
-            if (sh.groups[mid].first <= at) lo = gi = mid; else hi = mid;
-          }
-          f = fmaf(__ldcg(p.weights + pair), unshift(total_of(gi * strips + (r >> 5), r & 31, at - sh.groups[gi].first), row_shift<BF16>(sh.max[at])), f);
-        }
-        p.out[(int64_t)m * p.N + own0 + r] = to_half<BF16>(f);
-      }
     }
     __syncthreads();                                       // slots and columns are used again
     b0 = b1;
   }
-  if (OWN && sh.n_groups == 0) {                           // nobody has an expert
-    for (int i = threadIdx.x; i < p.T * own; i += blockDim.x) p.out[(int64_t)(i / own) * p.N + own0 + i % own] = 0;
-  }
+  if (!waited) grid_dep_wait();                            // the kernel behind waits for this one, and so for all before it
 }
 
 template <bool BF16> __global__ void __launch_bounds__(256) g4_pairs_sum_kernel(const float* y, const int32_t* ids, uint16_t* out, int64_t total, int N, int k, int E) {
@@ -291,42 +275,48 @@ template <bool BF16> __global__ void __launch_bounds__(256) g4_pairs_sum_kernel(
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const int64_t t = i / N, n = i - t * N;
     float f = 0.f;
-    for (int s = 0; s < k; ++s)
-      if ((uint32_t)__ldcg(ids + t * k + s) < (uint32_t)E) f += __ldcg(y + (t * k + s) * N + n);
+    for (int s0 = 0; s0 < k; s0 += 8) {                    // requested together
+      float v[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) v[s] = s0 + s < k && (uint32_t)__ldcg(ids + t * k + s0 + s) < (uint32_t)E ? __ldcg(y + (t * k + s0 + s) * N + n) : 0.f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) f += v[s];
+    }
     out[i] = to_half<BF16>(f);
   }
 }
 
 // ---- host ----
-struct Plan { int warps, up_columns, down_columns, smem_up, smem_down; bool own, fits; };
-// Columns and groups that shared memory has room for, one group for two columns and one more.
+// What shared memory has room for: tiles first, as many as a CTA is likely to have, as long as one group's columns fit beside them; then columns, with a group for two of them
+// and one more.
+struct Room { int columns, groups, cap, smem; };
 static int groups_of(int columns) { return columns / 2 + 1; }
 static int bytes_of(int columns, int K, int G) { const int steps = (K + STEP - 1) / STEP; return columns * steps * 256 + groups_of(columns) * steps * (STEP / G) * TOK * 4; }
-static int room_for(int most, int K, int G, int room) {
-  int n = most;
-  while (n > 0 && bytes_of(n, K, G) > room) --n;
-  return n;
+static Room room_for(int pairs, int E, int strips, int K, int G) {
+  const int least = std::min(pairs, TOK), groups = std::min(pairs, E + pairs / TOK);
+  Room r{};
+  r.cap = std::max(8, std::min(MAX_TILES, (int)((int64_t)groups * strips / sm_count()) + 1));
+  auto fixed = [](int cap) { return WARPS * WARP_BYTES + (cap + WARPS) * ROWS * TOK * 4; };
+  while (r.cap > 8 && fixed(r.cap) + bytes_of(least, K, G) > SMEM) --r.cap;
+  for (r.columns = pairs; r.columns > 0 && fixed(r.cap) + bytes_of(r.columns, K, G) > SMEM;) --r.columns;
+  if (r.columns < least) r.columns = 0;
+  r.groups = groups_of(r.columns);
+  r.smem = fixed(r.cap) + bytes_of(r.columns, K, G);
+  return r;
 }
+struct Plan { Room up, down; bool fits; };
 static Plan plan(const G4MoeArgs& a) {
   Plan q{};
-  const int pairs = a.T * a.k, most = std::min(pairs, TOK);
+  const int pairs = a.T * a.k;
   if (pairs > MAX_PAIRS) return q;
-  int fixed = 0;
-  for (q.warps = MOST_WARPS; q.warps >= LEAST_WARPS && !q.fits; q.warps -= 4) {
-    fixed = q.warps * WARP_BYTES + (CAP + q.warps) * ROWS * TOK * 4;
-    q.up_columns = room_for(pairs, a.H, a.G13, SMEM - fixed);
-    q.down_columns = room_for(pairs, a.I, a.G2, SMEM - fixed);
-    q.fits = most <= q.up_columns && most <= q.down_columns;
-  }
-  q.warps += 4;
-  const int strips = ((a.H + sm_count() - 1) / sm_count() + ROWS - 1) / ROWS;
-  q.own = q.down_columns == pairs && groups_of(pairs) >= pairs && pairs * strips <= CAP && (int64_t)pairs * a.I <= 16384;
-  q.smem_up = fixed + bytes_of(q.up_columns, a.H, a.G13);
-  q.smem_down = fixed + bytes_of(q.down_columns, a.I, a.G2);
+  q.up = room_for(pairs, a.E, a.I / 16, a.H, a.G13);
+  q.down = room_for(pairs, a.E, (a.H + ROWS - 1) / ROWS, a.I, a.G2);
+  q.fits = q.up.columns > 0 && q.down.columns > 0;
   return q;
 }
-template <int VEC, bool BF16, bool UP, bool OWN, bool PART> static int launch(const Params& p, int warps, int smem, cudaStream_t st) {
-  auto kern = g4_experts_kernel<VEC, BF16, UP, OWN, PART>;
+template <int VEC, bool BF16, bool UP, bool PART> static int launch(Params& p, const Room& r, cudaStream_t st) {
+  p.columns = r.columns; p.groups = r.groups; p.cap = r.cap;
+  auto kern = g4_experts_kernel<VEC, BF16, UP, PART>;
   static thread_local bool configured[16] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -334,20 +324,19 @@ template <int VEC, bool BF16, bool UP, bool OWN, bool PART> static int launch(co
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return B2Q_ERR_CUDA;
     if (dev < 16) configured[dev] = true;
   }
-  const int grid = OWN ? std::min(sm_count(), p.N) : sm_count();
-  launch_overlapped(kern, dim3(grid), dim3(32 * warps), smem, st, tls().overlap_mode > 0, p);
+  launch_overlapped(kern, dim3(sm_count()), dim3(THREADS), r.smem, st, tls().overlap_mode > 0, p);
   note_launch(UP ? "g4_experts_up" : "g4_experts_down");
   return launch_status();
 }
-template <bool UP, bool OWN> static int by_type(const Params& p, bool bf16, int G, int warps, int smem, cudaStream_t st) {
+template <bool UP> static int by_type(Params& p, bool bf16, int G, const Room& r, cudaStream_t st) {
   const bool part = p.K % STEP != 0;                       // groups of 128 leave no part of a step
-  if (G == 128) return bf16 ? launch<4, true, UP, OWN, false>(p, warps, smem, st) : launch<4, false, UP, OWN, false>(p, warps, smem, st);
+  if (G == 128) return bf16 ? launch<4, true, UP, false>(p, r, st) : launch<4, false, UP, false>(p, r, st);
   if (G == 64) {
-    if (part) return bf16 ? launch<2, true, UP, OWN, true>(p, warps, smem, st) : launch<2, false, UP, OWN, true>(p, warps, smem, st);
-    return bf16 ? launch<2, true, UP, OWN, false>(p, warps, smem, st) : launch<2, false, UP, OWN, false>(p, warps, smem, st);
+    if (part) return bf16 ? launch<2, true, UP, true>(p, r, st) : launch<2, false, UP, true>(p, r, st);
+    return bf16 ? launch<2, true, UP, false>(p, r, st) : launch<2, false, UP, false>(p, r, st);
   }
-  if (part) return bf16 ? launch<1, true, UP, OWN, true>(p, warps, smem, st) : launch<1, false, UP, OWN, true>(p, warps, smem, st);
-  return bf16 ? launch<1, true, UP, OWN, false>(p, warps, smem, st) : launch<1, false, UP, OWN, false>(p, warps, smem, st);
+  if (part) return bf16 ? launch<1, true, UP, true>(p, r, st) : launch<1, false, UP, true>(p, r, st);
+  return bf16 ? launch<1, true, UP, false>(p, r, st) : launch<1, false, UP, false>(p, r, st);
 }
 static size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 }  // namespace g4f
@@ -373,15 +362,15 @@ int moe_g4_few(const G4MoeArgs& a, void* scratch, cudaStream_t st) {
   p.x = reinterpret_cast<const uint16_t*>(a.x);
   p.w = Matrix{a.w13, reinterpret_cast<const uint16_t*>(a.s13), a.z13, a.H / 2, 2 * (int64_t)a.I};
   p.w_rows = 2 * (int64_t)a.I; p.s_expert = (int64_t)(a.H / a.G13) * 2 * a.I;
-  p.N = a.I; p.K = a.H; p.steps = (a.H + STEP - 1) / STEP; p.columns = q.up_columns; p.groups = groups_of(q.up_columns);
-  int rc = by_type<true, false>(p, a.bf16, a.G13, q.warps, q.smem_up, st);
+  p.N = a.I; p.K = a.H; p.steps = (a.H + STEP - 1) / STEP; 
+  int rc = by_type<true>(p, a.bf16, a.G13, q.up, st);
   if (rc) return rc;
   p.x = p.h;
   p.w = Matrix{a.w2, reinterpret_cast<const uint16_t*>(a.s2), a.z2, a.I / 2, a.H};
   p.w_rows = a.H; p.s_expert = (int64_t)(a.I / a.G2) * a.H;
-  p.N = a.H; p.K = a.I; p.steps = (a.I + STEP - 1) / STEP; p.columns = q.down_columns; p.groups = groups_of(q.down_columns);
-  if (q.own) return by_type<false, true>(p, a.bf16, a.G2, q.warps, q.smem_down, st);
-  rc = by_type<false, false>(p, a.bf16, a.G2, q.warps, q.smem_down, st);
+  p.N = a.H; p.K = a.I; p.steps = (a.I + STEP - 1) / STEP; 
+  p.early = tls().overlap_mode == 2;
+  rc = by_type<false>(p, a.bf16, a.G2, q.down, st);
   if (rc) return rc;
   const int64_t total = (int64_t)a.T * a.H, n = (total + 255) / 256;
   launch_overlapped(a.bf16 ? g4_pairs_sum_kernel<true> : g4_pairs_sum_kernel<false>, dim3((unsigned)std::min<int64_t>(n, 1184)), dim3(256), 0, st, tls().overlap_mode > 0, (const float*)p.y,
