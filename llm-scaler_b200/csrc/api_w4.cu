@@ -9,6 +9,9 @@ bool known(int dtype) { return dtype >= 0 && dtype <= 2; }
 bool is_group(int64_t g) { return g == 32 || g == 64 || g == 128; }
 constexpr int64_t MAX_ROWS = INT32_MAX - 4096;             // tokens and weight rows: rounded up to tiles and rounds of tiles, both below this
 constexpr int64_t MAX_K = 1 << 20;
+// set_force_kernel(2): tcgen05 for everything
+bool use_stream(int64_t M, int64_t N, int64_t K, int64_t group) { return tls().force_kernel != 2 && g4_stream_preferred((int)M, (int)N, (int)K, (int)group); }
+bool use_few(const G4MoeArgs& a) { return tls().force_kernel != 2 && moe_g4_few_preferred(a); }
 }  // namespace
 
 extern "C" {
@@ -33,7 +36,7 @@ int b2q_route_experts(const void* logits, int logits_dtype, int64_t ldl, const v
 
 size_t b2q_linear_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t group) {
   if (M <= 0 || N <= 0 || K <= 0 || !is_group(group) || M > MAX_ROWS || N > MAX_ROWS || K > MAX_K) return 0;
-  if (g4_stream_fits((int)M, (int)N, (int)K, (int)group)) return g4_stream_bytes((int)M, (int)N, (int)K, (int)group);
+  if (use_stream(M, N, K, group)) return g4_stream_bytes((int)M, (int)N, (int)K, (int)group);
   return umma_g4_bytes(nullptr, 0, (int)M, (int)N, (int)K, (int)group);
 }
 
@@ -54,7 +57,7 @@ int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8_t* w, c
   G4LinearArgs a{};
   a.x = x; a.ldx = ldx; a.bf16 = act_dtype == B2Q_BF16; a.w = w; a.scale = scale; a.zero = zero; a.bias = bias; a.out = out; a.ldo = ldo;
   a.M = (int)M; a.N = (int)N; a.K = (int)K; a.G = (int)group;
-  if (g4_stream_fits(a.M, a.N, a.K, a.G)) return g4_stream_linear(a, workspace, (cudaStream_t)stream);
+  if (use_stream(M, N, K, group)) return g4_stream_linear(a, workspace, (cudaStream_t)stream);
   return umma_g4_linear(a, workspace, (cudaStream_t)stream);
 }
 
@@ -83,7 +86,7 @@ int b2q_moe_forward_w4(const b2q_moe_w4* m, void* workspace, size_t workspace_by
   G4MoeArgs g{};
   g.x = a.x; g.bf16 = a.act_dtype == B2Q_BF16; g.weights = a.weights; g.ids = a.ids; g.w13 = a.w13; g.s13 = a.s13; g.z13 = a.z13; g.w2 = a.w2; g.s2 = a.s2; g.z2 = a.z2;
   g.out = a.out; g.T = (int)a.T; g.E = (int)a.E; g.k = (int)a.top_k; g.H = (int)a.H; g.I = (int)a.I; g.G13 = (int)a.group13; g.G2 = (int)a.group2;
-  if (moe_g4_few_preferred(g)) return moe_g4_few(g, workspace, (cudaStream_t)stream);
+  if (use_few(g)) return moe_g4_few(g, workspace, (cudaStream_t)stream);
   return moe_g4_many(g, workspace, (cudaStream_t)stream);
 }
 

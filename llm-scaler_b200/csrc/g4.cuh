@@ -23,7 +23,7 @@ struct G4LinearArgs {
   const void* bias; void* out; int64_t ldo;
   int M, N, K, G;
 };
-bool g4_stream_fits(int M, int N, int K, int G);           // up to sixteen tokens whose shares fit shared memory
+bool g4_stream_preferred(int M, int N, int K, int G);           // sixteen tokens at most
 size_t g4_stream_bytes(int M, int N, int K, int G);
 int g4_stream_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st);
 

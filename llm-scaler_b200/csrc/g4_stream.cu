@@ -277,7 +277,9 @@ template <int VEC, bool PART> static int by_type(Params& p, bool bf16, const Pla
 }
 }  // namespace g4s
 
-bool g4_stream_fits(int M, int N, int K, int G) { return M <= 16 && g4s::plan(M, N, K, G).smem > 0; }
+// Up to eight tokens, and up to sixteen of small layers (here / on tcgen05, us: 16 x 2048 x 2048 7.2 / 8.2, 16 x 1024 x 8192 9.1 / 11.2, 16 x 4096 x 4096 10.8 / 10.3, 12 x 28672 x
+// 2048 16.7 / 14.7, 16 x 17408 x 5120 24.0 / 18.8; 8 x 4096 x 4096 7.8 / 10.0).
+bool g4_stream_preferred(int M, int N, int K, int G) { return M <= (N * (int64_t)K <= 12 << 20 ? 16 : 8) && g4s::plan(M, N, K, G).smem > 0; }
 
 size_t g4_stream_bytes(int M, int N, int K, int G) {
   const g4s::Plan q = g4s::plan(M, N, K, G);

@@ -341,7 +341,9 @@ template <bool UP> static int by_type(Params& p, bool bf16, int G, const Room& r
 static size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 }  // namespace g4f
 
-bool moe_g4_few_preferred(const G4MoeArgs& a) { return g4f::plan(a).fits && a.T <= 32; }
+// Up to five rows per expert (few / many, us; rows per expert in brackets): 128 experts of 2048 x 768, top-8, 16 tokens [1] 67 / 89, 48 [3] 102 / 119; 8 of 4096 x 4096, top-2, 16 [4]
+// 70 / 90, 32 [8] 97 / 91; 64 of 2048 x 1408 in groups of 32, top-6, 32 [3] 123 / 124, 60 [5.6] 141 / 127; 16 of 2048 x 2048, top-4, 16 [4] 45 / 59, 32 [8] 57 / 60.
+bool moe_g4_few_preferred(const G4MoeArgs& a) { return (int64_t)a.T * a.k <= 5 * (int64_t)a.E && g4f::plan(a).fits; }
 
 size_t moe_g4_few_bytes(const G4MoeArgs& a) {
   const size_t pairs = (size_t)a.T * a.k;
