@@ -35,7 +35,7 @@ int b2q_route_experts(const void* logits, int logits_dtype, int64_t ldl, const v
 }
 
 size_t b2q_linear_w4_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t group) {
-  if (M <= 0 || N <= 0 || K <= 0 || !is_group(group) || M > MAX_ROWS || N > MAX_ROWS || K > MAX_K) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || !is_group(group) || K % group != 0 || M > MAX_ROWS || N > MAX_ROWS || K > MAX_K) return 0;
   if (use_stream(M, N, K, group)) return g4_stream_bytes((int)M, (int)N, (int)K, (int)group);
   return umma_g4_bytes(nullptr, 0, (int)M, (int)N, (int)K, (int)group);
 }
@@ -45,7 +45,7 @@ int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8_t* w, c
   if (!x || !w || !scale || !out) return B2Q_ERR_NULL;
   if (!is16(act_dtype)) return B2Q_ERR_DTYPE;
   if (M < 0 || N < 0 || K <= 0 || !is_group(group) || K % group != 0 || ldx < K || ldo < N) return B2Q_ERR_SHAPE;
-  if (M > MAX_ROWS || N > MAX_ROWS || K > MAX_K) return B2Q_ERR_LIMIT;
+  if (M > MAX_ROWS || N > MAX_ROWS || K > MAX_K || N > INT32_MAX / (K / group)) return B2Q_ERR_LIMIT;
   if (!aligned16(w) || !aligned_to(x, 2) || !aligned_to(scale, 2) || !aligned_to(bias, 2) || !aligned_to(out, 2)) return B2Q_ERR_ALIGN;
   if (M == 0 || N == 0) return B2Q_OK;
   const size_t need = b2q_linear_w4_workspace_bytes(M, N, K, group);
@@ -62,7 +62,7 @@ int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8_t* w, c
 }
 
 size_t b2q_moe_forward_w4_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I) {
-  if (T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || top_k > 32 || H <= 0 || I <= 0 || T > INT32_MAX / 32) return 0;
+  if (T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || top_k > 32 || H <= 0 || I <= 0 || H > MAX_K || I > MAX_K || T > INT32_MAX / 32) return 0;
   G4MoeArgs g{};
   g.T = (int)T; g.E = (int)E; g.k = (int)top_k; g.H = (int)H; g.I = (int)I;
   const size_t few = moe_g4_few_bytes(g), many = moe_g4_many_bytes(g);      // which form it will be depends on the groups too
@@ -75,7 +75,9 @@ int b2q_moe_forward_w4(const b2q_moe_w4* m, void* workspace, size_t workspace_by
   if (!a.x || !a.weights || !a.ids || !a.w13 || !a.s13 || !a.w2 || !a.s2 || !a.out) return B2Q_ERR_NULL;
   if (!is16(a.act_dtype)) return B2Q_ERR_DTYPE;
   if (a.T < 0 || a.E <= 0 || a.top_k <= 0 || a.H <= 0 || a.I <= 0 || !is_group(a.group13) || !is_group(a.group2) || a.H % a.group13 != 0 || a.I % a.group2 != 0) return B2Q_ERR_SHAPE;
-  if (a.E > 1024 || a.top_k > 32 || a.H > MAX_K || a.I > MAX_K || a.T > INT32_MAX / 32 || 2 * a.E * a.I > INT32_MAX || a.E * a.H > INT32_MAX) return B2Q_ERR_LIMIT;
+  if (a.E > 1024 || a.top_k > 32 || a.H > MAX_K || a.I > MAX_K || a.T > INT32_MAX / 32 || 2 * a.E * a.I > INT32_MAX || a.E * a.H > INT32_MAX ||
+      2 * a.I > INT32_MAX / (a.H / a.group13) || a.H > INT32_MAX / (a.I / a.group2) || !moe_g4_many_fits(a.T, a.E, a.top_k, a.H, a.I))
+    return B2Q_ERR_LIMIT;
   if (!aligned16(a.x) || !aligned16(a.w13) || !aligned16(a.w2) || !aligned16(a.out) || !aligned_to(a.s13, 2) || !aligned_to(a.s2, 2) || !aligned_to(a.weights, 4) ||
       !aligned_to(a.ids, 4))
     return B2Q_ERR_ALIGN;

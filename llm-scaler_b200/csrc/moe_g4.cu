@@ -84,6 +84,11 @@ static Parts parts_of(void* ws, const G4MoeArgs& a) {
 }
 }  // namespace g4m
 
+bool moe_g4_many_fits(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
+  const int64_t tile = g4_grouped_tile(T * k, (int)E), tiles = (T * k + tile - 1) / tile + E;
+  return tiles * ((I + 127) / 128) <= INT32_MAX / 2 && tiles * ((H + 255) / 256) <= INT32_MAX / 2;
+}
+
 size_t moe_g4_many_bytes(const G4MoeArgs& a) { return g4m::parts_of(nullptr, a).total; }
 
 int moe_g4_many(const G4MoeArgs& a, void* scratch, cudaStream_t st) {

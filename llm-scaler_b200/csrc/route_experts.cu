@@ -52,9 +52,9 @@ __device__ __forceinline__ double value(Key k) { return value_of(k); }
 __device__ __forceinline__ float value(uint32_t k) { return value32(k); }
 
 // How far the fp32 keys may be off, relative to the larger of 1 and the key.  __expf is good to 2 + 1.17 |x| units of 2^-23, so that a sigmoid's p (1 - p) |x| of it is below 2^-23, the
-// quotient's two units are another 2^-23 at most, and the sums with 1 and with the bias are rounded to 2^-24.  A softmax has 2^-22 of its exponential and as much
-// of the sum of all, and 2^-21 at most of that sum's roundings.
-template <bool SIGMOID> constexpr float EPS = SIGMOID ? 4.76837158203125e-7f : 9.5367431640625e-7f;      // 2^-21, 2^-20
+// quotient's two units are another 2^-23 at most, and the sums with 1 and with the bias are rounded to 2^-24.  A softmax has 2^-22 of its exponential and as much of those that its
+// sum is made of, and that sum's roundings: PER a lane, five over lanes, and a reciprocal.
+template <bool SIGMOID, int PER> constexpr float EPS = SIGMOID ? 4.76837158203125e-7f : 4.76837158203125e-7f + (PER + 6) * 5.9604644775390625e-8f;      // 2^-21; 2^-24
 
 // Values of experts lane + 32 j; `beyond` from E on.
 template <int PER> __device__ __forceinline__ void load_row(float (&v)[PER], const void* from, int64_t at, int dt, int E, float beyond) {
@@ -86,7 +86,7 @@ __device__ __forceinline__ bool choose(K (&key)[PER], const K (&gkey)[TOP2 ? PER
   bool sure = true;
   auto apart = [](K a, K b, float times) {                 // a >= b, both there
     const float x = (float)value(a), y = (float)value(b);
-    return x - y > times * EPS<SIGMOID> * fmaxf(1.f, fmaxf(fabsf(x), fabsf(y)));
+    return x - y > times * EPS<SIGMOID, PER> * fmaxf(1.f, fmaxf(fabsf(x), fabsf(y)));
   };
   if constexpr (GROUPS) {
     K mine = 0;                                            // lane g: of group g

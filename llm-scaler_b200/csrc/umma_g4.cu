@@ -692,6 +692,7 @@ int umma_g4_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st) {
   using namespace ug4;
   if (!tensor_map_encoder()) return B2Q_ERR_CUDA;
   const Plan q = plan(a.M, a.N, a.K);
+  if ((int64_t)q.n_strips * q.m_tiles * q.pieces > INT32_MAX / 8) return B2Q_ERR_LIMIT;
   uint8_t* at = reinterpret_cast<uint8_t*>(scratch);
   const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x);
   int64_t ldx = a.ldx;
@@ -708,7 +709,6 @@ int umma_g4_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st) {
   p.bias = reinterpret_cast<const uint16_t*>(a.bias); p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.ldo; p.vec_out = aligned16(a.out) && a.ldo % 8 == 0;
   p.M = a.M; p.N = a.N; p.K = a.K; p.groups = a.K / a.G; p.nks = (a.K + 127) / 128;
   p.n_strips = q.n_strips; p.m_tiles = q.m_tiles; p.m_group = q.m_tiles < 16 ? q.m_tiles : 16; p.pieces = q.pieces;
-  if ((int64_t)q.n_strips * q.m_tiles * q.pieces > INT32_MAX / 8) return B2Q_ERR_LIMIT;
   p.total = q.n_strips * q.m_tiles * q.pieces;
   if (q.pieces > 1) {
     p.partials = reinterpret_cast<float*>(at);
@@ -754,7 +754,6 @@ int umma_g4_grouped(const G4GroupedArgs& a, cudaStream_t st) {
   p.status = umma_status_ptr();
   if (!p.status) return B2Q_ERR_CUDA;
   const int64_t w_rows = (int64_t)a.E * p.s_rows;
-  if (w_rows > INT32_MAX || (int64_t)a.tile_cap * p.n_strips > INT32_MAX / 2) return B2Q_ERR_LIMIT;
   CUtensorMap tx, tw;
   int rc = make_tmap_2d(&tx, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.x, a.rows, a.K, (uint64_t)a.K * 2, a.tile / 2, 64,
                         CU_TENSOR_MAP_SWIZZLE_128B);
