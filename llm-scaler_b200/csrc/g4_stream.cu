@@ -224,7 +224,7 @@ static Plan plan(int M, int N, int K, int G) {
     const int rows = (N + q.clusters - 1) / q.clusters, most = (q.steps + q.C - 1) / q.C;
     q.cap = (rows + ROWS - 1) / ROWS;
     // (fewer where there is little for each to do: 1 x 2048 x 2048 4.6 us with sixteen, 4.15 with twelve; 1 x 28672 x 8192 28.1 and 30.4)
-    for (q.warps = q.cap * most >= 4 * MOST_WARPS ? MOST_WARPS : 12; q.warps >= 12; q.warps -= 4) {
+    for (q.warps = (int64_t)q.cap * most >= 4 * MOST_WARPS ? MOST_WARPS : 12; q.warps >= 12; q.warps -= 4) {
       const int64_t front = (int64_t)q.warps * WARP_BYTES + (int64_t)most * step_bytes(M, G, q.tt);
       const int64_t smem = front + (int64_t)(q.cap + q.warps) * ROWS * 8 * q.tt * 4;
       q.self = M * q.steps * (STEP / 8) <= SELF * 32 * q.warps;

@@ -21,6 +21,7 @@ int dtype_of(const Tensor& t) {
   TORCH_CHECK(false, "b2q: unsupported dtype ", t.scalar_type());
 }
 bool is16(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+// Messages are made of strings alone: a compiler that puts libstdc++ into the library gives it a second set of the facets that print numbers, and printing one ended the process.
 void check(int rc) { TORCH_CHECK(rc == 0, b2q_strerror(rc)); }
 
 // all on one CUDA device, that of the first
@@ -56,7 +57,7 @@ Weight weight_of(const char* name, const Tensor& x, const Tensor& w, const Tenso
               " tensor");
   TORCH_CHECK(r.K > 0 && r.K % s.size(d) == 0, name, " scale has a number of groups that does not divide K");
   r.group = r.K / s.size(d);
-  TORCH_CHECK(r.group == 32 || r.group == 64 || r.group == 128, name, " groups must have 32, 64 or 128 values, not ", r.group);
+  TORCH_CHECK(r.group == 32 || r.group == 64 || r.group == 128, name, " groups must have 32, 64 or 128 values");
   if (d) TORCH_CHECK(w.size(0) == experts && s.size(0) == experts, name, " weight and scale must have the same number of experts");
   if (z.has_value()) {
     same_device({&x, &*z});
