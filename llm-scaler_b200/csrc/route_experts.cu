@@ -5,9 +5,12 @@
 // the scores that a group's two best add up to.  So no rounding of the scores decides between two experts, and equal keys go to the lowest index.
 // Weights are fp32, of the scores without the bias.
 //
-// Latency-bound: a warp per token, its logits in registers, k rounds of a warp-wide maximum.  Scores are made in fp32 first, good to EPS; where no two
-// that the choice depends on are nearer to each other than their errors, it is the one of 64 bits, and only the other tokens are done again in those (in 64
-// bits throughout: 4093 tokens of 256 experts 24 us; see the table of cases for now).
+// Bound by issue slots (4093 tokens of 256 experts: 1090 instructions a token, nearly half of all slots) and, for a few tokens, by its chain of exchanges.  A warp per token,
+// its logits in registers.  The need-th largest of the lanes' maxima leaves a dozen experts or so, which are then ranked by counting, a lane each; k rounds of a
+// warp-wide maximum over all registers took 13.8 us where this takes 11.1 (16384 tokens of 128 experts: 10.5 and 9.5; one of 256: 4.5 and 3.6).  Groups of 32
+// experts are registers, whose two best change hands by halves, and are ranked in the same way.
+// Scores are made in fp32 first, good to EPS; where no two that the choice depends on are nearer to each other than their errors, it is the one of 64 bits, and
+// only the other tokens are done again in those (in 64 bits throughout: 24 us, when the rest took 14).
 #include "g4.cuh"
 
 namespace b2q {
@@ -100,12 +103,28 @@ __device__ __forceinline__ bool choose(K (&key)[PER], const K (&gkey)[TOP2 ? PER
       }
       return best;
     };
-    if (p.size == 32) {                                    // a register each
+    if (p.size == 32) {                                    // a register each: halves change hands until a lane has one group, then its lanes agree
+      K a[PER], b[PER];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const K best = of_group(TOP2 ? gkey[TOP2 ? j : 0] : key[j], 0);
-        if (lane == j) mine = best;
+      for (int j = 0; j < PER; ++j) { a[j] = TOP2 ? gkey[TOP2 ? j : 0] : key[j]; b[j] = 0; }
+#pragma unroll
+      for (int n = PER / 2, o = 16; o > 0; n /= 2, o /= 2) {
+        const bool upper = lane & o;
+#pragma unroll
+        for (int j = 0; j < (n ? n : 1); ++j) {
+          const K c = __shfl_xor_sync(0xffffffffu, n && !upper ? a[j + n] : a[j], o);
+          const K own = n && upper ? a[j + n] : a[j];
+          if (TOP2) {
+            const K d = __shfl_xor_sync(0xffffffffu, n && !upper ? b[j + n] : b[j], o);
+            b[j] = max(max(n && upper ? b[j + n] : b[j], d), min(own, c));
+          }
+          a[j] = max(own, c);
+        }
       }
+      K best = a[0];
+      if (TOP2) best = best && b[0] ? as_key(value(best) + value(b[0]), K{}) : 0;
+      mine = __shfl_sync(0xffffffffu, best, lane * (32 / PER) & 31);
+      if (lane >= p.groups) mine = 0;
     } else {
       for (int g = 0; g < p.groups; ++g) {
         const int lo = g * p.size, hi = lo + p.size;
@@ -121,18 +140,17 @@ __device__ __forceinline__ bool choose(K (&key)[PER], const K (&gkey)[TOP2 ? PER
         if (lane == g) mine = best;
       }
     }
-    uint32_t keep = 0;
-    K last = 0;
-    for (int i = 0; i < p.top_groups; ++i) {
-      const K best = warp_max(mine);
-      if (best == 0) break;
-      last = best;
-      const int g = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
-      keep |= 1u << g;
-      if (lane == g) mine = 0;
+    int rank = 0;                                          // among the groups; equal ones by their index
+#pragma unroll 8
+    for (int g = 0; g < p.groups; ++g) {
+      const K other = __shfl_sync(0xffffffffu, mine, g);
+      rank += other > mine || (other == mine && g < lane);
     }
+    if (lane >= p.groups) rank = 32;
+    const uint32_t keep = __ballot_sync(0xffffffffu, mine != 0 && rank < p.top_groups);
     if (CHECK) {
-      const K next = warp_max(mine);
+      const K last = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, rank == p.top_groups - 1)) - 1);
+      const K next = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, rank == p.top_groups)) - 1);
       if (next) sure = apart(last, next, TOP2 ? 4.f : 2.f);
     }
 #pragma unroll
@@ -143,26 +161,67 @@ __device__ __forceinline__ bool choose(K (&key)[PER], const K (&gkey)[TOP2 ? PER
   }
   id = -1;
   K mine = 0;                                              // lane i: the key of its choice; lane k: of the best that is left
-  for (int i = 0; i < p.k + (CHECK ? 1 : 0); ++i) {
-    K best = 0;
+  const int need = p.k + (CHECK ? 1 : 0);
+  // The need-th largest of the lanes' maxima (1, if there are fewer) is no larger than the need-th largest of all: what is below it is out.
+  K least = 1, top = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) best = max(best, key[j]);
-    best = warp_max(best);
+  for (int j = 0; j < PER; ++j) top = max(top, key[j]);
+  for (int left = need; left > 0;) {
+    const K best = warp_max(top);
+    least = max(best, (K)1);
     if (best == 0) break;
-    if (CHECK && (lane == i || (i == 32 && lane == 31))) {
-      if (i == 32) sure = sure && apart(mine, best, 2.f);
-      else mine = best;
+    left -= __popc(__ballot_sync(0xffffffffu, top == best));
+    if (top == best) top = 0;
+  }
+  // The others, a lane each in the order of their index, are ranked by counting.
+  __shared__ struct { K key[32]; int e[32]; } all[WARPS];
+  auto& of = all[threadIdx.x >> 5];
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const bool in = key[j] >= least;
+    const uint32_t who = __ballot_sync(0xffffffffu, in);
+    const int at = n + __popc(who & ((1u << lane) - 1));
+    if (in && at < 32) { of.key[at] = key[j]; of.e[at] = lane + 32 * j; }
+    n += __popc(who);
+  }
+  __syncwarp();
+  if (n <= 32) {
+    const K own = lane < n ? of.key[lane] : 0;
+    const int e = of.e[lane];
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const K other = of.key[i];
+      rank += other > own || (other == own && i < lane);
     }
-    if (i == p.k) break;
-    uint32_t e = 0xFFFFu;
+    __syncwarp();
+    if (lane < n) { of.key[rank] = own; of.e[rank] = e; }
+    __syncwarp();
+    if (lane < n && lane < need) mine = of.key[lane];
+    if (lane < n && lane < p.k) id = of.e[lane];
+  } else {                                                 // equal ones, for the most part
+    for (int i = 0; i < need; ++i) {
+      K best = 0;
 #pragma unroll
-    for (int j = PER - 1; j >= 0; --j)
-      if (key[j] == best) e = lane + 32 * j;
-    e = __reduce_min_sync(0xffffffffu, e);
+      for (int j = 0; j < PER; ++j) best = max(best, key[j]);
+      best = warp_max(best);
+      if (best == 0) break;
+      if (CHECK && (lane == i || (i == 32 && lane == 31))) {
+        if (i == 32) sure = sure && apart(mine, best, 2.f);
+        else mine = best;
+      }
+      if (i == p.k) break;
+      uint32_t e = 0xFFFFu;
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (lane + 32 * j == (int)e) key[j] = 0;
-    if (lane == i) id = (int)e;
+      for (int j = PER - 1; j >= 0; --j)
+        if (key[j] == best) e = lane + 32 * j;
+      e = __reduce_min_sync(0xffffffffu, e);
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (lane + 32 * j == (int)e) key[j] = 0;
+      if (lane == i) id = (int)e;
+    }
   }
   if (CHECK) {
     const K next = __shfl_down_sync(0xffffffffu, mine, 1);

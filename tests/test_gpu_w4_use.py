@@ -206,6 +206,33 @@ def test_route_of_one_expert():
         check_route(torch.randn(5, 1, generator=gen(0)).to(dt), 1, scoring="sigmoid", renormalize=False)
 
 
+@pytest.mark.parametrize("T,E", [(150, 128), (700, 4), (1500, 3)])
+def test_a_token_comes_out_the_same_wherever_it_stands(T, E):
+    """The rows of an expert are collected by atomics: their order, and so the tile a row is in, changes from call to call, its bits do not."""
+    a = dev(*moe_inputs(T, E, 2, 256, 288, 64, 32, "bf16"))
+    want = e.moe_forward_w4(*a)
+    for seed in range(6):
+        order = torch.randperm(T, generator=gen(seed)).to(DEV)
+        assert torch.equal(e.moe_forward_w4(*(t[order] for t in a[:3]), *a[3:]), want[order])
+
+
+def test_route_of_equal_and_of_many_near_experts():
+    """More than a warp's lanes of candidates, and choices that only 64 bits tell apart among them."""
+    g = gen(3)
+    l = torch.zeros(12, 256)
+    l[1] = 1 + torch.arange(256) % 3 * 2.0 ** -23
+    l[2, 100:] = -1
+    l[3] = torch.arange(256) // 8 * 0.5
+    l[4] = torch.randint(0, 2, (256,), generator=g) * 1.0
+    l[5:] = 0.5 + torch.randint(0, 4, (7, 256), generator=g) * 2.0 ** -24
+    bias = torch.randint(0, 3, (256,), generator=g) * 2.0 ** -24
+    for kw in ({}, dict(scoring="sigmoid"), dict(scoring="sigmoid", bias=bias), dict(bias=bias), dict(num_groups=8, top_groups=3), dict(num_groups=8, top_groups=3, group_score="top2"),
+               dict(scoring="sigmoid", bias=bias, num_groups=8, top_groups=4, group_score="top2"), dict(num_groups=16, top_groups=5, group_score="top2", bias=bias)):
+        for k in (1, 8, 32):
+            check_route(l, k, **kw)
+            check_route(l[:, :192].contiguous(), min(k, 24), **{n: v[:192].contiguous() if torch.is_tensor(v) else v for n, v in kw.items()})
+
+
 # ------------------------------------------------------------------------------------------- offsets beyond 32 bits
 def test_linear_weight_beyond_two_gib():
     N, K, G = 70000, 65536, 128
