@@ -2,7 +2,11 @@
 // in its epilogue, a grouped GEMM whose outputs are multiplied by the routes' weights, the sum of each token's rows.
 //
 // h and the weighted outputs have 16 bits in between: h because it is the second product's operand; the outputs, one rounding each before the sum of top_k of them,
-// because they are read and written once (67 M values for 4096 tokens, top-8, H = 2048).
+// because they are read and written once (67 M values for 4096 tokens, top-8, H = 2048).  An expert's rows come in any order, which changes no bits: a row's sums depend on the
+// expert and the output alone, not on the tile that it is in.
+//
+// Each kernel lets the next begin only when all before itself are done, so that the GEMMs read the tile list, weights and scales before the tokens are there (311 tokens of 64 experts
+// 127.8 -> 121.1 us; 4096 of 128 422 -> 387).
 #include "i8.cuh"
 #include "g4.cuh"
 
@@ -17,7 +21,8 @@ struct Copies {
 // A CTA per token: its row to the row of each of its pairs, the values of every eight in the order that the grouped kernel wants.
 __global__ void __launch_bounds__(256) g4_copies_kernel(const uint4* x, uint4* to, int per, const Copies c) {
   __shared__ int rows[32];
-  grid_dep_enter();
+  grid_dep_wait();
+  grid_dep_release();                                      // in this order: the next kernel may then read the tile list and weights at once
   const int t = blockIdx.x;
   if (threadIdx.x < c.k) {
     const int64_t pair = (int64_t)t * c.k + threadIdx.x;

@@ -60,7 +60,7 @@ struct Params {
   int n_strips, m_tiles, m_group, pieces, total;           // total: tiles of a dense launch
   float* partials; Arrivals* arrivals; Arrivals tag; const Arrivals* epoch;
   const int32_t* tiles; const int32_t* offsets;            // grouped
-  int early;
+  int early;                                               // weights (grouped: and the tile list) may be read before the kernel in front is done
   uint32_t mask, magic;                                    // of the decode: as constants they take an operation each
   int* status;
 };
@@ -228,7 +228,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
   const uint32_t rank = cluster_ctarank();
   const int first = (int)blockIdx.x / 2, step = (int)gridDim.x / 2;
 
-  grid_dep_release();
+  if (!GROUPED) grid_dep_release();
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::S; ++i) { mbar_init(full + 8 * i, 9); mbar_init(empty + 8 * i, 1); }
     for (int i = 0; i < C::RS; ++i) { mbar_init(raw_full + 8 * i, 1); mbar_init(raw_empty + 8 * i, 4); }
@@ -247,7 +247,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
   const uint32_t tmem = *tmem_slot;
   int total = p.total, known = 0;
   if constexpr (GROUPED) {
-    grid_dep_wait();                                       // the tile list is made by the kernels in front
+    if (!p.early) grid_dep_wait();                         // early: the tile list was there when the kernel in front let this one begin
     total = __ldcg(p.tiles) * p.n_strips;
     const int mine = first < total ? (total - first + step - 1) / step : 0;
     known = min(mine, C::TABLE);
@@ -289,6 +289,7 @@ umma_g4_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
     if (elect_one()) {
       tma_prefetch_desc(&tm_x);
       grid_dep_wait();
+      if (GROUPED) grid_dep_release();                     // the next one may read the tile list at once, and weights
       int s = 0, issued = 0;
       uint32_t par = 1u;
       bool ok = true;
@@ -753,6 +754,7 @@ int umma_g4_grouped(const G4GroupedArgs& a, cudaStream_t st) {
   p.mask = MASK; p.magic = a.bf16 ? MAGIC_BF16 : MAGIC_F16;
   p.status = umma_status_ptr();
   if (!p.status) return B2Q_ERR_CUDA;
+  p.early = tls().overlap_mode > 0;
   const int64_t w_rows = (int64_t)a.E * p.s_rows;
   CUtensorMap tx, tw;
   int rc = make_tmap_2d(&tx, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.x, a.rows, a.K, (uint64_t)a.K * 2, a.tile / 2, 64,
