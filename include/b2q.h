@@ -406,7 +406,8 @@ B2Q_API int b2q_route_experts(const void* logits, int logits_dtype, int64_t ldl,
                       int64_t T, int64_t E, int64_t top_k, int scoring, int64_t num_groups, int64_t top_groups, int group_score,
                       int renormalize, float scale, void* stream);
 
-/* out[m, n] = sum_k x[m, k] (q[n, k] - zero[k / group, n]) scale[k / group, n] (+ bias[n]), one rounding to act_dtype.  w holds q contiguous [N, K / 2], even k
+/* out[m, n] = sum_k x[m, k] (q[n, k] - zero[k / group, n]) scale[k / group, n] (+ bias[n]), sums in fp32, one rounding to act_dtype; with more than a few
+ * tokens each (q - zero) scale is rounded to act_dtype too.  w holds q contiguous [N, K / 2], even k
  * in the low half of a byte (as little-endian int32: eight values, lowest nibble first); scale [K / group, N] and zero [K / group, N] (uint8, any value;
  * NULL: 8 everywhere) contiguous.  x [M, K] with row pitch ldx, scale, bias, out (row pitch ldo) in act_dtype (bf16 / fp16).  group 32, 64 or 128,
  * K % group == 0, any M and N; w 16-byte aligned, the others to their elements (x rows that start on 16 bytes save a copy for many tokens).
@@ -419,7 +420,8 @@ B2Q_API int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8
 /* A whole expert layer on 4-bit experts for given routes: out[t] = sum over s of weights[t, s] y(ids[t, s], x[t]), y(e, x) = W2_e (silu(G_e x) * U_e x); ids outside
  * [0, E) contribute nothing (an expert of another rank, padding), an expert named twice counts twice.  w13 [E, 2I, H / 2] (gate rows, then up), s13 and z13
  * [E, H / group13, 2I], w2 [E, H, I / 2], s2 and z2 [E, I / group2, H], in the forms of b2q_linear_w4, all contiguous; z13, z2 may be NULL.  x, out
- * contiguous [T, H] and scales in act_dtype, 16-byte aligned; weights fp32 and ids int32 contiguous [T, top_k].  E <= 1024, top_k <= 32.             */
+ * contiguous [T, H] and scales in act_dtype; x, w13, w2 and out 16-byte aligned; weights fp32 and ids int32 contiguous [T, top_k].  E <= 1024, top_k <= 32.
+ * h is rounded to act_dtype; with many tokens so are the weights, and each weighted y before the sum.  workspace as above.                        */
 typedef struct b2q_moe_w4 {
   const void* x;
   const float* weights; const int32_t* ids;
@@ -568,8 +570,8 @@ B2Q_API int b2q_device_status_reset(void);
 B2Q_API int b2q_selftest_bounded_wait(int code, int* gave_up, void* stream);
 
 /* Kernel selection override for benchmarking: 0 = automatic, 1 = the mma.sync streaming kernel,
- * 2 = the tcgen05 kernel with 16-bit operands (8-bit integer operators: theirs, and an expert layer's grouped form; scratch
- * is asked for while the override is set), 3 = the same without activation pre-pass,
+ * 2 = the tcgen05 kernel with 16-bit operands (8-bit integer and 4-bit group-quantised operators: theirs, and an expert layer's
+ * grouped form; scratch is asked for while the override is set), 3 = the same without activation pre-pass,
  * 4 = the same with one CTA per strip (no strip cutting), 5 = INT4 decode on the int8 MMA (its scratch is asked for
  * while the override is set),
  * 6 = the CTA-pair (cta_group::2) variant of the W8A8 GEMM, 7 = the INT4 decode streaming kernel, 8 = the FP8 streaming

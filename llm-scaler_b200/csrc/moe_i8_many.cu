@@ -3,7 +3,8 @@
 // Routing.  A CTA routes a run of tokens, a warp each in turn, and counts its pairs per expert in shared memory; the place a pair is counted at
 // is its place among the CTA's pairs of that expert.  The last CTA to finish (arrivals.cuh) turns the counts into where each CTA's pairs of an
 // expert begin in the sorted order, and lists the tiles.  Where a pair's row is then follows from its expert, its CTA and its place.  Which
-// of a CTA's pairs comes first is a matter of chance, and no result depends on it: a row of the sorted order does not see the others.
+// of a CTA's pairs comes first is a matter of chance, and no result depends on it: a row of the sorted order does not see the others.  The 4-bit expert layer, whose
+// routes are given, has its pairs sorted here too.
 // 4096 tokens, 128 experts, top-8: five launches of 27 us before (top-k, a stable sort in three, tiles).
 //
 // Weighted sum.  Memory-bound; a thread has eight columns of a token and requests eight experts' rows at a time, or four in fp32.  An expert's output
