@@ -3,7 +3,8 @@
 // HBM-bound: the weights are read once, and there is little time to convert them (g4_stream.cuh has the mathematics and the layout).  A CTA per SM has rows of its own, dealt
 // out evenly.  Its units (32 rows of 128 k each) go to its warps in equal runs; a warp's next units are on their way while one is multiplied, and
 // nothing in the loop waits for another warp.  A warp leaves its sums of a tile of rows in a slot of shared memory; at the end they are added up in the
-// order of warps, so that results are the same every time.
+// order of warps, so that results are the same every time.  In graphs: 1 x 28672 x 8192 28.1 us (4.4 TB/s), 1 x 2048 x 2048 4.2, 7 x 5120 x 13824 in groups of 64 18.1.  Tiles of sixteen
+// rows or fewer count as whole ones: dealt out as halves they made the first 30.3.
 //
 // The tokens are scaled and permuted by each CTA for itself where that is one round of loads, else by a kernel in front, whose image of shared memory the CTAs
 // then fetch with one bulk copy, under the first weights.  Where the image does not fit, a cluster of two or four CTAs has rows together and a share of k each; their sums

@@ -1,7 +1,7 @@
 // The 4-bit expert layer of a few tokens for given routes: two kernels that stream the chosen experts' weights (g4_stream.cuh has the mathematics and the layout), and a sum where
 // tokens are more than a handful.
 //
-// HBM-bound for a batch, a chain of latencies for one token.  Every CTA sorts the routes by itself, in shared memory: the pairs (token, slot) of an expert form groups of
+// A chain of latencies for one token (128 experts of 2048 x 768, top-8: 20.8 us in a graph, 3.0 of bytes), issue slots and HBM for a batch (16 tokens: 71 us, 3.0 TB/s).  Every CTA sorts the routes by itself, in shared memory: the pairs (token, slot) of an expert form groups of
 // up to eight, whose tokens are the columns of one MMA.  A tile is 32 weight rows of one group; CTAs have equal runs of the tiles of all groups, and their
 // warps equal runs of the tiles' steps of 128 k, as in the linear.
 //  * up: a tile has sixteen gate rows and the sixteen up rows of the same outputs; h = silu(gate) * up goes out in 16 bits, with its largest magnitude per tile, from which the

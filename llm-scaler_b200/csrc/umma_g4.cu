@@ -15,6 +15,9 @@
 //  * Where strips of 256 rows are fewer than pairs of SMs, k is cut into pieces; whoever delivers the last of a strip's partial sums adds them up in order (arrivals.cuh).
 //  * GATED (expert up projection): a warp's 32 rows are 16 gate and 16 up rows of the same outputs, and the epilogue stores silu(gate) * up.
 //
+// In graphs: 4001 x 17408 x 5120 494 to 543 us by the GPU's power (1.3 to 1.44 PFLOP/s), 33 x 17408 x 5120 in groups of 32 22.2, 100 x 4096 x 4096 18.5; what bounds those up to 128 tokens is the
+// transform, 650 to 750 cycles for a stage.
+//
 // No multicast load; every mbarrier wait is bounded, as in the other tcgen05 kernels.
 #include <type_traits>
 #include "umma_gemm.cuh"
