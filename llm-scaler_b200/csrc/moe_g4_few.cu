@@ -1,7 +1,7 @@
 // The 4-bit expert layer of a few tokens for given routes: two kernels that stream the chosen experts' weights (g4_stream.cuh has the mathematics and the layout), and a sum where
 // tokens are more than a handful.
 //
-// A chain of latencies for one token (128 experts of 2048 x 768, top-8: 20.8 us in a graph, 3.0 of bytes), issue slots and HBM for a batch (16 tokens: 71 us, 3.0 TB/s).  Every CTA sorts the routes by itself, in shared memory: the pairs (token, slot) of an expert form groups of
+// A chain of latencies for one token (128 experts of 2048 x 768, top-8: 19.1 us in a graph, 3.0 of bytes), issue slots and HBM for a batch (16 tokens: 71 us, 3.0 TB/s).  Every CTA sorts the routes by itself, in shared memory: the pairs (token, slot) of an expert form groups of
 // up to eight, whose tokens are the columns of one MMA.  A tile is 32 weight rows of one group; CTAs have equal runs of the tiles of all groups, and their
 // warps equal runs of the tiles' steps of 128 k, as in the linear.
 //  * up: a tile has sixteen gate rows and the sixteen up rows of the same outputs; h = silu(gate) * up goes out in 16 bits, with its largest magnitude per tile, from which the
@@ -35,7 +35,6 @@ struct alignas(16) Shared {
   int ids[MAX_PAIRS];
   int count[MAX_E];                                        // pairs of an expert, then where they begin
   int16_t pairs[MAX_PAIRS];                                // sorted by expert
-  int16_t place[MAX_PAIRS];                                // of a pair among the sorted; -1: no expert
   Group groups[MAX_PAIRS];
   int warp_sum[WARPS][2];
   int n_groups;
@@ -46,6 +45,28 @@ struct alignas(16) Shared {
 // The routes' pairs sorted by expert, those of an expert by their number: all CTAs of both kernels have to agree on which group a pair is in.
 __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
   const int n = p.T * p.k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (n <= 32) {                                           // one warp, by counting (1 token, top-8: the layer 19.1 us in a graph, 20.8 with what is below)
+    if (warp == 0) {
+      int id = lane < n ? __ldcg(p.ids + lane) : -1;
+      if ((uint32_t)id >= (uint32_t)p.E) id = -1;
+      int at = 0, same = 0, all = 0;                       // pairs in front of this one; of its expert: in front, and in all
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const int other = __shfl_sync(0xffffffffu, id, j);
+        all += other == id;
+        same += other == id && j < lane;
+        at += other >= 0 && other < id;
+      }
+      at += same;
+      const bool first = id >= 0 && same % TOK == 0;
+      const uint32_t groups = __reduce_or_sync(0xffffffffu, first ? 1u << at : 0u);
+      if (first) sh.groups[__popc(groups & ((1u << at) - 1))] = Group{(int16_t)id, (int16_t)at, (int16_t)min(TOK, all - same)};
+      if (id >= 0) sh.pairs[at] = (int16_t)lane;
+      if (lane == 0) sh.n_groups = __popc(groups);
+    }
+    __syncthreads();
+    return;
+  }
   for (int e = threadIdx.x; e < p.E; e += THREADS) sh.count[e] = 0;
   __syncthreads();
   int id = -1, at = 0;
@@ -90,9 +111,7 @@ __device__ __forceinline__ void sort_routes(Shared& sh, const Params& p) {
   }
   __syncthreads();
   if (threadIdx.x < n) {
-    const int to = id >= 0 ? sh.count[id] + at : -1;
-    sh.place[threadIdx.x] = (int16_t)to;
-    if (to >= 0) sh.pairs[to] = (int16_t)threadIdx.x;
+    if (id >= 0) sh.pairs[sh.count[id] + at] = (int16_t)threadIdx.x;
   }
   __syncthreads();
 }
