@@ -3,7 +3,7 @@
 // HBM-bound: the weights are read once, and there is little time to convert them (g4_stream.cuh has the mathematics and the layout).  A CTA per SM has rows of its own, dealt
 // out evenly.  Its units (32 rows of 128 k each) go to its warps in equal runs; a warp's next units are on their way while one is multiplied, and
 // nothing in the loop waits for another warp.  A warp leaves its sums of a tile of rows in a slot of shared memory; at the end they are added up in the
-// order of warps, so that results are the same every time.  In graphs: 1 x 28672 x 8192 28.1 us (4.4 TB/s), 1 x 2048 x 2048 4.2, 7 x 5120 x 13824 in groups of 64 18.1.  Tiles of sixteen
+// order of warps, so that results are the same every time.  In graphs: 1 x 28672 x 8192 28.1 us (4.4 TB/s), 1 x 2048 x 2048 3.9, 7 x 5120 x 13824 in groups of 64 18.1.  Tiles of sixteen
 // rows or fewer count as whole ones: dealt out as halves they made the first 30.3.
 //
 // The tokens are scaled and permuted by each CTA for itself where that is one round of loads, else by a kernel in front, whose image of shared memory the CTAs
@@ -91,14 +91,14 @@ __global__ void __launch_bounds__(THREADS, 1) g4_stream_kernel(const Params p) {
   uint32_t C;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(C));
   const int rank = (int)sm100::cluster_ctarank();
-  const int cluster = blockIdx.x / C, clusters = gridDim.x / C;
-  const int s0 = rank * p.steps / (int)C, s1 = (rank + 1) * p.steps / (int)C, steps = s1 - s0;
+  const int log_c = (int)C >> 1, cluster = blockIdx.x >> log_c, clusters = gridDim.x >> log_c;      // of 1, 2, 4
+  const int s0 = rank * p.steps >> log_c, s1 = (rank + 1) * p.steps >> log_c, steps = s1 - s0;
   const int sb = step_bytes(p.M, G, TT);
   uint8_t* xs = smem + blockDim.x / 32 * WARP_BYTES;       // [steps][step_bytes]
-  float* slots = reinterpret_cast<float*>(xs + (p.steps + C - 1) / C * sb);      // [tiles + WARPS][ROWS][TOK]
+  float* slots = reinterpret_cast<float*>(xs + ((p.steps + (int)C - 1) >> log_c) * sb);      // [tiles + WARPS][ROWS][TOK]
 
   const int WARPS = blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int r0 = (int)((int64_t)cluster * p.N / clusters), rows = (int)((int64_t)(cluster + 1) * p.N / clusters) - r0;
+  const int share = p.N / clusters, more = p.N - share * clusters, r0 = cluster * share + min(cluster, more), rows = share + (cluster < more);
   const int tiles = (rows + ROWS - 1) / ROWS, units = tiles * steps;
   const int run = (units + WARPS - 1) / WARPS, u0 = min(units, warp * run), u1 = min(units, u0 + run);
 

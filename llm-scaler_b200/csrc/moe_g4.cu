@@ -44,11 +44,11 @@ __global__ void __launch_bounds__(256) g4_copies_kernel(const uint4* x, uint4* t
   }
 }
 
-template <bool BF16> __global__ void __launch_bounds__(256) g4_sum_kernel(const uint4* y, const int32_t* rows, uint4* out, int64_t total, int per, int k) {
+template <bool BF16> __global__ void __launch_bounds__(256) g4_sum_kernel(const uint4* y, const int32_t* rows, uint4* out, int per, int k) {
   constexpr int AT_ONCE = 8;
   grid_dep_enter();
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t t = i / per, c = i - t * per;
+  const int64_t t = blockIdx.x;
+  for (int c = threadIdx.x; c < per; c += 256) {
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < k; s0 += AT_ONCE) {
       uint4 v[AT_ONCE];
@@ -69,7 +69,7 @@ template <bool BF16> __global__ void __launch_bounds__(256) g4_sum_kernel(const 
         }
       }
     }
-    out[i] = make_uint4(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]), pack2<BF16>(acc[4], acc[5]), pack2<BF16>(acc[6], acc[7]));
+    out[t * per + c] = make_uint4(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]), pack2<BF16>(acc[4], acc[5]), pack2<BF16>(acc[6], acc[7]));
   }
 }
 
@@ -117,9 +117,8 @@ int moe_g4_many(const G4MoeArgs& a, void* scratch, cudaStream_t st) {
   g.x = p.h; g.w = a.w2; g.scale = a.s2; g.zero = a.z2; g.out_w = c.row_w; g.out = p.y; g.N = a.H; g.K = a.I; g.G = a.G2; g.gated = false;
   if (!rc) rc = umma_g4_grouped(g, st);
   if (rc) return rc;
-  const int64_t total = (int64_t)a.T * (a.H / 8), n = (total + 255) / 256;
-  launch_overlapped(a.bf16 ? g4_sum_kernel<true> : g4_sum_kernel<false>, dim3((unsigned)(n < 148 * 8 ? n : 148 * 8)), dim3(256), 0, st, overlap, reinterpret_cast<const uint4*>(p.y),
-                    (const int32_t*)out_rows, reinterpret_cast<uint4*>(a.out), total, a.H / 8, a.k);
+  launch_overlapped(a.bf16 ? g4_sum_kernel<true> : g4_sum_kernel<false>, dim3(a.T), dim3(256), 0, st, overlap, reinterpret_cast<const uint4*>(p.y),
+                    (const int32_t*)out_rows, reinterpret_cast<uint4*>(a.out), a.H / 8, a.k);
   note_launch("g4_sum");
   return launch_status();
 }

@@ -1,7 +1,8 @@
 // The 4-bit expert layer of a few tokens for given routes: two kernels that stream the chosen experts' weights (g4_stream.cuh has the mathematics and the layout), and a sum where
 // tokens are more than a handful.
 //
-// A chain of latencies for one token (128 experts of 2048 x 768, top-8: 19.1 us in a graph, 3.0 of bytes), issue slots and HBM for a batch (16 tokens: 71 us, 3.0 TB/s).  Every CTA sorts the routes by itself, in shared memory: the pairs (token, slot) of an expert form groups of
+// A chain of latencies for one token (128 experts of 2048 x 768, top-8: 18.1 us in a graph, 3.0 of bytes), issue slots and HBM for a batch (16 tokens: 70 us, 3.0 TB/s).  64-bit divisions ahead of the
+// first load cost a microsecond a layer, so there are none.  Every CTA sorts the routes by itself, in shared memory: the pairs (token, slot) of an expert form groups of
 // up to eight, whose tokens are the columns of one MMA.  A tile is 32 weight rows of one group; CTAs have equal runs of the tiles of all groups, and their
 // warps equal runs of the tiles' steps of 128 k, as in the linear.
 //  * up: a tile has sixteen gate rows and the sixteen up rows of the same outputs; h = silu(gate) * up goes out in 16 bits, with its largest magnitude per tile, from which the
@@ -136,8 +137,9 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
   // this CTA's tiles: strip by strip of every group in turn
   constexpr int STRIP = UP ? 16 : 32;                      // outputs of a tile
   const int strips = (p.N + STRIP - 1) / STRIP, all = sh.n_groups * strips;
-  const int begin = (int)((int64_t)blockIdx.x * all / gridDim.x), end = (int)((int64_t)(blockIdx.x + 1) * all / gridDim.x);
-  const int batches = (end - begin + p.cap - 1) / p.cap, cap = batches ? (end - begin + batches - 1) / batches : 0;
+  const int share = all / (int)gridDim.x, more = all - share * (int)gridDim.x, begin = (int)blockIdx.x * share + min((int)blockIdx.x, more), end = begin + share + ((int)blockIdx.x < more);
+  int cap = end - begin;
+  if (cap > p.cap) { const int batches = (cap + p.cap - 1) / p.cap; cap = (cap + batches - 1) / batches; }
   const uint32_t ring = smem_addr(smem) + warp * WARP_BYTES;
 
   for (int b0 = begin; b0 < end;) {
@@ -288,11 +290,12 @@ __global__ void __launch_bounds__(THREADS, 1) g4_experts_kernel(const Params p) 
   if (!waited) grid_dep_wait();                            // the kernel behind waits for this one, and so for all before it
 }
 
-template <bool BF16> __global__ void __launch_bounds__(256) g4_pairs_sum_kernel(const float* y, const int32_t* ids, uint16_t* out, int64_t total, int N, int k, int E) {
+template <bool BF16> __global__ void __launch_bounds__(256) g4_pairs_sum_kernel(const float* y, const int32_t* ids, uint16_t* out, int N, int k, int E) {
   grid_dep_release();
   grid_dep_wait();
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t t = i / N, n = i - t * N;
+  const int64_t t = blockIdx.y;
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n < N) {
     float f = 0.f;
     for (int s0 = 0; s0 < k; s0 += 8) {                    // requested together
       float v[8];
@@ -301,7 +304,7 @@ template <bool BF16> __global__ void __launch_bounds__(256) g4_pairs_sum_kernel(
 #pragma unroll
       for (int s = 0; s < 8; ++s) f += v[s];
     }
-    out[i] = to_half<BF16>(f);
+    out[t * N + n] = to_half<BF16>(f);
   }
 }
 
@@ -393,9 +396,7 @@ int moe_g4_few(const G4MoeArgs& a, void* scratch, cudaStream_t st) {
   p.early = tls().overlap_mode == 2;
   rc = by_type<false>(p, a.bf16, a.G2, q.down, st);
   if (rc) return rc;
-  const int64_t total = (int64_t)a.T * a.H, n = (total + 255) / 256;
-  launch_overlapped(a.bf16 ? g4_pairs_sum_kernel<true> : g4_pairs_sum_kernel<false>, dim3((unsigned)std::min<int64_t>(n, 1184)), dim3(256), 0, st, tls().overlap_mode > 0, (const float*)p.y,
-                    a.ids, p.out, total, a.H, a.k, a.E);
+  launch_overlapped(a.bf16 ? g4_pairs_sum_kernel<true> : g4_pairs_sum_kernel<false>, dim3((a.H + 255) / 256, a.T), dim3(256), 0, st, tls().overlap_mode > 0, (const float*)p.y, a.ids, p.out, a.H, a.k, a.E);
   note_launch("g4_pairs_sum");
   return launch_status();
 }
