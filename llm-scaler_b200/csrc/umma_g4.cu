@@ -15,7 +15,7 @@
 //  * Where strips of 256 rows are fewer than pairs of SMs, k is cut into pieces; whoever delivers the last of a strip's partial sums adds them up in order (arrivals.cuh).
 //  * GATED (expert up projection): a warp's 32 rows are 16 gate and 16 up rows of the same outputs, and the epilogue stores silu(gate) * up.
 //
-// In graphs: 4001 x 17408 x 5120 494 to 543 us by the GPU's power (1.3 to 1.44 PFLOP/s), 33 x 17408 x 5120 in groups of 32 22.2, 100 x 4096 x 4096 18.5; what bounds those up to 128 tokens is the
+// In graphs: 4001 x 17408 x 5120 484 to 587 us by the GPU's power (1.22 to 1.47 PFLOP/s), 33 x 17408 x 5120 in groups of 32 22.0, 100 x 4096 x 4096 18.5; what bounds those up to 128 tokens is the
 // transform, 650 to 750 cycles for a stage.
 //
 // No multicast load; every mbarrier wait is bounded, as in the other tcgen05 kernels.
@@ -100,8 +100,8 @@ template <int NT, bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile
     if (p.pieces > 1) {
       t.strip = id / p.pieces;
       t.piece = id - t.strip * p.pieces;
-      t.ks0 = (int)((int64_t)t.piece * p.nks / p.pieces);
-      t.n = (int)((int64_t)(t.piece + 1) * p.nks / p.pieces) - t.ks0;
+      t.ks0 = t.piece * p.nks / p.pieces;
+      t.n = (t.piece + 1) * p.nks / p.pieces - t.ks0;
       id = t.strip;
     }
     const int per = p.m_group * p.n_strips, gi = id / per, left = id - gi * per, m0 = gi * p.m_group;
@@ -113,7 +113,7 @@ template <int NT, bool GROUPED, bool GATED> __device__ __forceinline__ Tile tile
     t.n0 = st * WIDTH;
     t.w0 = t.n0;
   }
-  t.turn = (int)((int64_t)st * t.n / p.n_strips);
+  t.turn = st * t.n / p.n_strips;                          // below 2^23, since a matrix has fewer than 2^31 scales
   return t;
 }
 
