@@ -395,9 +395,10 @@ B2Q_API int b2q_moe_forward_int8(const b2q_moe_int8* args, void* workspace, size
  * in it, or with B2Q_GROUP_TOP2 the sum of its two largest p (+ bias) (of its one, where groups have one).  ids = the top_k largest keys of what stays,
  * in that order; equal keys, of experts and of groups, go to the lowest index first.  weights = scale * p, or scale * p / (sum of the chosen p) if
  * renormalize, in fp32.  No rounding decides: sums of p and bias are compared in 64 bits.
- * A logit of -inf, or a bias of -inf or NaN, takes an expert out of the choice; where fewer than top_k are left the last ids are -1 with the weight 0.  A token
- * whose logits hold a NaN or +inf, or nothing above -inf, gets no expert at all.  logits [T, E] with row pitch ldl, bias [E], any of the three
- * types each; weights, ids contiguous [T, top_k].  E <= 1024, num_groups <= 32 and a divisor of E, top_k <= 32 and <= top_groups * E / num_groups.   */
+ * A logit of -inf, or a bias of -inf or NaN, takes an expert out of the choice, and neither its p nor its bias counts for its group: with one expert left a group counts
+ * by that one, with none it is out.  Where fewer than top_k are left the last ids are -1 with the weight 0.  A token whose logits hold a NaN or +inf, or
+ * nothing above -inf, gets no expert at all.  logits [T, E] with row pitch ldl, bias [E], any of the three types each;
+ * weights, ids contiguous [T, top_k].  E <= 1024, num_groups <= 32 and a divisor of E, top_k <= 32 and <= top_groups * E / num_groups.   */
 #define B2Q_SCORE_SOFTMAX 0
 #define B2Q_SCORE_SIGMOID 1
 #define B2Q_GROUP_MAX  0

@@ -99,7 +99,7 @@ __device__ __forceinline__ bool choose(K (&key)[PER], const K (&gkey)[TOP2 ? PER
         const uint32_t who = __ballot_sync(0xffffffffu, a == best);
         if (lane == __ffs(who) - 1) a = b;
         const K second = warp_max(a);
-        best = best && second ? as_key(value(best) + value(second), K{}) : 0;
+        if (second) best = as_key(value(best) + value(second), K{});      // the only one left counts for itself
       }
       return best;
     };
@@ -122,7 +122,7 @@ __device__ __forceinline__ bool choose(K (&key)[PER], const K (&gkey)[TOP2 ? PER
         }
       }
       K best = a[0];
-      if (TOP2) best = best && b[0] ? as_key(value(best) + value(b[0]), K{}) : 0;
+      if (TOP2 && b[0]) best = as_key(value(best) + value(b[0]), K{});
       mine = __shfl_sync(0xffffffffu, best, lane * (32 / PER) & 31);
       if (lane >= p.groups) mine = 0;
     } else {

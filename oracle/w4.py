@@ -22,7 +22,8 @@ def route(logits, top_k, scoring="softmax", bias=None, num_groups=1, top_groups=
             of = []
             for g in range(num_groups):
                 best = sorted((with_bias if group_score == "top2" else key)[g * size:(g + 1) * size].tolist(), reverse=True)
-                of.append(sum(best[:2]) if group_score == "top2" else best[0])
+                left = [b for b in best[:2 if group_score == "top2" else 1] if b > -math.inf]      # what is out of the choice does not count
+                of.append(sum(left) if left else -math.inf)
             keep = sorted(range(num_groups), key=lambda g: (-of[g], g))[:top_groups]
             for g in range(num_groups):
                 if g not in keep:
