@@ -11,6 +11,7 @@
 // experts are registers, whose two best change hands by halves, and are ranked in the same way.
 // Scores are made in fp32 first, good to EPS; where no two that the choice depends on are nearer to each other than their errors, it is the one of 64 bits, and
 // only the other tokens are done again in those (in 64 bits throughout: 24 us, when the rest took 14).
+#include <cfloat>
 #include "g4.cuh"
 
 namespace b2q {
@@ -53,6 +54,9 @@ __device__ __forceinline__ Key as_key(double v, Key) { return key_of(v); }
 __device__ __forceinline__ uint32_t as_key(float v, uint32_t) { return key32(v); }
 __device__ __forceinline__ double value(Key k) { return value_of(k); }
 __device__ __forceinline__ float value(uint32_t k) { return value32(k); }
+// The key of what two add up to.  In fp32 a sum below all finite values is the lowest of those and not -inf, which would be no key; apart() then tells it from nothing near it.
+__device__ __forceinline__ Key both(Key a, Key b) { return key_of(value_of(a) + value_of(b)); }
+__device__ __forceinline__ uint32_t both(uint32_t a, uint32_t b) { return key32(fmaxf(value32(a) + value32(b), -FLT_MAX)); }
 
 // How far the fp32 keys may be off, relative to the larger of 1 and the key.  __expf is good to 2 + 1.17 |x| units of 2^-23, so that a sigmoid's p (1 - p) |x| of it is below 2^-23, the
 // quotient's two units are another 2^-23 at most, and the sums with 1 and with the bias are rounded to 2^-24.  A softmax has 2^-22 of its exponential and as much of those that its
@@ -99,7 +103,7 @@ __device__ __forceinline__ bool choose(K (&key)[PER], const K (&gkey)[TOP2 ? PER
         const uint32_t who = __ballot_sync(0xffffffffu, a == best);
         if (lane == __ffs(who) - 1) a = b;
         const K second = warp_max(a);
-        if (second) best = as_key(value(best) + value(second), K{});      // the only one left counts for itself
+        if (second) best = both(best, second);      // the only one left counts for itself
       }
       return best;
     };
@@ -122,7 +126,7 @@ __device__ __forceinline__ bool choose(K (&key)[PER], const K (&gkey)[TOP2 ? PER
         }
       }
       K best = a[0];
-      if (TOP2 && b[0]) best = as_key(value(best) + value(b[0]), K{});
+      if (TOP2 && b[0]) best = both(best, b[0]);
       mine = __shfl_sync(0xffffffffu, best, lane * (32 / PER) & 31);
       if (lane >= p.groups) mine = 0;
     } else {

@@ -46,6 +46,22 @@ def test_groups_with_one_expert_left(E, groups, scoring, dt):
                 check_route(l, min(8, top * (E // groups)), scoring=scoring, bias=b, num_groups=groups, top_groups=top, group_score=score)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("E,groups", [(16, 4), (128, 4), (60, 6)])
+def test_biases_of_the_types_lowest_value(E, groups, scoring, bt):
+    """They put an expert behind all others but do not take it out, two in a group neither, whose sum fp32 does not hold."""
+    size, low = E // groups, torch.finfo(bt).min
+    l = torch.randn(5, E, generator=gen(1))
+    for left in range(groups):      # groups whose biases are ordinary
+        bias = torch.full((E,), low, dtype=bt)
+        bias[:left * size] = (0.2 * torch.randn(left * size, generator=gen(2))).to(bt)
+        bias[-size:-1] = -INF       # and one expert of the last group
+        for top in range(1, groups + 1):
+            for score in ("top2", "max"):
+                check_route(l, min(6, top * size), scoring=scoring, bias=bias, num_groups=groups, top_groups=top, group_score=score)
+
+
 def test_sigmoids_that_are_not_renormalised():
     """Without a bias, at the edges: masked rows, scores that underflow and scores that round to one."""
     l = torch.randn(10, 64, generator=gen(7))
