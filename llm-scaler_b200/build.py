@@ -82,10 +82,14 @@ def build(force=False, verbose=False):
 def build_torch_ops(force=False, out=OUT_TORCH, source="torch_ops.cpp"):
     """libb2q_torch.so: the C++ torch-op registration of the dense linears (csrc/torch_ops.cpp) over libb2q.so; libb2q_int8.so: that of
     the 8-bit integer operators (csrc/torch_int8.cpp); libb2q_w4.so: that of expert routing and the 4-bit group-quantised layers (csrc/torch_w4.cpp).
-    Host code only: compiled with g++ against the installed torch's headers and linked with its libraries."""
+    Host code only: compiled with g++ against the installed torch's headers and linked with its libraries.
+
+    Linked with the shared libstdc++ that torch itself has loaded.  A compiler that comes with the archive alone would put a second one into the library, whose
+    streams find no facets that print numbers: a refusal with a number in its message ended the process.  Where the compiler does not know the option, the messages
+    are safe because they are made of strings alone."""
     src = os.path.join(CSRC, source)
     hdr = os.path.join(INCLUDE, "b2q.h")
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(hdr), os.path.getmtime(OUT)):
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(f) for f in (src, hdr, OUT, os.path.abspath(__file__))):
         return out
     import torch
     tdir = os.path.dirname(torch.__file__)
@@ -99,7 +103,9 @@ def build_torch_ops(force=False, out=OUT_TORCH, source="torch_ops.cpp"):
            "-I", os.path.join(cuda_home, "include"), src, "-o", out,
            "-L", os.path.dirname(OUT), "-l:libb2q.so", "-L", os.path.join(tdir, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
            "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    r = subprocess.run(cmd + ["-nostdlib++", "-l:libstdc++.so.6"], capture_output=True, text=True)
+    if r.returncode != 0:
+        r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("g++ failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
     return out

@@ -67,7 +67,7 @@ Int4View int4_view(const at::Tensor& weight, const at::Tensor& scale) {
   const int64_t G = v.K / GROUP;
   if (scale.size(0) == v.N && scale.size(1) == G) { v.sn = scale.stride(0); v.sg = scale.stride(1); }
   else if (scale.size(0) == G && scale.size(1) == v.N) { v.sn = scale.stride(1); v.sg = scale.stride(0); }
-  else TORCH_CHECK(false, "int4 scale shape [", scale.size(0), ", ", scale.size(1), "] does not match N=", v.N, ", K/128=", G);
+  else TORCH_CHECK(false, "int4 scale shape matches neither [N, K/128] nor [K/128, N] of the weight");      // strings alone: see build.py, build_torch_ops
   return v;
 }
 

@@ -21,7 +21,7 @@ int dtype_of(const Tensor& t) {
   TORCH_CHECK(false, "b2q: unsupported dtype ", t.scalar_type());
 }
 bool is16(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
-// Messages are made of strings alone: a compiler that puts libstdc++ into the library gives it a second set of the facets that print numbers, and printing one ended the process.
+// Messages are made of strings alone: see build.py, build_torch_ops.
 void check(int rc) { TORCH_CHECK(rc == 0, b2q_strerror(rc)); }
 
 // all on one CUDA device, that of the first
