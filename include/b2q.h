@@ -422,7 +422,7 @@ B2Q_API int b2q_linear_w4(const void* x, int act_dtype, int64_t ldx, const uint8
  * [0, E) contribute nothing (an expert of another rank, padding), an expert named twice counts twice.  w13 [E, 2I, H / 2] (gate rows, then up), s13 and z13
  * [E, H / group13, 2I], w2 [E, H, I / 2], s2 and z2 [E, I / group2, H], in the forms of b2q_linear_w4, all contiguous; z13, z2 may be NULL.  x, out
  * contiguous [T, H] and scales in act_dtype; x, w13, w2 and out 16-byte aligned; weights fp32 and ids int32 contiguous [T, top_k].  E <= 1024, top_k <= 32.
- * h is rounded to act_dtype; with many tokens so are the weights, and each weighted y before the sum.  workspace as above.                        */
+ * h is rounded to act_dtype; with many tokens so are the weights, and each weighted y before the sum (unless act_dtype cannot hold it).  workspace as above.                        */
 typedef struct b2q_moe_w4 {
   const void* x;
   const float* weights; const int32_t* ids;

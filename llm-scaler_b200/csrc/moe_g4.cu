@@ -44,10 +44,59 @@ __global__ void __launch_bounds__(256) g4_copies_kernel(const uint4* x, uint4* t
   }
 }
 
-template <bool BF16> __global__ void __launch_bounds__(256) g4_sum_kernel(const uint4* y, const int32_t* rows, uint4* out, int per, int k) {
+struct Outputs {                                           // what the outputs are made of: h by row, the experts' matrices, the pairs' experts and weights
+  const uint16_t* h; const uint8_t* w; const uint16_t* s; const uint8_t* z; const int32_t* ids; const float* weights; int I, G;
+};
+template <bool BF16> __device__ __forceinline__ float half_f(uint32_t raw) { return scalar_from_raw(raw, BF16 ? B2Q_BF16 : B2Q_F16); }
+// Expert e's output n of row r of h, in fp32.
+template <bool BF16> __device__ __forceinline__ float output(const Outputs& of, int64_t r, int64_t e, int H, int n) {
+  const uint16_t* h = of.h + r * of.I;
+  const uint8_t* w = of.w + (e * H + n) * (of.I / 2);
+  const int groups = of.I / of.G;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int g = 0; g < groups; ++g) {
+    const int64_t at = (e * groups + g) * H + n;
+    const float zero = of.z ? (float)of.z[at] : 8.f;
+    float d = 0.f;
+#pragma unroll 1
+    for (int k = g * of.G; k < (g + 1) * of.G; k += 8) {
+      const uint4 v = ld_vec(h + k);
+      const uint32_t q = *reinterpret_cast<const uint32_t*>(w + k / 2), x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {                        // h has them as g4_position says
+        d = fmaf(half_f<BF16>(x[j] & 0xFFFFu), (float)(q >> 4 * j & 15u) - zero, d);
+        d = fmaf(half_f<BF16>(x[j] >> 16), (float)(q >> (4 * j + 16) & 15u) - zero, d);
+      }
+    }
+    sum = fmaf(half_f<BF16>(of.s[at]), d, sum);
+  }
+  return sum;
+}
+// Eight columns n of token t once more, with every weighted output that is infinite in y made anew.
+template <bool BF16> __device__ __forceinline__ void sum_again(const uint16_t* y, const int32_t* rows, const Outputs& of, uint16_t* out, int64_t t, int n, int H, int k) {
+#pragma unroll 1
+  for (int j = n; j < n + 8; ++j) {
+    float acc = 0.f;
+#pragma unroll 1
+    for (int s = 0; s < k; ++s) {
+      const int64_t pair = t * k + s, r = __ldcg(rows + pair);
+      if (r < 0) continue;
+      float f = half_f<BF16>(__ldcg(reinterpret_cast<const unsigned short*>(y) + r * H + j));
+      if (fabsf(f) == INFINITY) f = __ldcg(of.weights + pair) * output<BF16>(of, r, __ldcg(of.ids + pair), H, j);
+      acc += f;
+    }
+    out[t * H + j] = (uint16_t)pack2<BF16>(acc, 0.f);
+  }
+}
+
+// A weighted output that its 16 bits cannot hold (fp16 beyond 65504) would make a sum infinite that is not, and is not so for few tokens, whose outputs stay in fp32: where a thread's
+// sums are not finite, it adds them up again and takes such outputs from h.
+template <bool BF16> __global__ void __launch_bounds__(256) g4_sum_kernel(const uint4* y, const int32_t* rows, uint4* out, int per, int k, const Outputs of) {
   constexpr int AT_ONCE = 8;
   grid_dep_enter();
   const int64_t t = blockIdx.x;
+  float none = 0.f;                                        // NaN once a sum of this thread's was not finite
   for (int c = threadIdx.x; c < per; c += 256) {
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < k; s0 += AT_ONCE) {
@@ -69,7 +118,13 @@ template <bool BF16> __global__ void __launch_bounds__(256) g4_sum_kernel(const 
         }
       }
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) none = fmaf(acc[j], 0.f, none);
     out[t * per + c] = make_uint4(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]), pack2<BF16>(acc[4], acc[5]), pack2<BF16>(acc[6], acc[7]));
+  }
+  if (none != 0.f) {
+#pragma unroll 1
+    for (int c = threadIdx.x; c < per; c += 256) sum_again<BF16>(reinterpret_cast<const uint16_t*>(y), rows, of, reinterpret_cast<uint16_t*>(out), t, 8 * c, 8 * per, k);
   }
 }
 
@@ -117,8 +172,9 @@ int moe_g4_many(const G4MoeArgs& a, void* scratch, cudaStream_t st) {
   g.x = p.h; g.w = a.w2; g.scale = a.s2; g.zero = a.z2; g.out_w = c.row_w; g.out = p.y; g.N = a.H; g.K = a.I; g.G = a.G2; g.gated = false;
   if (!rc) rc = umma_g4_grouped(g, st);
   if (rc) return rc;
+  const Outputs of{reinterpret_cast<const uint16_t*>(p.h), a.w2, reinterpret_cast<const uint16_t*>(a.s2), a.z2, a.ids, a.weights, a.I, a.G2};
   launch_overlapped(a.bf16 ? g4_sum_kernel<true> : g4_sum_kernel<false>, dim3(a.T), dim3(256), 0, st, overlap, reinterpret_cast<const uint4*>(p.y),
-                    (const int32_t*)out_rows, reinterpret_cast<uint4*>(a.out), a.H / 8, a.k);
+                    (const int32_t*)out_rows, reinterpret_cast<uint4*>(a.out), a.H / 8, a.k, of);
   note_launch("g4_sum");
   return launch_status();
 }
