@@ -65,7 +65,7 @@ size_t b2q_moe_forward_w4_workspace_bytes(int64_t T, int64_t E, int64_t top_k, i
   if (T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || top_k > 32 || H <= 0 || I <= 0 || H > MAX_K || I > MAX_K || T > INT32_MAX / 32) return 0;
   G4MoeArgs g{};
   g.T = (int)T; g.E = (int)E; g.k = (int)top_k; g.H = (int)H; g.I = (int)I;
-  const size_t few = moe_g4_few_bytes(g), many = moe_g4_many_bytes(g);      // which form it will be depends on the groups too
+  const size_t few = moe_g4_few_bytes(g), many = moe_g4_many_bytes(g);      // which form a few tokens get depends on the groups too
   return few > many ? few : many;
 }
 

@@ -50,7 +50,7 @@ struct G4MoeArgs {
   int T, E, k, H, I, G13, G2;
 };
 bool moe_g4_few_preferred(const G4MoeArgs& a);
-size_t moe_g4_few_bytes(const G4MoeArgs& a);
+size_t moe_g4_few_bytes(const G4MoeArgs& a);               // 0 where it serves with no groups
 int moe_g4_few(const G4MoeArgs& a, void* scratch, cudaStream_t st);
 bool moe_g4_many_fits(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I);      // its tiles can be counted
 size_t moe_g4_many_bytes(const G4MoeArgs& a);

@@ -329,8 +329,7 @@ static Room room_for(int pairs, int E, int strips, int K, int G) {
 struct Plan { Room up, down; bool fits; };
 static Plan plan(const G4MoeArgs& a) {
   Plan q{};
-  const int pairs = a.T * a.k;
-  if (pairs > MAX_PAIRS) return q;
+  const int pairs = a.T * a.k;                             // few_pairs()
   q.up = room_for(pairs, a.E, a.I / 16, a.H, a.G13);
   q.down = room_for(pairs, a.E, (a.H + ROWS - 1) / ROWS, a.I, a.G2);
   q.fits = q.up.columns > 0 && q.down.columns > 0;
@@ -365,9 +364,11 @@ static size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 
 // Up to five rows per expert (few / many, us; rows per expert in brackets): 128 experts of 2048 x 768, top-8, 16 tokens [1] 67 / 89, 48 [3] 102 / 119; 8 of 4096 x 4096, top-2, 16 [4]
 // 70 / 90, 32 [8] 97 / 91; 64 of 2048 x 1408 in groups of 32, top-6, 32 [3] 123 / 124, 60 [5.6] 141 / 127; 16 of 2048 x 2048, top-4, 16 [4] 45 / 59, 32 [8] 57 / 60.
-bool moe_g4_few_preferred(const G4MoeArgs& a) { return (int64_t)a.T * a.k <= 5 * (int64_t)a.E && g4f::plan(a).fits; }
+static bool few_pairs(const G4MoeArgs& a) { const int64_t pairs = (int64_t)a.T * a.k; return pairs <= g4f::MAX_PAIRS && pairs <= 5 * (int64_t)a.E; }
+bool moe_g4_few_preferred(const G4MoeArgs& a) { return few_pairs(a) && g4f::plan(a).fits; }
 
 size_t moe_g4_few_bytes(const G4MoeArgs& a) {
+  if (!few_pairs(a)) return 0;                             // I / 4 bytes more for each pair than the form of many tokens takes
   const size_t pairs = (size_t)a.T * a.k;
   return g4f::align_up(pairs * a.I * 2) + g4f::align_up(pairs * (a.I / 16) * 4) + g4f::align_up(pairs * a.H * 4);
 }
