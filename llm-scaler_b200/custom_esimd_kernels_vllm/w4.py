@@ -20,29 +20,64 @@ if not _MISSING:
 
 
 def _fakes():
-    """Outputs without data, for tracing: the sizes are checked as the ops check them, pointers and strides are not."""
+    """Outputs without data, for tracing: types and sizes are checked as csrc/torch_w4.cpp checks them; pointers, strides and the C functions' limits are not."""
     fake, check = torch.library.register_fake, torch._check
     half = (torch.bfloat16, torch.float16)
 
-    def width(w):
-        check(w.dtype in (torch.uint8, torch.int32), lambda: "weight must be uint8 or int32")
-        return w.shape[-1] * (2 if w.dtype == torch.uint8 else 8)
+    def refuse(condition, message):
+        check(condition, lambda: message)
+
+    def weight(name, x, w, s, z, experts=()):
+        """(N, K) of a weight, [N, K / 2] behind `experts`."""
+        d = len(experts)
+        refuse(w.dtype in (torch.uint8, torch.int32), name + " weight must be uint8 (two codes to a byte) or int32 (eight)")
+        refuse(w.dim() == 2 + d and s.dim() == 2 + d, name + " weight must be [.., N, K / 2] (int32: K / 8), its scale [.., K / group, N]")
+        N, K, groups = w.shape[d], w.shape[d + 1] * (2 if w.dtype == torch.uint8 else 8), s.shape[d]
+        refuse(s.dtype == x.dtype, name + " scale must have the activations' type")
+        refuse(s.shape[d + 1] == N, name + " scale must be [.., K / group, N]")
+        refuse(groups > 0, name + " scale has no groups")
+        refuse(K > 0 and K % groups == 0, name + " scale has a number of groups that does not divide K")
+        refuse(K // groups in (32, 64, 128), name + " groups must have 32, 64 or 128 values")
+        if experts:
+            refuse(w.shape[0] == experts[0] and s.shape[0] == experts[0], name + " weight and scale must have the same number of experts")
+        if z is not None:
+            refuse(z.dtype == torch.uint8 and z.dim() == s.dim() and all(i == j for i, j in zip(z.shape, s.shape)), name + " zero must be uint8 of the scale's shape")
+        return N, K
 
     @fake("b2q_w4::route_experts")
     def _(logits, top_k, scoring, bias, num_groups, top_groups, group_score, renormalize, scale):
-        check(logits.dim() == 2 and logits.dtype in half + (torch.float32,), lambda: "logits must be 2-D bf16, fp16 or fp32")
-        return logits.new_empty((logits.shape[0], top_k), dtype=torch.float32), logits.new_empty((logits.shape[0], top_k), dtype=torch.int32)
+        refuse(logits.dim() == 2 and logits.dtype in half + (torch.float32,), "logits must be 2-D bf16, fp16 or fp32")
+        T, E = logits.shape
+        refuse(scoring in (0, 1) and group_score in (0, 1), "scoring must be 0 (softmax) or 1 (sigmoid), group_score 0 (max) or 1 (top2)")
+        refuse(num_groups > 0, "num_groups must divide the number of experts")
+        refuse(E > 0 and E % num_groups == 0, "num_groups must divide the number of experts")
+        refuse(0 < top_groups and top_groups <= num_groups, "top_groups must be between 1 and num_groups")
+        refuse(0 < top_k and top_k <= E // num_groups * top_groups, "top_k must be between 1 and the number of experts in top_groups groups")
+        if bias is not None:
+            refuse(bias.dim() == 1 and bias.shape[0] == E and bias.dtype in half + (torch.float32,), "bias must be a bf16, fp16 or fp32 [E] tensor")
+        return logits.new_empty((T, top_k), dtype=torch.float32), logits.new_empty((T, top_k), dtype=torch.int32)
 
     @fake("b2q_w4::linear")
-    def _(x, weight, scale, zero, bias):
-        check(x.dim() == 2 and x.dtype in half and weight.dim() == 2 and width(weight) == x.shape[1], lambda: "x must be 2-D bf16 / fp16, weight [N, K / 2]")
-        check(scale.dim() == 2 and scale.shape[1] == weight.shape[0], lambda: "scale must be [K / group, N]")
-        return x.new_empty((x.shape[0], weight.shape[0]))
+    def _(x, w, scale, zero, bias):
+        refuse(x.dim() == 2 and x.dtype in half, "x must be 2-D bf16 or fp16")
+        N, K = weight("the", x, w, scale, zero)
+        refuse(x.shape[1] == K, "weight has another K than x")
+        if bias is not None:
+            refuse(bias.dim() == 1 and bias.shape[0] == N and bias.dtype == x.dtype, "bias must be an [N] tensor of x's type")
+        return x.new_empty((x.shape[0], N))
 
     @fake("b2q_w4::moe_forward")
     def _(x, topk_weights, topk_ids, gate_up_weight, gate_up_scale, down_weight, down_scale, gate_up_zero, down_zero):
-        check(x.dim() == 2 and x.dtype in half and topk_ids.dim() == 2 and topk_ids.shape[0] == x.shape[0], lambda: "x must be a bf16 / fp16 [T, H] tensor, topk_ids [T, top_k]")
-        check(down_weight.dim() == 3 and down_weight.shape[1] == x.shape[1], lambda: "the down weight must be of [E, H, I]")
+        refuse(x.dim() == 2 and x.dtype in half, "x must be a bf16 / fp16 [T, H] tensor")
+        refuse(topk_ids.dim() == 2 and topk_ids.shape[0] == x.shape[0] and topk_ids.shape[1] > 0 and topk_ids.dtype == torch.int32, "topk_ids must be an int32 [T, top_k] tensor")
+        refuse(topk_weights.dim() == 2 and topk_weights.shape[0] == topk_ids.shape[0] and topk_weights.shape[1] == topk_ids.shape[1] and topk_weights.dtype == torch.float32,
+               "topk_weights must be an fp32 tensor of the shape of topk_ids")
+        refuse(gate_up_weight.dim() == 3 and gate_up_weight.shape[0] > 0, "the gate_up weight must be of [E, 2I, H], with experts")
+        E, H = gate_up_weight.shape[0], x.shape[1]
+        two_i, k_up = weight("the gate_up", x, gate_up_weight, gate_up_scale, gate_up_zero, (E,))
+        n_down, k_down = weight("the down", x, down_weight, down_scale, down_zero, (E,))
+        refuse(k_up == H and two_i % 2 == 0, "the gate_up weight must be of [E, 2I, H]")
+        refuse(n_down == H and 2 * k_down == two_i, "the down weight must be of [E, H, I]")
         return x.new_empty(x.shape)
 
 
