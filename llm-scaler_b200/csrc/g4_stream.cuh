@@ -304,7 +304,8 @@ template <bool BF16> __device__ __forceinline__ int row_shift(uint32_t mx) {
   const int ex = (int)(__float_as_uint(half_f<BF16>(mx)) >> 23);
   return mx == 0 || ex == 255 ? 0 : min(126, max(-126, 14 - (ex - 127)));
 }
-__device__ __forceinline__ float unshift(float v, int shift) { return v * 16777216.f * pow2(-shift); }
+// v 2^(24 - shift), in two halves, so that what lies between them is beyond fp32 only where v or the result is
+__device__ __forceinline__ float unshift(float v, int shift) { const int e = 24 - shift, half = e >> 1; return v * pow2(half) * pow2(e - half); }
 __device__ __forceinline__ uint32_t max_bits(const uint4& v) {      // of eight magnitudes, which order as their bits
   const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
   return max(m & 0xFFFFu, m >> 16);
