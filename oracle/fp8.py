@@ -98,8 +98,8 @@ def linear_tensor(x, wq, s, e5m2=False):
 
 
 def linear_block_w8a16(x, wq, ws):
-    """The reference's block path keeps the activation in 16 bit (vllm/patches/vllm_for_multi_arc.patch:2671-2683)."""
-    return x.float() @ dequant_block(wq, ws).T
+    """The reference's block path keeps the activation in 16 bit (vllm/patches/vllm_for_multi_arc.patch:2671-2683).  Sums in 64 bits: those of fp32 depend on the machine."""
+    return (x.double() @ dequant_block(wq, ws).double().T).float()
 
 
 def linear_block_w8a8(xq, xs, wq, ws):
