@@ -24,7 +24,7 @@ struct Params {
   const uint16_t* x; int64_t ldx; int vec;
   const uint8_t* image; const int* shifts;                 // of the kernel in front, or null
   Matrix w; const uint16_t* bias; uint16_t* out; int64_t ldo;
-  int M, N, K, steps, cap;                                 // steps: of all K; cap: tiles of rows a CTA or cluster may have
+  int M, N, K, steps;                                      // steps: of all K
   int early;
   int* status;
 };
@@ -237,7 +237,6 @@ static Plan plan(int M, int N, int K, int G) {
 }
 
 template <int VEC, int TT, bool BF16, bool PART> static int launch(Params& p, const Plan& q, cudaStream_t st) {
-  p.cap = q.cap;
   const bool overlap = tls().overlap_mode > 0;
   if (p.image) {
     launch_overlapped(g4_prep_kernel<32 * VEC, TT, BF16>, dim3(p.M), dim3(256), 0, st, overlap, p.x, p.ldx, p.vec, const_cast<uint8_t*>(p.image), const_cast<int*>(p.shifts), p.M, p.K, p.steps);
