@@ -1,6 +1,6 @@
 // Linear of a few tokens on 4-bit group-quantised weights: out[m, n] = sum_g s[g, n] (sum_k x[m, k] q[n, k] - z[g, n] X[m, g]) (+ bias[n]).
 //
-// HBM-bound: the weights are read once, and there is little time to convert them (g4_stream.cuh has the mathematics and the layout).  A CTA per SM has rows of its own, dealt
+// The weights are read once, and there is little time to convert them (g4_stream.cuh has the mathematics, the layout and what holds the loop).  A CTA per SM has rows of its own, dealt
 // out evenly.  Its units (32 rows of 128 k each) go to its warps in equal runs; a warp's next units are on their way while one is multiplied, and
 // nothing in the loop waits for another warp.  A warp leaves its sums of a tile of rows in a slot of shared memory; at the end they are added up in the
 // order of warps, so that results are the same every time.  In graphs: 1 x 28672 x 8192 28.1 us (4.4 TB/s), 1 x 2048 x 2048 3.9, 7 x 5120 x 13824 in groups of 64 18.1.  Tiles of sixteen
@@ -278,7 +278,8 @@ template <int VEC, bool PART> static int by_type(Params& p, bool bf16, const Pla
 }  // namespace g4s
 
 // Up to eight tokens, and up to sixteen of small layers (here / on tcgen05, us: 16 x 2048 x 2048 7.2 / 8.2, 16 x 1024 x 8192 9.1 / 11.2, 16 x 4096 x 4096 10.8 / 10.3, 12 x 28672 x
-// 2048 16.7 / 14.7, 16 x 17408 x 5120 24.0 / 18.8; 8 x 4096 x 4096 7.8 / 10.0).
+// 2048 16.7 / 14.7, 16 x 17408 x 5120 24.0 / 18.8; 8 x 4096 x 4096 7.8 / 10.0).  Eight tokens of a K above some 25000 have no room in shared memory and go to tcgen05, for want of another form: 8 x 4096 x 24576
+// 22.6 / 28.4, 7 x 4096 x 28672 25.7 / 32.3, 8 x 4096 x 28672 - / 32.2.
 bool g4_stream_preferred(int M, int N, int K, int G) { return M <= (N * (int64_t)K <= 12 << 20 ? 16 : 8) && g4s::plan(M, N, K, G).smem > 0; }
 
 size_t g4_stream_bytes(int M, int N, int K, int G) {

@@ -5,7 +5,7 @@
 // the scores that a group's two best add up to.  So no rounding of the scores decides between two experts, and equal keys go to the lowest index.
 // Weights are fp32, of the scores without the bias.
 //
-// Bound by issue slots (4093 tokens of 256 experts: 1090 instructions a token, nearly half of all slots) and, for a few tokens, by its chain of exchanges.  A warp per token,
+// Held by latencies: for many tokens those of loads, arithmetic and exchanges together (4093 tokens of 256 experts: 1090 instructions a token, 47 % of the issue slots), for a few by one chain of exchanges.  A warp per token,
 // its logits in registers.  The need-th largest of the lanes' maxima leaves a dozen experts or so, which are then ranked by counting, a lane each; k rounds of a
 // warp-wide maximum over all registers took 13.8 us where this takes 11.1 (16384 tokens of 128 experts: 10.5 and 9.5; one of 256: 4.5 and 3.6).  Groups of 32
 // experts are registers, whose two best change hands by halves, and are ranked in the same way.

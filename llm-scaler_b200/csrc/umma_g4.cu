@@ -6,7 +6,7 @@
 // subtracted), times s is the one rounding; it is of the size of the output's own.
 //
 // Two CTAs share a tile of 256 rows (cta_group::2), each with its own 128 rows in tensor memory and half of the tokens in shared memory: a CTA alone would pull twice the
-// tokens through L2, which at 9 TB/s is what bounds narrow tiles too (64 x 17408 x 5120: 97 MB of tokens beside 46 of weights).
+// tokens through L2, which at 9 TB/s is what bounds narrow tiles too (64 x 17408 x 5120: 89 MB of tokens, 45 in pairs, beside 46 of weights).
 //
 // A persistent CTA has separate warps for the weights' copies, the tokens' copies, the MMA, the epilogue and the transform, so that nothing of one tile stops the stream of the
 // next.  An operand stage is 128 k; each ring stage stays with one group of four transform warps, since a parity wait cannot tell a phase from the one before the
@@ -15,8 +15,10 @@
 //  * Where strips of 256 rows are fewer than pairs of SMs, k is cut into pieces; whoever delivers the last of a strip's partial sums adds them up in order (arrivals.cuh).
 //  * GATED (expert up projection): a warp's 32 rows are 16 gate and 16 up rows of the same outputs, and the epilogue stores silu(gate) * up.
 //
-// In graphs: 4001 x 17408 x 5120 484 to 587 us by the GPU's power (1.22 to 1.47 PFLOP/s), 33 x 17408 x 5120 in groups of 32 22.0, 100 x 4096 x 4096 18.5; what bounds those up to 128 tokens is the
-// transform, 650 to 750 cycles for a stage.
+// In graphs: 4001 x 17408 x 5120 484 to 587 us by the GPU's power (1.22 to 1.47 PFLOP/s), 33 x 17408 x 5120 in groups of 32 22.0, 100 x 4096 x 4096 18.5.  Up to 128 tokens the
+// transform sets the pace, 650 to 750 cycles for a stage, and no unit is full while it does: of 33 x 17408 x 5120 issue slots 52 %, the ALU pipe 45, the 16-bit one 26, tensor cores 26 (grouped
+// 64, 54, 32, 32); fp16, whose decode has two operations fewer for a word, takes 24.0 us where bf16 takes 25.2 (cold, one launch).  Of the 9.6 cycles between two instructions of a warp 2.1 wait for
+// loads, 1.7 at barriers, 1.1 for fixed latencies.  What would shorten the chain is not known; more groups and more slots did not.
 //
 // No multicast load; every mbarrier wait is bounded, as in the other tcgen05 kernels.
 #include <type_traits>
@@ -667,6 +669,11 @@ static int by_type(bool bf16, int G, const CUtensorMap& tx, const CUtensorMap& t
 static size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 struct Plan { int nt, pieces, m_tiles, n_strips; };
+// Heights, us in graphs, K = 5120, N = 17408: 32 tokens 19.8 in a tile of 32, 20.2 of 64; 48 tokens 32.9, 20.5 and 23.0 of 32, 64 and 128; 96 tokens 34.2, 24.0 and 33.4 of 64, 128 and 256; 128 tokens 34.5,
+// 26.0, 33.9; 129 tokens 38.0 and 35.6 of 128 and 256, 256 tokens 41.4 and 37.6, 1024 142 and 127, 4001 581 and 506.  Where strips are few, 256 loses up to 512 tokens (4096 x 4096: 129 tokens
+// 18.8 and 22.3, 512 21.3 and 26.5, 1024 33.8 and 31.2); the rule does not tell these apart.
+// Pieces, at most eight: 24 x 512 x 14336 19.2 with four, 16.3 with eight, 18.3 with sixteen; 40 x 1024 x 8192 15.1, 15.6, 20.2; 100 x 1024 x 8192 20.4, 24.1, 34.2.  Of four stages at least: 40 x 1024 x 2048 12.7 of
+// two, 10.4 of four, 9.8 of eight; 300 x 512 x 2048 27.4, 20.7, 19.1; 100 x 512 x 1024 13.4, 11.1, 6.8.
 static Plan plan(int M, int N, int K) {
   Plan q{};
   q.nt = M <= 32 ? 32 : (M <= 64 ? 64 : (M <= 128 ? 128 : 256));
@@ -712,6 +719,7 @@ int umma_g4_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st) {
   p.s = reinterpret_cast<const uint16_t*>(a.scale); p.z = a.zero; p.s_rows = a.N;
   p.bias = reinterpret_cast<const uint16_t*>(a.bias); p.out = reinterpret_cast<uint16_t*>(a.out); p.ldo = a.ldo; p.vec_out = aligned16(a.out) && a.ldo % 8 == 0;
   p.M = a.M; p.N = a.N; p.K = a.K; p.groups = a.K / a.G; p.nks = (a.K + 127) / 128;
+  // sixteen tiles of tokens take turns at a strip: 2048 x 8192 x 8192 191 us with 4 or 16, 197 with 8 or 32, 244 with 64 (which is none); 4001 x 17408 x 5120 482 to 508 with 4 to 32, 530 with 64
   p.n_strips = q.n_strips; p.m_tiles = q.m_tiles; p.m_group = q.m_tiles < 16 ? q.m_tiles : 16; p.pieces = q.pieces;
   p.total = q.n_strips * q.m_tiles * q.pieces;
   if (q.pieces > 1) {
@@ -737,7 +745,9 @@ int umma_g4_linear(const G4LinearArgs& a, void* scratch, cudaStream_t st) {
   return by_type<256, false, false>(a.bf16, a.G, tx, tw, p, grid, st);
 }
 
-// Token height of the tiles, from the mean rows per expert.
+// Token height of the tiles, from the mean rows per expert (in brackets; us in graphs of the layer in tiles of 32, 64, 128): 64 experts of 2048 x 1408, top-8, groups of 64 [16] 109, 110, 133, [24] 113, 111, 135,
+// [32] 149, 113, 137, [48] 191, 118, 141, [64] 233, 157, 143, [96] 315, 201, 151, [128] 399, 244, 203; 128 of 2048 x 768 [24] 117, 119, 143, [32] 151, 122, 146, [48] 203, 133, 153, [64] 246, 172, 158; 8 of
+// 4096 x 4096, top-2 [24] 87, 90, 99, [32] 113, 90, 102, [48] 138, 93, 104, [64] 174, 125, 103.
 int g4_grouped_tile(int64_t rows, int E) {
   const int64_t avg = (rows + E - 1) / E;
   return avg <= 24 ? 32 : (avg <= 48 ? 64 : 128);
